@@ -464,6 +464,30 @@ int p2b_mean_over_hand_perms(const float* values, const int32_t* perms, int32_t 
 int p2b_indexed_add_rows(float* out, const int64_t* index, const float* src, int64_t num_src, int64_t num_out,
                          int64_t width, int mean, int accumulate, void* stream);
 
+/* ---- network operators (no counterpart upstream, whose networks are torch modules) -------------------
+ * The gated hidden layer of a value or policy network and its gradients on the tensor cores.
+ * x [rows,width], gate_weight and up_weight [hidden,width], gate_bias and up_bias [hidden] (either may be NULL),
+ * all of one type: dtype 0 bf16, 1 fp16; rows x_stride, ... elements apart, elements of a row next to each other.
+ * activation 0: gelu (with erf), 1: silu.  Sums in fp32.
+ *   h = act(x gate_weight^T + gate_bias) * (x up_weight^T + up_bias)        [rows,hidden], one rounding
+ * Rows of x and of the weights start on 16-byte boundaries, unless there are at most p2b_gated_few_rows() rows
+ * (forward only).  A wait that runs out inside a kernel leaves NaN in the outputs that hung on it.
+ * p2b_gated_backward: gradients of sum(grad_h * h); dgate = grad_h * up * act' and dup = grad_h * act are rounded to the type
+ * once on their way into the products.  dx [rows,width] (dx_stride), dwg and dwu [hidden,width], dbg and dbu [hidden]
+ * packed; any of the five may be NULL.  scratch: p2b_gated_backward_scratch_bytes(rows, hidden), 16-byte aligned.
+ * The same inputs give the same bits. */
+int p2b_gated_few_rows(void);
+int p2b_gated_forward(const void* x, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
+                      const void* up_weight, int64_t up_stride, const void* gate_bias, const void* up_bias,
+                      int64_t rows, int32_t width, int32_t hidden, int32_t dtype, int32_t activation, void* h,
+                      int64_t h_stride, void* stream);
+int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t hidden);
+int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, int64_t x_stride,
+                       const void* gate_weight, int64_t gate_stride, const void* up_weight, int64_t up_stride,
+                       const void* gate_bias, const void* up_bias, int64_t rows, int32_t width, int32_t hidden,
+                       int32_t dtype, int32_t activation, void* dx, int64_t dx_stride, void* dwg, void* dwu,
+                       void* dbg, void* dbu, void* scratch, int64_t scratch_bytes, void* stream);
+
 /* ---- self-test (no counterpart in the reference) ------------------------------------------
  * The solver's divisions share divisors and run through a short correctly rounded sequence
  * (csrc/exactdiv.cuh).  p2b_selftest_division compares it with the compiler's IEEE division

@@ -77,6 +77,9 @@ _SIGNATURES = {
     "p2b_mean_over_hand_perms": [_vp, _vp, _i32, _i64, _vp, _vp],
     "p2b_tree_count": [_vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp],
     "p2b_tree_records": [_vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "p2b_gated_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
+    "p2b_gated_backward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp,
+                           _vp, _vp, _vp, _vp, _i64, _vp],
     "p2b_selftest_division": [ctypes.c_uint64, ctypes.c_uint32, _vp, _vp, _vp],
     "p2b_selftest_division_sweep": [_vp, _vp, _vp],
 }
@@ -85,6 +88,7 @@ _VALUE_FUNCS = {"p2b_cfr_scratch_floats": ([_i32, _i32], _i64), "p2b_cfr_default
                 "p2b_cfr_solve_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_solve_block_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_step_scratch_floats": ([_i32, _i32, _i64], _i64),
+                "p2b_gated_few_rows": ([], _i32), "p2b_gated_backward_scratch_bytes": ([_i64, _i32], _i64),
                 "p2b_cfr_noalloc_scratch_floats": ([], _i64), "p2b_cfr_path_policy": ([_i32], _i32)}
 
 
@@ -166,3 +170,20 @@ def card_ids(t: torch.Tensor):
 def require_cuda(t: torch.Tensor, what: str) -> None:
     if t.device.type != "cuda":
         raise ValueError(f"{what} requires a CUDA tensor.")
+
+
+def plain_rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix whose rows are packed and do not overlap: `t` itself where it is one."""
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) or t.shape[1] == 1 and t.stride(0) >= 1 else t.contiguous()
+
+
+def wide_rows(t: torch.Tensor) -> torch.Tensor:
+    """The same with every row on a 16-byte boundary, as the tensor-memory kernels load them: copied where it is not."""
+    per = 16 // t.element_size()
+    rows, columns = t.shape
+    if t.data_ptr() % 16 == 0 and (columns == 1 or t.stride(1) == 1) and t.stride(0) >= columns and t.stride(0) % per == 0:
+        return t
+    if rows <= 1 and t.data_ptr() % 16 == 0 and (columns == 1 or t.stride(1) == 1) and columns % per == 0:
+        return t
+    out = torch.empty(rows, (columns + per - 1) // per * per, dtype=t.dtype, device=t.device)[:, :columns]
+    return out.copy_(t)

@@ -9,7 +9,8 @@ import sys
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libpoker2_b200.so")
-SOURCES = ["common.cu", "rank7.cu", "showdown.cu", "cfr.cu", "cfr_wide.cu", "cfr_iter.cu", "cfr_split.cu", "stepops.cu", "chance.cu", "treebuild.cu", "selftest.cu", "api.cu"]
+SOURCES = ["common.cu", "rank7.cu", "showdown.cu", "cfr.cu", "cfr_wide.cu", "cfr_iter.cu", "cfr_split.cu", "stepops.cu", "chance.cu", "treebuild.cu", "selftest.cu", "api.cu",
+           "tensor.cu", "gated.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -19,6 +20,8 @@ NVCC_FLAGS = [
     "-fmad=false",
     "-Xcompiler", "-fPIC",
 ]
+# The network operators have no upstream bits to match: their sums contract.
+CONTRACTED = {"gated.cu"}
 
 
 def nvcc_path() -> str:
@@ -59,7 +62,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
             newest_source = max(newest_source, os.path.getmtime(os.path.join(CSRC, "cfr.cu")))
         if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(newest_source, newest_header):
             continue
-        cmd = [nvcc, *NVCC_FLAGS, "-c", src_path, "-o", obj]
+        flags = [f for f in NVCC_FLAGS if f != "-fmad=false" or src not in CONTRACTED]
+        cmd = [nvcc, *flags, "-c", src_path, "-o", obj]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

@@ -1,0 +1,82 @@
+"""Plain 64-bit forms of the network operators, and bounds on how far a kernel may be from them."""
+import math
+
+import torch
+
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}  # of the value
+SMALLEST = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}  # half a step below the normal numbers
+
+
+def activation(z, name):
+    if name == "none":
+        return z
+    return z * 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5))) if name == "gelu" else z * torch.sigmoid(z)
+
+
+def slope(z, name):
+    if name == "gelu":
+        return 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
+    s = torch.sigmoid(z)
+    return s * (1.0 + z * (1.0 - s))
+
+
+def rounded(value, dtype):
+    """How far a rounding to dtype may move each value."""
+    return value.abs() * HALF_STEP[dtype] + SMALLEST[dtype]
+
+
+def summed(magnitudes, terms):
+    """Error of a sum of `terms` fp32 terms whose magnitudes add up to `magnitudes`: a step of 2^-23 an addition (the tensor cores
+    need not round to nearest), two more for what is added to the sum."""
+    return magnitudes * ((terms + 2) * 2.0 ** -23)
+
+
+def gated(x, wg, wu, bg, bu, name, dtype):
+    """(h, bound) in 64 bits; h before its rounding to dtype."""
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    zero = torch.zeros(wg.shape[0], dtype=torch.float64, device=x.device)
+    bg, bu = (zero if b is None else b.double() for b in (bg, bu))
+    gate, up = x @ wg.T + bg, x @ wu.T + bu
+    mag_g, mag_u = x.abs() @ wg.abs().T + bg.abs(), x.abs() @ wu.abs().T + bu.abs()
+    K = x.shape[-1]
+    a = activation(gate, name)
+    # |act'| <= 1.13; the activation itself: 2^-20 of its argument's size (a handful of fp32 steps); the product's own step
+    err_a = 1.13 * summed(mag_g, K) + gate.abs() * 2.0 ** -20
+    err = err_a * (up.abs() + summed(mag_u, K)) + a.abs() * summed(mag_u, K) + (a * up).abs() * 2.0 ** -22
+    h = a * up
+    return h, err + rounded(h.abs() + err, dtype)
+
+
+def gated_backward(dh, x, wg, wu, bg, bu, name, dtype):
+    """{name: (gradient, bound)}: the rounding of dgate and dup, taken at its worst in every term, the fp32 sums, the last rounding."""
+    dh, x, wg, wu = dh.double(), x.double(), wg.double(), wu.double()
+    zero = torch.zeros(wg.shape[0], dtype=torch.float64, device=x.device)
+    bg, bu = (zero if b is None else b.double() for b in (bg, bu))
+    gate, up = x @ wg.T + bg, x @ wu.T + bu
+    K, F, M = x.shape[-1], wg.shape[0], x.shape[0]
+    err_g, err_u = summed(x.abs() @ wg.abs().T + bg.abs(), K), summed(x.abs() @ wu.abs().T + bu.abs(), K)
+    a, s = activation(gate, name), slope(gate, name)
+    dg, du = dh * up * s, dh * a
+    # |act''| <= 0.8, |act'| <= 1.13, functions to 2^-20
+    e_dg = dh.abs() * (err_u * s.abs() + (up.abs() + err_u) * (0.8 * err_g + 2.0 ** -20 * (1 + gate.abs())))
+    e_du = dh.abs() * (1.13 * err_g + gate.abs() * 2.0 ** -20)
+    e_dg, e_du = e_dg + rounded(dg.abs() + e_dg, dtype), e_du + rounded(du.abs() + e_du, dtype)
+
+    def with_bound(value, err, mag, terms):
+        err = err + summed(mag + err, terms)
+        return value, err + rounded(value.abs() + err, dtype)
+
+    return {
+        "dx": with_bound(dg @ wg + du @ wu, e_dg @ wg.abs() + e_du @ wu.abs(), dg.abs() @ wg.abs() + du.abs() @ wu.abs(), 2 * F),
+        "dwg": with_bound(dg.T @ x, e_dg.T @ x.abs(), dg.abs().T @ x.abs(), M),
+        "dwu": with_bound(du.T @ x, e_du.T @ x.abs(), du.abs().T @ x.abs(), M),
+        "dbg": with_bound(dg.sum(0), e_dg.sum(0), dg.abs().sum(0), M),
+        "dbu": with_bound(du.sum(0), e_du.sum(0), du.abs().sum(0), M),
+    }
+
+
+def assert_within(got, value, bound, what=""):
+    off = (got.double() - value).abs() - bound
+    worst = off.max().item() if off.numel() else 0.0
+    assert torch.isfinite(got.double()).all(), what
+    assert worst <= 0.0, f"{what}: {int((off > 0).sum())} of {off.numel()} outside, worst by {worst:.3g} (bound {bound.flatten()[off.argmax()].item():.3g})"
