@@ -488,6 +488,27 @@ int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, i
                        int32_t dtype, int32_t activation, void* dx, int64_t dx_stride, void* dwg, void* dwu,
                        void* dbg, void* dbu, void* scratch, int64_t scratch_bytes, void* stream);
 
+/* Microscaled 4-bit values: a row in blocks of 32, each with a power-of-two scale, the smallest that brings the block's largest
+ * magnitude to 6 or below; values are the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, ties to the even code.  A
+ * block with an infinity or a NaN reads back as NaN.
+ *  values  p2b_mx4_value_bytes(rows, width): rows of ceil(width/32)*16 bytes, two values a byte, the first in the low half
+ *  scales  p2b_mx4_scale_bytes(rows, width): exponent + 127 (255: NaN) in pieces of 512 bytes for 128 rows x 4 blocks,
+ *          ceil(width/256)*2 pieces for a group of 128 rows; (row % 32)*16 + (row % 128)/32*4 + block % 4 inside a piece
+ * Both on 16-byte boundaries.  dtype of x and out 0 bf16, 1 fp16, 2 fp32 (p2b_mx4_linear: 0 or 1); rows x_stride elements
+ * apart, any alignment.
+ * p2b_mx4_linear: out [rows,columns] = act(A W^T + bias) of two quantised matrices of the same width, fp32 sums, bias [columns]
+ * (may be NULL) and out of one type; activation 0 gelu (with erf), 1 silu, 2 none.  A wait that runs out inside the kernel
+ * leaves NaN in the outputs that hung on it. */
+int64_t p2b_mx4_value_bytes(int64_t rows, int32_t width);
+int64_t p2b_mx4_scale_bytes(int64_t rows, int32_t width);
+int p2b_mx4_quantise(const void* x, int64_t x_stride, int64_t rows, int32_t width, int32_t dtype, void* values, void* scales,
+                     void* stream);
+int p2b_mx4_dequantise(const void* values, const void* scales, int64_t rows, int32_t width, int32_t dtype, void* out,
+                       int64_t out_stride, void* stream);
+int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales,
+                   int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out,
+                   int64_t out_stride, void* stream);
+
 /* ---- self-test (no counterpart in the reference) ------------------------------------------
  * The solver's divisions share divisors and run through a short correctly rounded sequence
  * (csrc/exactdiv.cuh).  p2b_selftest_division compares it with the compiler's IEEE division

@@ -1,0 +1,403 @@
+// Microscaled 4-bit values: rows in blocks of 32 that share a power-of-two scale; quantising, reading back, and the product
+// of two such matrices on the block-scaled matrix instructions.
+//
+// A block's scale is the smallest power of two that brings its largest magnitude to 6 or below (no value is cut off); a
+// value then goes to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even code.  Both steps are exact in fp32.
+//
+// Layout: values two a byte, the first in the low half, a row of ceil(width/32) * 16 bytes.  Scales (exponent + 127 in a byte,
+// 255: the block holds an infinity or a NaN) as the matrix instructions read them: 512 bytes hold 128 rows x 4 blocks, at
+// (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4; an even number of these along the row, so that a step of 256 columns
+// always finds two.  The entries behind the last row and the last block are zero.
+#include "layer.cuh"
+#include "tensor.cuh"
+
+namespace p2b {
+
+using namespace tc;
+
+// pieces of 512 scale bytes along a row of `width` values
+__host__ __device__ __forceinline__ int64_t scale_pieces(int64_t width) { return (width + 255) / 256 * 2; }
+
+template <typename T> struct Eight;  // 8 neighbouring values as fp32
+template <> struct Eight<float> {
+    static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    static __device__ __forceinline__ float one(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+};
+template <bool kBf16> struct EightHalf {
+    static __device__ __forceinline__ void load(const void* p, float (&v)[8]) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack<kBf16>(w[i]);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ float one(const void* p) { return widen<kBf16>(*reinterpret_cast<const uint16_t*>(p)); }
+    static __device__ __forceinline__ void put(void* p, float v) { *reinterpret_cast<uint16_t*>(p) = narrow<kBf16>(v); }
+    static __device__ __forceinline__ void store(void* p, const float (&v)[8]) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack<kBf16>(v[0], v[1]), pack<kBf16>(v[2], v[3]), pack<kBf16>(v[4], v[5]), pack<kBf16>(v[6], v[7]));
+    }
+};
+template <> struct Eight<__nv_bfloat16> : EightHalf<true> {};
+template <> struct Eight<__half> : EightHalf<false> {};
+
+// Scale byte of a block whose largest magnitude is `top`: top = 2^E m, 1 <= m < 2, is at most 6 * 2^(E-2) where m <= 1.5.
+__device__ __forceinline__ uint32_t scale_byte(float top) {
+    const uint32_t bits = __float_as_uint(top);
+    if (bits >= 0x7F800000u) return 255u;
+    const int e = (int)(bits >> 23) - ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 2);
+    return (uint32_t)(e > 0 ? e : 0);
+}
+// 2^(127 - byte) for the bytes that a finite block gets, 0 to 253
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return byte == 255u ? __int_as_float(0x7FC00000) : byte ? __uint_as_float(byte << 23) : 5.8774717541114375e-39f;
+}
+__device__ __forceinline__ uint32_t four_bit_pair(float lo, float hi) {
+    uint32_t v;
+    asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ float four_bit_value(uint32_t code) {
+    // magnitudes 0, 0.5 and then sign and two exponent bits, one mantissa bit
+    const uint32_t m = code & 7u;
+    const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+    return code & 8u ? -v : v;
+}
+
+// Four lanes take a block, a warp 256 neighbouring columns of a row: 16-byte loads (16-bit types), 128 bytes of values and two
+// scale words out.  Bound by memory: 2 + 17/32 bytes a value.
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t stride, int64_t rows, int64_t width, uint8_t* values,
+                                                           uint8_t* scales, int vector) {
+    const int lane = threadIdx.x % 32;
+    const int64_t row_bytes = (width + 31) / 32 * 16, pieces = scale_pieces(width), spans = pieces / 2;
+    const int64_t all = (rows + 127) / 128 * 128 * spans;
+    for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < all; job += (int64_t)gridDim.x * 8) {
+        const int64_t row = job / spans, span = job - row * spans;
+        const int64_t col = span * 256 + lane * 8;
+        float v[8];
+        const T* p = x + row * stride + col;
+        if (row < rows && col + 8 <= width && vector) {
+            Eight<T>::load(p, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = row < rows && col + i < width ? Eight<T>::one(p + i) : 0.0f;
+        }
+        // (as bits: a NaN counts as the largest)
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(~0u, top, 1));
+        top = max(top, __shfl_xor_sync(~0u, top, 2));
+        const uint32_t byte = scale_byte(__uint_as_float(top));
+        const float inverse = byte == 255u ? 0.0f : inverse_scale(byte);
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word |= four_bit_pair(v[2 * i] * inverse, v[2 * i + 1] * inverse) << (8 * i);
+        if (row < rows && col < (width + 31) / 32 * 32) *reinterpret_cast<uint32_t*>(values + row * row_bytes + col / 2) = word;
+        uint32_t four = byte << (8 * (lane / 4 % 4));
+        four |= __shfl_xor_sync(~0u, four, 4);
+        four |= __shfl_xor_sync(~0u, four, 8);
+        if (lane % 16 == 0) {
+            const int64_t piece = row / 128 * pieces + span * 2 + lane / 16;
+            *reinterpret_cast<uint32_t*>(scales + piece * 512 + row % 32 * 16 + row % 128 / 32 * 4) = four;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* values, const uint8_t* scales, int64_t rows, int64_t width, T* out,
+                                                             int64_t stride, int vector) {
+    const int lane = threadIdx.x % 32;
+    const int64_t row_bytes = (width + 31) / 32 * 16, pieces = scale_pieces(width), spans = pieces / 2;
+    for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < rows * spans; job += (int64_t)gridDim.x * 8) {
+        const int64_t row = job / spans, span = job - row * spans, col = span * 256 + lane * 8;
+        if (col >= width) continue;
+        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(values + row * row_bytes + col / 2));
+        const int64_t piece = row / 128 * pieces + span * 2 + lane / 16;
+        const float scale = scale_of(__ldg(scales + piece * 512 + row % 32 * 16 + row % 128 / 32 * 4 + lane / 4 % 4));
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = four_bit_value(word >> (4 * i) & 15u) * scale;
+        T* p = out + row * stride + col;
+        if (vector && col + 8 <= width) {
+            Eight<T>::store(p, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (col + i < width) Eight<T>::put(p + i, v[i]);
+        }
+    }
+}
+
+// y = act(A W^T + bias): tiles of 128 rows x 128 columns, steps of 256 columns of A and W (128 bytes a row), the scales of a step
+// copied from shared to tensor memory by the thread that issues the matrix instructions, in their order.
+struct Mx4Args {
+    CUtensorMap a, w;
+    const uint8_t *a_scales, *w_scales;
+    const void* bias;
+    void* out;
+    int64_t out_stride, rows;
+    int columns, steps, tiles_m, tiles_n;
+    int vector_out;
+};
+
+constexpr int kTile = 128;
+constexpr int kMxStages = 5;
+constexpr int kScaleBytes = 1024;  // two pieces
+constexpr int kMxStage = 2 * (kTile * 128 + kScaleBytes);
+constexpr int kMxShared = kMxStages * kMxStage + 1024;
+constexpr int kMxThreads = 320;
+constexpr int kScaleSets = 4;      // sets of scale columns in tensor memory, used in turn
+constexpr uint32_t kMxTmem = 512;  // two accumulators, scales behind them
+constexpr uint32_t kScaleColumn = 2 * kTile;
+
+template <int kOut, int kActivation>  // kOut 0 bf16, 1 fp16
+__global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_constant__ Mx4Args args) {
+    constexpr bool kBf16 = kOut == 0;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t bars[2 * kMxStages + 5];
+    __shared__ uint32_t tmem_at;
+    __shared__ volatile int given_up;
+    const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, bar0 = smem_addr(bars);
+    auto full = [&](int s) { return bar0 + 8 * s; };
+    auto empty = [&](int s) { return bar0 + 8 * (kMxStages + s); };
+    auto acc_full = [&](int s) { return bar0 + 8 * (2 * kMxStages + s); };
+    auto acc_empty = [&](int s) { return bar0 + 8 * (2 * kMxStages + 2 + s); };
+    const uint32_t last = bar0 + 8 * (2 * kMxStages + 4);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        given_up = 0;
+        for (int s = 0; s < kMxStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(acc_full(s), 1);
+            mbar_init(acc_empty(s), 256);
+        }
+        mbar_init(last, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) tmem_alloc(smem_addr(&tmem_at), kMxTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    const int tiles = args.tiles_m * args.tiles_n, steps = args.steps;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            tma_prefetch_map(&args.a);
+            tma_prefetch_map(&args.w);
+            int64_t issued = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                const int m = tile / args.tiles_n, n = tile % args.tiles_n;
+                for (int k = 0; k < steps; ++k, ++issued) {
+                    const int s = (int)(issued % kMxStages);
+                    if (issued >= kMxStages && !mbar_wait(empty(s), (uint32_t)(issued / kMxStages - 1) & 1, &given_up)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t a = ring + s * kMxStage;
+                    mbar_expect(full(s), kMxStage);
+                    tma_load_2d(a, &args.a, k * 128, m * kTile, full(s));
+                    tma_load_2d(a + kTile * 128, &args.w, k * 128, n * kTile, full(s));
+                    bulk_load(a + 2 * kTile * 128, args.a_scales + ((int64_t)m * steps + k) * kScaleBytes, kScaleBytes, full(s));
+                    bulk_load(a + 2 * kTile * 128 + kScaleBytes, args.w_scales + ((int64_t)n * steps + k) * kScaleBytes, kScaleBytes, full(s));
+                }
+            }
+            if (!ok)  // the copies in flight land before the block's memory goes
+                for (int64_t i = issued > kMxStages ? issued - kMxStages : 0; i < issued; ++i) {
+                    volatile int still = 0;
+                    mbar_wait(full((int)(i % kMxStages)), (uint32_t)(i / kMxStages) & 1, &still);
+                }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            int64_t used = 0;
+            int turn = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++turn) {
+                const int acc = turn & 1;
+                if (turn >= 2 && !mbar_wait(acc_empty(acc), (uint32_t)(turn / 2 - 1) & 1, &given_up)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                for (int k = 0; k < steps; ++k, ++used) {
+                    const int s = (int)(used % kMxStages);
+                    if (!mbar_wait(full(s), (uint32_t)(used / kMxStages) & 1, &given_up)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = ring + s * kMxStage, w = a + kTile * 128, sa = w + kTile * 128, sw = sa + kScaleBytes;
+                    const uint32_t ta = tmem + kScaleColumn + (uint32_t)(used % kScaleSets) * 16, tw = ta + 8;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        tmem_copy_scales(ta + 4 * i, scale_desc(sa + 512 * i));
+                        tmem_copy_scales(tw + 4 * i, scale_desc(sw + 512 * i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mma_mx4(tmem + acc * kTile, operand_desc(a + 32 * i, 1024, 16), operand_desc(w + 32 * i, 1024, 16), mx4_idesc(kTile, kTile, i & 1),
+                                ta + 4 * (i >> 1), tw + 4 * (i >> 1), k > 0 || i > 0);
+                    tc_commit(empty(s));
+                }
+                if (ok) tc_commit(acc_full(acc));
+            }
+            if (!ok) {  // the matrix instructions in flight end before their tensor memory is freed
+                volatile int still = 0;
+                tc_commit(last);
+                mbar_wait(last, 0, &still);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quadrant = warp % 4, half = warp / 4;
+        int turn = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
+            const int64_t row = (int64_t)(tile / args.tiles_n) * kTile + quadrant * 32 + lane;
+            const int n0 = tile % args.tiles_n * kTile, acc = turn & 1;
+            const bool ok = mbar_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
+            tc_fence_after();
+            for (int c = 32 * half; c < kTile; c += 64) {
+                const int col = n0 + c;
+                uint32_t g[32];
+                float v[32];
+                tmem_load_32(tmem + ((uint32_t)(quadrant * 32) << 16) + acc * kTile + c, g);
+                const float bias = args.bias && col + lane < args.columns ? widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias)[col + lane]) : 0.0f;
+                tmem_load_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float slope;
+                    const float y = activate<kActivation, false>(__uint_as_float(g[i]) + __shfl_sync(~0u, bias, i), slope);
+                    v[i] = ok ? y : __int_as_float(0x7FC00000);
+                }
+                if (row < args.rows) store_row<kBf16>(args.out, row * args.out_stride + col, v, args.columns - col, args.vector_out);
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty(acc));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_free(tmem, kMxTmem);
+    }
+}
+
+static SharedLimit g_limit[2][3];
+
+template <int kOut, int kActivation> static int launch_linear(const Mx4Args& args, cudaStream_t stream) {
+    auto* kernel = mx4_linear_kernel<kOut, kActivation>;
+    int rc = allow_shared(g_limit[kOut][kActivation], (const void*)kernel, kMxShared);
+    if (rc) return rc;
+    const int tiles = args.tiles_m * args.tiles_n;
+    kernel<<<tiles < sm_count() ? tiles : sm_count(), kMxThreads, kMxShared, stream>>>(args);
+    return check_cuda(cudaGetLastError(), "mx4_linear_kernel");
+}
+
+constexpr int64_t kMostRows = 1ll << 30;
+constexpr int32_t kMostWidth = 1 << 20;
+
+static int check_matrix(const char* name, int64_t rows, int32_t width) {
+    if (rows < 0 || rows > kMostRows || width < 1 || width > kMostWidth)
+        return set_error(P2B_ERR_ARG, "%s: %lld rows of %d are out of range", name, (long long)rows, width);
+    return P2B_OK;
+}
+static unsigned warp_grid(int64_t jobs) {
+    const int64_t blocks = blocks_of(jobs, 8), most = (int64_t)sm_count() * 8;
+    return (unsigned)(blocks < most ? blocks : most);
+}
+
+}  // namespace p2b
+
+using namespace p2b;
+
+extern "C" int64_t p2b_mx4_value_bytes(int64_t rows, int32_t width) { return rows < 0 || width < 1 ? -1 : rows * blocks_of(width, 32) * 16; }
+extern "C" int64_t p2b_mx4_scale_bytes(int64_t rows, int32_t width) {
+    return rows < 0 || width < 1 ? -1 : blocks_of(rows, 128) * scale_pieces(width) * 512;
+}
+
+extern "C" int p2b_mx4_quantise(const void* x, int64_t x_stride, int64_t rows, int32_t width, int32_t dtype, void* values, void* scales, void* stream) {
+    int rc = check_matrix("p2b_mx4_quantise", rows, width);
+    if (rc) return rc;
+    if (dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: unknown type %d (0 bf16, 1 fp16, 2 fp32)", dtype);
+    if (rows == 0) return P2B_OK;
+    if (!x || !values || !scales || x_stride < 0) return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: null array or negative stride");
+    if (((uintptr_t)values % 16) || ((uintptr_t)scales % 16) || (uintptr_t)x % (dtype == 2 ? 4 : 2))
+        return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: values and scales must lie on 16-byte boundaries, x on its element's");
+    const int vector = (uintptr_t)x % 16 == 0 && x_stride % (dtype == 2 ? 4 : 8) == 0;
+    const unsigned grid = warp_grid(blocks_of(rows, 128) * 128 * (scale_pieces(width) / 2));
+    cudaStream_t st = (cudaStream_t)stream;
+    uint8_t *v = (uint8_t*)values, *s = (uint8_t*)scales;
+    if (dtype == 0) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, x_stride, rows, (int64_t)width, v, s, vector);
+    if (dtype == 1) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __half*)x, x_stride, rows, (int64_t)width, v, s, vector);
+    if (dtype == 2) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const float*)x, x_stride, rows, (int64_t)width, v, s, vector);
+    return check_cuda(cudaGetLastError(), "mx4_quantise_kernel");
+}
+
+extern "C" int p2b_mx4_dequantise(const void* values, const void* scales, int64_t rows, int32_t width, int32_t dtype, void* out, int64_t out_stride,
+                                  void* stream) {
+    int rc = check_matrix("p2b_mx4_dequantise", rows, width);
+    if (rc) return rc;
+    if (dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "p2b_mx4_dequantise: unknown type %d (0 bf16, 1 fp16, 2 fp32)", dtype);
+    if (rows == 0) return P2B_OK;
+    if (!out || !values || !scales || (rows > 1 && out_stride < width))
+        return set_error(P2B_ERR_ARG, "p2b_mx4_dequantise: null array or rows that overlap");
+    if (((uintptr_t)values % 16) || ((uintptr_t)scales % 16) || (uintptr_t)out % (dtype == 2 ? 4 : 2))
+        return set_error(P2B_ERR_ARG, "p2b_mx4_dequantise: values and scales must lie on 16-byte boundaries, out on its element's");
+    const int vector = (uintptr_t)out % 16 == 0 && out_stride % (dtype == 2 ? 4 : 8) == 0;
+    const unsigned grid = warp_grid(rows * (scale_pieces(width) / 2));
+    cudaStream_t st = (cudaStream_t)stream;
+    const uint8_t *v = (const uint8_t*)values, *s = (const uint8_t*)scales;
+    if (dtype == 0) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, (int64_t)width, (__nv_bfloat16*)out, out_stride, vector);
+    if (dtype == 1) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, (int64_t)width, (__half*)out, out_stride, vector);
+    if (dtype == 2) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, (int64_t)width, (float*)out, out_stride, vector);
+    return check_cuda(cudaGetLastError(), "mx4_dequantise_kernel");
+}
+
+extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
+                              int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* stream) {
+    int rc = check_matrix("p2b_mx4_linear", rows, width);
+    if (!rc) rc = check_matrix("p2b_mx4_linear", columns, width);
+    if (rc) return rc;
+    if (columns < 1 || blocks_of(rows, kTile) * blocks_of(columns, kTile) > 0x7FFF0000ll)
+        return set_error(P2B_ERR_ARG, "p2b_mx4_linear: %lld x %d outputs are out of range", (long long)rows, columns);
+    if (dtype < 0 || dtype > 1) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: unknown type %d (0 bf16, 1 fp16)", dtype);
+    if (activation < 0 || activation > 2) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: unknown activation %d (0 gelu, 1 silu, 2 none)", activation);
+    if (rows == 0) return P2B_OK;
+    if (!a_values || !a_scales || !w_values || !w_scales || !out || (rows > 1 && out_stride < columns))
+        return set_error(P2B_ERR_ARG, "p2b_mx4_linear: null array or rows that overlap");
+    for (const void* p : {a_values, a_scales, w_values, w_scales})
+        if ((uintptr_t)p % 16) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: values and scales must lie on 16-byte boundaries");
+    if ((uintptr_t)out % 2 || (uintptr_t)bias % 2) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: out and bias must lie on 2-byte boundaries");
+    Mx4Args args{};
+    const int64_t row_bytes = blocks_of(width, 32) * 16;
+    rc = encode_rows(&args.a, a_values, 1, row_bytes, rows, row_bytes, kTile);
+    if (!rc) rc = encode_rows(&args.w, w_values, 1, row_bytes, columns, row_bytes, kTile);
+    if (rc) return rc;
+    args.a_scales = (const uint8_t*)a_scales, args.w_scales = (const uint8_t*)w_scales, args.bias = bias, args.out = out;
+    args.out_stride = out_stride, args.rows = rows, args.columns = columns;
+    args.steps = (int)blocks_of(width, 256), args.tiles_m = (int)blocks_of(rows, kTile), args.tiles_n = (int)blocks_of(columns, kTile);
+    args.vector_out = aligned16(out, out_stride);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == 0)
+        return activation == 0 ? launch_linear<0, 0>(args, st) : activation == 1 ? launch_linear<0, 1>(args, st) : launch_linear<0, 2>(args, st);
+    return activation == 0 ? launch_linear<1, 0>(args, st) : activation == 1 ? launch_linear<1, 1>(args, st) : launch_linear<1, 2>(args, st);
+}

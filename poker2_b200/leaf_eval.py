@@ -17,7 +17,7 @@ import threading
 import numpy as np
 import torch
 
-from . import _lib, chance
+from . import _lib, chance, gated, mx4
 
 NUM_HANDS = 1326
 
@@ -81,6 +81,71 @@ class ValueMLP(torch.nn.Module):
         return x
 
 
+class GatedBlock(torch.nn.Module):
+    """x + Wd (act(Wg n(x) + bg) * (Wu n(x) + bu)) + bd with n a layer norm: the gated hidden layer as a residual block."""
+
+    def __init__(self, width: int, hidden: int, *, activation: str = "gelu", generator: torch.Generator | None = None):
+        super().__init__()
+        self.norm = torch.nn.LayerNorm(width)
+        new = lambda rows, columns: torch.nn.Parameter(torch.randn(rows, columns, generator=generator) / columns ** 0.5)  # noqa: E731
+        self.gate_weight, self.up_weight = new(hidden, width), new(hidden, width)
+        self.gate_bias, self.up_bias = torch.nn.Parameter(torch.zeros(hidden)), torch.nn.Parameter(torch.zeros(hidden))
+        self.down = torch.nn.Linear(hidden, width)
+        with torch.no_grad():
+            self.down.weight.copy_(new(width, hidden))
+            self.down.bias.zero_()
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        h = gated.gated_linear(self.norm(x), self.gate_weight, self.up_weight, self.gate_bias, self.up_bias, activation=self.activation)
+        return x + self.down(h)
+
+
+class GatedValueMLP(ValueMLP):
+    """`ValueMLP` with `depth - 1` gated residual blocks of `hidden` units for its inner layers; same input and output rows, so
+    the leaf evaluators take it on the same paths.  Runs on the GPU, bf16 or fp16."""
+
+    def __init__(self, width: int = 1536, depth: int = 4, *, hidden: int | None = None, activation: str = "gelu", dtype=torch.bfloat16, seed: int = 0):
+        super().__init__(width, 1, dtype=dtype, seed=seed)
+        g = torch.Generator().manual_seed(seed + 1)
+        first, act, last = self.net
+        blocks = [GatedBlock(width, hidden or 2 * width // 3, activation=activation, generator=g) for _ in range(depth - 1)]
+        self.net = torch.nn.Sequential(first, act, *blocks, last).to(dtype)
+
+
+class Mx4Linear(torch.nn.Module):
+    """act(q(x) q(W)^T + b) with W quantised once, when the layer is made."""
+
+    def __init__(self, linear: torch.nn.Linear, activation: str = "none"):
+        super().__init__()
+        self.weight = mx4.quantise(linear.weight.detach())
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return mx4.linear(x, self.weight, self.bias, activation=self.activation)
+
+
+class Mx4ValueMLP(ValueMLP):
+    """A `ValueMLP` as it serves in 4 bits: every linear layer with its GELU becomes an `Mx4Linear`.  A copy of the weights as
+    they are now, on the GPU where they lie; for leaf values, not for training."""
+
+    def __init__(self, source: ValueMLP):
+        torch.nn.Module.__init__(self)
+        if type(source) is not ValueMLP or source.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("a bf16 or fp16 ValueMLP is quantised")
+        layers = list(source.net)
+        if any(type(m) not in (torch.nn.Linear, torch.nn.GELU) or type(m) is torch.nn.GELU and m.approximate != "none" for m in layers):
+            raise ValueError("linear layers and GELUs are quantised, nothing else")
+        if any(type(m) is torch.nn.GELU and (i == 0 or type(layers[i - 1]) is not torch.nn.Linear) for i, m in enumerate(layers)):
+            raise ValueError("a GELU follows a linear layer")
+        after = lambda i: "gelu" if i + 1 < len(layers) and type(layers[i + 1]) is torch.nn.GELU else "none"  # noqa: E731
+        self.net = torch.nn.Sequential(*(Mx4Linear(m, after(i)) for i, m in enumerate(layers) if type(m) is torch.nn.Linear))
+        self.dtype = source.dtype
+
+
+# networks whose input and output rows are those of `ValueMLP`
+_ROW_NETWORKS = (ValueMLP, GatedValueMLP, Mx4ValueMLP)
 _module_hooks = torch.nn.modules.module
 
 
@@ -172,7 +237,7 @@ class DirectLeafEvaluator:
         # one-hot, context, padding) are filled in once
         self._rows = None
         self._rows_lock = threading.RLock()
-        if type(model) is ValueMLP and model.dtype == torch.bfloat16 and self.boards.is_cuda and self.boards.shape[0] > 0:
+        if type(model) in _ROW_NETWORKS and model.dtype == torch.bfloat16 and self.boards.is_cuda and self.boards.shape[0] > 0:
             L, first = self.boards.shape[0], 2 * NUM_HANDS
             x = torch.zeros(L, ValueMLP.IN_PADDED, device=device, dtype=torch.bfloat16)
             card = torch.arange(52, device=device)
@@ -206,7 +271,7 @@ class DirectLeafEvaluator:
 
     def _direct(self) -> bool:
         """The model's layers may be called on rows kept here instead of the model itself."""
-        return self._rows is not None and type(self.model) is ValueMLP and _bare(self.model)
+        return self._rows is not None and type(self.model) in _ROW_NETWORKS and _bare(self.model)
 
     def __call__(self, leaf_beliefs: torch.Tensor) -> torch.Tensor:
         if not self._direct():

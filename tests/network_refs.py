@@ -80,3 +80,37 @@ def assert_within(got, value, bound, what=""):
     worst = off.max().item() if off.numel() else 0.0
     assert torch.isfinite(got.double()).all(), what
     assert worst <= 0.0, f"{what}: {int((off > 0).sum())} of {off.numel()} outside, worst by {worst:.3g} (bound {bound.flatten()[off.argmax()].item():.3g})"
+
+
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def mx4_values(x):
+    """What x [rows, width] reads back as, in 64 bits: every scale from 2^-127 up is tried against the block's largest magnitude,
+    every level against the value."""
+    x = x.double()
+    rows, width = x.shape
+    padded = torch.zeros(rows, (width + 31) // 32 * 32, dtype=torch.float64, device=x.device)
+    padded[:, :width] = x
+    blocks = padded.view(rows, -1, 32)
+    top = blocks.abs().amax(dim=-1)
+    scales = torch.exp2(torch.arange(-127, 127, dtype=torch.float64, device=x.device))
+    scale = scales[torch.searchsorted(6.0 * scales, torch.nan_to_num(top, nan=0.0, posinf=0.0))][..., None]
+    levels = torch.tensor(LEVELS, dtype=torch.float64, device=x.device)
+    distance = ((blocks.abs() / scale)[..., None] - levels).abs()
+    best = distance == distance.amin(dim=-1, keepdim=True)
+    even = torch.arange(8, device=x.device) % 2 == 0
+    best = torch.where((best.sum(dim=-1, keepdim=True) > 1), best & even, best)
+    value = levels[best.int().argmax(dim=-1)] * scale * torch.sign(blocks)
+    value = torch.where(torch.isfinite(top)[..., None], value, float("nan"))
+    return value.reshape(rows, -1)[:, :width]
+
+
+def mx4_linear(a, w, bias, name, dtype):
+    """(y, bound) of act(a w^T + bias) for matrices of 4-bit values in 64 bits."""
+    zero = torch.zeros(w.shape[0], dtype=torch.float64, device=w.device)
+    bias = zero if bias is None else bias.double()
+    z, mag = a @ w.T + bias, a.abs() @ w.abs().T + bias.abs()
+    y = activation(z, name)
+    err = 1.13 * summed(mag, a.shape[1]) + z.abs() * 2.0 ** -20
+    return y, err + rounded(y.abs() + err, dtype)

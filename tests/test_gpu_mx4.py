@@ -1,0 +1,136 @@
+"""4-bit rows and their products against a search over all scales and levels in 64 bits."""
+import pytest
+import torch
+
+import network_refs as refs
+from poker2_b200 import mx4
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _same(got, want):
+    want = want.to(got.dtype).double()  # (the largest finite magnitude rounds up to 4 * 2^126, which is an infinity in fp32)
+    assert torch.equal(torch.isnan(got.double()), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got.double()), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 32), (3, 31), (2, 33), (129, 255), (128, 256), (5, 257), (40, 1300), (300, 2720), (17, 1536)])
+def test_quantise_reads_back_as_its_definition(cuda_device, rows, width, dtype):
+    g = torch.Generator(device=cuda_device).manual_seed(rows + width)
+    x = torch.randn(rows, width, device=cuda_device, generator=g) * torch.exp2(torch.randint(-12, 6, (rows, 1), device=cuda_device, generator=g).float())
+    x = x.to(dtype)
+    q = mx4.quantise(x)
+    assert q.values.shape == (rows, (width + 31) // 32 * 16) and q.shape == (rows, width)
+    _same(q.dequantise(), refs.mx4_values(x))
+    for to in TYPES[:2]:
+        assert torch.equal(q.dequantise(to), refs.mx4_values(x).to(to))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_borders_and_special_values(cuda_device, dtype):
+    """Every border between two levels and its neighbours in the type, at several scales; largest magnitudes at and next to the
+    borders between scales; zeros, the smallest and largest numbers, infinities and NaN."""
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0], dtype=torch.float64)
+    info = torch.finfo(dtype)
+    near = [borders, borders * (1 + info.eps), borders * (1 - info.eps / 2), -borders]
+    row = torch.cat(near)  # 32 values, the largest above 6: their block's scale is one power higher
+    rows = [row, row.clamp(-6, 6), torch.zeros(32, dtype=torch.float64)]
+    for exponent in (-9, 0, 7):
+        for top in (1.5, 1.5 * (1 + info.eps), 1.5 * (1 - info.eps), 1.0, 2.0 * (1 - info.eps)):
+            block = torch.linspace(-1, 1, 32, dtype=torch.float64) * 2.0 ** exponent
+            block[7] = -top * 2.0 ** exponent
+            rows.append(block)
+    for value in (info.max, info.min, info.tiny, info.smallest_normal / 4, float("inf"), float("-inf"), float("nan")):
+        block = torch.ones(32, dtype=torch.float64) * 0.5
+        block[31] = value
+        rows.append(block)
+        rows.append(torch.full((32,), value, dtype=torch.float64))
+    x = torch.stack(rows).to(dtype).to(cuda_device)
+    _same(mx4.quantise(x).dequantise(), refs.mx4_values(x))
+    # the same blocks side by side: nothing of one reaches its neighbours
+    wide = x.reshape(1, -1)
+    _same(mx4.quantise(wide).dequantise().view(-1, 32), refs.mx4_values(x))
+
+
+def test_strides_and_shapes(cuda_device):
+    x = torch.randn(70, 96, device=cuda_device).bfloat16()
+    want = mx4.quantise(x)
+    area = torch.zeros(70 * 96 + 1, device=cuda_device, dtype=x.dtype)[1:].view(70, 96).copy_(x)
+    wide = torch.randn(70, 200, device=cuda_device).bfloat16()
+    wide[:, 3:99] = x
+    for other in (area, wide[:, 3:99], x.t().contiguous().t(), x.view(7, 10, 96)):
+        q = mx4.quantise(other)
+        assert torch.equal(q.values, want.values) and torch.equal(q.scales, want.scales)
+        assert q.dequantise(x.dtype).shape == other.shape
+    row = mx4.quantise(x[:1].expand(70, 96))
+    assert torch.equal(row.values, want.values[:1].expand(70, -1))
+    assert mx4.quantise(x[:0]).dequantise().shape == (0, 96)
+    assert mx4.quantise(x[0]).dequantise().shape == (96,)
+    # a quantised row is left as it is when quantised again
+    back = want.dequantise(torch.bfloat16)
+    assert torch.equal(mx4.quantise(back).dequantise(torch.bfloat16), back)
+
+
+@pytest.mark.parametrize("activation", ["none", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("rows,width,columns", [(1, 1536, 1536), (1, 32, 1), (2, 31, 7), (33, 256, 128), (128, 300, 129), (129, 64, 40),
+                                                (200, 2720, 333), (385, 1000, 257), (600, 513, 2652)])
+def test_linear(cuda_device, rows, width, columns, dtype, activation):
+    g = torch.Generator(device=cuda_device).manual_seed(rows + width + columns)
+    x = torch.randn(rows, width, device=cuda_device, generator=g).to(dtype)
+    w = (torch.randn(columns, width, device=cuda_device, generator=g) / width ** 0.5).to(dtype)
+    bias = torch.randn(columns, device=cuda_device, generator=g).to(dtype)
+    q = mx4.quantise(w)
+    want = refs.mx4_linear(refs.mx4_values(x), refs.mx4_values(w), bias, activation, dtype)
+    y = mx4.linear(x, q, bias, activation=activation)
+    assert y.dtype == dtype and y.shape == (rows, columns)
+    refs.assert_within(y, *want)
+    assert torch.equal(mx4.linear(mx4.quantise(x), q, bias, activation=activation, dtype=dtype), y)
+    if activation == "none":
+        refs.assert_within(mx4.linear(x, q), *refs.mx4_linear(refs.mx4_values(x), refs.mx4_values(w), None, activation, dtype))
+
+
+def test_linear_types_shapes_and_bad_rows(cuda_device):
+    x = torch.randn(140, 96, device=cuda_device)
+    q = mx4.quantise(torch.randn(50, 96, device=cuda_device))
+    y = mx4.linear(x, q)
+    assert y.dtype == torch.bfloat16
+    assert mx4.linear(x, q, dtype=torch.float16).dtype == torch.float16
+    assert torch.equal(mx4.linear(x.view(14, 10, 96), q), y.view(14, 10, 50))
+    assert mx4.linear(x[:0], q).shape == (0, 50) and torch.equal(mx4.linear(x[0], q), y[0])
+    x[5, 40], x[139, 0] = float("nan"), float("inf")
+    bad = mx4.linear(x, q)
+    others = torch.ones(140, dtype=torch.bool, device=cuda_device)
+    others[[5, 139]] = False
+    assert torch.equal(bad[others], y[others]) and torch.isnan(bad[[5, 139]]).all()
+    # wide ranges: scales from one end to the other, the sum stays exact where one term carries it
+    a = torch.zeros(3, 64, device=cuda_device)
+    w = torch.zeros(2, 64, device=cuda_device)
+    a[0, 0], a[1, 33], a[2, 40], w[0, 0], w[1, 33], w[1, 40] = 2.0 ** 100, 3.0 * 2.0 ** -100, -1.5, 2.0 ** -90, 2.0 ** 110, 0.5 * 2.0 ** 110
+    got = mx4.linear(a, mx4.quantise(w)).double()
+    assert torch.equal(got, (refs.mx4_values(a) @ refs.mx4_values(w).T).bfloat16().double())
+
+
+def test_streams_and_capture(cuda_device):
+    x = torch.randn(300, 512, device=cuda_device).bfloat16()
+    q = mx4.quantise(torch.randn(160, 512, device=cuda_device))
+    y = mx4.linear(x, q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        aside = mx4.linear(x, q)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(aside, y)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append((mx4.linear(x, q, activation="silu"), mx4.quantise(x).dequantise(x.dtype)))
+        graphs.append(graph)
+    x.copy_(torch.randn(300, 512, device=cuda_device))
+    graphs[0].replay()
+    graphs[1].replay()
+    for a, b in outs:
+        assert torch.equal(a, mx4.linear(x, q, activation="silu")) and torch.equal(b, mx4.quantise(x).dequantise(x.dtype))

@@ -88,3 +88,64 @@ def test_gated_linear_refuses():
         args.update(change)
         with pytest.raises(ValueError):
             gated._check(*args.values())
+
+
+def _refused(handle, name, **change):
+    area, p = _area()
+    calls = {
+        "p2b_mx4_quantise": dict(x=p, stride=64, rows=4, width=64, dtype=0, values=p, scales=p, stream=None),
+        "p2b_mx4_dequantise": dict(values=p, scales=p, rows=4, width=64, dtype=0, out=p, stride=64, stream=None),
+        "p2b_mx4_linear": dict(a=p, sa=p, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
+    }
+    args = calls[name]
+    args.update({k: p + v[0] if isinstance(v, tuple) else v for k, v in change.items()})
+    return getattr(handle, name)(*args.values()) == -1 and name.encode() in handle.p2b_last_error()
+
+
+MATRIX = [dict(rows=-1), dict(rows=1 << 40), dict(width=0), dict(width=-5), dict(width=1 << 24), dict(dtype=3), dict(dtype=-1)]
+
+
+@pytest.mark.parametrize("change", MATRIX + [dict(x=None), dict(values=None), dict(scales=None), dict(stride=-1), dict(values=(8,)), dict(scales=(4,)), dict(x=(1,))])
+def test_mx4_quantise_refuses(handle, change):
+    assert _refused(handle, "p2b_mx4_quantise", **change)
+
+
+@pytest.mark.parametrize("change", MATRIX + [dict(out=None), dict(values=None), dict(scales=None), dict(stride=63), dict(values=(8,)), dict(scales=(4,)), dict(out=(1,))])
+def test_mx4_dequantise_refuses(handle, change):
+    assert _refused(handle, "p2b_mx4_dequantise", **change)
+
+
+@pytest.mark.parametrize("change", MATRIX + [dict(dtype=2), dict(act=3), dict(act=-1), dict(columns=0), dict(columns=1 << 30), dict(a=None), dict(sa=None), dict(w=None),
+                                             dict(sw=None), dict(out=None), dict(stride=7), dict(a=(8,)), dict(sa=(1,)), dict(w=(4,)), dict(sw=(8,)), dict(out=(1,)),
+                                             dict(bias=(1,)), dict(rows=1 << 30, columns=1 << 20)])
+def test_mx4_linear_refuses(handle, change):
+    assert _refused(handle, "p2b_mx4_linear", **change)
+
+
+def test_mx4_sizes(handle):
+    assert handle.p2b_mx4_value_bytes(3, 33) == 96 and handle.p2b_mx4_scale_bytes(129, 257) == 2 * 4 * 512
+    assert handle.p2b_mx4_value_bytes(-1, 33) == -1 and handle.p2b_mx4_scale_bytes(1, 0) == -1
+    assert handle.p2b_mx4_quantise(None, 0, 0, 64, 0, None, None, None) == 0
+    assert handle.p2b_mx4_linear(None, None, 0, None, None, 8, 64, None, 0, 0, None, 8, None) == 0
+
+
+def test_mx4_python_refuses():
+    from poker2_b200 import mx4
+
+    with pytest.raises(ValueError, match="CUDA"):
+        mx4.quantise(torch.zeros(2, 32))
+    for bad in (_there(2, 0), _there(2, 32, dtype=torch.float64), torch.zeros((), dtype=torch.bfloat16).as_subclass(_Elsewhere)):
+        with pytest.raises(ValueError):
+            mx4.quantise(bad)
+    w = mx4.Mx4(_there(4, 16, dtype=torch.uint8), _there(1024, dtype=torch.uint8), (4, 32))
+    x = mx4.Mx4(_there(2, 16, dtype=torch.uint8), _there(1024, dtype=torch.uint8), (2, 32))
+    with pytest.raises(ValueError):
+        w.dequantise(torch.float64)
+    for change in (dict(weight=_there(4, 32)), dict(activation="relu"), dict(dtype=torch.float32), dict(bias=_there(3)), dict(bias=_there(4, dtype=torch.float16)),
+                   dict(x=mx4.Mx4(x.values, x.scales, (2, 31))), dict(weight=mx4.Mx4(w.values, w.scales, (2, 2, 32))), dict(weight=mx4.Mx4(w.values, w.scales, (0, 32)))):
+        args = dict(x=x, weight=w, bias=None, activation="none", dtype=None)
+        args.update(change)
+        with pytest.raises(ValueError):
+            mx4.linear(args["x"], args["weight"], args["bias"], activation=args["activation"], dtype=args["dtype"])
+    with pytest.raises(RuntimeError, match="gradient"):
+        mx4.linear(_there(2, 32).requires_grad_(True), w)
