@@ -509,6 +509,22 @@ int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, con
                    int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out,
                    int64_t out_stride, void* stream);
 
+/* Clipped policy loss with a KL term over the hands of a batch of states, and its gradient.  Per state and hand, over the legal
+ * actions a, p = softmax(logits) and q = old_policy:
+ *   l = -sum_a min(p_a A_a, clip(p_a, (1-clip) q_a, (1+clip) q_a) A_a) + kl sum_a t_a (log t_a - log p_a)
+ * loss = sum(w l) / sum(w) over the hands of states that have a legal action; 0 where sum(w) is 0.
+ *  logits, grad [states,hands,actions] of dtype 0 bf16, 1 fp16, 2 fp32 (grad may be NULL); old_policy, advantages (both NULL: the
+ *  KL term alone), target [states,hands,actions] fp32; legal [states,actions] bytes; weights [states,hands] fp32, none
+ *  negative (NULL: 1).  All packed.  1 to 16 actions, 0 <= clip < 1, kl >= 0.
+ * Nothing is read into the result from illegal actions, hands of weight 0 and hands whose legal logits are all -inf; their
+ * gradients are 0.  loss: one fp32, summed in 64 bits in a fixed order.  scratch: p2b_policy_loss_scratch_bytes(states, hands),
+ * 8-byte aligned.  p2b_policy_loss_scale: out = grad * *factor (device), n values. */
+int64_t p2b_policy_loss_scratch_bytes(int64_t states, int32_t hands);
+int p2b_policy_loss(const void* logits, const float* old_policy, const float* advantages, const float* target,
+                    const uint8_t* legal, const float* weights, int64_t states, int32_t hands, int32_t actions, int32_t dtype,
+                    double clip, float kl, float* loss, void* grad, void* scratch, int64_t scratch_bytes, void* stream);
+int p2b_policy_loss_scale(const void* grad, const float* factor, int64_t n, int32_t dtype, void* out, void* stream);
+
 /* ---- self-test (no counterpart in the reference) ------------------------------------------
  * The solver's divisions share divisors and run through a short correctly rounded sequence
  * (csrc/exactdiv.cuh).  p2b_selftest_division compares it with the compiler's IEEE division

@@ -10,7 +10,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libpoker2_b200.so")
 SOURCES = ["common.cu", "rank7.cu", "showdown.cu", "cfr.cu", "cfr_wide.cu", "cfr_iter.cu", "cfr_split.cu", "stepops.cu", "chance.cu", "treebuild.cu", "selftest.cu", "api.cu",
-           "tensor.cu", "gated.cu", "mx4.cu"]
+           "tensor.cu", "gated.cu", "mx4.cu", "policy_loss.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -21,7 +21,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
 ]
 # The network operators have no upstream bits to match: their sums contract.
-CONTRACTED = {"gated.cu", "mx4.cu"}
+CONTRACTED = {"gated.cu", "mx4.cu", "policy_loss.cu"}
 
 
 def nvcc_path() -> str:

@@ -1,0 +1,120 @@
+"""The loss that trains a policy head on what a search returned, with its gradient: a clipped policy term and the KL divergence to a
+target policy, over all 1326 hands (or any number) of a batch of states and their legal actions.
+
+Per state and hand, with p = softmax(logits) over the legal actions, q the old policy and t the target,
+
+    l = -sum_a min(p_a A_a, clip(p_a, (1-clip) q_a, (1+clip) q_a) A_a) + kl * sum_a t_a (log t_a - log p_a)
+
+is the clipped surrogate of the ratio p/q summed over the actions (a search gives every action's advantage, none is sampled)
+plus the divergence from the target.  The loss is the mean over the hands by their weights.  `RebelBatchLike.policy_loss` calls it
+on a minibatch of the replay ring.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+NUM_HANDS = _lib.NUM_HANDS
+MAX_ACTIONS = 16
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def clipped_policy_loss(logits: torch.Tensor, old_policy: torch.Tensor | None, advantages: torch.Tensor | None, target: torch.Tensor,
+                        legal: torch.Tensor, weights: torch.Tensor | None = None, *, clip: float = 0.2, kl: float = 1.0) -> torch.Tensor:
+    """logits [states, hands, actions] bf16, fp16 or fp32; old_policy and advantages (both None: the KL term alone) and target of that
+    shape in fp32; legal [states, actions] bool; weights [states, hands] fp32, none negative (None: 1) -> the loss, an fp32 scalar
+    that differentiates to the logits.
+
+    Illegal actions, hands of weight 0, states without a legal action and hands whose legal logits are all -inf add nothing
+    and get a zero gradient, whatever their entries hold.  With gradients wanted the gradient is computed in the same pass (rounded
+    to the logits' type; a factor that the backward pass brings is rounded in once more) and the call is refused while a CUDA graph is
+    being captured: use `clipped_policy_loss_and_grad` there."""
+    _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
+    if not (torch.is_grad_enabled() and logits.requires_grad):
+        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, False)[0]
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("clipped_policy_loss cannot be captured into a CUDA graph through autograd; call clipped_policy_loss_and_grad, which can.")
+    return _Loss.apply(logits, old_policy, advantages, target, legal, weights, clip, kl)
+
+
+def clipped_policy_loss_and_grad(logits: torch.Tensor, old_policy: torch.Tensor | None, advantages: torch.Tensor | None, target: torch.Tensor,
+                                 legal: torch.Tensor, weights: torch.Tensor | None = None, *, clip: float = 0.2, kl: float = 1.0):
+    """(loss, its gradient to the logits in their type) of `clipped_policy_loss`, in one pass and without autograd: hand the gradient
+    to `logits.backward(grad)`, or scale it first."""
+    _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
+    return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, True)
+
+
+def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tensor) -> torch.Tensor:
+    """[n, 1326] fp32: the chance that the player to act holds a hand, times the chance that the other player's range leaves it
+    open; 0 for hands with a card on the board.  beliefs [n, 2*1326], to_act [n], board [n, L] with -1 for cards not dealt."""
+    from .fused_cfr import unblocked_mass_triton
+
+    _lib.require_cuda(beliefs, "hand_weights")
+    n = beliefs.shape[0]
+    if tuple(beliefs.shape) != (n, 2 * NUM_HANDS) or tuple(to_act.shape) != (n,) or board.dim() != 2 or board.shape[0] != n:
+        raise ValueError("beliefs [n, 2652], to_act [n] and board [n, L] are wanted")
+    device = beliefs.device
+    ranges = beliefs.to(torch.float32).view(n, 2, NUM_HANDS)
+    actor, rows = to_act.to(device=device, dtype=torch.int64), torch.arange(n, device=device)
+    held = ranges[rows, actor] * unblocked_mass_triton(ranges[rows, 1 - actor].contiguous()).clamp(min=0.0)
+    c1, c2 = torch.triu_indices(52, 52, 1, device=device)
+    board = board.to(device=device, dtype=torch.int64)
+    dealt = torch.zeros(n, 53, dtype=torch.bool, device=device).scatter_(1, torch.where(board >= 0, board, 52), True)
+    return torch.where(dealt[:, c1] | dealt[:, c2], 0.0, held)
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, old_policy, advantages, target, legal, weights, clip, kl):
+        loss, grad = _run(logits, old_policy, advantages, target, legal, weights, clip, kl, True)
+        ctx.save_for_backward(grad)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, factor):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the backward pass of clipped_policy_loss cannot be captured into a CUDA graph; call clipped_policy_loss_and_grad, which can.")
+        grad, = ctx.saved_tensors
+        out = torch.empty_like(grad)
+        p = _lib.ptr
+        with _lib.on(grad.device):
+            _lib.call("p2b_policy_loss_scale", p(grad), p(factor.contiguous()), grad.numel(), _TYPES[grad.dtype], p(out), _lib.stream_ptr(grad.device))
+        return out, None, None, None, None, None, None, None
+
+
+def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, with_grad):
+    states, hands, actions = logits.shape
+    device = logits.device
+    packed = lambda t: None if t is None else t.detach().contiguous()  # noqa: E731
+    logits, old_policy, advantages, target, legal, weights = map(packed, (logits, old_policy, advantages, target, legal, weights))
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if with_grad else None
+    p = _lib.ptr
+    with _lib.on(device):
+        size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
+        scratch = torch.empty(max(size, 8), dtype=torch.uint8, device=device)
+        _lib.call("p2b_policy_loss", p(logits), p(old_policy), p(advantages), p(target), p(legal), p(weights), states, hands, actions,
+                  _TYPES[logits.dtype], float(clip), float(kl), p(loss), p(grad), p(scratch), scratch.numel(), _lib.stream_ptr(device))
+    return loss, grad
+
+
+def _check(logits, old_policy, advantages, target, legal, weights, clip, kl) -> None:
+    _lib.require_cuda(logits, "clipped_policy_loss")
+    if logits.dtype not in _TYPES or logits.dim() != 3 or logits.shape[1] < 1 or not 1 <= logits.shape[2] <= MAX_ACTIONS:
+        raise ValueError(f"logits [states, hands, actions] in bf16, fp16 or fp32 with 1 to {MAX_ACTIONS} actions are wanted")
+    if (old_policy is None) != (advantages is None):
+        raise ValueError("the old policy and the advantages come together")
+    for t in (old_policy, advantages, target):
+        if t is not None and (t.shape != logits.shape or t.dtype != torch.float32 or t.device != logits.device):
+            raise ValueError("old policy, advantages and target have the logits' shape and device, in fp32")
+    if tuple(legal.shape) != (logits.shape[0], logits.shape[2]) or legal.dtype != torch.bool or legal.device != logits.device:
+        raise ValueError("legal [states, actions] bool on the logits' device is wanted")
+    if weights is not None and (weights.shape != logits.shape[:2] or weights.dtype != torch.float32 or weights.device != logits.device):
+        raise ValueError("weights [states, hands] fp32 on the logits' device are wanted")
+    if any(t is not None and t.requires_grad for t in (old_policy, advantages, target, weights)) and torch.is_grad_enabled():
+        raise RuntimeError("the loss differentiates to the logits alone: detach the policies, advantages and weights")
+    if not 0.0 <= clip < 1.0 or not 0.0 <= kl < float("inf"):
+        raise ValueError("clip lies in [0, 1), kl is not negative")

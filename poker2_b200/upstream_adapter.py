@@ -149,6 +149,18 @@ class RebelBatchLike:
         return RebelBatchLike(self.features.to(device), self.legal_masks.to(device), mv(self.policy_targets),
                               mv(self.value_targets), {k: v.to(device) for k, v in self.statistics.items()})
 
+    def policy_loss(self, logits: torch.Tensor, old_policy: torch.Tensor | None = None, advantages: torch.Tensor | None = None, *,
+                    clip: float = 0.2, kl: float = 1.0) -> torch.Tensor:
+        """Loss of a policy head's logits [n,1326,A] on this batch: its policy targets as the KL term's, its legal masks, every hand by the
+        chance that it is held (`policy_loss.hand_weights`); with an old policy and advantages the clipped term too."""
+        from . import policy_loss
+
+        if self.policy_targets is None:
+            raise ValueError("the batch has no policy targets")
+        f = self.features
+        return policy_loss.clipped_policy_loss(logits, old_policy, advantages, self.policy_targets.to(torch.float32), self.legal_masks,
+                                               policy_loss.hand_weights(f.beliefs, f.to_act, f.board), clip=clip, kl=kl)
+
     @classmethod
     def cat(cls, batches) -> "RebelBatchLike":
         if not batches or any(b is None for b in batches):

@@ -114,3 +114,50 @@ def mx4_linear(a, w, bias, name, dtype):
     y = activation(z, name)
     err = 1.13 * summed(mag, a.shape[1]) + z.abs() * 2.0 ** -20
     return y, err + rounded(y.abs() + err, dtype)
+
+
+def policy_loss(logits, old, adv, target, legal, weights, clip, kl, dtype):
+    """(loss, its bound, gradient, its bound) in 64 bits, from the definition."""
+    z = logits.double()
+    N, H, A = z.shape
+    legal = legal[:, None, :].expand(N, H, A)
+    w = torch.ones(N, H, dtype=torch.float64, device=z.device) if weights is None else weights.double()
+    w = torch.where(legal.any(-1), w, 0.0)
+    mass = w.sum()
+    z = torch.where(legal, z, -math.inf)
+    top = z.amax(-1, keepdim=True)
+    counts = (w != 0) & (top[..., 0] != -math.inf)
+    legal = legal & counts[..., None]
+    d = torch.where(legal, z - torch.where(counts[..., None], top, 0.0), 0.0)
+    e = torch.where(legal, torch.exp(d), 0.0)
+    total = torch.where(counts, e.sum(-1), 1.0)[..., None]
+    p = e / total
+    t = torch.where(legal, target.double(), 0.0)
+    logp = d - torch.log(total)
+    kl_terms = torch.where(t > 0, t * (torch.log(torch.where(t > 0, t, 1.0)) - torch.where(t > 0, logp, 0.0)), 0.0)
+    if old is None:
+        surr, g = torch.zeros_like(p), torch.zeros_like(p)
+    else:
+        q, a = torch.where(legal, old.double(), 0.0), torch.where(legal, adv.double(), 0.0)
+        low, high = (1.0 - clip) * q, (1.0 + clip) * q
+        free = torch.where(a > 0, p <= high, p >= low)
+        surr = torch.minimum(p * a, torch.minimum(torch.maximum(p, low), high) * a)
+        g = torch.where(free, a, 0.0)
+    per_hand = torch.where(counts, kl * kl_terms.sum(-1) - surr.sum(-1), 0.0)
+    some = mass > 0
+    loss = (w * per_hand).sum() / mass if some else torch.zeros_like(mass)
+    scale = (w / mass if some else torch.zeros_like(w))[..., None]
+    pull, targets = (g * p).sum(-1, keepdim=True), t.sum(-1, keepdim=True)
+    grad = torch.where(legal, scale * (kl * (p * targets - t) - p * (g - pull)), 0.0)
+    # fp32 steps u: z - top is off by u |d|, the exponential by 4 u, the sum by A u and its terms' own |d|; log by 4 u of its
+    # value and u of the total's error
+    u = 2.0 ** -24
+    finite = torch.where(torch.isfinite(d), d, 0.0).abs()
+    reach = finite.clamp(max=104.0).amax(-1, keepdim=True)
+    e_p = u * (finite + reach + A + 16)
+    size = kl * (p * targets + t) + p * (g.abs() + (g.abs() * p).sum(-1, keepdim=True))
+    err = scale * size * (3 * e_p + (A + 12) * u)
+    hand_size = kl * torch.where(t > 0, t * (torch.log(torch.where(t > 0, t, 1.0)).abs() + finite + torch.log(total) + 1), 0.0).sum(-1) + surr.abs().sum(-1)
+    hand_err = hand_size * (3 * e_p.amax(-1) + (A + 12) * u)
+    loss_err = (w * hand_err).sum() / mass if some else torch.zeros_like(mass)
+    return loss, loss_err + loss.abs() * 2 * u + 1e-300, grad, err + rounded(grad.abs() + err, dtype)

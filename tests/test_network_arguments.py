@@ -149,3 +149,46 @@ def test_mx4_python_refuses():
             mx4.linear(args["x"], args["weight"], args["bias"], activation=args["activation"], dtype=args["dtype"])
     with pytest.raises(RuntimeError, match="gradient"):
         mx4.linear(_there(2, 32).requires_grad_(True), w)
+
+
+def _loss(p, **change):
+    a = dict(logits=p, old=p, adv=p, target=p, legal=p, weights=p, states=2, hands=3, actions=4, dtype=0, clip=0.2, kl=1.0, loss=p, grad=p, scratch=p, size=1 << 20)
+    a.update({k: p + v[0] if isinstance(v, tuple) else v for k, v in change.items()})
+    return [*a.values(), None]
+
+
+@pytest.mark.parametrize("change", [dict(states=-1), dict(states=1 << 40), dict(hands=0), dict(actions=0), dict(actions=17), dict(dtype=3), dict(clip=1.0), dict(clip=-0.1),
+                                    dict(clip=float("nan")), dict(kl=-1.0), dict(kl=float("inf")), dict(kl=float("nan")), dict(loss=None), dict(scratch=None),
+                                    dict(size=8), dict(scratch=(4,)), dict(old=None), dict(adv=None), dict(logits=None), dict(target=None), dict(legal=None),
+                                    dict(logits=(1,)), dict(old=(2,)), dict(target=(1,)), dict(weights=(2,)), dict(grad=(1,)), dict(loss=(2,)),
+                                    dict(dtype=2, logits=(2,))])
+def test_policy_loss_refuses(handle, change):
+    area, p = _area()
+    assert handle.p2b_policy_loss(*_loss(p, **change)) == -1 and b"p2b_policy_loss" in handle.p2b_last_error()
+
+
+def test_policy_loss_scale_refuses(handle):
+    area, p = _area()
+    for args in ((None, p, 4, 0, p), (p, None, 4, 0, p), (p, p, 4, 0, None), (p, p, -1, 0, p), (p, p, 4, 3, p)):
+        assert handle.p2b_policy_loss_scale(*args, None) == -1
+    assert handle.p2b_policy_loss_scale(None, None, 0, 0, None, None) == 0
+    assert handle.p2b_policy_loss_scratch_bytes(-1, 4) == -1 and handle.p2b_policy_loss_scratch_bytes(1, 0) == -1
+
+
+def test_policy_loss_python_refuses():
+    from poker2_b200 import policy_loss as pl
+
+    with pytest.raises(ValueError, match="CUDA"):
+        pl.clipped_policy_loss(torch.zeros(2, 3, 4), None, None, torch.zeros(2, 3, 4), torch.ones(2, 4, dtype=torch.bool))
+    f32 = torch.float32
+    good = dict(logits=_there(2, 3, 4), old_policy=_there(2, 3, 4, dtype=f32), advantages=_there(2, 3, 4, dtype=f32), target=_there(2, 3, 4, dtype=f32),
+                legal=_there(2, 4, dtype=torch.bool), weights=_there(2, 3, dtype=f32), clip=0.2, kl=1.0)
+    pl._check(*good.values())
+    for change in (dict(logits=_there(2, 12)), dict(logits=_there(2, 3, 17)), dict(logits=_there(2, 3, 4, dtype=torch.float64)), dict(old_policy=None),
+                   dict(advantages=None), dict(target=_there(2, 3, 4)), dict(target=_there(2, 3, 5, dtype=f32)), dict(target=torch.zeros(2, 3, 4)),
+                   dict(legal=_there(2, 3, 4, dtype=torch.bool)), dict(legal=_there(2, 4, dtype=torch.uint8)), dict(weights=_there(2, 4, dtype=f32)),
+                   dict(weights=_there(2, 3)), dict(clip=1.0), dict(clip=-0.5), dict(kl=-1.0), dict(kl=float("nan"))):
+        with pytest.raises(ValueError):
+            pl._check(*{**good, **change}.values())
+    with pytest.raises(RuntimeError, match="detach"):
+        pl._check(*{**good, "target": _there(2, 3, 4, dtype=f32).requires_grad_(True)}.values())
