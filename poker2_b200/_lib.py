@@ -179,18 +179,31 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} requires a CUDA tensor.")
 
 
+
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def call_on(device: int, name: str, *args) -> None:
+    """`call` with the device's current stream behind the arguments, made where that device is the current one."""
+    if device == _get_device():
+        call(name, *args, _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
 def plain_rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix whose rows are packed and do not overlap: `t` itself where it is one."""
-    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) or t.shape[1] == 1 and t.stride(0) >= 1 else t.contiguous()
+    rows, columns = t.shape
+    apart, step = t.stride()
+    return t if (step == 1 or columns == 1) and (apart >= columns or rows <= 1) else t.contiguous()
 
 
 def wide_rows(t: torch.Tensor) -> torch.Tensor:
-    """The same with every row on a 16-byte boundary, as the tensor-memory kernels load them: copied where it is not."""
-    per = 16 // t.element_size()
+    """The same with every row of 16-bit elements on a 16-byte boundary, as the tensor-memory kernels load them: copied where it
+    is not."""
     rows, columns = t.shape
-    if t.data_ptr() % 16 == 0 and (columns == 1 or t.stride(1) == 1) and t.stride(0) >= columns and t.stride(0) % per == 0:
+    apart, step = t.stride()
+    if (step == 1 or columns == 1) and (apart >= columns and apart % 8 == 0 or rows <= 1) and t.data_ptr() % 16 == 0:
         return t
-    if rows <= 1 and t.data_ptr() % 16 == 0 and (columns == 1 or t.stride(1) == 1) and columns % per == 0:
-        return t
-    out = torch.empty(rows, (columns + per - 1) // per * per, dtype=t.dtype, device=t.device)[:, :columns]
-    return out.copy_(t)
+    return t.new_empty((rows, (columns + 7) // 8 * 8))[:, :columns].copy_(t)

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -40,6 +41,20 @@ def needs_build() -> bool:
     return any(os.path.getmtime(d) > lib_m for d in deps)
 
 
+def _sources_of(path: str, seen: set | None = None) -> set:
+    """A source file and what it includes by a quoted name, itself or through others."""
+    seen = set() if seen is None else seen
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', f.read(), flags=re.M):
+                for place in (os.path.dirname(path), os.path.join(PKG_DIR, "..", "include")):
+                    if os.path.exists(os.path.join(place, name)):
+                        _sources_of(os.path.normpath(os.path.join(place, name)), seen)
+                        break
+    return seen
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB_PATH
@@ -47,20 +62,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
     build_dir = os.path.join(PKG_DIR, "build")
     os.makedirs(build_dir, exist_ok=True)
     nvcc = nvcc_path()
-    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    headers.append(os.path.join(PKG_DIR, "..", "include", "poker2_b200.h"))
-    newest_header = max(os.path.getmtime(h) for h in headers)
     procs = []
     for src in SOURCES:
         obj = os.path.join(build_dir, src.replace(".cu", ".o"))
         objs.append(obj)
         src_path = os.path.join(CSRC, src)
-        # an object is reused when it is newer than its source (cfr_wide.cu is cfr.cu compiled a second time)
-        # and than every header
-        newest_source = os.path.getmtime(src_path)
-        if src == "cfr_wide.cu":
-            newest_source = max(newest_source, os.path.getmtime(os.path.join(CSRC, "cfr.cu")))
-        if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(newest_source, newest_header):
+        # an object is reused when it is newer than its source and than every file that includes
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(map(os.path.getmtime, _sources_of(src_path))):
             continue
         flags = [f for f in NVCC_FLAGS if f != "-fmad=false" or src not in CONTRACTED]
         cmd = [nvcc, *flags, "-c", src_path, "-o", obj]

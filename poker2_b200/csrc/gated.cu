@@ -12,247 +12,400 @@ namespace p2b {
 
 using namespace tc;
 
-enum GatedMode { kForward = 0, kGradHidden = 1, kGradInput = 2, kGradWeight = 3 };
+enum GatedMode { kForward = 0, kGradHidden = 1, kGradients = 2 };
 
 struct GatedArgs {
-    CUtensorMap a, b0, b1;
+    CUtensorMap a, b0, b1;   // kForward, kGradHidden: x, Wg, Wu; kGradients: dgate | dup by rows, Wg, Wu
+    CUtensorMap at, bt;      // kGradients: dgate | dup and x with the reduction along their rows
     const void *bias_gate, *bias_up, *grad_h;
-    void *out0, *out1;
+    void *out, *dwg, *dwu;   // h, dgate | dup or dx; the gradients of the weights
+    float* sums;             // kGradHidden: column sums of dgate | dup over 32 rows each (NULL: not wanted)
     int64_t grad_stride, out_stride;
-    int64_t rows;         // rows of x
-    int width, hidden;    // columns of x, rows of either weight
-    int hidden_padded;    // columns of dgate (and dup) in work space: a multiple of 128
-    int k_blocks;         // steps of 64 along the reduction (kGradInput: of each half)
-    int tiles_m, tiles_n;
-    int activation;
-    int vector_in, vector_out;  // 16-byte loads of grad_h, stores of the outputs
+    int64_t rows;            // rows of x
+    int width, hidden;       // columns of x, rows of either weight
+    int hidden_padded;       // columns of dgate (and dup) in work space: a multiple of 128
+    int steps, steps_w;      // steps of 64 along the reduction of a tile; kGradients: of dx, of the weights
+    int tiles_n, tiles;      // tiles of out
+    int tiles_w_n, tiles_w;  // kGradients: tiles of the weights' gradients, and how many of the
+    int ahead;               //   other tiles a pair without a last one of those takes in its place
+    int vector_in, vector_out, vector_w;  // 16-byte loads of grad_h, stores of the outputs
 };
 
-constexpr int kRows = 128;     // rows of a tile
-constexpr int kStep = 64;      // reduction columns of a stage: 128 bytes
+constexpr int kRows = 128;   // rows of a block's tile
+constexpr int kStep = 64;    // reduction columns of a stage: 128 bytes
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 
-template <int kCols> __host__ __device__ constexpr int stages() { return kCols == 256 ? 4 : 6; }
-template <int kCols> __host__ __device__ constexpr int stage_bytes() { return kRows * 128 + kCols * 128; }
-template <int kCols> __host__ __device__ constexpr int shared_bytes() { return stages<kCols>() * stage_bytes<kCols>() + 1024; }
+// Sum over the warp's lanes of each of 32 values: lane l ends with the sum of value l.  Half of the values change places in
+// every round, 31 exchanges in all.
+__device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float give = upper ? v[i] : v[i + o], keep = upper ? v[i + o] : v[i];
+            v[i] = keep + __shfl_xor_sync(~0u, give, o);
+        }
+    }
+    return v[0];
+}
 
-template <int kMode, int kCols, bool kBf16, int kActivation>
-__global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ GatedArgs args) {
-    constexpr int kStages = stages<kCols>();
-    constexpr bool kPaired = kMode == kForward || kMode == kGradHidden;  // gate and up columns in one tile
-    constexpr int kTileCols = kPaired ? kCols / 2 : kCols;               // output columns of a tile
-    constexpr uint32_t kTmem = 2 * kCols < 32 ? 32 : 2 * kCols;
+// 32 hidden columns of a warp's 32 rows, from the accumulators of gate and up to h or to dgate and dup.
+template <int kMode, bool kBf16, int kActivation>
+__device__ __forceinline__ void finish_hidden(const GatedArgs& args, uint32_t gate_at, uint32_t up_at, int64_t row, int col, bool ok, int lane) {
+    uint32_t g[32], u[32];
+    tmem_load_32(gate_at, g);
+    tmem_load_32(up_at, u);
+    float bias_g = 0.0f, bias_u = 0.0f;
+    if (col + lane < args.hidden) {
+        if (args.bias_gate) bias_g = widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias_gate)[col + lane]);
+        if (args.bias_up) bias_u = widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias_up)[col + lane]);
+    }
+    const bool inside = row < args.rows;
+    float v[32];
+    if (kMode == kForward) {
+        tmem_load_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            float slope;
+            const float gate = __uint_as_float(g[i]) + __shfl_sync(~0u, bias_g, i);
+            const float up = __uint_as_float(u[i]) + __shfl_sync(~0u, bias_u, i);
+            v[i] = ok ? activate<kActivation, false>(gate, slope) * up : __int_as_float(0x7FC00000);
+        }
+        if (inside) store_row<kBf16>(args.out, row * args.out_stride + col, v, args.hidden - col, args.vector_out);
+        return;
+    }
+    const uint16_t* dh = reinterpret_cast<const uint16_t*>(args.grad_h) + row * args.grad_stride + col;
+    uint32_t d[16];
+    if (inside && args.vector_in && col + 32 <= args.hidden) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(dh) + i);
+            d[4 * i] = q.x, d[4 * i + 1] = q.y, d[4 * i + 2] = q.z, d[4 * i + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            d[i] = inside && col + 2 * i < args.hidden ? dh[2 * i] : 0;
+            d[i] |= inside && col + 2 * i + 1 < args.hidden ? (uint32_t)dh[2 * i + 1] << 16 : 0;
+        }
+    }
+    tmem_load_wait();
+    float w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        float slope;
+        const float gate = __uint_as_float(g[i]) + __shfl_sync(~0u, bias_g, i);
+        const float up = __uint_as_float(u[i]) + __shfl_sync(~0u, bias_u, i);
+        const float a = activate<kActivation, true>(gate, slope);
+        const float2 pair = unpack<kBf16>(d[i / 2]);
+        const float grad = i % 2 ? pair.y : pair.x;
+        // (zero behind the last row and column, also where x is not finite)
+        const bool counts = inside && col + i < args.hidden;
+        v[i] = !ok ? __int_as_float(0x7FC00000) : counts ? grad * up * slope : 0.0f;
+        w[i] = !ok ? __int_as_float(0x7FC00000) : counts ? grad * a : 0.0f;
+    }
+    if (inside) {
+        store_row<kBf16>(args.out, row * args.out_stride + col, v, 32, true);
+        store_row<kBf16>(args.out, row * args.out_stride + args.hidden_padded + col, w, 32, true);
+    }
+    if (args.sums && row - lane < args.rows) {
+        float* sums = args.sums + (row / 32) * 2 * args.hidden_padded + col + lane;
+        sums[0] = lane_sums(v, lane);
+        sums[args.hidden_padded] = lane_sums(w, lane);
+    }
+}
+
+// Which tiles a pair takes, the same for its producers, its matrix instructions and its epilogues.  kGradients: first the tiles
+// of the weights' gradients, pair after pair; the pairs that get one less of them go ahead on the tiles of dx.
+template <int kMode> struct Walk {
+    int pair, pairs, next, free_pairs, ahead_left, behind;
+    bool on_weights;
+    __device__ __forceinline__ Walk(const GatedArgs& args, int pair_, int pairs_) : pair(pair_), pairs(pairs_), next(pair_) {
+        on_weights = kMode == kGradients && args.tiles_w > 0;
+        const int extra = kMode == kGradients ? args.tiles_w % pairs : 0;
+        free_pairs = extra > 0 ? pairs - extra : 0;
+        ahead_left = extra > 0 && pair >= extra ? args.ahead : 0;
+        behind = extra > 0 ? min(args.ahead * free_pairs, args.tiles) : 0;
+        if (!on_weights) enter(args);
+    }
+    __device__ __forceinline__ void enter(const GatedArgs& args) {
+        on_weights = false;
+        next = ahead_left > 0 ? pair - (pairs - free_pairs) : behind + pair;
+    }
+    // the next tile; false when there is none left
+    __device__ __forceinline__ bool take(const GatedArgs& args, int& tile, bool& weights) {
+        if (on_weights) {
+            if (next < args.tiles_w) {
+                tile = next, weights = true;
+                next += pairs;
+                return true;
+            }
+            enter(args);
+        }
+        weights = false;
+        if (ahead_left > 0) {
+            if (next < behind) {
+                tile = next;
+                next += free_pairs;
+                if (--ahead_left == 0) next = behind + pair;
+                return true;
+            }
+            ahead_left = 0;
+            next = behind + pair;
+        }
+        if (next >= args.tiles) return false;
+        tile = next;
+        next += pairs;
+        return true;
+    }
+};
+
+// Pairs of blocks: 256 rows x 256 accumulator columns a tile, of which a block holds 128 rows of one operand and 128 of the other, so
+// that a step of 64 brings 32 KB to each multiprocessor for 512 clocks of matrix instructions (a block by itself: 48 KB).
+// Accumulators in turn: the epilogue of a tile runs beside the products of the next.
+constexpr int kPairStages = 6;
+constexpr int kPairStage = 2 * kRows * 128;
+constexpr int kPairShared = kPairStages * kPairStage + 1024;
+
+template <int kMode, bool kBf16, int kActivation>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_pair_kernel(const __grid_constant__ GatedArgs args) {
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t bars[2 * kStages + 5];
+    __shared__ uint64_t bars[2 * kPairStages + 5];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int given_up;
-
-    const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u;
-    const uint32_t bar0 = smem_addr(bars);
+    const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, bar0 = smem_addr(bars);
     auto full = [&](int s) { return bar0 + 8 * s; };
-    auto empty = [&](int s) { return bar0 + 8 * (kStages + s); };
-    auto acc_full = [&](int s) { return bar0 + 8 * (2 * kStages + s); };
-    auto acc_empty = [&](int s) { return bar0 + 8 * (2 * kStages + 2 + s); };
-    const uint32_t last = bar0 + 8 * (2 * kStages + 4);
+    auto empty = [&](int s) { return bar0 + 8 * (kPairStages + s); };
+    auto acc_full = [&](int s) { return bar0 + 8 * (2 * kPairStages + s); };
+    auto acc_empty = [&](int s) { return bar0 + 8 * (2 * kPairStages + 2 + s); };
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-
+    const int rank = (int)pair_rank(), pair = blockIdx.x / 2, pairs = gridDim.x / 2;
     if (threadIdx.x == 0) {
         given_up = 0;
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < kPairStages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(acc_full(s), 1);
-            mbar_init(acc_empty(s), 32 * kEpilogueWarps);
+            mbar_init(acc_empty(s), 2 * kEpilogueWarps);
         }
-        mbar_init(last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kEpilogueWarps + 1) tmem_alloc(smem_addr(&tmem_at), kTmem);
+    if (warp == kEpilogueWarps + 1) pair_tmem_alloc(smem_addr(&tmem_at), 512);
     tc_fence_before();
     __syncthreads();
+    pair_sync();
     tc_fence_after();
     const uint32_t tmem = tmem_at;
-    const int tiles = args.tiles_m * args.tiles_n;
-    const int steps = kMode == kGradInput ? 2 * args.k_blocks : args.k_blocks;
+    Walk<kMode> walk(args, pair, pairs);
+    int tile;
+    bool weights;
 
     if (warp == kEpilogueWarps) {
         if (lane == 0) {
             tma_prefetch_map(&args.a);
             tma_prefetch_map(&args.b0);
-            if (kMode != kGradWeight) tma_prefetch_map(&args.b1);
-            int64_t issued = 0;
+            tma_prefetch_map(&args.b1);
+            uint32_t issued = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-                const int m0 = tile / args.tiles_n * kRows, n0 = tile % args.tiles_n * kTileCols;
+            while (ok && walk.take(args, tile, weights)) {
+                const int across = weights ? args.tiles_w_n : args.tiles_n, steps = weights ? args.steps_w : args.steps;
+                const int m0 = tile / across * 256 + rank * 128, n = tile % across;
                 for (int k = 0; k < steps; ++k, ++issued) {
-                    const int s = (int)(issued % kStages);
-                    if (issued >= kStages && !mbar_wait(empty(s), (uint32_t)(issued / kStages - 1) & 1, &given_up)) {
+                    const int s = (int)(issued % kPairStages);
+                    if (issued >= kPairStages && !pair_wait(empty(s), (issued / kPairStages - 1) & 1, &given_up)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t a = ring + s * stage_bytes<kCols>(), b = a + kRows * 128;
-                    mbar_expect(full(s), stage_bytes<kCols>());
-                    if (kPaired) {
-                        tma_load_2d(a, &args.a, k * kStep, m0, full(s));
-                        tma_load_2d(b, &args.b0, k * kStep, n0, full(s));
-                        tma_load_2d(b + kTileCols * 128, &args.b1, k * kStep, n0, full(s));
-                    } else if (kMode == kGradInput) {
-                        const bool second = k >= args.k_blocks;
-                        const int f0 = (second ? k - args.k_blocks : k) * kStep;
-                        tma_load_2d(a, &args.a, f0 + (second ? args.hidden_padded : 0), m0, full(s));
-                        for (int c = 0; c < kCols / 64; ++c)
-                            tma_load_2d(b + c * 8192, second ? &args.b1 : &args.b0, n0 + 64 * c, f0, full(s));
+                    const uint32_t a = ring + s * kPairStage, b = a + kRows * 128, bar = in_leader(full(s));
+                    if (rank == 0) mbar_expect(full(s), 2 * kPairStage);
+                    if (kMode != kGradients) {
+                        pair_load_2d(a, &args.a, k * kStep, m0, bar);
+                        pair_load_2d(b, rank == 0 ? &args.b0 : &args.b1, k * kStep, n * 128, bar);
+                    } else if (weights) {
+                        for (int c = 0; c < 2; ++c) {
+                            pair_load_2d(a + c * 8192, &args.at, m0 + 64 * c, k * kStep, bar);
+                            pair_load_2d(b + c * 8192, &args.bt, n * 256 + rank * 128 + 64 * c, k * kStep, bar);
+                        }
                     } else {
-                        for (int c = 0; c < kRows / 64; ++c) tma_load_2d(a + c * 8192, &args.a, m0 + 64 * c, k * kStep, full(s));
-                        for (int c = 0; c < kCols / 64; ++c) tma_load_2d(b + c * 8192, &args.b0, n0 + 64 * c, k * kStep, full(s));
+                        const bool second = 2 * k >= steps;
+                        const int f0 = (second ? k - steps / 2 : k) * kStep;
+                        pair_load_2d(a, &args.a, f0 + (second ? args.hidden_padded : 0), m0, bar);
+                        for (int c = 0; c < 2; ++c)
+                            pair_load_2d(b + c * 8192, second ? &args.b1 : &args.b0, n * 256 + rank * 128 + 64 * c, f0, bar);
                     }
                 }
             }
-            if (!ok)  // the copies in flight land before the block's memory goes
-                for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
-                    volatile int still = 0;
-                    mbar_wait(full((int)(i % kStages)), (uint32_t)(i / kStages) & 1, &still);
-                }
+            if (!ok) let_settle();
         }
         __syncwarp();
     } else if (warp == kEpilogueWarps + 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = f16_idesc(kBf16, kMode == kGradWeight, !kPaired, kRows, kCols);
-            int64_t used = 0;
+        if (lane == 0 && rank == 0) {
+            uint32_t used = 0;
             int turn = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++turn) {
-                const int acc = turn & 1;
-                if (turn >= 2 && !mbar_wait(acc_empty(acc), (uint32_t)(turn / 2 - 1) & 1, &given_up)) {
+            for (; ok && walk.take(args, tile, weights); ++turn) {
+                const int acc = turn & 1, steps = weights ? args.steps_w : args.steps;
+                if (turn >= 2 && !pair_wait(acc_empty(acc), (uint32_t)(turn / 2 - 1) & 1, &given_up)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
+                const uint32_t idesc = f16_idesc(kBf16, weights, kMode == kGradients, 256, 256);
                 for (int k = 0; k < steps; ++k, ++used) {
-                    const int s = (int)(used % kStages);
-                    if (!mbar_wait(full(s), (uint32_t)(used / kStages) & 1, &given_up)) {
+                    const int s = (int)(used % kPairStages);
+                    if (!pair_wait(full(s), (used / kPairStages) & 1, &given_up)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = ring + s * stage_bytes<kCols>(), b = a + kRows * 128;
+                    const uint32_t a = ring + s * kPairStage, b = a + kRows * 128;
 #pragma unroll
                     for (int i = 0; i < kStep / 16; ++i) {
                         // rows along the reduction: 32 bytes on within the swizzled row, else 16 rows of 128 bytes
-                        const uint64_t da = kMode == kGradWeight ? operand_desc(a + 2048 * i, 1024, 8192) : operand_desc(a + 32 * i, 1024, 16);
-                        const uint64_t db = kPaired ? operand_desc(b + 32 * i, 1024, 16) : operand_desc(b + 2048 * i, 1024, 8192);
-                        mma_f16(tmem + acc * kCols, da, db, idesc, k > 0 || i > 0);
+                        const uint64_t da = weights ? operand_desc(a + 2048 * i, 1024, 8192) : operand_desc(a + 32 * i, 1024, 16);
+                        const uint64_t db = kMode == kGradients ? operand_desc(b + 2048 * i, 1024, 8192) : operand_desc(b + 32 * i, 1024, 16);
+                        pair_mma_f16(tmem + acc * 256, da, db, idesc, k > 0 || i > 0);
                     }
-                    tc_commit(empty(s));
+                    pair_commit(empty(s));
                 }
-                if (ok) tc_commit(acc_full(acc));
+                if (ok) pair_commit(acc_full(acc));
             }
-            if (!ok) {  // the matrix instructions in flight end before their tensor memory is freed
-                volatile int still = 0;
-                tc_commit(last);
-                mbar_wait(last, 0, &still);
-            }
+            if (!ok) let_settle();
         }
         __syncwarp();
     } else {
         const int quadrant = warp % 4, half = warp / 4;
         const uint32_t lanes = (uint32_t)(quadrant * 32) << 16;
-        int turn = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
-            const int64_t row = (int64_t)(tile / args.tiles_n) * kRows + quadrant * 32 + lane;
-            const int n0 = tile % args.tiles_n * kTileCols, acc = turn & 1;
-            const bool ok = mbar_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
+        for (int turn = 0; walk.take(args, tile, weights); ++turn) {
+            const int across = weights ? args.tiles_w_n : args.tiles_n, n = tile % across, acc = turn & 1;
+            const int64_t row = (int64_t)(tile / across) * 256 + rank * 128 + quadrant * 32 + lane;
+            const uint32_t from = tmem + lanes + acc * 256;
+            const bool ok = pair_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
             tc_fence_after();
-            for (int c = 32 * half; c < kTileCols; c += 64) {
-                const uint32_t from = tmem + lanes + acc * kCols + c;
-                const int col = n0 + c;
-                float v[32];
-                if (kPaired) {
-                    uint32_t g[32], u[32];
-                    tmem_load_32(from, g);
-                    tmem_load_32(from + kTileCols, u);
-                    float bias_g = 0.0f, bias_u = 0.0f;
-                    if (col + lane < args.hidden) {
-                        if (args.bias_gate) bias_g = widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias_gate)[col + lane]);
-                        if (args.bias_up) bias_u = widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias_up)[col + lane]);
-                    }
-                    if (kMode == kForward) {
-                        tmem_load_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float slope;
-                            const float gate = __uint_as_float(g[i]) + __shfl_sync(~0u, bias_g, i);
-                            const float up = __uint_as_float(u[i]) + __shfl_sync(~0u, bias_u, i);
-                            v[i] = activate<kActivation, false>(gate, slope) * up;
-                        }
-                    } else {
-                        const uint16_t* dh = reinterpret_cast<const uint16_t*>(args.grad_h) + row * args.grad_stride + col;
-                        const bool inside = row < args.rows;
-                        uint32_t d[16];
-                        if (inside && args.vector_in && col + 32 <= args.hidden) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint4 q = __ldg(reinterpret_cast<const uint4*>(dh) + i);
-                                d[4 * i] = q.x, d[4 * i + 1] = q.y, d[4 * i + 2] = q.z, d[4 * i + 3] = q.w;
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                d[i] = inside && col + 2 * i < args.hidden ? dh[2 * i] : 0;
-                                d[i] |= inside && col + 2 * i + 1 < args.hidden ? (uint32_t)dh[2 * i + 1] << 16 : 0;
-                            }
-                        }
-                        tmem_load_wait();
-                        float w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float slope;
-                            const float gate = __uint_as_float(g[i]) + __shfl_sync(~0u, bias_g, i);
-                            const float up = __uint_as_float(u[i]) + __shfl_sync(~0u, bias_u, i);
-                            const float a = activate<kActivation, true>(gate, slope);
-                            const float2 pair = unpack<kBf16>(d[i / 2]);
-                            const float grad = i % 2 ? pair.y : pair.x;
-                            // (zero behind the last column, also where a row of x is not finite)
-                            v[i] = !ok ? __int_as_float(0x7FC00000) : col + i < args.hidden ? grad * up * slope : 0.0f;
-                            w[i] = !ok ? __int_as_float(0x7FC00000) : col + i < args.hidden ? grad * a : 0.0f;
-                        }
-                        if (inside) store_row<kBf16>(args.out0, row * args.out_stride + args.hidden_padded + col, w, 32, true);
-                    }
-                } else {
+            if (kMode != kGradients) {
+                for (int c = 32 * half; c < 128; c += 64)
+                    finish_hidden<kMode, kBf16, kActivation>(args, from + c, from + 128 + c, row, n * 128 + c, ok, lane);
+            } else {
+                const bool up = weights && row >= args.hidden_padded;
+                const int64_t at = up ? row - args.hidden_padded : row;
+                void* out = weights ? (up ? args.dwu : args.dwg) : args.out;
+                const bool inside = weights ? at < args.hidden && out : at < args.rows;
+                const int64_t stride = weights ? args.width : args.out_stride;
+                const bool vector = weights ? args.vector_w : args.vector_out;
+                for (int c = 32 * half; c < 256; c += 64) {
                     uint32_t g[32];
-                    tmem_load_32(from, g);
+                    float v[32];
+                    tmem_load_32(from + c, g);
                     tmem_load_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(g[i]);
-                }
-                if (kMode != kGradHidden && !ok)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7FC00000);
-                if (kMode == kForward) {
-                    if (row < args.rows) store_row<kBf16>(args.out0, row * args.out_stride + col, v, args.hidden - col, args.vector_out);
-                } else if (kMode == kGradHidden) {
-                    if (row < args.rows) store_row<kBf16>(args.out0, row * args.out_stride + col, v, 32, true);
-                } else if (kMode == kGradInput) {
-                    if (row < args.rows) store_row<kBf16>(args.out0, row * args.out_stride + col, v, args.width - col, args.vector_out);
-                } else {
-                    const bool up = row >= args.hidden_padded;
-                    const int64_t f = up ? row - args.hidden_padded : row;
-                    if (f < args.hidden && (up ? args.out1 : args.out0))
-                        store_row<kBf16>(up ? args.out1 : args.out0, f * args.out_stride + col, v, args.width - col, args.vector_out);
+                    for (int i = 0; i < 32; ++i) v[i] = ok ? __uint_as_float(g[i]) : __int_as_float(0x7FC00000);
+                    const int col = n * 256 + c;
+                    if (inside) store_row<kBf16>(out, at * stride + col, v, args.width - col, vector);
                 }
             }
             tc_fence_before();
-            mbar_arrive(acc_empty(acc));
+            __syncwarp();
+            if (lane == 0) pair_arrive(in_leader(acc_empty(acc)));
         }
     }
     tc_fence_before();
     __syncthreads();
+    pair_sync();
     if (warp == kEpilogueWarps + 1) {
         tc_fence_after();
-        tmem_free(tmem, kTmem);
+        pair_tmem_free(tmem, 512);
+    }
+}
+
+// Blocks by themselves, 128 rows x 32 hidden columns: for few rows, where tiles of the pairs would leave most multiprocessors
+// without work and what counts is the length of a block's walk along the reduction.
+constexpr int kSlimStages = 8;
+constexpr int kSlimStage = (kRows + 64) * 128;
+constexpr int kSlimShared = kSlimStages * kSlimStage + 1024;
+
+template <int kMode, bool kBf16, int kActivation>
+__global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constant__ GatedArgs args) {
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t bars[2 * kSlimStages + 1];
+    __shared__ uint32_t tmem_at;
+    __shared__ volatile int given_up;
+    const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, bar0 = smem_addr(bars), done = bar0 + 16 * kSlimStages;
+    auto full = [&](int s) { return bar0 + 8 * s; };
+    auto empty = [&](int s) { return bar0 + 8 * (kSlimStages + s); };
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t m0 = (int64_t)(blockIdx.x / args.tiles_n) * kRows;
+    const int n0 = blockIdx.x % args.tiles_n * 32;
+    if (threadIdx.x == 0) {
+        given_up = 0;
+        for (int s = 0; s < kSlimStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 5) tmem_alloc(smem_addr(&tmem_at), 64);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    const int steps = args.steps;
+    if (warp == 4) {
+        if (lane == 0) {
+            bool ok = true;
+            int issued = 0;
+            for (; issued < steps; ++issued) {
+                const int s = issued % kSlimStages, round = issued / kSlimStages;
+                if (round > 0 && !mbar_wait(empty(s), (round - 1) & 1, &given_up)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t a = ring + s * kSlimStage, b = a + kRows * 128;
+                mbar_expect(full(s), kSlimStage);
+                tma_load_2d(a, &args.a, issued * kStep, (int)m0, full(s));
+                tma_load_2d(b, &args.b0, issued * kStep, n0, full(s));
+                tma_load_2d(b + 32 * 128, &args.b1, issued * kStep, n0, full(s));
+            }
+            if (!ok) let_settle();
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int k = 0; k < steps; ++k) {
+                const int s = k % kSlimStages;
+                if (!mbar_wait(full(s), (k / kSlimStages) & 1, &given_up)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t a = ring + s * kSlimStage, b = a + kRows * 128;
+#pragma unroll
+                for (int i = 0; i < kStep / 16; ++i)
+                    mma_f16(tmem, operand_desc(a + 32 * i, 1024, 16), operand_desc(b + 32 * i, 1024, 16), f16_idesc(kBf16, false, false, kRows, 64), k > 0 || i > 0);
+                tc_commit(empty(s));
+            }
+            if (ok)
+                tc_commit(done);
+            else
+                let_settle();
+        }
+        __syncwarp();
+    } else {
+        const bool ok = mbar_wait(done, 0, &given_up);
+        tc_fence_after();
+        const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16);
+        finish_hidden<kMode, kBf16, kActivation>(args, from, from + 32, m0 + warp * 32 + lane, n0, ok, lane);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_free(tmem, 64);
     }
 }
 
@@ -313,62 +466,49 @@ __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64
         }
 }
 
-// Column sums of dgate | dup: a block adds `chunk` rows of 64 columns, and a second launch the blocks' sums in their order.
+// Gradients of the biases: the column sums of 32 rows each, added up.  A block takes 32 columns, a warp every eighth part.
 template <bool kBf16>
-__global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* d, int64_t stride, int64_t rows, int64_t chunk, float* partial, int columns) {
-    __shared__ float2 part[8][32];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int col = blockIdx.x * 64 + 2 * lane;
-    const int64_t first = blockIdx.y * chunk, end = first + chunk < rows ? first + chunk : rows;
-    float2 sum = {0.0f, 0.0f};
-    for (int64_t r = first + warp; r < end; r += 8) {
-        const float2 v = unpack<kBf16>(*reinterpret_cast<const uint32_t*>(d + r * stride + col));
-        sum.x += v.x;
-        sum.y += v.y;
-    }
+__global__ void __launch_bounds__(256) bias_gradient_kernel(const float* sums, int64_t parts, int hidden, int hidden_padded, uint16_t* gate, uint16_t* up) {
+    __shared__ float part[8][32];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int64_t p = warp; p < parts; p += 8) sum += sums[p * 2 * hidden_padded + c];
     part[warp][lane] = sum;
     __syncthreads();
-    if (warp == 0) {
+    if (warp > 0) return;
 #pragma unroll
-        for (int w = 1; w < 8; ++w) {
-            sum.x += part[w][lane].x;
-            sum.y += part[w][lane].y;
-        }
-        float* p = partial + (int64_t)blockIdx.y * columns + col;
-        p[0] = sum.x;
-        p[1] = sum.y;
-    }
-}
-template <bool kBf16>
-__global__ void __launch_bounds__(128) column_totals_kernel(const float* partial, int parts, int hidden, int hidden_padded, uint16_t* gate, uint16_t* up) {
-    const int c = blockIdx.x * 128 + threadIdx.x;
-    if (c >= 2 * hidden_padded) return;
-    float sum = 0.0f;
-    for (int p = 0; p < parts; ++p) sum += partial[(int64_t)p * 2 * hidden_padded + c];
+    for (int w = 1; w < 8; ++w) sum += part[w][lane];
     const bool second = c >= hidden_padded;
     const int f = second ? c - hidden_padded : c;
     uint16_t* out = second ? up : gate;
     if (f < hidden && out) out[f] = narrow<kBf16>(sum);
 }
 
-static SharedLimit g_limit[4][2][2][2];
+static SharedLimit g_pair_limit[3][2][2], g_slim_limit[2][2][2];
 
-template <int kMode, int kCols, bool kBf16, int kActivation> static int launch(const GatedArgs& args, cudaStream_t stream) {
-    auto* kernel = gated_kernel<kMode, kCols, kBf16, kActivation>;
-    int rc = allow_shared(g_limit[kMode][kCols == 256][kBf16][kActivation], (const void*)kernel, shared_bytes<kCols>());
+template <int kMode, bool kBf16, int kActivation> static int launch_pairs(const GatedArgs& args, cudaStream_t stream) {
+    auto* kernel = gated_pair_kernel<kMode, kBf16, kActivation>;
+    int rc = allow_shared(g_pair_limit[kMode][kBf16][kActivation], (const void*)kernel, kPairShared);
     if (rc) return rc;
-    const int tiles = args.tiles_m * args.tiles_n;
-    kernel<<<tiles < sm_count() ? tiles : sm_count(), kThreads, shared_bytes<kCols>(), stream>>>(args);
-    return check_cuda(cudaGetLastError(), "gated_kernel");
+    const int tiles = args.tiles + args.tiles_w, pairs = sm_count() / 2;
+    kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, kPairShared, stream>>>(args);
+    return check_cuda(cudaGetLastError(), "gated_pair_kernel");
 }
-template <int kMode, int kCols> static int launch(const GatedArgs& args, bool bf16, cudaStream_t stream) {
-    if (kMode == kGradInput || kMode == kGradWeight)
-        return bf16 ? launch<kMode, kCols, true, 0>(args, stream) : launch<kMode, kCols, false, 0>(args, stream);
-    if (args.activation == kGelu)
-        return bf16 ? launch<kMode, kCols, true, kGelu>(args, stream) : launch<kMode, kCols, false, kGelu>(args, stream);
-    return bf16 ? launch<kMode, kCols, true, kSilu>(args, stream) : launch<kMode, kCols, false, kSilu>(args, stream);
+template <int kMode, bool kBf16, int kActivation> static int launch_slim(const GatedArgs& args, cudaStream_t stream) {
+    auto* kernel = gated_slim_kernel<kMode, kBf16, kActivation>;
+    int rc = allow_shared(g_slim_limit[kMode][kBf16][kActivation], (const void*)kernel, kSlimShared);
+    if (rc) return rc;
+    kernel<<<args.tiles, 192, kSlimShared, stream>>>(args);
+    return check_cuda(cudaGetLastError(), "gated_slim_kernel");
 }
-
+template <int kMode> static int launch_hidden(const GatedArgs& args, bool slim, bool bf16, int activation, cudaStream_t st) {
+    if (slim)
+        return activation == kGelu ? (bf16 ? launch_slim<kMode, true, kGelu>(args, st) : launch_slim<kMode, false, kGelu>(args, st))
+                                   : (bf16 ? launch_slim<kMode, true, kSilu>(args, st) : launch_slim<kMode, false, kSilu>(args, st));
+    return activation == kGelu ? (bf16 ? launch_pairs<kMode, true, kGelu>(args, st) : launch_pairs<kMode, false, kGelu>(args, st))
+                               : (bf16 ? launch_pairs<kMode, true, kSilu>(args, st) : launch_pairs<kMode, false, kSilu>(args, st));
+}
 
 constexpr int kFewRows = 8;
 constexpr int64_t kMostRows = 1ll << 30;
@@ -389,19 +529,19 @@ static int check_layer(const char* name, const void* x, int64_t x_stride, const 
     return P2B_OK;
 }
 
-// Maps of x (rows x 64 boxes) and of the weights for the paired products.
-static int paired_maps(GatedArgs& args, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride, int cols) {
+// Slim tiles where they fit the chip at once.
+static bool slim_tiles(int64_t rows, int32_t hidden) { return blocks_of(rows, kRows) * blocks_of(hidden, 32) <= sm_count(); }
+
+// Tiles and maps of x and the weights for the products that end in hidden columns.
+static int hidden_maps(GatedArgs& args, bool slim, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride) {
     int rc = encode_rows(&args.a, x, 2, args.width, args.rows, 2 * x_stride, kRows);
-    if (!rc) rc = encode_rows(&args.b0, wg, 2, args.width, args.hidden, 2 * wg_stride, cols / 2);
-    if (!rc) rc = encode_rows(&args.b1, wu, 2, args.width, args.hidden, 2 * wu_stride, cols / 2);
-    args.k_blocks = (int)blocks_of(args.width, kStep);
-    args.tiles_m = (int)blocks_of(args.rows, kRows);
-    args.tiles_n = (int)blocks_of(args.hidden, cols / 2);
+    if (!rc) rc = encode_rows(&args.b0, wg, 2, args.width, args.hidden, 2 * wg_stride, slim ? 32 : 128);
+    if (!rc) rc = encode_rows(&args.b1, wu, 2, args.width, args.hidden, 2 * wu_stride, slim ? 32 : 128);
+    args.steps = (int)blocks_of(args.width, kStep);
+    args.tiles_n = (int)blocks_of(args.hidden, slim ? 32 : 128);
+    args.tiles = (int)blocks_of(args.rows, slim ? kRows : 256) * args.tiles_n;
     return rc;
 }
-
-// A tile of 32 hidden columns where the wide ones would leave more than half of the multiprocessors without one.
-static bool narrow_tiles(int64_t rows, int32_t hidden) { return 2 * blocks_of(rows, kRows) * blocks_of(hidden, 128) <= sm_count(); }
 
 template <bool kBf16, int kActivation>
 static int launch_few(const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride, const void* bg,
@@ -435,20 +575,18 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
     if (!aligned16(x, x_stride) || !aligned16(wg, hidden > 1 ? wg_stride : 0) || !aligned16(wu, hidden > 1 ? wu_stride : 0))
         return set_error(P2B_ERR_ARG, "p2b_gated_forward: rows of x and of the weights must start on 16-byte boundaries");
     GatedArgs args{};
-    args.rows = rows, args.width = width, args.hidden = hidden, args.activation = activation;
-    args.bias_gate = bg, args.bias_up = bu, args.out0 = h, args.out_stride = h_stride, args.vector_out = aligned16(h, h_stride);
-    const bool slim = narrow_tiles(rows, hidden);
-    rc = paired_maps(args, x, x_stride, wg, hidden > 1 ? wg_stride : blocks_of(width, 8) * 8, wu, hidden > 1 ? wu_stride : blocks_of(width, 8) * 8, slim ? 64 : 256);
-    if (rc) return rc;
-    return slim ? launch<kForward, 64>(args, bf16, st) : launch<kForward, 256>(args, bf16, st);
+    args.rows = rows, args.width = width, args.hidden = hidden;
+    args.bias_gate = bg, args.bias_up = bu, args.out = h, args.out_stride = h_stride, args.vector_out = aligned16(h, h_stride);
+    if (hidden == 1) wg_stride = wu_stride = blocks_of(width, 8) * 8;
+    const bool slim = slim_tiles(rows, hidden);
+    rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
+    return rc ? rc : launch_hidden<kForward>(args, slim, bf16, activation, st);
 }
-
-static int sum_parts(int64_t rows) { return (int)(rows < 64 * 64 ? blocks_of(rows, 64) : 64); }
 
 extern "C" int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t hidden) {
     if (rows < 0 || rows > kMostRows || hidden < 1 || hidden > kMostColumns) return -1;
     const int64_t columns = 2 * blocks_of(hidden, 128) * 128;
-    return 2 * rows * columns + 4 * columns * sum_parts(rows);
+    return 2 * rows * columns + 4 * columns * blocks_of(rows, 32);  // dgate | dup, their column sums
 }
 
 extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride,
@@ -477,50 +615,43 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     if (rows == 1) x_stride = whole;
     if (hidden == 1) wg_stride = wu_stride = whole;
     GatedArgs args{};
-    args.rows = rows, args.width = width, args.hidden = hidden, args.activation = activation;
+    args.rows = rows, args.width = width, args.hidden = hidden;
     args.hidden_padded = (int)blocks_of(hidden, 128) * 128;
+    const int64_t columns = 2 * (int64_t)args.hidden_padded;
+    GatedArgs next = args;
     args.bias_gate = bg, args.bias_up = bu, args.grad_h = grad_h, args.grad_stride = grad_stride;
     args.vector_in = aligned16(grad_h, rows > 1 ? grad_stride : 0);
-    const int64_t columns = 2 * (int64_t)args.hidden_padded;
-    args.out0 = scratch, args.out_stride = columns;
-    rc = paired_maps(args, x, x_stride, wg, wg_stride, wu, wu_stride, 256);
-    if (!rc) rc = launch<kGradHidden, 256>(args, bf16, st);
+    args.out = scratch, args.out_stride = columns;
+    args.sums = dbg || dbu ? (float*)((char*)scratch + 2 * rows * columns) : nullptr;
+    const bool slim = slim_tiles(rows, args.hidden_padded);
+    rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
+    // every column of the work space is written, those behind the last hidden unit as zeros
+    args.tiles_n = args.hidden_padded / (slim ? 32 : 128);
+    args.tiles = (int)blocks_of(rows, slim ? kRows : 256) * args.tiles_n;
+    if (!rc) rc = launch_hidden<kGradHidden>(args, slim, bf16, activation, st);
     if (rc) return rc;
-    if (dx) {
-        GatedArgs in = args;
-        rc = encode_rows(&in.a, scratch, 2, columns, rows, 2 * columns, kRows);
-        if (!rc) rc = encode_rows(&in.b0, wg, 2, width, hidden, 2 * wg_stride, kStep);
-        if (!rc) rc = encode_rows(&in.b1, wu, 2, width, hidden, 2 * wu_stride, kStep);
+    if (dx || dwg || dwu) {
+        rc = encode_rows(&next.a, scratch, 2, columns, rows, 2 * columns, kRows);
+        if (!rc) rc = encode_rows(&next.b0, wg, 2, width, hidden, 2 * wg_stride, kStep);
+        if (!rc) rc = encode_rows(&next.b1, wu, 2, width, hidden, 2 * wu_stride, kStep);
+        if (!rc) rc = encode_rows(&next.at, scratch, 2, columns, rows, 2 * columns, kStep);
+        if (!rc) rc = encode_rows(&next.bt, x, 2, width, rows, 2 * x_stride, kStep);
         if (rc) return rc;
-        in.k_blocks = (int)blocks_of(hidden, kStep);
-        in.tiles_n = (int)blocks_of(width, 256);
-        in.out0 = dx, in.out_stride = dx_stride, in.vector_out = aligned16(dx, rows > 1 ? dx_stride : 0);
-        rc = launch<kGradInput, 256>(in, bf16, st);
-        if (rc) return rc;
-    }
-    if (dwg || dwu) {
-        GatedArgs in = args;
-        rc = encode_rows(&in.a, scratch, 2, columns, rows, 2 * columns, kStep);
-        if (!rc) rc = encode_rows(&in.b0, x, 2, width, rows, 2 * x_stride, kStep);
-        if (rc) return rc;
-        in.k_blocks = (int)blocks_of(rows, kStep);
-        in.tiles_m = (int)(columns / kRows);
-        in.tiles_n = (int)blocks_of(width, 256);
-        in.out0 = dwg, in.out1 = dwu, in.out_stride = width;
-        in.vector_out = (!dwg || aligned16(dwg, width)) && (!dwu || aligned16(dwu, width));
-        rc = launch<kGradWeight, 256>(in, bf16, st);
+        next.steps = 2 * (int)blocks_of(hidden, kStep);
+        next.steps_w = (int)blocks_of(rows, kStep);
+        next.tiles_n = next.tiles_w_n = (int)blocks_of(width, 256);
+        next.tiles = dx ? (int)blocks_of(rows, 256) * next.tiles_n : 0;
+        next.tiles_w = dwg || dwu ? (int)(columns / 256) * next.tiles_w_n : 0;
+        next.ahead = (next.steps_w + next.steps / 2) / next.steps;
+        next.out = dx, next.out_stride = dx_stride, next.vector_out = aligned16(dx, rows > 1 ? dx_stride : 0);
+        next.dwg = dwg, next.dwu = dwu, next.vector_w = (!dwg || aligned16(dwg, width)) && (!dwu || aligned16(dwu, width));
+        rc = bf16 ? launch_pairs<kGradients, true, 0>(next, st) : launch_pairs<kGradients, false, 0>(next, st);
         if (rc) return rc;
     }
-    if (dbg || dbu) {
-        float* partial = (float*)((char*)scratch + 2 * rows * columns);
-        const int parts = sum_parts(rows);
-        const dim3 grid((unsigned)(columns / 64), parts);
-        const int64_t chunk = blocks_of(rows, parts);
-        auto* sums = bf16 ? column_sums_kernel<true> : column_sums_kernel<false>;
-        auto* totals = bf16 ? column_totals_kernel<true> : column_totals_kernel<false>;
-        sums<<<grid, 256, 0, st>>>((const uint16_t*)scratch, columns, rows, chunk, partial, (int)columns);
-        totals<<<(unsigned)(columns / 128), 128, 0, st>>>(partial, parts, hidden, args.hidden_padded, (uint16_t*)dbg, (uint16_t*)dbu);
-        rc = check_cuda(cudaGetLastError(), "column sums");
+    if (args.sums) {
+        auto* kernel = bf16 ? bias_gradient_kernel<true> : bias_gradient_kernel<false>;
+        kernel<<<(unsigned)(columns / 32), 256, 0, st>>>(args.sums, blocks_of(rows, 32), hidden, args.hidden_padded, (uint16_t*)dbg, (uint16_t*)dbu);
+        rc = check_cuda(cudaGetLastError(), "bias_gradient_kernel");
     }
     return rc;
 }

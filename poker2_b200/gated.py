@@ -13,6 +13,7 @@ from . import _lib
 
 ACTIVATIONS = {"gelu": 0, "silu": 1}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
+FEW_ROWS = 8  # up to so many rows the forward pass reads operands of any alignment (p2b_gated_few_rows)
 
 
 def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, gate_bias: torch.Tensor | None = None,
@@ -21,12 +22,12 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
     -> act(x Wg^T + bg) * (x Wu^T + bu) [..., hidden].  Sums are fp32 and the result is rounded once.  `activation` is
     "gelu" (with erf) or "silu".  Any strides; rows that start on 16-byte boundaries (and weights likewise) are read in place.
     With gradients wanted the call is refused while a CUDA graph is being captured: use `gated_linear_backward` there."""
-    _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
-    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_weight, up_weight, gate_bias, up_bias))
-    if not wanted:
-        return _forward(x, gate_weight, up_weight, gate_bias, up_bias, activation)
-    _refuse_capture("gated_linear", "gated_linear_backward")
-    return _Gated.apply(x, gate_weight, up_weight, gate_bias, up_bias, activation)
+    act = _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
+    if torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad
+                                    or gate_bias is not None and gate_bias.requires_grad or up_bias is not None and up_bias.requires_grad):
+        _refuse_capture("gated_linear")
+        return _Gated.apply(x, gate_weight, up_weight, gate_bias, up_bias, act)
+    return _forward(x, gate_weight, up_weight, gate_bias, up_bias, act)
 
 
 def gated_linear_backward(grad_h: torch.Tensor, x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor,
@@ -34,85 +35,93 @@ def gated_linear_backward(grad_h: torch.Tensor, x: torch.Tensor, gate_weight: to
                           needs: tuple = (True, True, True, True, True)):
     """Gradients of sum(grad_h * gated_linear(x, ...)) for (x, gate_weight, up_weight, gate_bias, up_bias); None where `needs` says
     so or the bias is None.  The same inputs give the same bits."""
-    _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
-    width, hidden = x.shape[-1], gate_weight.shape[0]
-    if tuple(grad_h.shape) != (*x.shape[:-1], hidden) or grad_h.dtype != x.dtype or grad_h.device != x.device:
+    act = _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
+    if grad_h.shape != (*x.shape[:-1], gate_weight.shape[0]) or grad_h.dtype != x.dtype or grad_h.get_device() != x.get_device():
         raise ValueError("the gradient of the hidden layer must have its shape, type and device")
     with torch.no_grad():
-        rows_of = x.reshape(-1, width)
-        rows = rows_of.shape[0]
-        new = lambda wanted, *shape: torch.empty(*shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
-        dx = new(needs[0], rows, width)
-        dwg, dwu = new(needs[1], hidden, width), new(needs[2], hidden, width)
-        dbg, dbu = new(needs[3] and gate_bias is not None, hidden), new(needs[4] and up_bias is not None, hidden)
-        xr, gw, uw = _lib.wide_rows(rows_of), _lib.wide_rows(gate_weight), _lib.wide_rows(up_weight)
-        gh = grad_h.reshape(-1, hidden)
-        gh = gh if gh.stride(1) == 1 and (rows <= 1 or gh.stride(0) >= hidden) else gh.contiguous()
-        gb, ub = _packed(gate_bias), _packed(up_bias)
-        p = _lib.ptr
-        with _lib.on(x.device):
-            size = _lib.lib().p2b_gated_backward_scratch_bytes(rows, hidden)
-            scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
-            _lib.call("p2b_gated_backward", p(gh), gh.stride(0), p(xr), xr.stride(0), p(gw), gw.stride(0), p(uw), uw.stride(0), p(gb), p(ub),
-                      rows, width, hidden, _TYPES[x.dtype], ACTIVATIONS[activation], p(dx), width, p(dwg), p(dwu), p(dbg), p(dbu), p(scratch),
-                      scratch.numel(), _lib.stream_ptr(x.device))
-    return dx if dx is None else dx.view(x.shape), dwg, dwu, dbg, dbu
+        return _backward(grad_h, x, gate_weight, up_weight, gate_bias, up_bias, act, needs)
 
 
-def _forward(x, gate_weight, up_weight, gate_bias, up_bias, activation):
-    width, hidden = x.shape[-1], gate_weight.shape[0]
-    with torch.no_grad():
-        h = torch.empty(*x.shape[:-1], hidden, dtype=x.dtype, device=x.device)
-        xr, gw, uw = x.reshape(-1, width), gate_weight, up_weight
-        rows = xr.shape[0]
-        whole = _lib.wide_rows if rows > _lib.lib().p2b_gated_few_rows() else _lib.plain_rows
-        xr, gw, uw = whole(xr), whole(gw), whole(uw)
-        gb, ub = _packed(gate_bias), _packed(up_bias)
-        p = _lib.ptr
-        with _lib.on(x.device):
-            _lib.call("p2b_gated_forward", p(xr), xr.stride(0), p(gw), gw.stride(0), p(uw), uw.stride(0), p(gb), p(ub), rows, width, hidden,
-                      _TYPES[x.dtype], ACTIVATIONS[activation], p(h), hidden, _lib.stream_ptr(x.device))
-    return h
+def _forward(x, gate_weight, up_weight, gate_bias, up_bias, act):
+    shape, hidden = x.shape, gate_weight.shape[0]
+    width = shape[-1]
+    xr = x if len(shape) == 2 else x.reshape(-1, width)
+    rows = xr.shape[0]
+    h = x.new_empty((rows, hidden))
+    whole = _lib.wide_rows if rows > FEW_ROWS else _lib.plain_rows
+    xr, gw, uw = whole(xr), whole(gate_weight), whole(up_weight)
+    gb = None if gate_bias is None else gate_bias.contiguous()
+    ub = None if up_bias is None else up_bias.contiguous()
+    _lib.call_on(x.get_device(), "p2b_gated_forward", xr.data_ptr(), xr.stride(0), gw.data_ptr(), gw.stride(0), uw.data_ptr(), uw.stride(0),
+                 None if gb is None else gb.data_ptr(), None if ub is None else ub.data_ptr(), rows, width, hidden, _TYPES[x.dtype], act,
+                 h.data_ptr(), hidden)
+    return h if len(shape) == 2 else h.view(*shape[:-1], hidden)
+
+
+def _backward(grad_h, x, gate_weight, up_weight, gate_bias, up_bias, act, needs):
+    shape, hidden, p = x.shape, gate_weight.shape[0], _lib.ptr
+    width = shape[-1]
+    xr, gh = (x, grad_h) if len(shape) == 2 else (x.reshape(-1, width), grad_h.reshape(-1, hidden))
+    rows, new = xr.shape[0], x.new_empty
+    dx = new((rows, width)) if needs[0] else None
+    dwg = new((hidden, width)) if needs[1] else None
+    dwu = new((hidden, width)) if needs[2] else None
+    dbg = new((hidden,)) if needs[3] and gate_bias is not None else None
+    dbu = new((hidden,)) if needs[4] and up_bias is not None else None
+    xr, gw, uw, gh = _lib.wide_rows(xr), _lib.wide_rows(gate_weight), _lib.wide_rows(up_weight), _lib.plain_rows(gh)
+    gb = None if gate_bias is None else gate_bias.contiguous()
+    ub = None if up_bias is None else up_bias.contiguous()
+    size = _lib.lib().p2b_gated_backward_scratch_bytes(rows, hidden)
+    scratch = new((max(size, 16) // 2,))
+    _lib.call_on(x.get_device(), "p2b_gated_backward", gh.data_ptr(), gh.stride(0), xr.data_ptr(), xr.stride(0), gw.data_ptr(), gw.stride(0),
+                 uw.data_ptr(), uw.stride(0), p(gb), p(ub), rows, width, hidden, _TYPES[x.dtype], act, p(dx), width, p(dwg), p(dwu), p(dbg),
+                 p(dbu), scratch.data_ptr(), size)
+    return dx if dx is None or len(shape) == 2 else dx.view(shape), dwg, dwu, dbg, dbu
 
 
 class _Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, activation):
+    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, act):
         ctx.save_for_backward(x, gate_weight, up_weight, gate_bias, up_bias)
-        ctx.activation = activation
-        return _forward(x, gate_weight, up_weight, gate_bias, up_bias, activation)
+        ctx.act = act
+        return _forward(x, gate_weight, up_weight, gate_bias, up_bias, act)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_h):
-        _refuse_capture("the backward pass of gated_linear", "gated_linear_backward")
-        return (*gated_linear_backward(grad_h, *ctx.saved_tensors, activation=ctx.activation, needs=ctx.needs_input_grad[:5]), None)
+        _refuse_capture("the backward pass of gated_linear")
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_linear has no second derivatives (create_graph=True)")
+        return (*_backward(grad_h, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad), None)
 
 
-def _refuse_capture(what: str, instead: str) -> None:
+def _refuse_capture(what: str) -> None:
     """Autograd joins a leaf's gradient on the stream that the leaf was first used on; with an eager graph of the same leaves alive that
     stream lies outside the capture, and the process ends in the engine's thread."""
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what} cannot be captured into a CUDA graph through autograd; call {instead}, which can.")
+        raise RuntimeError(f"{what} cannot be captured into a CUDA graph through autograd; call gated_linear_backward, which can.")
 
 
-def _packed(bias):
-    return None if bias is None else bias.contiguous()
-
-
-def _check(x, gate_weight, up_weight, gate_bias, up_bias, activation) -> None:
-    _lib.require_cuda(x, "gated_linear")
-    if activation not in ACTIVATIONS:
+def _check(x, gate_weight, up_weight, gate_bias, up_bias, activation) -> int:
+    """The activation's number; ValueError where the arguments do not fit (asked once a call: the smallest calls last as long as the
+    host takes to make them)."""
+    device, dtype, shape = x.get_device(), x.dtype, gate_weight.shape
+    if device < 0:
+        _lib.require_cuda(x, "gated_linear")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
-    if x.dtype not in _TYPES:
+    if dtype not in _TYPES:
         raise ValueError("gated_linear takes bf16 or fp16 tensors")
-    if x.dim() < 1 or gate_weight.dim() != 2 or gate_weight.shape != up_weight.shape or gate_weight.shape[1] != x.shape[-1]:
+    if len(shape) != 2 or up_weight.shape != shape or x.dim() < 1 or x.shape[-1] != shape[1]:
         raise ValueError("x [..., width] and two weights [hidden, width] are wanted")
-    if gate_weight.numel() == 0:
+    if shape[0] == 0 or shape[1] == 0:
         raise ValueError("width and hidden must not be zero")
-    for t in (gate_weight, up_weight, gate_bias, up_bias):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise ValueError("x, weights and biases must have one type and lie on one device")
+    if gate_weight.dtype != dtype or up_weight.dtype != dtype or gate_weight.get_device() != device or up_weight.get_device() != device:
+        raise ValueError("x, weights and biases must have one type and lie on one device")
     for b in (gate_bias, up_bias):
-        if b is not None and tuple(b.shape) != (gate_weight.shape[0],):
-            raise ValueError("a bias has one entry for each hidden unit")
+        if b is not None:
+            if b.dtype != dtype or b.get_device() != device:
+                raise ValueError("x, weights and biases must have one type and lie on one device")
+            if b.dim() != 1 or b.shape[0] != shape[0]:
+                raise ValueError("a bias has one entry for each hidden unit")
+    return act

@@ -17,7 +17,7 @@ ACTIVATIONS = {"gelu": 0, "silu": 1, "none": 2}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-@dataclass(frozen=True)
+@dataclass
 class Mx4:
     """A matrix in 4 bits: `values` [rows, ceil(width/32)*16] bytes, two values a byte; `scales`, the blocks' exponents in the
     order in which the matrix instructions read them (include/poker2_b200.h); `shape` of what was quantised."""
@@ -40,32 +40,34 @@ class Mx4:
 
     def dequantise(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values stood for, in bf16, fp16 or fp32 (exact but for what lies outside the type's range)."""
-        if dtype not in _TYPES:
+        kind, values = _TYPES.get(dtype), self.values
+        if kind is None:
             raise ValueError("values are read back in bf16, fp16 or fp32")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _lib.on(self.device):
-            _lib.call("p2b_mx4_dequantise", _lib.ptr(self.values), _lib.ptr(self.scales), self.rows, self.width, _TYPES[dtype], _lib.ptr(out),
-                      self.width, _lib.stream_ptr(self.device))
+        out, width = values.new_empty(self.shape, dtype=dtype), self.shape[-1]
+        _lib.call_on(values.get_device(), "p2b_mx4_dequantise", values.data_ptr(), self.scales.data_ptr(), values.shape[0], width, kind,
+                     out.data_ptr(), width)
         return out
 
 
 def quantise(x: torch.Tensor) -> Mx4:
     """x [..., width], bf16, fp16 or fp32, any strides; the blocks lie along the last dimension, the last one may be short."""
-    _lib.require_cuda(x, "quantise")
-    if x.dtype not in _TYPES:
+    kind, shape, device = _TYPES.get(x.dtype), x.shape, x.get_device()
+    if device < 0:
+        _lib.require_cuda(x, "quantise")
+    if kind is None:
         raise ValueError("quantise takes bf16, fp16 or fp32 tensors")
-    if x.dim() < 1 or x.shape[-1] == 0:
+    if len(shape) < 1 or shape[-1] == 0:
         raise ValueError("quantise wants rows of at least one value")
-    width = x.shape[-1]
-    flat = x.detach().reshape(-1, width)
-    flat = flat if flat.stride(1) == 1 else flat.contiguous()
+    width = shape[-1]
+    flat = x if len(shape) == 2 else x.detach().reshape(-1, width)
     rows = flat.shape[0]
-    values = torch.empty(rows, (width + 31) // 32 * 16, dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows + 127) // 128 * ((width + 255) // 256) * 1024, dtype=torch.uint8, device=x.device)
-    with _lib.on(x.device):
-        _lib.call("p2b_mx4_quantise", _lib.ptr(flat), flat.stride(0), rows, width, _TYPES[x.dtype], _lib.ptr(values), _lib.ptr(scales),
-                  _lib.stream_ptr(x.device))
-    return Mx4(values, scales, tuple(x.shape))
+    if width > 1 and flat.stride(1) != 1:
+        flat = flat.detach().contiguous()
+    bytes_ = (width + 31) // 32 * 16
+    values = flat.new_empty((rows, bytes_), dtype=torch.uint8)
+    scales = flat.new_empty(((rows + 127) // 128 * ((width + 255) // 256) * 1024,), dtype=torch.uint8)
+    _lib.call_on(device, "p2b_mx4_quantise", flat.data_ptr(), flat.stride(0), rows, width, kind, values.data_ptr(), scales.data_ptr())
+    return Mx4(values, scales, tuple(shape))
 
 
 def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None, *, activation: str = "none",
@@ -75,26 +77,28 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
     unless `dtype` says bf16 or fp16.  `activation`: "none", "gelu" (with erf) or "silu".  Sums are fp32, one rounding at the end."""
     if not isinstance(weight, Mx4) or len(weight.shape) != 2:
         raise ValueError("the weight is a quantised matrix [columns, width]")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, bias)):
+    tensor = isinstance(x, torch.Tensor)
+    if torch.is_grad_enabled() and (tensor and x.requires_grad or bias is not None and bias.requires_grad):
         raise RuntimeError("mx4.linear has no gradient: call it under torch.no_grad(), or train the layer that was quantised")
     if dtype is None:
-        dtype = x.dtype if isinstance(x, torch.Tensor) and x.dtype == torch.float16 else torch.bfloat16
-    if dtype not in (torch.bfloat16, torch.float16):
+        dtype = torch.float16 if tensor and x.dtype == torch.float16 else torch.bfloat16
+    elif dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("the result is bf16 or fp16")
-    if len(x.shape) < 1 or x.shape[-1] != weight.width or x.device != weight.device:
+    columns, width = weight.shape
+    device = weight.values.get_device()
+    if len(x.shape) < 1 or x.shape[-1] != width or (x if tensor else x.values).get_device() != device:
         raise ValueError("x must have the weight's width and device")
-    columns = weight.shape[0]
     if columns == 0:
         raise ValueError("the weight has no row")
-    if bias is not None and (tuple(bias.shape) != (columns,) or bias.dtype != dtype or bias.device != weight.device):
-        raise ValueError("the bias has one entry for each output, in the type of the result and on its device")
-    a = x if isinstance(x, Mx4) else quantise(x)
-    out = torch.empty(*a.shape[:-1], columns, dtype=dtype, device=weight.device)
-    bias = None if bias is None else bias.contiguous()
-    p = _lib.ptr
-    with _lib.on(weight.device):
-        _lib.call("p2b_mx4_linear", p(a.values), p(a.scales), a.rows, p(weight.values), p(weight.scales), columns, weight.width, p(bias),
-                  _TYPES[dtype], ACTIVATIONS[activation], p(out), columns, _lib.stream_ptr(weight.device))
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != columns or bias.dtype != dtype or bias.get_device() != device:
+            raise ValueError("the bias has one entry for each output, in the type of the result and on its device")
+        bias = bias.contiguous()
+    a = quantise(x) if tensor else x
+    out = a.values.new_empty((*a.shape[:-1], columns), dtype=dtype)
+    _lib.call_on(device, "p2b_mx4_linear", a.values.data_ptr(), a.scales.data_ptr(), a.values.shape[0], weight.values.data_ptr(),
+                 weight.scales.data_ptr(), columns, width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, out.data_ptr(), columns)
     return out

@@ -73,48 +73,51 @@ class _Loss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, factor):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the backward pass of clipped_policy_loss cannot be captured into a CUDA graph; call clipped_policy_loss_and_grad, which can.")
+        if torch.is_grad_enabled():
+            raise RuntimeError("clipped_policy_loss has no second derivatives (create_graph=True)")
         grad, = ctx.saved_tensors
         out = torch.empty_like(grad)
-        p = _lib.ptr
-        with _lib.on(grad.device):
-            _lib.call("p2b_policy_loss_scale", p(grad), p(factor.contiguous()), grad.numel(), _TYPES[grad.dtype], p(out), _lib.stream_ptr(grad.device))
+        _lib.call_on(grad.get_device(), "p2b_policy_loss_scale", grad.data_ptr(), factor.data_ptr(), grad.numel(), _TYPES[grad.dtype], out.data_ptr())
         return out, None, None, None, None, None, None, None
+
+
+def _packed(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, with_grad):
     states, hands, actions = logits.shape
-    device = logits.device
-    packed = lambda t: None if t is None else t.detach().contiguous()  # noqa: E731
-    logits, old_policy, advantages, target, legal, weights = map(packed, (logits, old_policy, advantages, target, legal, weights))
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if with_grad else None
+    with torch.no_grad():
+        logits, old_policy, advantages, target, legal, weights = map(_packed, (logits, old_policy, advantages, target, legal, weights))
+    loss = target.new_empty(())
+    grad = logits.new_empty((states, hands, actions)) if with_grad else None
     p = _lib.ptr
-    with _lib.on(device):
-        size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
-        scratch = torch.empty(max(size, 8), dtype=torch.uint8, device=device)
-        _lib.call("p2b_policy_loss", p(logits), p(old_policy), p(advantages), p(target), p(legal), p(weights), states, hands, actions,
-                  _TYPES[logits.dtype], float(clip), float(kl), p(loss), p(grad), p(scratch), scratch.numel(), _lib.stream_ptr(device))
+    size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
+    scratch = target.new_empty((size // 4,))
+    _lib.call_on(logits.get_device(), "p2b_policy_loss", logits.data_ptr(), p(old_policy), p(advantages), target.data_ptr(), legal.data_ptr(),
+                 p(weights), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(), p(grad), scratch.data_ptr(), size)
     return loss, grad
 
 
 def _check(logits, old_policy, advantages, target, legal, weights, clip, kl) -> None:
-    _lib.require_cuda(logits, "clipped_policy_loss")
-    if logits.dtype not in _TYPES or logits.dim() != 3 or logits.shape[1] < 1 or not 1 <= logits.shape[2] <= MAX_ACTIONS:
+    device, shape, f32 = logits.get_device(), logits.shape, torch.float32
+    if device < 0:
+        _lib.require_cuda(logits, "clipped_policy_loss")
+    if logits.dtype not in _TYPES or len(shape) != 3 or shape[1] < 1 or not 1 <= shape[2] <= MAX_ACTIONS:
         raise ValueError(f"logits [states, hands, actions] in bf16, fp16 or fp32 with 1 to {MAX_ACTIONS} actions are wanted")
     if (old_policy is None) != (advantages is None):
         raise ValueError("the old policy and the advantages come together")
-    for t in (old_policy, advantages, target):
-        if t is not None and (t.shape != logits.shape or t.dtype != torch.float32 or t.device != logits.device):
+    for t in (target, old_policy, advantages):
+        if t is not None and (t.shape != shape or t.dtype != f32 or t.get_device() != device):
             raise ValueError("old policy, advantages and target have the logits' shape and device, in fp32")
-    if tuple(legal.shape) != (logits.shape[0], logits.shape[2]) or legal.dtype != torch.bool or legal.device != logits.device:
+    if legal.shape != (shape[0], shape[2]) or legal.dtype != torch.bool or legal.get_device() != device:
         raise ValueError("legal [states, actions] bool on the logits' device is wanted")
-    if weights is not None and (weights.shape != logits.shape[:2] or weights.dtype != torch.float32 or weights.device != logits.device):
+    if weights is not None and (weights.shape != shape[:2] or weights.dtype != f32 or weights.get_device() != device):
         raise ValueError("weights [states, hands] fp32 on the logits' device are wanted")
-    if any(t is not None and t.requires_grad for t in (old_policy, advantages, target, weights)) and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (old_policy, advantages, target, weights)):
         raise RuntimeError("the loss differentiates to the logits alone: detach the policies, advantages and weights")
     if not 0.0 <= clip < 1.0 or not 0.0 <= kl < float("inf"):
         raise ValueError("clip lies in [0, 1), kl is not negative")

@@ -54,6 +54,7 @@ def test_gated_addresses_off_their_boundaries_are_refused(handle):
         assert handle.p2b_gated_backward(*_gated_backward(p, **{name: p + 8})) == -1 and b"16-byte" in handle.p2b_last_error()
     assert handle.p2b_gated_backward(*_gated_backward(p, scratch=p + 4)) == -1
     assert handle.p2b_gated_forward(*_gated_forward(None, rows=0, wg=p, wu=p)) == 0  # no rows: nothing to do
+    assert handle.p2b_gated_few_rows() == gated.FEW_ROWS
     assert handle.p2b_gated_backward_scratch_bytes(-1, 8) == -1 and handle.p2b_gated_backward_scratch_bytes(8, 0) == -1
 
 
@@ -69,6 +70,9 @@ class _Elsewhere(torch.Tensor):
     @property
     def device(self):
         return torch.device("cuda:0")
+
+    def get_device(self):
+        return 0
 
 
 def _there(*shape, dtype=torch.bfloat16):
