@@ -17,6 +17,7 @@ enum GatedMode { kForward = 0, kGradHidden = 1, kGradients = 2 };
 struct GatedArgs {
     CUtensorMap a, b0, b1;   // kForward, kGradHidden: x, Wg, Wu; kGradients: dgate | dup by rows, Wg, Wu
     CUtensorMap at, bt;      // kGradients: dgate | dup and x with the reduction along their rows
+    CUtensorMap to, to_wg, to_wu;  // the outputs out, dwg, dwu, where their rows start on 16-byte boundaries
     const void *bias_gate, *bias_up, *grad_h;
     void *out, *dwg, *dwu;   // h, dgate | dup or dx; the gradients of the weights
     float* sums;             // kGradHidden: column sums of dgate | dup over 32 rows each (NULL: not wanted)
@@ -28,12 +29,13 @@ struct GatedArgs {
     int tiles_n, tiles;      // tiles of out
     int tiles_w_n, tiles_w;  // kGradients: tiles of the weights' gradients, and how many of the
     int ahead;               //   other tiles a pair without a last one of those takes in its place
-    int vector_in, vector_out, vector_w;  // 16-byte loads of grad_h, stores of the outputs
+    int vector_in, vector_bias;      // 16-byte loads of grad_h and of the biases
+    int align_out, align_w;          // row_alignment of the outputs
 };
 
 constexpr int kRows = 128;   // rows of a block's tile
 constexpr int kStep = 64;    // reduction columns of a stage: 128 bytes
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 
 // Sum over the warp's lanes of each of 32 values: lane l ends with the sum of value l.  Half of the values change places in
@@ -51,70 +53,64 @@ __device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
     return v[0];
 }
 
-// 32 hidden columns of a warp's 32 rows, from the accumulators of gate and up to h or to dgate and dup.
+// The biases as the epilogues read them: of up to kBiasColumns hidden units from shared memory, zeros behind the last, else from
+// where they are.
+constexpr int kBiasColumns = 2048;
+struct Biases {
+    const uint16_t *gate, *up;
+    int count_gate, count_up;  // entries that may be read
+    bool vector;
+};
+__device__ __forceinline__ Biases stage_biases(const GatedArgs& args, uint16_t* area, int threads) {
+    const uint16_t *gate = reinterpret_cast<const uint16_t*>(args.bias_gate), *up = reinterpret_cast<const uint16_t*>(args.bias_up);
+    if (args.hidden_padded > kBiasColumns) return {gate, up, gate ? args.hidden : 0, up ? args.hidden : 0, (bool)args.vector_bias};
+    for (int f = threadIdx.x; f < args.hidden_padded; f += threads) {
+        area[f] = gate && f < args.hidden ? gate[f] : 0;
+        area[args.hidden_padded + f] = up && f < args.hidden ? up[f] : 0;
+    }
+    return {area, area + args.hidden_padded, args.hidden_padded, args.hidden_padded, true};
+}
+
+// 16 hidden columns of a warp's 32 rows, from the accumulators of gate and up to h (v[0..15]) or to dgate and dup (v[0..15], v[16..31]).
+// (grad: 16 columns of grad_h, loaded before the accumulators were waited for.)
 template <int kMode, bool kBf16, int kActivation>
-__device__ __forceinline__ void finish_hidden(const GatedArgs& args, uint32_t gate_at, uint32_t up_at, int64_t row, int col, bool ok, int lane) {
-    uint32_t g[32], u[32];
-    tmem_load_32(gate_at, g);
-    tmem_load_32(up_at, u);
-    float bias_g = 0.0f, bias_u = 0.0f;
-    if (col + lane < args.hidden) {
-        if (args.bias_gate) bias_g = widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias_gate)[col + lane]);
-        if (args.bias_up) bias_u = widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias_up)[col + lane]);
-    }
+__device__ __forceinline__ void finish_hidden(const GatedArgs& args, const Biases& bias, const uint32_t (&grad)[8], uint32_t gate_at, uint32_t up_at,
+                                              int64_t row, int col, bool ok, float (&v)[32]) {
+    uint32_t g[16], u[16], bg[8], bu[8];
+    tmem_load_16(gate_at, g);
+    tmem_load_16(up_at, u);
+    load_words(bias.gate + col, bias.count_gate - col, bias.vector, bg);
+    load_words(bias.up + col, bias.count_up - col, bias.vector, bu);
     const bool inside = row < args.rows;
-    float v[32];
-    if (kMode == kForward) {
-        tmem_load_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float slope;
-            const float gate = __uint_as_float(g[i]) + __shfl_sync(~0u, bias_g, i);
-            const float up = __uint_as_float(u[i]) + __shfl_sync(~0u, bias_u, i);
-            v[i] = ok ? activate<kActivation, false>(gate, slope) * up : __int_as_float(0x7FC00000);
-        }
-        if (inside) store_row<kBf16>(args.out, row * args.out_stride + col, v, args.hidden - col, args.vector_out);
-        return;
-    }
-    const uint16_t* dh = reinterpret_cast<const uint16_t*>(args.grad_h) + row * args.grad_stride + col;
-    uint32_t d[16];
-    if (inside && args.vector_in && col + 32 <= args.hidden) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(dh) + i);
-            d[4 * i] = q.x, d[4 * i + 1] = q.y, d[4 * i + 2] = q.z, d[4 * i + 3] = q.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            d[i] = inside && col + 2 * i < args.hidden ? dh[2 * i] : 0;
-            d[i] |= inside && col + 2 * i + 1 < args.hidden ? (uint32_t)dh[2 * i + 1] << 16 : 0;
-        }
-    }
     tmem_load_wait();
-    float w[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
         float slope;
-        const float gate = __uint_as_float(g[i]) + __shfl_sync(~0u, bias_g, i);
-        const float up = __uint_as_float(u[i]) + __shfl_sync(~0u, bias_u, i);
-        const float a = activate<kActivation, true>(gate, slope);
-        const float2 pair = unpack<kBf16>(d[i / 2]);
-        const float grad = i % 2 ? pair.y : pair.x;
-        // (zero behind the last row and column, also where x is not finite)
-        const bool counts = inside && col + i < args.hidden;
-        v[i] = !ok ? __int_as_float(0x7FC00000) : counts ? grad * up * slope : 0.0f;
-        w[i] = !ok ? __int_as_float(0x7FC00000) : counts ? grad * a : 0.0f;
+        const float2 two_g = unpack<kBf16>(bg[i / 2]), two_u = unpack<kBf16>(bu[i / 2]);
+        const float gate = __uint_as_float(g[i]) + (i % 2 ? two_g.y : two_g.x);
+        const float up = __uint_as_float(u[i]) + (i % 2 ? two_u.y : two_u.x);
+        const float a = activate<kActivation, kMode == kGradHidden>(gate, slope);
+        if (kMode == kForward) {
+            v[i] = ok ? a * up : __int_as_float(0x7FC00000);
+        } else {
+            const float2 two = unpack<kBf16>(grad[i / 2]);
+            const float dh = i % 2 ? two.y : two.x;
+            // (zero behind the last row and column, also where x is not finite)
+            const bool counts = inside && col + i < args.hidden;
+            v[i] = !ok ? __int_as_float(0x7FC00000) : counts ? dh * up * slope : 0.0f;
+            v[16 + i] = !ok ? __int_as_float(0x7FC00000) : counts ? dh * a : 0.0f;
+        }
     }
-    if (inside) {
-        store_row<kBf16>(args.out, row * args.out_stride + col, v, 32, true);
-        store_row<kBf16>(args.out, row * args.out_stride + args.hidden_padded + col, w, 32, true);
-    }
-    if (args.sums && row - lane < args.rows) {
-        float* sums = args.sums + (row / 32) * 2 * args.hidden_padded + col + lane;
-        sums[0] = lane_sums(v, lane);
-        sums[args.hidden_padded] = lane_sums(w, lane);
-    }
+}
+__device__ __forceinline__ void split(const float (&v)[32], float (&lower)[16], float (&upper)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lower[i] = v[i], upper[i] = v[16 + i];
+}
+// Column sums of dgate and dup (16 columns each) over the warp's 32 rows.
+__device__ __forceinline__ void sum_hidden(const GatedArgs& args, float (&v)[32], int64_t row, int col, int lane) {
+    if (!args.sums || row - lane >= args.rows) return;
+    const float sum = lane_sums(v, lane);
+    args.sums[(row / 32) * 2 * args.hidden_padded + (lane < 16 ? 0 : args.hidden_padded - 16) + col + lane] = sum;
 }
 
 // Which tiles a pair takes, the same for its producers, its matrix instructions and its epilogues.  kGradients: first the tiles
@@ -165,9 +161,10 @@ template <int kMode> struct Walk {
 // Pairs of blocks: 256 rows x 256 accumulator columns a tile, of which a block holds 128 rows of one operand and 128 of the other, so
 // that a step of 64 brings 32 KB to each multiprocessor for 512 clocks of matrix instructions (a block by itself: 48 KB).
 // Accumulators in turn: the epilogue of a tile runs beside the products of the next.
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
 constexpr int kPairStage = 2 * kRows * 128;
-constexpr int kPairShared = kPairStages * kPairStage + 1024;
+constexpr int kBiasBytes = 4 * kBiasColumns;
+constexpr int kPairShared = kPairStages * kPairStage + 2 * kPanelBytes + kBiasBytes + 1024;
 
 template <int kMode, bool kBf16, int kActivation>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_pair_kernel(const __grid_constant__ GatedArgs args) {
@@ -195,6 +192,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kEpilogueWarps + 1) pair_tmem_alloc(smem_addr(&tmem_at), 512);
+    Biases bias{};
+    uint8_t* const panels = raw + (ring - smem_addr(raw)) + kPairStages * kPairStage;
+    if (kMode != kGradients) bias = stage_biases(args, reinterpret_cast<uint16_t*>(panels + 2 * kPanelBytes), kThreads);
     tc_fence_before();
     __syncthreads();
     pair_sync();
@@ -278,39 +278,87 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
         }
         __syncwarp();
     } else {
-        const int quadrant = warp % 4, half = warp / 4;
+        // The four warps of a quadrant (32 rows) fill its part of the panels; their first thread stores it.
+        const int quadrant = warp % 4, part = warp / 4, r = quadrant * 32 + lane;
+        const bool storer = part == 0 && lane == 0;
         const uint32_t lanes = (uint32_t)(quadrant * 32) << 16;
         for (int turn = 0; walk.take(args, tile, weights); ++turn) {
             const int across = weights ? args.tiles_w_n : args.tiles_n, n = tile % across, acc = turn & 1;
-            const int64_t row = (int64_t)(tile / across) * 256 + rank * 128 + quadrant * 32 + lane;
+            const int64_t row = (int64_t)(tile / across) * 256 + rank * 128 + r, row0 = row - lane;
             const uint32_t from = tmem + lanes + acc * 256;
+            const bool up = weights && row0 >= args.hidden_padded;  // (a block's 128 rows lie on one side)
+            const int64_t first = up ? row0 - args.hidden_padded : row0, rows = weights ? args.hidden : args.rows;
+            void* const out = weights ? (up ? args.dwu : args.dwg) : args.out;
+            const CUtensorMap* const map = weights ? (up ? &args.to_wu : &args.to_wg) : &args.to;
+            const int64_t stride = weights ? args.width : args.out_stride;
+            const int alignment = weights ? args.align_w : args.align_out;
+            uint32_t grad[2][8];
+            if (kMode == kGradHidden)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int col = n * 128 + 64 * j + 16 * part;
+                    load_words(reinterpret_cast<const uint16_t*>(args.grad_h) + row * args.grad_stride + col, row < args.rows ? args.hidden - col : 0,
+                               args.vector_in, grad[j]);
+                }
             const bool ok = pair_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
             tc_fence_after();
-            if (kMode != kGradients) {
-                for (int c = 32 * half; c < 128; c += 64)
-                    finish_hidden<kMode, kBf16, kActivation>(args, from + c, from + 128 + c, row, n * 128 + c, ok, lane);
-            } else {
-                const bool up = weights && row >= args.hidden_padded;
-                const int64_t at = up ? row - args.hidden_padded : row;
-                void* out = weights ? (up ? args.dwu : args.dwg) : args.out;
-                const bool inside = weights ? at < args.hidden && out : at < args.rows;
-                const int64_t stride = weights ? args.width : args.out_stride;
-                const bool vector = weights ? args.vector_w : args.vector_out;
-                for (int c = 32 * half; c < 256; c += 64) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                // forward: 64 columns, one panel after the other; dgate and dup: 64 columns each; other gradients: 128 columns
+                if (storer) {
+                    if (kMode == kForward)
+                        store_wait_read<1>();
+                    else
+                        store_wait_read<0>();
+                }
+                group_sync(1 + quadrant, 128);
+                const int col = kMode == kGradients ? n * 256 + 128 * j : n * 128 + 64 * j;
+                float v[32];
+                if (kMode == kGradients) {
                     uint32_t g[32];
-                    float v[32];
-                    tmem_load_32(from + c, g);
+                    tmem_load_32(from + 128 * j + 32 * part, g);
                     tmem_load_wait();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = ok ? __uint_as_float(g[i]) : __int_as_float(0x7FC00000);
-                    const int col = n * 256 + c;
-                    if (inside) store_row<kBf16>(out, at * stride + col, v, args.width - col, vector);
+                    put_panel<kBf16>(panels + part / 2 * kPanelBytes, r, part % 2 * 32, v);
+                } else {
+                    float lower[16], upper[16];
+                    const int c = 64 * j + 16 * part;
+                    finish_hidden<kMode, kBf16, kActivation>(args, bias, grad[j], from + c, from + 128 + c, row, n * 128 + c, ok, v);
+                    split(v, lower, upper);
+                    put_panel<kBf16>(panels + (kMode == kForward ? j : 0) * kPanelBytes, r, 16 * part, lower);
+                    if (kMode == kGradHidden) put_panel<kBf16>(panels + kPanelBytes, r, 16 * part, upper);
                 }
+                if (j == 1) {  // the accumulators are read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) pair_arrive(in_leader(acc_empty(acc)));
+                }
+                if (alignment == 16) {
+                    async_fence();
+                    group_sync(1 + quadrant, 128);
+                    if (storer) {
+                        if (first < rows && out) {
+                            const uint32_t src = smem_addr(panels) + quadrant * 4096;
+                            const int columns = kMode == kForward ? args.hidden : kMode == kGradHidden ? args.hidden_padded : args.width;
+                            if (col < columns) tma_store_2d(map, col, (int)first, src + (kMode == kForward ? j : 0) * kPanelBytes);
+                            if (kMode == kGradHidden) tma_store_2d(map, args.hidden_padded + col, (int)first, src + kPanelBytes);
+                            if (kMode == kGradients && col + 64 < columns) tma_store_2d(map, col + 64, (int)first, src + kPanelBytes);
+                        }
+                        store_commit();
+                    }
+                } else {
+                    group_sync(1 + quadrant, 128);
+                    const int columns = kMode == kForward ? args.hidden : args.width;
+                    if (out)
+                        for (int p = 0; p < (kMode == kGradients ? 2 : 1); ++p)
+                            copy_panel(panels + (kMode == kForward ? j : p) * kPanelBytes, quadrant * 32, part, 4, out, stride, first, rows, col + 64 * p, columns,
+                                       alignment >= 4, lane);
+                }
+                if (kMode == kGradHidden) sum_hidden(args, v, row, n * 128 + 64 * j + 16 * part, lane);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) pair_arrive(in_leader(acc_empty(acc)));
         }
+        if (storer) store_wait();
     }
     tc_fence_before();
     __syncthreads();
@@ -325,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
 // without work and what counts is the length of a block's walk along the reduction.
 constexpr int kSlimStages = 8;
 constexpr int kSlimStage = (kRows + 64) * 128;
-constexpr int kSlimShared = kSlimStages * kSlimStage + 1024;
+constexpr int kSlimShared = kSlimStages * kSlimStage + kBiasBytes + 1024;
 
 template <int kMode, bool kBf16, int kActivation>
 __global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constant__ GatedArgs args) {
@@ -349,6 +397,7 @@ __global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constan
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 5) tmem_alloc(smem_addr(&tmem_at), 64);
+    const Biases bias = stage_biases(args, reinterpret_cast<uint16_t*>(raw + (ring - smem_addr(raw)) + kSlimStages * kSlimStage), 192);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -396,10 +445,32 @@ __global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constan
         }
         __syncwarp();
     } else {
+        const int64_t row = m0 + warp * 32 + lane;
+        uint32_t grad[2][8];
+        if (kMode == kGradHidden)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                load_words(reinterpret_cast<const uint16_t*>(args.grad_h) + row * args.grad_stride + n0 + 16 * j,
+                           row < args.rows ? args.hidden - n0 - 16 * j : 0, args.vector_in, grad[j]);
         const bool ok = mbar_wait(done, 0, &given_up);
         tc_fence_after();
         const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16);
-        finish_hidden<kMode, kBf16, kActivation>(args, from, from + 32, m0 + warp * 32 + lane, n0, ok, lane);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float v[32], lower[16], upper[16];
+            const int col = n0 + 16 * j;
+            finish_hidden<kMode, kBf16, kActivation>(args, bias, grad[j], from + 16 * j, from + 32 + 16 * j, row, col, ok, v);
+            split(v, lower, upper);
+            if (row < args.rows) {
+                if (kMode == kForward) {
+                    store_row<kBf16>(args.out, row * args.out_stride + col, lower, args.hidden - col, args.align_out);
+                } else {
+                    store_row<kBf16>(args.out, row * args.out_stride + col, lower, 16, 16);
+                    store_row<kBf16>(args.out, row * args.out_stride + args.hidden_padded + col, upper, 16, 16);
+                }
+            }
+            if (kMode == kGradHidden) sum_hidden(args, v, row, col, lane);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -576,10 +647,13 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
         return set_error(P2B_ERR_ARG, "p2b_gated_forward: rows of x and of the weights must start on 16-byte boundaries");
     GatedArgs args{};
     args.rows = rows, args.width = width, args.hidden = hidden;
-    args.bias_gate = bg, args.bias_up = bu, args.out = h, args.out_stride = h_stride, args.vector_out = aligned16(h, h_stride);
+    args.hidden_padded = (int)blocks_of(hidden, 128) * 128;
+    args.bias_gate = bg, args.bias_up = bu, args.out = h, args.out_stride = h_stride, args.align_out = row_alignment(h, rows > 1 ? h_stride : 0);
+    args.vector_bias = aligned16(bg, 0) && aligned16(bu, 0);
     if (hidden == 1) wg_stride = wu_stride = blocks_of(width, 8) * 8;
     const bool slim = slim_tiles(rows, hidden);
     rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
+    if (!rc && !slim && args.align_out == 16) rc = encode_rows(&args.to, h, 2, hidden, rows, 2 * (rows > 1 ? h_stride : blocks_of(hidden, 8) * 8), 32);
     return rc ? rc : launch_hidden<kForward>(args, slim, bf16, activation, st);
 }
 
@@ -620,7 +694,7 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     const int64_t columns = 2 * (int64_t)args.hidden_padded;
     GatedArgs next = args;
     args.bias_gate = bg, args.bias_up = bu, args.grad_h = grad_h, args.grad_stride = grad_stride;
-    args.vector_in = aligned16(grad_h, rows > 1 ? grad_stride : 0);
+    args.vector_in = aligned16(grad_h, rows > 1 ? grad_stride : 0), args.vector_bias = aligned16(bg, 0) && aligned16(bu, 0);
     args.out = scratch, args.out_stride = columns;
     args.sums = dbg || dbu ? (float*)((char*)scratch + 2 * rows * columns) : nullptr;
     const bool slim = slim_tiles(rows, args.hidden_padded);
@@ -628,14 +702,22 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     // every column of the work space is written, those behind the last hidden unit as zeros
     args.tiles_n = args.hidden_padded / (slim ? 32 : 128);
     args.tiles = (int)blocks_of(rows, slim ? kRows : 256) * args.tiles_n;
+    args.align_out = 16;
+    if (!rc && !slim) rc = encode_rows(&args.to, scratch, 2, columns, rows, 2 * columns, 32);
     if (!rc) rc = launch_hidden<kGradHidden>(args, slim, bf16, activation, st);
     if (rc) return rc;
     if (dx || dwg || dwu) {
+        next.out = dx, next.out_stride = dx_stride, next.align_out = row_alignment(dx, rows > 1 ? dx_stride : 0);
+        next.dwg = dwg, next.dwu = dwu, next.align_w = row_alignment((const void*)((uintptr_t)dwg | (uintptr_t)dwu), hidden > 1 ? width : 0);
         rc = encode_rows(&next.a, scratch, 2, columns, rows, 2 * columns, kRows);
         if (!rc) rc = encode_rows(&next.b0, wg, 2, width, hidden, 2 * wg_stride, kStep);
         if (!rc) rc = encode_rows(&next.b1, wu, 2, width, hidden, 2 * wu_stride, kStep);
         if (!rc) rc = encode_rows(&next.at, scratch, 2, columns, rows, 2 * columns, kStep);
         if (!rc) rc = encode_rows(&next.bt, x, 2, width, rows, 2 * x_stride, kStep);
+        if (!rc && dx && next.align_out == 16) rc = encode_rows(&next.to, dx, 2, width, rows, 2 * (rows > 1 ? dx_stride : whole), 32);
+        for (int i = 0; i < 2; ++i)
+            if (!rc && (i ? dwu : dwg) && next.align_w == 16)
+                rc = encode_rows(i ? &next.to_wu : &next.to_wg, i ? dwu : dwg, 2, width, hidden, 2 * (hidden > 1 ? (int64_t)width : whole), 32);
         if (rc) return rc;
         next.steps = 2 * (int)blocks_of(hidden, kStep);
         next.steps_w = (int)blocks_of(rows, kStep);
@@ -643,8 +725,6 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
         next.tiles = dx ? (int)blocks_of(rows, 256) * next.tiles_n : 0;
         next.tiles_w = dwg || dwu ? (int)(columns / 256) * next.tiles_w_n : 0;
         next.ahead = (next.steps_w + next.steps / 2) / next.steps;
-        next.out = dx, next.out_stride = dx_stride, next.vector_out = aligned16(dx, rows > 1 ? dx_stride : 0);
-        next.dwg = dwg, next.dwu = dwu, next.vector_w = (!dwg || aligned16(dwg, width)) && (!dwu || aligned16(dwu, width));
         rc = bf16 ? launch_pairs<kGradients, true, 0>(next, st) : launch_pairs<kGradients, false, 0>(next, st);
         if (rc) return rc;
     }

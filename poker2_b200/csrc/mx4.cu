@@ -143,21 +143,22 @@ __global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* valu
 // y = act(A W^T + bias): tiles of 128 rows x 128 columns, steps of 256 columns of A and W (128 bytes a row), the scales of a step
 // copied from shared to tensor memory by the thread that issues the matrix instructions, in their order.
 struct Mx4Args {
-    CUtensorMap a, w;
+    CUtensorMap a, w, to;
     const uint8_t *a_scales, *w_scales;
     const void* bias;
     void* out;
     int64_t out_stride, rows;
     int columns, steps, tiles_m, tiles_n;
-    int vector_out;
+    int vector_bias, align_out;
 };
 
 constexpr int kTile = 128;
 constexpr int kMxStages = 5;
 constexpr int kScaleBytes = 1024;  // two pieces
 constexpr int kMxStage = 2 * (kTile * 128 + kScaleBytes);
-constexpr int kMxShared = kMxStages * kMxStage + 1024;
-constexpr int kMxThreads = 320;
+constexpr int kMxShared = kMxStages * kMxStage + 2 * kPanelBytes + 1024;
+constexpr int kMxEpilogueWarps = 16;
+constexpr int kMxThreads = 32 * (kMxEpilogueWarps + 2);
 constexpr int kScaleSets = 4;      // sets of scale columns in tensor memory, used in turn
 constexpr uint32_t kMxTmem = 512;  // two accumulators, scales behind them
 constexpr uint32_t kScaleColumn = 2 * kTile;
@@ -184,19 +185,19 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(acc_full(s), 1);
-            mbar_init(acc_empty(s), 256);
+            mbar_init(acc_empty(s), kMxEpilogueWarps);
         }
         mbar_init(last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) tmem_alloc(smem_addr(&tmem_at), kMxTmem);
+    if (warp == kMxEpilogueWarps + 1) tmem_alloc(smem_addr(&tmem_at), kMxTmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_at;
     const int tiles = args.tiles_m * args.tiles_n, steps = args.steps;
 
-    if (warp == 8) {
+    if (warp == kMxEpilogueWarps) {
         if (lane == 0) {
             tma_prefetch_map(&args.a);
             tma_prefetch_map(&args.w);
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
                 }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == kMxEpilogueWarps + 1) {
         if (lane == 0) {
             int64_t used = 0;
             int turn = 0;
@@ -267,35 +268,57 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
         }
         __syncwarp();
     } else {
-        const int quadrant = warp % 4, half = warp / 4;
+        // The four warps of a quadrant (32 rows) fill its part of the two panels; their first thread stores it.
+        const int quadrant = warp % 4, part = warp / 4, r = quadrant * 32 + lane;
+        const bool storer = part == 0 && lane == 0;
+        uint8_t* const panels = raw + (ring - smem_addr(raw)) + kMxStages * kMxStage;
         int turn = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
-            const int64_t row = (int64_t)(tile / args.tiles_n) * kTile + quadrant * 32 + lane;
-            const int n0 = tile % args.tiles_n * kTile, acc = turn & 1;
+            const int64_t row0 = (int64_t)(tile / args.tiles_n) * kTile + quadrant * 32;
+            const int n0 = tile % args.tiles_n * kTile, col = n0 + 32 * part, acc = turn & 1;
+            uint32_t bias[16];
+            load_words(reinterpret_cast<const uint16_t*>(args.bias) + col, args.bias ? args.columns - col : 0, args.vector_bias, bias);
             const bool ok = mbar_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
             tc_fence_after();
-            for (int c = 32 * half; c < kTile; c += 64) {
-                const int col = n0 + c;
-                uint32_t g[32];
-                float v[32];
-                tmem_load_32(tmem + ((uint32_t)(quadrant * 32) << 16) + acc * kTile + c, g);
-                const float bias = args.bias && col + lane < args.columns ? widen<kBf16>(reinterpret_cast<const uint16_t*>(args.bias)[col + lane]) : 0.0f;
-                tmem_load_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    float slope;
-                    const float y = activate<kActivation, false>(__uint_as_float(g[i]) + __shfl_sync(~0u, bias, i), slope);
-                    v[i] = ok ? y : __int_as_float(0x7FC00000);
-                }
-                if (row < args.rows) store_row<kBf16>(args.out, row * args.out_stride + col, v, args.columns - col, args.vector_out);
-            }
+            uint32_t g[32];
+            float v[32];
+            tmem_load_32(tmem + ((uint32_t)(quadrant * 32) << 16) + acc * kTile + 32 * part, g);
+            tmem_load_wait();
             tc_fence_before();
-            mbar_arrive(acc_empty(acc));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty(acc));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                float slope;
+                const float2 two = unpack<kBf16>(bias[i / 2]);
+                const float y = activate<kActivation, false>(__uint_as_float(g[i]) + (i % 2 ? two.y : two.x), slope);
+                v[i] = ok ? y : __int_as_float(0x7FC00000);
+            }
+            if (storer) store_wait_read<0>();
+            group_sync(1 + quadrant, 128);
+            put_panel<kBf16>(panels + part / 2 * kPanelBytes, r, part % 2 * 32, v);
+            if (args.align_out == 16) {
+                async_fence();
+                group_sync(1 + quadrant, 128);
+                if (storer) {
+                    if (row0 < args.rows)
+                        for (int p = 0; p < 2; ++p)
+                            if (n0 + 64 * p < args.columns)
+                                tma_store_2d(&args.to, n0 + 64 * p, (int)row0, smem_addr(panels) + p * kPanelBytes + quadrant * 4096);
+                    store_commit();
+                }
+            } else {
+                group_sync(1 + quadrant, 128);
+                for (int p = 0; p < 2; ++p)
+                    copy_panel(panels + p * kPanelBytes, quadrant * 32, part, 4, args.out, args.out_stride, row0, args.rows, n0 + 64 * p, args.columns,
+                               args.align_out >= 4, lane);
+            }
         }
+        if (storer) store_wait();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kMxEpilogueWarps + 1) {
         tc_fence_after();
         tmem_free(tmem, kMxTmem);
     }
@@ -392,10 +415,13 @@ extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_
     rc = encode_rows(&args.a, a_values, 1, row_bytes, rows, row_bytes, kTile);
     if (!rc) rc = encode_rows(&args.w, w_values, 1, row_bytes, columns, row_bytes, kTile);
     if (rc) return rc;
+    args.align_out = row_alignment(out, rows > 1 ? out_stride : 0);
+    if (args.align_out == 16) rc = encode_rows(&args.to, out, 2, columns, rows, 2 * (rows > 1 ? out_stride : blocks_of(columns, 8) * 8), 32);
+    if (rc) return rc;
     args.a_scales = (const uint8_t*)a_scales, args.w_scales = (const uint8_t*)w_scales, args.bias = bias, args.out = out;
     args.out_stride = out_stride, args.rows = rows, args.columns = columns;
     args.steps = (int)blocks_of(width, 256), args.tiles_m = (int)blocks_of(rows, kTile), args.tiles_n = (int)blocks_of(columns, kTile);
-    args.vector_out = aligned16(out, out_stride);
+    args.vector_bias = aligned16(bias, 0);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == 0)
         return activation == 0 ? launch_linear<0, 0>(args, st) : activation == 1 ? launch_linear<0, 1>(args, st) : launch_linear<0, 2>(args, st);
