@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64
     for (int r = 0; r < kMost; ++r) g[r] = u[r] = 0.0f;
     const uint16_t *pg = wg + f * wg_stride, *pu = wu + f * wu_stride;
     if (vector) {
-#pragma unroll 2
+#pragma unroll(kMost == 1 ? 6 : kMost == 4 ? 3 : 2)
         for (int k = lane * 8; k + 8 <= width; k += 256) {
             const uint4 a = __ldg(reinterpret_cast<const uint4*>(pg + k)), b = __ldg(reinterpret_cast<const uint4*>(pu + k));
             const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};

@@ -11,6 +11,8 @@
 #include "layer.cuh"
 #include "tensor.cuh"
 
+#include <type_traits>
+
 namespace p2b {
 
 using namespace tc;
@@ -18,37 +20,56 @@ using namespace tc;
 // pieces of 512 scale bytes along a row of `width` values
 __host__ __device__ __forceinline__ int64_t scale_pieces(int64_t width) { return (width + 255) / 256 * 2; }
 
-template <typename T> struct Eight;  // 8 neighbouring values as fp32
-template <> struct Eight<float> {
-    static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-    static __device__ __forceinline__ float one(const float* p) { return *p; }
-    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
-    static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-};
-template <bool kBf16> struct EightHalf {
-    static __device__ __forceinline__ void load(const void* p, float (&v)[8]) {
+// Eight neighbouring values as they lie in memory, and what is asked of them.
+template <typename T> struct Eight {  // 16-bit types
+    static constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const T* p) {
         const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    }
+    __device__ __forceinline__ void load_some(const T* p, int64_t count) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack<kBf16>(w[i]);
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-        }
+        for (int i = 0; i < 4; ++i) w[i] = (2 * i < count ? h[2 * i] : 0) | (2 * i + 1 < count ? (uint32_t)h[2 * i + 1] << 16 : 0);
     }
-    static __device__ __forceinline__ float one(const void* p) { return widen<kBf16>(*reinterpret_cast<const uint16_t*>(p)); }
-    static __device__ __forceinline__ void put(void* p, float v) { *reinterpret_cast<uint16_t*>(p) = narrow<kBf16>(v); }
-    static __device__ __forceinline__ void store(void* p, const float (&v)[8]) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack<kBf16>(v[0], v[1]), pack<kBf16>(v[2], v[3]), pack<kBf16>(v[4], v[5]), pack<kBf16>(v[6], v[7]));
+    // the largest magnitude as an ordered number (a NaN counts as the largest), to be taken over lanes, and the float it stands for
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        return max(m & 0xFFFFu, m >> 16);
     }
+    static __device__ __forceinline__ float magnitude(uint32_t top) { return widen<kBf16>((uint16_t)top); }
+    __device__ __forceinline__ float2 pair(int i) const { return unpack<kBf16>(w[i]); }
+    static __device__ __forceinline__ void store(T* p, const float2 (&v)[4]) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack<kBf16>(v[0].x, v[0].y), pack<kBf16>(v[1].x, v[1].y), pack<kBf16>(v[2].x, v[2].y), pack<kBf16>(v[3].x, v[3].y));
+    }
+    static __device__ __forceinline__ void put(T* p, float v) { *reinterpret_cast<uint16_t*>(p) = narrow<kBf16>(v); }
 };
-template <> struct Eight<__nv_bfloat16> : EightHalf<true> {};
-template <> struct Eight<__half> : EightHalf<false> {};
+template <> struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = __ldg(reinterpret_cast<const float4*>(p));
+        b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+    __device__ __forceinline__ void load_some(const float* p, int64_t count) {
+        a = make_float4(count > 0 ? p[0] : 0.0f, count > 1 ? p[1] : 0.0f, count > 2 ? p[2] : 0.0f, count > 3 ? p[3] : 0.0f);
+        b = make_float4(count > 4 ? p[4] : 0.0f, count > 5 ? p[5] : 0.0f, count > 6 ? p[6] : 0.0f, count > 7 ? p[7] : 0.0f);
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        const uint32_t m = max(max(__float_as_uint(a.x) & 0x7FFFFFFFu, __float_as_uint(a.y) & 0x7FFFFFFFu), max(__float_as_uint(a.z) & 0x7FFFFFFFu, __float_as_uint(a.w) & 0x7FFFFFFFu));
+        const uint32_t n = max(max(__float_as_uint(b.x) & 0x7FFFFFFFu, __float_as_uint(b.y) & 0x7FFFFFFFu), max(__float_as_uint(b.z) & 0x7FFFFFFFu, __float_as_uint(b.w) & 0x7FFFFFFFu));
+        return max(m, n);
+    }
+    static __device__ __forceinline__ float magnitude(uint32_t top) { return __uint_as_float(top); }
+    __device__ __forceinline__ float2 pair(int i) const { return i == 0 ? make_float2(a.x, a.y) : i == 1 ? make_float2(a.z, a.w) : i == 2 ? make_float2(b.x, b.y) : make_float2(b.z, b.w); }
+    static __device__ __forceinline__ void store(float* p, const float2 (&v)[4]) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
 
 // Scale byte of a block whose largest magnitude is `top`: top = 2^E m, 1 <= m < 2, is at most 6 * 2^(E-2) where m <= 1.5.
 __device__ __forceinline__ uint32_t scale_byte(float top) {
@@ -67,75 +88,97 @@ __device__ __forceinline__ uint32_t four_bit_pair(float lo, float hi) {
     asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(v) : "f"(lo), "f"(hi));
     return v;
 }
-__device__ __forceinline__ float four_bit_value(uint32_t code) {
-    // magnitudes 0, 0.5 and then sign and two exponent bits, one mantissa bit
-    const uint32_t m = code & 7u;
-    const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-    return code & 8u ? -v : v;
+__device__ __forceinline__ float2 four_bit_values(uint32_t byte) {
+    uint32_t v;
+    asm("{\n\t.reg .b8 q;\n\tcvt.u8.u32 q, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, q;\n\t}" : "=r"(v) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// Four lanes take a block, a warp 256 neighbouring columns of a row: 16-byte loads (16-bit types), 128 bytes of values and two
-// scale words out.  Bound by memory: 2 + 17/32 bytes a value.
+// Four lanes take a block, a warp kSpans times 256 neighbouring columns of a row: 16-byte loads (16-bit types), kSpans of them on
+// their way at once, 128 bytes of values and two scale words out.  Bound by memory: 2 + 17/32 bytes a value.
+constexpr int kSpans = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t stride, int64_t rows, int64_t width, uint8_t* values,
-                                                           uint8_t* scales, int vector) {
+__global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t stride, int64_t rows, int width, uint8_t* values, uint8_t* scales,
+                                                           int vector) {
     const int lane = threadIdx.x % 32;
-    const int64_t row_bytes = (width + 31) / 32 * 16, pieces = scale_pieces(width), spans = pieces / 2;
-    const int64_t all = (rows + 127) / 128 * 128 * spans;
+    const int blocks = (width + 31) / 32, spans = (width + 255) / 256, row_jobs = (spans + kSpans - 1) / kSpans;
+    const int64_t row_bytes = (int64_t)blocks * 16, all = (rows + 127) / 128 * 128 * row_jobs;
     for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < all; job += (int64_t)gridDim.x * 8) {
-        const int64_t row = job / spans, span = job - row * spans;
-        const int64_t col = span * 256 + lane * 8;
-        float v[8];
-        const T* p = x + row * stride + col;
-        if (row < rows && col + 8 <= width && vector) {
-            Eight<T>::load(p, v);
-        } else {
+        const int64_t row = all < (1ll << 31) ? (uint32_t)job / (uint32_t)row_jobs : job / row_jobs;
+        const int first = (int)(job - row * row_jobs) * kSpans;
+        const T* p = x + row * stride + first * 256 + lane * 8;
+        Eight<T> v[kSpans];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = row < rows && col + i < width ? Eight<T>::one(p + i) : 0.0f;
+        for (int i = 0; i < kSpans; ++i) {
+            const int col = (first + i) * 256 + lane * 8;
+            if (row < rows && vector && col + 8 <= width)
+                v[i].load(p + i * 256);
+            else
+                v[i].load_some(p + i * 256, row < rows ? width - col : 0);
         }
-        // (as bits: a NaN counts as the largest)
-        uint32_t top = 0;
+        uint8_t* const row_scales = scales + (row / 128 * spans * 2 + lane / 16) * 512 + row % 32 * 16 + row % 128 / 32 * 4;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(~0u, top, 1));
-        top = max(top, __shfl_xor_sync(~0u, top, 2));
-        const uint32_t byte = scale_byte(__uint_as_float(top));
-        const float inverse = byte == 255u ? 0.0f : inverse_scale(byte);
-        uint32_t word = 0;
+        for (int i = 0; i < kSpans; ++i) {
+            if (first + i >= spans) break;
+            uint32_t top = v[i].top();
+            top = max(top, __shfl_xor_sync(~0u, top, 1));
+            top = max(top, __shfl_xor_sync(~0u, top, 2));
+            const uint32_t byte = scale_byte(Eight<T>::magnitude(top));
+            const float inverse = byte == 255u ? 0.0f : inverse_scale(byte);
+            uint32_t word = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) word |= four_bit_pair(v[2 * i] * inverse, v[2 * i + 1] * inverse) << (8 * i);
-        if (row < rows && col < (width + 31) / 32 * 32) *reinterpret_cast<uint32_t*>(values + row * row_bytes + col / 2) = word;
-        uint32_t four = byte << (8 * (lane / 4 % 4));
-        four |= __shfl_xor_sync(~0u, four, 4);
-        four |= __shfl_xor_sync(~0u, four, 8);
-        if (lane % 16 == 0) {
-            const int64_t piece = row / 128 * pieces + span * 2 + lane / 16;
-            *reinterpret_cast<uint32_t*>(scales + piece * 512 + row % 32 * 16 + row % 128 / 32 * 4) = four;
+            for (int j = 0; j < 4; ++j) {
+                const float2 two = v[i].pair(j);
+                word |= four_bit_pair(two.x * inverse, two.y * inverse) << (8 * j);
+            }
+            const int col = (first + i) * 256 + lane * 8;
+            if (row < rows && col < blocks * 32) *reinterpret_cast<uint32_t*>(values + row * row_bytes + col / 2) = word;
+            uint32_t four = byte << (8 * (lane / 4 % 4));
+            four |= __shfl_xor_sync(~0u, four, 4);
+            four |= __shfl_xor_sync(~0u, four, 8);
+            if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(row_scales + (int64_t)(first + i) * 1024) = four;
         }
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* values, const uint8_t* scales, int64_t rows, int64_t width, T* out,
+__global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* values, const uint8_t* scales, int64_t rows, int width, T* out,
                                                              int64_t stride, int vector) {
     const int lane = threadIdx.x % 32;
-    const int64_t row_bytes = (width + 31) / 32 * 16, pieces = scale_pieces(width), spans = pieces / 2;
-    for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < rows * spans; job += (int64_t)gridDim.x * 8) {
-        const int64_t row = job / spans, span = job - row * spans, col = span * 256 + lane * 8;
-        if (col >= width) continue;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(values + row * row_bytes + col / 2));
-        const int64_t piece = row / 128 * pieces + span * 2 + lane / 16;
-        const float scale = scale_of(__ldg(scales + piece * 512 + row % 32 * 16 + row % 128 / 32 * 4 + lane / 4 % 4));
-        float v[8];
+    const int spans = (width + 255) / 256, row_jobs = (spans + kSpans - 1) / kSpans;
+    const int64_t row_bytes = (int64_t)((width + 31) / 32) * 16, all = rows * row_jobs;
+    for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < all; job += (int64_t)gridDim.x * 8) {
+        const int64_t row = all < (1ll << 31) ? (uint32_t)job / (uint32_t)row_jobs : job / row_jobs;
+        const int first = (int)(job - row * row_jobs) * kSpans;
+        const uint8_t* const row_scales = scales + (row / 128 * spans * 2 + lane / 16) * 512 + row % 32 * 16 + row % 128 / 32 * 4 + lane / 4 % 4;
+        uint32_t word[kSpans], byte[kSpans];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = four_bit_value(word >> (4 * i) & 15u) * scale;
-        T* p = out + row * stride + col;
-        if (vector && col + 8 <= width) {
-            Eight<T>::store(p, v);
-        } else {
+        for (int i = 0; i < kSpans; ++i) {
+            const int col = (first + i) * 256 + lane * 8;
+            word[i] = col < width ? __ldg(reinterpret_cast<const uint32_t*>(values + row * row_bytes + col / 2)) : 0;
+            byte[i] = col < width ? __ldg(row_scales + (int64_t)(first + i) * 1024) : 0;
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (col + i < width) Eight<T>::put(p + i, v[i]);
+        for (int i = 0; i < kSpans; ++i) {
+            const int col = (first + i) * 256 + lane * 8;
+            const float scale = scale_of(byte[i]);
+            float2 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = four_bit_values(word[i] >> (8 * j) & 255u);
+                v[j].x *= scale, v[j].y *= scale;
+            }
+            T* p = out + row * stride + col;
+            if (vector && col + 8 <= width) {
+                Eight<T>::store(p, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (col + 2 * j < width) Eight<T>::put(p + 2 * j, v[j].x);
+                    if (col + 2 * j + 1 < width) Eight<T>::put(p + 2 * j + 1, v[j].y);
+                }
+            }
         }
     }
 }
@@ -366,12 +409,12 @@ extern "C" int p2b_mx4_quantise(const void* x, int64_t x_stride, int64_t rows, i
     if (((uintptr_t)values % 16) || ((uintptr_t)scales % 16) || (uintptr_t)x % (dtype == 2 ? 4 : 2))
         return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: values and scales must lie on 16-byte boundaries, x on its element's");
     const int vector = (uintptr_t)x % 16 == 0 && x_stride % (dtype == 2 ? 4 : 8) == 0;
-    const unsigned grid = warp_grid(blocks_of(rows, 128) * 128 * (scale_pieces(width) / 2));
+    const unsigned grid = warp_grid(blocks_of(rows, 128) * 128 * blocks_of(width, 256 * kSpans));
     cudaStream_t st = (cudaStream_t)stream;
     uint8_t *v = (uint8_t*)values, *s = (uint8_t*)scales;
-    if (dtype == 0) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, x_stride, rows, (int64_t)width, v, s, vector);
-    if (dtype == 1) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __half*)x, x_stride, rows, (int64_t)width, v, s, vector);
-    if (dtype == 2) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const float*)x, x_stride, rows, (int64_t)width, v, s, vector);
+    if (dtype == 0) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, x_stride, rows, width, v, s, vector);
+    if (dtype == 1) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __half*)x, x_stride, rows, width, v, s, vector);
+    if (dtype == 2) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const float*)x, x_stride, rows, width, v, s, vector);
     return check_cuda(cudaGetLastError(), "mx4_quantise_kernel");
 }
 
@@ -386,12 +429,12 @@ extern "C" int p2b_mx4_dequantise(const void* values, const void* scales, int64_
     if (((uintptr_t)values % 16) || ((uintptr_t)scales % 16) || (uintptr_t)out % (dtype == 2 ? 4 : 2))
         return set_error(P2B_ERR_ARG, "p2b_mx4_dequantise: values and scales must lie on 16-byte boundaries, out on its element's");
     const int vector = (uintptr_t)out % 16 == 0 && out_stride % (dtype == 2 ? 4 : 8) == 0;
-    const unsigned grid = warp_grid(rows * (scale_pieces(width) / 2));
+    const unsigned grid = warp_grid(rows * blocks_of(width, 256 * kSpans));
     cudaStream_t st = (cudaStream_t)stream;
     const uint8_t *v = (const uint8_t*)values, *s = (const uint8_t*)scales;
-    if (dtype == 0) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, (int64_t)width, (__nv_bfloat16*)out, out_stride, vector);
-    if (dtype == 1) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, (int64_t)width, (__half*)out, out_stride, vector);
-    if (dtype == 2) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, (int64_t)width, (float*)out, out_stride, vector);
+    if (dtype == 0) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, width, (__nv_bfloat16*)out, out_stride, vector);
+    if (dtype == 1) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, width, (__half*)out, out_stride, vector);
+    if (dtype == 2) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, width, (float*)out, out_stride, vector);
     return check_cuda(cudaGetLastError(), "mx4_dequantise_kernel");
 }
 

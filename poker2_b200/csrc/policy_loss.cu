@@ -18,8 +18,11 @@ using namespace tc;
 
 constexpr int kHands = 256;       // hands of a block
 constexpr int kMostActions = 16;
-constexpr int kMassBlocks = 296;  // two a multiprocessor
+constexpr int kMassBlocks = 592;  // four a multiprocessor
 constexpr int kMassChunk = 2048;
+constexpr int kLossStages = 3;
+constexpr int kLossBlocks = 1024;  // at most
+constexpr int kAlone = 8;         // tiles that one block takes by itself, in one launch (2 launches: 14 us for 6 tiles)
 
 struct LossArgs {
     const void* logits;
@@ -33,7 +36,9 @@ struct LossArgs {
     // scratch: [0] blocks done, then the mass sums, then the loss sums
     unsigned long long* done;
     double *mass, *sums;
+    uint32_t* masks;  // legal actions of every state, a bit each (with mass_parts > 0)
     int mass_parts;
+    uint64_t magic;   // ceil(2^64 / hands)
     float* loss;
     void* grad;
 };
@@ -49,19 +54,35 @@ __device__ __forceinline__ double block_sum(double v, double* area) {
     return sum;
 }
 
-// Sum of the weights of the hands whose state has a legal action: a part for every block, in a fixed order.
+// Sum of the weights of the hands whose state has a legal action: a warp takes a state's hands, kMassChunk at most; a part for
+// every block, in a fixed order.
 __global__ void __launch_bounds__(kHands) loss_mass_kernel(const float* weights, const uint8_t* legal, int64_t states, int hands, int actions,
-                                                           unsigned long long* done, double* mass) {
+                                                           unsigned long long* done, double* mass, uint32_t* masks) {
     __shared__ double area[kHands / 32];
-    const int64_t chunks = (hands + kMassChunk - 1) / kMassChunk;
+    const int lane = threadIdx.x % 32, chunks = (hands + kMassChunk - 1) / kMassChunk;
     double sum = 0.0;
-    for (int64_t job = blockIdx.x; job < states * chunks; job += gridDim.x) {
-        const int64_t state = job / chunks;
-        const int first = (int)(job - state * chunks) * kMassChunk, end = min(hands, first + kMassChunk);
-        bool any = false;
-        for (int a = 0; a < actions; ++a) any |= legal[state * actions + a] != 0;
-        if (!any) continue;
-        for (int h = first + threadIdx.x; h < end; h += kHands) sum += weights ? (double)weights[state * hands + h] : 1.0;
+    for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < states * chunks; job += (int64_t)gridDim.x * 8) {
+        const int64_t state = chunks == 1 ? job : job / chunks;
+        const int first = (int)(job - state * chunks) * kMassChunk, count = min(hands - first, kMassChunk);
+        const uint32_t open = __ballot_sync(~0u, lane < actions && legal[state * actions + min(lane, actions - 1)] != 0);
+        if (lane == 0 && first == 0) masks[state] = open;
+        if (open == 0) continue;
+        if (!weights) {
+            if (lane == 0) sum += (double)count;
+            continue;
+        }
+        const float* w = weights + state * hands + first;
+        double part[4] = {0.0, 0.0, 0.0, 0.0};
+        int h = lane;
+        for (; h + 7 * 32 < count; h += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __ldg(w + h + 32 * i);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part[i % 4] += (double)v[i];
+        }
+        for (; h < count; h += 32) part[0] += (double)w[h];
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
     }
     sum = block_sum(sum, area);
     if (threadIdx.x == 0) {
@@ -79,170 +100,272 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16(v); }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half(v); }
 
-// The probability of action `which` in 64 bits.
-template <int kActions, typename T> __device__ __noinline__ double exact_probability(const T* z, uint32_t open, int which) {
-    double top = -INFINITY, sum = 0.0;
+__device__ __forceinline__ float small_power_of_two(float x) {  // (subnormal results are kept)
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A hand's kActions values from shared memory, in reads as wide as the hands' distance allows (8 fp32 values apart, single reads would
+// meet in four banks).
+template <int kActions, typename T> __device__ __forceinline__ void read_hand(const T* p, float (&v)[kActions]) {
+    constexpr int kBytes = kActions * (int)sizeof(T), kWide = kBytes % 16 == 0 ? 16 : kBytes % 8 == 0 ? 8 : kBytes % 4 == 0 ? 4 : 2;
+    constexpr int kEach = kWide / (int)sizeof(T) > 0 ? kWide / (int)sizeof(T) : 1;
+#pragma unroll
+    for (int i = 0; i < kActions / kEach; ++i) {
+        T part[kEach];
+        if (kWide == 16) *reinterpret_cast<uint4*>(part) = reinterpret_cast<const uint4*>(p)[i];
+        if (kWide == 8) *reinterpret_cast<uint2*>(part) = reinterpret_cast<const uint2*>(p)[i];
+        if (kWide == 4) *reinterpret_cast<uint32_t*>(part) = reinterpret_cast<const uint32_t*>(p)[i];
+        if (kWide == 2) *reinterpret_cast<uint16_t*>(part) = reinterpret_cast<const uint16_t*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) v[i * kEach + j] = as_float(part[j]);
+    }
+}
+template <int kActions, typename T> __device__ __forceinline__ void write_hand(T* p, const float (&v)[kActions]) {
+    constexpr int kBytes = kActions * (int)sizeof(T), kWide = kBytes % 16 == 0 ? 16 : kBytes % 8 == 0 ? 8 : kBytes % 4 == 0 ? 4 : 2;
+    constexpr int kEach = kWide / (int)sizeof(T) > 0 ? kWide / (int)sizeof(T) : 1;
+#pragma unroll
+    for (int i = 0; i < kActions / kEach; ++i) {
+        T part[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) part[j] = from_float<T>(v[i * kEach + j]);
+        if (kWide == 16) reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(part);
+        if (kWide == 8) reinterpret_cast<uint2*>(p)[i] = *reinterpret_cast<const uint2*>(part);
+        if (kWide == 4) reinterpret_cast<uint32_t*>(p)[i] = *reinterpret_cast<const uint32_t*>(part);
+        if (kWide == 2) reinterpret_cast<uint16_t*>(p)[i] = *reinterpret_cast<const uint16_t*>(part);
+    }
+}
+
+__device__ __forceinline__ float log_two(float x) {  // of a positive number (a subnormal one counts as the smallest normal)
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 1.17549435e-38f)));
+    return y;
+}
+
+// Which of the doubtful actions of a hand are free: probabilities so near an end of their interval that 32 bits may put them on the
+// wrong side are compared in 64.  (Masks go in and out: an address taken of the caller's arrays would put them into memory.)
+template <int kActions, typename T>
+__device__ __noinline__ uint32_t settle_hand(const T* z, const float* old, const float* adv, uint32_t open, uint32_t doubtful, double clip) {
+    double top = -INFINITY, total = 0.0;
     for (int a = 0; a < kActions; ++a)
         if (open >> a & 1) top = fmax(top, (double)as_float(z[a]));
     for (int a = 0; a < kActions; ++a)
-        if (open >> a & 1) sum += exp((double)as_float(z[a]) - top);
-    return exp((double)as_float(z[which]) - top) / sum;
+        if (open >> a & 1) total += exp((double)as_float(z[a]) - top);
+    uint32_t free = 0;
+    for (int a = 0; a < kActions; ++a)
+        if (doubtful >> a & 1) {
+            const double exact = exp((double)as_float(z[a]) - top) / total, end = (adv[a] > 0.0f ? 1.0 + clip : 1.0 - clip) * (double)old[a];
+            free |= (adv[a] > 0.0f ? exact <= end : exact >= end) ? 1u << a : 0u;
+        }
+    return free;
 }
 
+// Blocks stay: each takes every gridDim.x-th tile of 256 hands, with the tiles after the present one on their way into the other
+// two of three stages.  The gradient overwrites the logits of its stage and leaves from there.
 template <int kActions, typename T>
 __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_constant__ LossArgs args) {
     extern __shared__ __align__(16) uint8_t area[];
     __shared__ double sums[kHands / 32];
-    __shared__ uint64_t bar_word;
+    __shared__ uint64_t bar_words[kLossStages];
     __shared__ volatile int given_up;
     __shared__ bool last_block;
-    T* z_s = reinterpret_cast<T*>(area);
-    float* old_s = reinterpret_cast<float*>(area + kHands * kActions * sizeof(T));
-    float* adv_s = old_s + kHands * kActions;
-    float* target_s = adv_s + kHands * kActions;
-    float* weight_s = target_s + kHands * kActions;
-    const int64_t first = (int64_t)blockIdx.x * kHands;
-    const int count = (int)(args.total - first < kHands ? args.total - first : kHands);
-    const bool bulk = args.bulk && count == kHands;
-    const uint32_t bar = smem_addr(&bar_word);
+    constexpr int kStage = kHands * (kActions * ((int)sizeof(T) + 12) + 4), kWords = kHands * kActions * 4, kLogits = kHands * kActions * (int)sizeof(T);
     const int tid = threadIdx.x;
+    const int64_t tiles = (args.total + kHands - 1) / kHands;
+    auto bar = [&](int s) { return smem_addr(bar_words + s); };
+    auto whole = [&](int64_t tile) { return args.bulk && tile < tiles && (tile + 1) * kHands <= args.total; };
+    auto fetch = [&](int64_t tile, int s) {
+        const int64_t first = tile * kHands;
+        const uint32_t at = smem_addr(area) + s * kStage, b = bar(s);
+        mbar_expect(b, kLogits + kWords + (args.old_policy ? 2 * kWords : 0) + (args.weights ? kHands * 4 : 0));
+        bulk_load(at, reinterpret_cast<const T*>(args.logits) + first * kActions, kLogits, b);
+        bulk_load(at + kLogits + 2 * kWords, args.target + first * kActions, kWords, b);
+        if (args.old_policy) {
+            bulk_load(at + kLogits, args.old_policy + first * kActions, kWords, b);
+            bulk_load(at + kLogits + kWords, args.advantages + first * kActions, kWords, b);
+        }
+        if (args.weights) bulk_load(at + kLogits + 3 * kWords, args.weights + first, kHands * 4, b);
+    };
     if (tid == 0) {
         given_up = 0;
-        mbar_init(bar, 1);
+        for (int s = 0; s < kLossStages; ++s) mbar_init(bar(s), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (bulk) {
-            constexpr uint32_t words = kHands * kActions * 4, z_bytes = kHands * kActions * sizeof(T);
-            mbar_expect(bar, z_bytes + words + (args.old_policy ? 2 * words : 0) + (args.weights ? kHands * 4 : 0));
-            bulk_load(smem_addr(z_s), reinterpret_cast<const T*>(args.logits) + first * kActions, z_bytes, bar);
-            bulk_load(smem_addr(target_s), args.target + first * kActions, words, bar);
-            if (args.old_policy) {
-                bulk_load(smem_addr(old_s), args.old_policy + first * kActions, words, bar);
-                bulk_load(smem_addr(adv_s), args.advantages + first * kActions, words, bar);
-            }
-            if (args.weights) bulk_load(smem_addr(weight_s), args.weights + first, kHands * 4, bar);
-        }
+        for (int s = 0; s < kLossStages - 1; ++s)
+            if (whole(blockIdx.x + (int64_t)s * gridDim.x)) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
     }
-    if (!bulk) {
-        for (int i = tid; i < count * kActions; i += kHands) {
-            z_s[i] = reinterpret_cast<const T*>(args.logits)[first * kActions + i];
-            target_s[i] = args.target[first * kActions + i];
-            if (args.old_policy) {
-                old_s[i] = args.old_policy[first * kActions + i];
-                adv_s[i] = args.advantages[first * kActions + i];
-            }
-        }
-        if (args.weights && tid < count) weight_s[tid] = args.weights[first + tid];
-    }
-    // meanwhile the sum of the weights, and the hand's legal actions
+    // meanwhile the sum of the weights
     double mass = 0.0;
-    for (int i = tid; i < args.mass_parts; i += kHands) mass += args.mass[i];
-    mass = block_sum(mass, sums);  // (a barrier of the block: what the threads copied is there)
-    const float inverse = mass > 0.0 ? (float)(1.0 / mass) : 0.0f;
-    uint32_t open = 0;
-    if (tid < count) {
-        const int64_t state0 = first / args.hands;
-        const int64_t state = state0 + ((int)(first - state0 * args.hands) + tid) / args.hands;
-#pragma unroll
-        for (int a = 0; a < kActions; ++a) open |= (args.legal[state * kActions + a] != 0 ? 1u : 0u) << a;
-    }
-    const bool ok = !bulk || mbar_wait(bar, 0, &given_up);
-    if (!ok && tid == 0) {  // the copies in flight land before the block's memory goes
-        volatile int still = 0;
-        mbar_wait(bar, 0, &still);
-    }
-
-    double loss = 0.0;
-    if (tid < count) {
-        const float weight = args.weights ? weight_s[tid] : 1.0f;
-        T* z_own = z_s + tid * kActions;
-        float p[kActions], d[kActions];
-        float top = -INFINITY;
-#pragma unroll
-        for (int a = 0; a < kActions; ++a) {
-            p[a] = as_float(z_own[a]);
-            if (open >> a & 1) top = fmaxf(top, p[a]);
+    if (args.mass_parts > 0) {
+        for (int i = tid; i < args.mass_parts; i += kHands) mass += args.mass[i];
+    } else {  // a single block, few hands
+        for (int i = tid; i < (int)args.total; i += kHands) {
+            bool open = false;
+            for (int a = 0; a < kActions; ++a) open |= args.legal[i / args.hands * kActions + a] != 0;
+            if (open) mass += args.weights ? (double)args.weights[i] : 1.0;
         }
-        // no legal action, or none that the logits leave, or a hand that does not count: nothing, whatever else is there
-        if (weight != 0.0f && open != 0 && top != -INFINITY) {
-            float total = 0.0f;
-#pragma unroll
-            for (int a = 0; a < kActions; ++a) {
-                d[a] = p[a] - top;
-                p[a] = open >> a & 1 ? expf(d[a]) : 0.0f;
-                total += p[a];
-            }
-            const float log_total = logf(total), rcp = 1.0f / total;
-            float surrogate = 0.0f, divergence = 0.0f, targets = 0.0f, pull = 0.0f;
-            float g[kActions];
-#pragma unroll
-            for (int a = 0; a < kActions; ++a) {
-                p[a] *= rcp;
-                g[a] = 0.0f;
-                if (open >> a & 1) {
-                    const float t = target_s[tid * kActions + a];
-                    targets += t;
-                    if (t > 0.0f) divergence = fmaf(t, logf(t) - (d[a] - log_total), divergence);
-                    if (args.old_policy) {
-                        const float q = old_s[tid * kActions + a], adv = adv_s[tid * kActions + a];
-                        const float low = (float)(1.0 - args.clip) * q, high = (float)(1.0 + args.clip) * q;
-                        bool free = adv > 0.0f ? p[a] <= high : p[a] >= low;
-                        const float border = adv > 0.0f ? high : low;
-                        if (fabsf(p[a] - border) <= border * fmaf(fabsf(d[a]), 1e-7f, 1e-5f)) {
-                            const double exact = exact_probability<kActions>(z_own, open, a);
-                            free = adv > 0.0f ? exact <= (1.0 + args.clip) * (double)q : exact >= (1.0 - args.clip) * (double)q;
-                        }
-                        g[a] = free ? adv : 0.0f;
-                        surrogate = fmaf(free ? p[a] : border, adv, surrogate);
-                        pull = fmaf(g[a], p[a], pull);
-                    }
+    }
+    mass = block_sum(mass, sums);
+    const float inverse = mass > 0.0 ? (float)(1.0 / mass) : 0.0f;
+    const float low_end = (float)(1.0 - args.clip), high_end = (float)(1.0 + args.clip);
+
+    double loss_sum = 0.0;
+    int turn = 0;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
+        const int s = turn % kLossStages;
+        const int64_t first = tile * kHands;
+        const int count = (int)(args.total - first < kHands ? args.total - first : kHands);
+        const bool bulk = whole(tile);
+        uint8_t* const stage = area + s * kStage;
+        T* const z_s = reinterpret_cast<T*>(stage);
+        float* const old_s = reinterpret_cast<float*>(stage + kLogits);
+        float *const adv_s = old_s + kHands * kActions, *const target_s = adv_s + kHands * kActions, *const weight_s = target_s + kHands * kActions;
+        if (!bulk) {
+            for (int i = tid; i < count * kActions; i += kHands) {
+                z_s[i] = reinterpret_cast<const T*>(args.logits)[first * kActions + i];
+                target_s[i] = args.target[first * kActions + i];
+                if (args.old_policy) {
+                    old_s[i] = args.old_policy[first * kActions + i];
+                    adv_s[i] = args.advantages[first * kActions + i];
                 }
             }
-            loss = (double)weight * (double)(args.kl * divergence - surrogate);
-            const float scale = weight * inverse;
+            if (args.weights && tid < count) weight_s[tid] = args.weights[first + tid];
+            __syncthreads();
+        }
+        uint32_t open = 0;
+        if (tid < count) {
+            // the hand's state, a multiplication instead of a division: one too large where the product carries the reciprocal's excess
+            const int64_t at = first + tid;
+            int64_t state = args.magic ? (int64_t)__umul64hi((uint64_t)at, args.magic) : at;
+            state -= state * args.hands > at;
+            if (args.mass_parts > 0) {
+                open = __ldcg(args.masks + state);
+            } else {
+#pragma unroll
+                for (int a = 0; a < kActions; ++a) open |= (args.legal[state * kActions + a] != 0 ? 1u : 0u) << a;
+            }
+        }
+        // (a stage that no bulk copy filled has not moved its barrier: only the last tile of all is one)
+        const bool ok = !bulk || mbar_wait(bar(s), (uint32_t)(turn / kLossStages) & 1, &given_up);
+        if (!ok && tid == 0) let_settle();  // the copies in flight land before the block's memory goes
+
+        if (tid < count) {
+            const float weight = args.weights ? weight_s[tid] : 1.0f;
+            T* const z_own = z_s + tid * kActions;
+            float p[kActions], t[kActions], q[kActions], g[kActions];
+            read_hand<kActions, T>(z_own, p);
+            read_hand<kActions, float>(target_s + tid * kActions, t);
+            if (args.old_policy) {
+                read_hand<kActions, float>(old_s + tid * kActions, q);
+                read_hand<kActions, float>(adv_s + tid * kActions, g);
+            }
+            float top = -INFINITY;
 #pragma unroll
             for (int a = 0; a < kActions; ++a) {
-                const float t = open >> a & 1 ? target_s[tid * kActions + a] : 0.0f;
-                d[a] = scale * (args.kl * (p[a] * targets - t) - p[a] * (g[a] - pull));
+                const bool legal = open & 1u << a;
+                p[a] = legal ? p[a] : -INFINITY;
+                t[a] = legal ? t[a] : 0.0f;
+                q[a] = legal ? q[a] : 1.0f;
+                g[a] = legal ? g[a] : 0.0f;
+                top = fmaxf(top, p[a]);
             }
-        } else {
+            // no legal action, or none that the logits leave, or a hand that does not count: nothing, whatever else is there
+            if (weight != 0.0f && top != -INFINITY) {
+                float d[kActions], total = 0.0f, targets = 0.0f, divergence = 0.0f;
+                // (in powers of two; logarithms are lg2.approx, off by 2^-22, of which the loss averages a whole batch)
 #pragma unroll
-            for (int a = 0; a < kActions; ++a) d[a] = 0.0f;
+                for (int a = 0; a < kActions; ++a) {
+                    d[a] = (p[a] - top) * 1.4426950408889634f;
+                    p[a] = small_power_of_two(d[a]);
+                    total += p[a];
+                    targets += t[a];
+                    const float more = fmaf(t[a], log_two(t[a]) - d[a], divergence);
+                    divergence = t[a] > 0.0f ? more : divergence;
+                }
+                divergence = 0.69314718055994531f * fmaf(targets, log_two(total), divergence);
+                const float rcp = reciprocal(total), scale = weight * inverse, pulled = scale * args.kl;
+                float surrogate = 0.0f, pull = 0.0f;
+                if (args.old_policy) {
+                    uint32_t doubtful = 0;
+#pragma unroll
+                    for (int a = 0; a < kActions; ++a) {
+                        p[a] *= rcp;
+                        q[a] *= g[a] > 0.0f ? high_end : low_end;
+                        // p is off by 1.5e-6 of itself and 1e-7 for every halving below the top, and by its last bits where those are few
+                        doubtful |= fabsf(p[a] - q[a]) <= fmaf(q[a], fmaf(fminf(-d[a], 200.0f), 1e-7f, 2e-6f), 1e-43f) ? 1u << a : 0u;
+                        const float moving = p[a] * g[a], fixed = q[a] * g[a];
+                        const bool free = moving <= fixed;
+                        surrogate += free ? moving : fixed;
+                        d[a] = free ? g[a] : 0.0f;
+                        pull += free ? moving : 0.0f;
+                    }
+                    if (doubtful) {
+                        const uint32_t free = settle_hand<kActions, T>(z_own, old_s + tid * kActions, adv_s + tid * kActions, open, doubtful, args.clip);
+                        surrogate = pull = 0.0f;
+#pragma unroll
+                        for (int a = 0; a < kActions; ++a) {
+                            const bool moves = doubtful >> a & 1 ? free >> a & 1 : p[a] * g[a] <= q[a] * g[a];
+                            surrogate = fmaf(moves ? p[a] : q[a], g[a], surrogate);
+                            d[a] = moves ? g[a] : 0.0f;
+                            pull = fmaf(d[a], p[a], pull);
+                        }
+                    }
+                    const float base = fmaf(pulled, targets, scale * pull);
+#pragma unroll
+                    for (int a = 0; a < kActions; ++a) p[a] = fmaf(p[a], fmaf(-scale, d[a], base), -pulled * t[a]);
+                } else {
+#pragma unroll
+                    for (int a = 0; a < kActions; ++a) p[a] = pulled * fmaf(p[a] * rcp, targets, -t[a]);
+                }
+                loss_sum += (double)weight * (double)(args.kl * divergence - surrogate);
+            } else {
+#pragma unroll
+                for (int a = 0; a < kActions; ++a) p[a] = 0.0f;
+            }
+            if (!ok) loss_sum = __longlong_as_double(0x7FF8000000000000ll);
+            if (args.grad) {
+                if (!ok)
+#pragma unroll
+                    for (int a = 0; a < kActions; ++a) p[a] = __int_as_float(0x7FC00000);
+                write_hand<kActions, T>(z_own, p);
+            }
         }
-        if (args.grad)
-#pragma unroll
-            for (int a = 0; a < kActions; ++a) z_own[a] = from_float<T>(ok ? d[a] : __int_as_float(0x7FC00000));
-    }
-    if (!ok) loss = __longlong_as_double(0x7FF8000000000000ll);
-    loss = block_sum(loss, sums);
-    if (args.grad) {
-        if (bulk) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncthreads();
-            if (tid == 0) {
+        if (bulk) async_fence();
+        __syncthreads();
+        if (bulk && tid == 0) {
+            if (args.grad)
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<T*>(args.grad) + first * kActions),
-                             "r"(smem_addr(z_s)), "r"((uint32_t)(kHands * kActions * sizeof(T)))
+                             "r"(smem_addr(z_s)), "r"((uint32_t)kLogits)
                              : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-        } else {
+            store_commit();
+            store_wait_read<1>();  // the gradient of the tile before has left its stage, which takes the tile after the next
+            const int64_t next = tile + (int64_t)(kLossStages - 1) * gridDim.x;
+            if (whole(next)) fetch(next, (turn + kLossStages - 1) % kLossStages);
+        }
+        if (!bulk && args.grad)
             for (int i = tid; i < count * kActions; i += kHands) reinterpret_cast<T*>(args.grad)[first * kActions + i] = z_s[i];
+        if (!args.bulk) __syncthreads();
+    }
+    loss_sum = block_sum(loss_sum, sums);
+    // the block that comes last adds the parts up, in their order
+    if (gridDim.x == 1) {
+        if (tid == 0) *args.loss = mass > 0.0 ? (float)(loss_sum / mass) : 0.0f;
+    } else {
+        if (tid == 0) {
+            args.sums[blockIdx.x] = loss_sum;
+            __threadfence();
+            last_block = atomicAdd(args.done, 1ull) == gridDim.x - 1;
+        }
+        __syncthreads();
+        if (last_block) {
+            __threadfence();
+            double sum = 0.0;
+            for (int i = tid; i < (int)gridDim.x; i += kHands) sum += __ldcg(args.sums + i);
+            sum = block_sum(sum, sums);
+            if (tid == 0) *args.loss = mass > 0.0 ? (float)(sum / mass) : 0.0f;
         }
     }
-    // the block that comes last adds the parts up, in their order
-    if (tid == 0) {
-        args.sums[blockIdx.x] = loss;
-        __threadfence();
-        last_block = atomicAdd(args.done, 1ull) == gridDim.x - 1;
-    }
-    __syncthreads();
-    if (last_block) {
-        __threadfence();
-        double sum = 0.0;
-        for (int64_t i = tid; i < gridDim.x; i += kHands) sum += __ldcg(args.sums + i);
-        sum = block_sum(sum, sums);
-        if (tid == 0) *args.loss = mass > 0.0 ? (float)(sum / mass) : 0.0f;
-    }
-    if (bulk && args.grad && tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (tid == 0) store_wait();
 }
 
 // grad * factor, the factor on the device
@@ -255,10 +378,12 @@ static SharedLimit g_limit[kMostActions + 1][3];
 
 template <int kActions, typename T> static int launch_loss(const LossArgs& args, int type, cudaStream_t stream) {
     auto* kernel = policy_loss_kernel<kActions, T>;
-    constexpr int shared = kHands * (kActions * (int)(sizeof(T) + 12) + 4);
+    constexpr int shared = kLossStages * kHands * (kActions * (int)(sizeof(T) + 12) + 4);
     int rc = allow_shared(g_limit[kActions][type], (const void*)kernel, shared);
     if (rc) return rc;
-    kernel<<<(unsigned)blocks_of(args.total, kHands), kHands, shared, stream>>>(args);
+    const int64_t tiles = blocks_of(args.total, kHands), fit = (int64_t)sm_count() * (shared <= 56 * 1024 ? 4 : shared <= 75 * 1024 ? 3 : shared <= 113 * 1024 ? 2 : 1);
+    const int64_t blocks = args.mass_parts == 0 ? 1 : tiles < fit ? tiles : fit;
+    kernel<<<(unsigned)(blocks < kLossBlocks ? blocks : kLossBlocks), kHands, shared, stream>>>(args);
     return check_cuda(cudaGetLastError(), "policy_loss_kernel");
 }
 template <typename T, int kActions = kMostActions> static int launch_actions(const LossArgs& args, int actions, int type, cudaStream_t stream) {
@@ -276,7 +401,7 @@ static bool loss_sizes(int64_t states, int32_t hands, int32_t actions) {
 }
 
 extern "C" int64_t p2b_policy_loss_scratch_bytes(int64_t states, int32_t hands) {
-    return loss_sizes(states, hands, 1) ? 8 * (1 + kMassBlocks + blocks_of(states * hands, kHands)) : -1;
+    return loss_sizes(states, hands, 1) ? 8 * (1 + kMassBlocks + kLossBlocks) + blocks_of(states, 2) * 8 : -1;
 }
 
 extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, const float* advantages, const float* target, const uint8_t* legal,
@@ -304,11 +429,15 @@ extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, cons
     args.done = (unsigned long long*)scratch;
     args.mass = (double*)scratch + 1;
     args.sums = args.mass + kMassBlocks;
-    const int64_t jobs = states * blocks_of(hands, kMassChunk);
-    args.mass_parts = (int)(jobs < kMassBlocks ? jobs : kMassBlocks);
-    loss_mass_kernel<<<args.mass_parts, kHands, 0, st>>>(weights, legal, states, hands, actions, args.done, args.mass);
-    int rc = check_cuda(cudaGetLastError(), "loss_mass_kernel");
-    if (rc) return rc;
+    args.masks = (uint32_t*)(args.sums + kLossBlocks);
+    args.magic = hands == 1 ? 0 : ~0ull / (uint64_t)hands + 1;
+    if (args.total > kAlone * kHands) {
+        const int64_t jobs = states * blocks_of(hands, kMassChunk);
+        args.mass_parts = (int)(jobs < 8 * kMassBlocks ? blocks_of(jobs, 8) : kMassBlocks);
+        loss_mass_kernel<<<args.mass_parts, kHands, 0, st>>>(weights, legal, states, hands, actions, args.done, args.mass, args.masks);
+        int rc = check_cuda(cudaGetLastError(), "loss_mass_kernel");
+        if (rc) return rc;
+    }
     if (dtype == 0) return launch_actions<__nv_bfloat16>(args, actions, 0, st);
     if (dtype == 1) return launch_actions<__half>(args, actions, 1, st);
     return launch_actions<float>(args, actions, 2, st);
