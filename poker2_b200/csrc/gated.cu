@@ -84,21 +84,24 @@ __device__ __forceinline__ void finish_hidden(const GatedArgs& args, const Biase
     const bool inside = row < args.rows;
     tmem_load_wait();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float slope;
-        const float2 two_g = unpack<kBf16>(bg[i / 2]), two_u = unpack<kBf16>(bu[i / 2]);
-        const float gate = __uint_as_float(g[i]) + (i % 2 ? two_g.y : two_g.x);
-        const float up = __uint_as_float(u[i]) + (i % 2 ? two_u.y : two_u.x);
-        const float a = activate<kActivation, kMode == kGradHidden>(gate, slope);
+    for (int i = 0; i < 8; ++i) {
+        Two slope;
+        const Two gate = Two(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])) + two_of<kBf16>(bg[i]);
+        const Two up = Two(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])) + two_of<kBf16>(bu[i]);
+        const Two a = activate<kActivation, kMode == kGradHidden>(gate, slope);
         if (kMode == kForward) {
-            v[i] = ok ? a * up : __int_as_float(0x7FC00000);
+            const float2 h = (a * up).apart();
+            v[2 * i] = ok ? h.x : __int_as_float(0x7FC00000);
+            v[2 * i + 1] = ok ? h.y : __int_as_float(0x7FC00000);
         } else {
-            const float2 two = unpack<kBf16>(grad[i / 2]);
-            const float dh = i % 2 ? two.y : two.x;
+            const Two dh = two_of<kBf16>(grad[i]);
+            const float2 dgate = (dh * up * slope).apart(), dup = (dh * a).apart();
             // (zero behind the last row and column, also where x is not finite)
-            const bool counts = inside && col + i < args.hidden;
-            v[i] = !ok ? __int_as_float(0x7FC00000) : counts ? dh * up * slope : 0.0f;
-            v[16 + i] = !ok ? __int_as_float(0x7FC00000) : counts ? dh * a : 0.0f;
+            const bool first = inside && col + 2 * i < args.hidden, second = inside && col + 2 * i + 1 < args.hidden;
+            v[2 * i] = !ok ? __int_as_float(0x7FC00000) : first ? dgate.x : 0.0f;
+            v[2 * i + 1] = !ok ? __int_as_float(0x7FC00000) : second ? dgate.y : 0.0f;
+            v[16 + 2 * i] = !ok ? __int_as_float(0x7FC00000) : first ? dup.x : 0.0f;
+            v[17 + 2 * i] = !ok ? __int_as_float(0x7FC00000) : second ? dup.y : 0.0f;
         }
     }
 }
@@ -531,9 +534,9 @@ __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64
 #pragma unroll
     for (int r = 0; r < kMost; ++r)
         if (lane == r && r < rows) {
-            float slope;
+            Two slope;
             const float gate = g[r] + (bg ? widen<kBf16>(bg[f]) : 0.0f), up = u[r] + (bu ? widen<kBf16>(bu[f]) : 0.0f);
-            h[r * h_stride + f] = narrow<kBf16>(activate<kActivation, false>(gate, slope) * up);
+            h[r * h_stride + f] = narrow<kBf16>(activate<kActivation, false>(Two(gate), slope).apart().x * up);
         }
 }
 

@@ -45,24 +45,66 @@ __device__ __forceinline__ float reciprocal(float x) {
     return y;
 }
 
+// Two fp32 numbers in one register pair: an instruction works on both.
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ explicit Two(float both) : Two(both, both) {}
+    __device__ __forceinline__ float2 apart() const {
+        float2 r;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+        return r;
+    }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+template <bool kBf16> __device__ __forceinline__ Two two_of(uint32_t word) {
+    const float2 f = unpack<kBf16>(word);
+    return Two(f.x, f.y);
+}
+
 // act(z), and act'(z) where asked for.  The normal distribution of the gelu is Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at
 // most), about half the instructions of erff, whose exponential is the density that the slope needs.  The epilogues of the
 // layers last as long as their instructions: with erff a 128 x 128 tile took 14,000 clocks beside 12,300 of products.
-template <int kActivation, bool kSlope> __device__ __forceinline__ float activate(float z, float& slope) {
+template <int kActivation, bool kSlope> __device__ __forceinline__ Two activate(Two z, Two& slope) {
     if (kActivation == kNoActivation) {
-        slope = 1.0f;
+        slope = Two(1.0f);
         return z;
     }
+    const float2 zs = z.apart();
     if (kActivation == kGelu) {
-        const float density = power_of_two(z * z * -0.72134752044448170f);  // exp(-z^2 / 2)
-        const float t = reciprocal(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.0f));
-        const float tail = (((((0.5f * 1.061405429f * t - 0.5f * 1.453152027f) * t + 0.5f * 1.421413741f) * t - 0.5f * 0.284496736f) * t + 0.5f * 0.254829592f) * t) * density;
-        const float below = z < 0.0f ? tail : 1.0f - tail;
-        if (kSlope) slope = fmaf(z * 0.39894228040143268f, density, below);
+        const float2 power = (z * z * Two(-0.72134752044448170f)).apart();
+        const Two density(power_of_two(power.x), power_of_two(power.y));  // exp(-z^2 / 2)
+        const float2 below_t = fma2(Two(fabsf(zs.x), fabsf(zs.y)), Two(0.3275911f * 0.70710678118654752f), Two(1.0f)).apart();
+        const Two t(reciprocal(below_t.x), reciprocal(below_t.y));
+        Two tail = fma2(t, Two(0.5f * 1.061405429f), Two(-0.5f * 1.453152027f));
+        tail = fma2(tail, t, Two(0.5f * 1.421413741f));
+        tail = fma2(tail, t, Two(-0.5f * 0.284496736f));
+        tail = fma2(tail, t, Two(0.5f * 0.254829592f));
+        // half less the tail beyond |z|, with z's sign, on half
+        const float2 middle = fma2(tail * t, density * Two(-1.0f), Two(0.5f)).apart();
+        const Two below = Two(copysignf(middle.x, zs.x), copysignf(middle.y, zs.y)) + Two(0.5f);
+        if (kSlope) slope = fma2(z * Two(0.39894228040143268f), density, below);
         return z * below;
     }
-    const float s = reciprocal(1.0f + power_of_two(z * -1.4426950408889634f));
-    if (kSlope) slope = s * fmaf(z, 1.0f - s, 1.0f);
+    const float2 power = (z * Two(-1.4426950408889634f)).apart();
+    const float2 over = (Two(power_of_two(power.x), power_of_two(power.y)) + Two(1.0f)).apart();
+    const Two s(reciprocal(over.x), reciprocal(over.y));
+    if (kSlope) slope = s * fma2(z, fma2(s, Two(-1.0f), Two(1.0f)), Two(1.0f));
     return z * s;
 }
 

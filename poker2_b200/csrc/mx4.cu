@@ -331,11 +331,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty(acc));
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                float slope;
-                const float2 two = unpack<kBf16>(bias[i / 2]);
-                const float y = activate<kActivation, false>(__uint_as_float(g[i]) + (i % 2 ? two.y : two.x), slope);
-                v[i] = ok ? y : __int_as_float(0x7FC00000);
+            for (int i = 0; i < 16; ++i) {
+                Two slope;
+                const float2 y = activate<kActivation, false>(Two(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])) + two_of<kBf16>(bias[i]), slope).apart();
+                v[2 * i] = ok ? y.x : __int_as_float(0x7FC00000);
+                v[2 * i + 1] = ok ? y.y : __int_as_float(0x7FC00000);
             }
             if (storer) store_wait_read<0>();
             group_sync(1 + quadrant, 128);
@@ -365,6 +365,100 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
         tc_fence_after();
         tmem_free(tmem, kMxTmem);
     }
+}
+
+// Few rows of x as they are: every block quantises them for itself (a chunk of kChunk columns at a time, in shared memory as the
+// values they stand for), a warp takes a column of the product.  One launch, and no 128 rows of which most are empty: at 1 row,
+// 1536 x 1536, the two launches of the general way took 4 + 9 us.
+constexpr int kFewRows = 8;
+constexpr int kChunk = 1024;
+
+template <typename T, int kMost, bool kBf16, int kActivation>
+__global__ void __launch_bounds__(256) mx4_few_kernel(const T* x, int64_t x_stride, int rows, int width, const uint8_t* w_values, const uint8_t* w_scales,
+                                                      const uint16_t* bias, int columns, uint16_t* out, int64_t out_stride, int vector) {
+    __shared__ __align__(16) float values[kMost][kChunk];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = blockIdx.x * 8 + warp;
+    const int blocks = (width + 31) / 32, spans = (width + 255) / 256;
+    const int64_t row_bytes = (int64_t)blocks * 16;
+    const uint8_t* const w = w_values + column * row_bytes;
+    const uint8_t* const scale_at = w_scales + ((int64_t)(column / 128) * spans * 2 + lane / 16) * 512 + column % 32 * 16 + column % 128 / 32 * 4 + lane / 4 % 4;
+    float sum[kMost];
+#pragma unroll
+    for (int r = 0; r < kMost; ++r) sum[r] = 0.0f;
+    for (int first = 0; first < spans; first += kChunk / 256) {
+        uint32_t word[kChunk / 256], byte[kChunk / 256];
+#pragma unroll
+        for (int i = 0; i < kChunk / 256; ++i) {
+            const int col = (first + i) * 256 + lane * 8;
+            const bool there = column < columns && col < blocks * 32;
+            word[i] = there ? __ldg(reinterpret_cast<const uint32_t*>(w + col / 2)) : 0;
+            byte[i] = there ? __ldg(scale_at + (int64_t)(first + i) * 1024) : 0;
+        }
+        if (first > 0) __syncthreads();
+        for (int job = warp; job < rows * (kChunk / 256); job += 8) {
+            const int r = job / (kChunk / 256), i = job % (kChunk / 256), col = (first + i) * 256 + lane * 8;
+            Eight<T> v;
+            if (vector && col + 8 <= width)
+                v.load(x + r * x_stride + col);
+            else
+                v.load_some(x + r * x_stride + col, width - col);
+            uint32_t top = v.top();
+            top = max(top, __shfl_xor_sync(~0u, top, 1));
+            top = max(top, __shfl_xor_sync(~0u, top, 2));
+            const uint32_t b = scale_byte(Eight<T>::magnitude(top));
+            const float inverse = b == 255u ? 0.0f : inverse_scale(b), scale = scale_of(b);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 two = v.pair(j), q = four_bit_values(four_bit_pair(two.x * inverse, two.y * inverse));
+                *reinterpret_cast<float2*>(&values[r][i * 256 + lane * 8 + 2 * j]) = make_float2(q.x * scale, q.y * scale);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kChunk / 256; ++i) {
+            if (first + i >= spans) break;
+            float2 f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[j] = four_bit_values(word[i] >> (8 * j) & 255u);
+                f[j].x *= scale_of(byte[i]), f[j].y *= scale_of(byte[i]);
+            }
+#pragma unroll
+            for (int r = 0; r < kMost; ++r)
+                if (r < rows) {
+                    const float4 a = *reinterpret_cast<const float4*>(&values[r][i * 256 + lane * 8]), b = *reinterpret_cast<const float4*>(&values[r][i * 256 + lane * 8 + 4]);
+                    float part = fmaf(a.x, f[0].x, sum[r]);
+                    part = fmaf(a.y, f[0].y, part);
+                    part = fmaf(a.z, f[1].x, part);
+                    part = fmaf(a.w, f[1].y, part);
+                    part = fmaf(b.x, f[2].x, part);
+                    part = fmaf(b.y, f[2].y, part);
+                    part = fmaf(b.z, f[3].x, part);
+                    sum[r] = fmaf(b.w, f[3].y, part);
+                }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kMost; ++r)
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) sum[r] += __shfl_xor_sync(~0u, sum[r], o);
+    if (column >= columns) return;
+#pragma unroll
+    for (int r = 0; r < kMost; ++r)
+        if (lane == r && r < rows) {
+            Two slope;
+            out[r * out_stride + column] = narrow<kBf16>(activate<kActivation, false>(Two(sum[r] + (bias ? widen<kBf16>(bias[column]) : 0.0f)), slope).apart().x);
+        }
+}
+
+template <typename T, bool kBf16, int kActivation>
+static int launch_few(const void* x, int64_t x_stride, int rows, int width, const void* w_values, const void* w_scales, const void* bias, int columns, void* out,
+                      int64_t out_stride, cudaStream_t stream) {
+    const int vector = (uintptr_t)x % 16 == 0 && (rows == 1 || x_stride % (16 / (int)sizeof(T)) == 0);
+    auto* kernel = rows == 1 ? mx4_few_kernel<T, 1, kBf16, kActivation> : rows <= 4 ? mx4_few_kernel<T, 4, kBf16, kActivation> : mx4_few_kernel<T, kFewRows, kBf16, kActivation>;
+    kernel<<<(unsigned)blocks_of(columns, 8), 256, 0, stream>>>((const T*)x, x_stride, rows, width, (const uint8_t*)w_values, (const uint8_t*)w_scales,
+                                                               (const uint16_t*)bias, columns, (uint16_t*)out, out_stride, vector);
+    return check_cuda(cudaGetLastError(), "mx4_few_kernel");
 }
 
 static SharedLimit g_limit[2][3];
@@ -436,6 +530,30 @@ extern "C" int p2b_mx4_dequantise(const void* values, const void* scales, int64_
     if (dtype == 1) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, width, (__half*)out, out_stride, vector);
     if (dtype == 2) mx4_dequantise_kernel<<<grid, 256, 0, st>>>(v, s, rows, width, (float*)out, out_stride, vector);
     return check_cuda(cudaGetLastError(), "mx4_dequantise_kernel");
+}
+
+extern "C" int p2b_mx4_few_rows(void) { return kFewRows; }
+
+extern "C" int p2b_mx4_linear_few(const void* x, int64_t x_stride, int32_t x_dtype, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
+                                  int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* stream) {
+    const char* name = "p2b_mx4_linear_few";
+    int rc = check_matrix(name, columns, width);
+    if (rc) return rc;
+    if (rows < 0 || rows > kFewRows || columns < 1) return set_error(P2B_ERR_ARG, "%s: %lld rows and %d columns (0 to %d rows)", name, (long long)rows, columns, kFewRows);
+    if (dtype < 0 || dtype > 1 || x_dtype < 0 || x_dtype > 2) return set_error(P2B_ERR_ARG, "%s: unknown type (x %d, result %d)", name, x_dtype, dtype);
+    if (activation < 0 || activation > 2) return set_error(P2B_ERR_ARG, "%s: unknown activation %d (0 gelu, 1 silu, 2 none)", name, activation);
+    if (rows == 0) return P2B_OK;
+    if (!x || !w_values || !w_scales || !out || x_stride < 0 || (rows > 1 && out_stride < columns))
+        return set_error(P2B_ERR_ARG, "%s: null array or rows that overlap", name);
+    if ((uintptr_t)w_values % 16 || (uintptr_t)w_scales % 16) return set_error(P2B_ERR_ARG, "%s: values and scales must lie on 16-byte boundaries", name);
+    if ((uintptr_t)out % 2 || (uintptr_t)bias % 2 || (uintptr_t)x % (x_dtype == 2 ? 4 : 2)) return set_error(P2B_ERR_ARG, "%s: x, out and bias must lie on their elements' boundaries", name);
+    auto few = [&](auto element) {
+        using T = decltype(element);
+        auto* f = dtype == 0 ? (activation == 0 ? launch_few<T, true, 0> : activation == 1 ? launch_few<T, true, 1> : launch_few<T, true, 2>)
+                             : (activation == 0 ? launch_few<T, false, 0> : activation == 1 ? launch_few<T, false, 1> : launch_few<T, false, 2>);
+        return f(x, x_stride, (int)rows, width, w_values, w_scales, bias, columns, out, out_stride, (cudaStream_t)stream);
+    };
+    return x_dtype == 0 ? few(__nv_bfloat16()) : x_dtype == 1 ? few(__half()) : few(0.0f);
 }
 
 extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,

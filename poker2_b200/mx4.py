@@ -15,6 +15,7 @@ from . import _lib
 
 ACTIVATIONS = {"gelu": 0, "silu": 1, "none": 2}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+FEW_ROWS = 8  # up to so many rows are quantised by the product itself (p2b_mx4_few_rows)
 
 
 @dataclass
@@ -97,6 +98,15 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
         if bias.dim() != 1 or bias.shape[0] != columns or bias.dtype != dtype or bias.get_device() != device:
             raise ValueError("the bias has one entry for each output, in the type of the result and on its device")
         bias = bias.contiguous()
+    if tensor and x.numel() <= FEW_ROWS * width and x.dtype in _TYPES:
+        flat = x if x.dim() == 2 else x.reshape(-1, width)
+        if width > 1 and flat.stride(1) != 1:
+            flat = flat.contiguous()
+        rows = flat.shape[0]
+        out = x.new_empty((rows, columns), dtype=dtype)
+        _lib.call_on(device, "p2b_mx4_linear_few", flat.data_ptr(), flat.stride(0), _TYPES[x.dtype], rows, weight.values.data_ptr(),
+                     weight.scales.data_ptr(), columns, width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, out.data_ptr(), columns)
+        return out if x.dim() == 2 else out.view(*x.shape[:-1], columns)
     a = quantise(x) if tensor else x
     out = a.values.new_empty((*a.shape[:-1], columns), dtype=dtype)
     _lib.call_on(device, "p2b_mx4_linear", a.values.data_ptr(), a.scales.data_ptr(), a.values.shape[0], weight.values.data_ptr(),

@@ -75,7 +75,7 @@ def test_strides_and_shapes(cuda_device):
 
 @pytest.mark.parametrize("activation", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("dtype", TYPES[:2])
-@pytest.mark.parametrize("rows,width,columns", [(1, 1536, 1536), (1, 32, 1), (2, 31, 7), (33, 256, 128), (128, 300, 129), (129, 64, 40),
+@pytest.mark.parametrize("rows,width,columns", [(1, 1536, 1536), (1, 32, 1), (2, 31, 7), (4, 1023, 9), (8, 2720, 130), (8, 1025, 16), (9, 1025, 16), (33, 256, 128), (128, 300, 129), (129, 64, 40),
                                                 (200, 2720, 333), (385, 1000, 257), (600, 513, 2652)])
 def test_linear(cuda_device, rows, width, columns, dtype, activation):
     g = torch.Generator(device=cuda_device).manual_seed(rows + width + columns)
@@ -87,7 +87,14 @@ def test_linear(cuda_device, rows, width, columns, dtype, activation):
     y = mx4.linear(x, q, bias, activation=activation)
     assert y.dtype == dtype and y.shape == (rows, columns)
     refs.assert_within(y, *want)
-    assert torch.equal(mx4.linear(mx4.quantise(x), q, bias, activation=activation, dtype=dtype), y)
+    general = mx4.linear(mx4.quantise(x), q, bias, activation=activation, dtype=dtype)
+    if rows > mx4.FEW_ROWS:
+        assert torch.equal(general, y)
+    else:  # another order of sums
+        refs.assert_within(general, *want)
+        fp32 = mx4.linear(x.float(), q, bias, activation=activation, dtype=dtype)
+        assert torch.equal(fp32, y)
+        assert torch.equal(mx4.linear(x.t().contiguous().t(), q, bias, activation=activation), y)
     if activation == "none":
         refs.assert_within(mx4.linear(x, q), *refs.mx4_linear(refs.mx4_values(x), refs.mx4_values(w), None, activation, dtype))
 
@@ -99,7 +106,12 @@ def test_linear_types_shapes_and_bad_rows(cuda_device):
     assert y.dtype == torch.bfloat16
     assert mx4.linear(x, q, dtype=torch.float16).dtype == torch.float16
     assert torch.equal(mx4.linear(x.view(14, 10, 96), q), y.view(14, 10, 50))
-    assert mx4.linear(x[:0], q).shape == (0, 50) and torch.equal(mx4.linear(x[0], q), y[0])
+    assert mx4.linear(x[:0], q).shape == (0, 50) and mx4.linear(x[:6].view(2, 3, 96), q).shape == (2, 3, 50)
+    assert torch.equal(mx4.linear(x[0], q), mx4.linear(x[:1], q)[0])
+    broken = x[:3].clone()
+    broken[1, 3] = float("inf")
+    few = mx4.linear(broken, q)
+    assert torch.equal(few[[0, 2]], mx4.linear(x[:3], q)[[0, 2]]) and torch.isnan(few[1]).all()
     x[5, 40], x[139, 0] = float("nan"), float("inf")
     bad = mx4.linear(x, q)
     others = torch.ones(140, dtype=torch.bool, device=cuda_device)
@@ -109,8 +121,9 @@ def test_linear_types_shapes_and_bad_rows(cuda_device):
     a = torch.zeros(3, 64, device=cuda_device)
     w = torch.zeros(2, 64, device=cuda_device)
     a[0, 0], a[1, 33], a[2, 40], w[0, 0], w[1, 33], w[1, 40] = 2.0 ** 100, 3.0 * 2.0 ** -100, -1.5, 2.0 ** -90, 2.0 ** 110, 0.5 * 2.0 ** 110
-    got = mx4.linear(a, mx4.quantise(w)).double()
-    assert torch.equal(got, (refs.mx4_values(a) @ refs.mx4_values(w).T).bfloat16().double())
+    for rows in (a, a.repeat(4, 1)):
+        got = mx4.linear(rows, mx4.quantise(w)).double()[:3]
+        assert torch.equal(got, (refs.mx4_values(a) @ refs.mx4_values(w).T).bfloat16().double())
 
 
 def test_streams_and_capture(cuda_device):

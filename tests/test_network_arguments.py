@@ -99,6 +99,7 @@ def _refused(handle, name, **change):
     calls = {
         "p2b_mx4_quantise": dict(x=p, stride=64, rows=4, width=64, dtype=0, values=p, scales=p, stream=None),
         "p2b_mx4_dequantise": dict(values=p, scales=p, rows=4, width=64, dtype=0, out=p, stride=64, stream=None),
+        "p2b_mx4_linear_few": dict(x=p, xs=64, xdtype=0, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
         "p2b_mx4_linear": dict(a=p, sa=p, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
     }
     args = calls[name]
@@ -126,7 +127,17 @@ def test_mx4_linear_refuses(handle, change):
     assert _refused(handle, "p2b_mx4_linear", **change)
 
 
+@pytest.mark.parametrize("change", [dict(rows=-1), dict(rows=9), dict(width=0), dict(columns=0), dict(columns=1 << 30), dict(dtype=2), dict(xdtype=3), dict(xdtype=-1), dict(act=3),
+                                    dict(x=None), dict(w=None), dict(sw=None), dict(out=None), dict(xs=-1), dict(stride=7), dict(w=(8,)), dict(sw=(4,)), dict(x=(1,)),
+                                    dict(xdtype=2, x=(2,)), dict(out=(1,)), dict(bias=(1,))])
+def test_mx4_linear_few_refuses(handle, change):
+    assert _refused(handle, "p2b_mx4_linear_few", **change)
+
+
 def test_mx4_sizes(handle):
+    from poker2_b200 import mx4
+
+    assert handle.p2b_mx4_few_rows() == mx4.FEW_ROWS
     assert handle.p2b_mx4_value_bytes(3, 33) == 96 and handle.p2b_mx4_scale_bytes(129, 257) == 2 * 4 * 512
     assert handle.p2b_mx4_value_bytes(-1, 33) == -1 and handle.p2b_mx4_scale_bytes(1, 0) == -1
     assert handle.p2b_mx4_quantise(None, 0, 0, 64, 0, None, None, None) == 0
@@ -151,6 +162,8 @@ def test_mx4_python_refuses():
         args.update(change)
         with pytest.raises(ValueError):
             mx4.linear(args["x"], args["weight"], args["bias"], activation=args["activation"], dtype=args["dtype"])
+    with pytest.raises(ValueError):
+        mx4.linear(_there(2, 32, dtype=torch.float64), w)
     with pytest.raises(RuntimeError, match="gradient"):
         mx4.linear(_there(2, 32).requires_grad_(True), w)
 
