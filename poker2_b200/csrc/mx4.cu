@@ -186,13 +186,13 @@ __global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* valu
 // y = act(A W^T + bias): tiles of 128 rows x 128 columns, steps of 256 columns of A and W (128 bytes a row), the scales of a step
 // copied from shared to tensor memory by the thread that issues the matrix instructions, in their order.
 struct Mx4Args {
-    CUtensorMap a, w, to;
+    CUtensorMap a, w, to, sa, sw;  // (the maps of the scales: pairs alone)
     const uint8_t *a_scales, *w_scales;
     const void* bias;
     void* out;
     int64_t out_stride, rows;
     int columns, steps, tiles_m, tiles_n;
-    int vector_bias, align_out;
+    int vector_bias, align_out, pairs;
 };
 
 constexpr int kTile = 128;
@@ -367,6 +367,174 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
     }
 }
 
+// Pairs of blocks, 256 x 256 outputs: each block brings its 128 rows of A, 128 of the 256 rows of W, and the scales of the former
+// and of all of the latter: 35 KB a step for 512 clocks of matrix instructions, where the blocks by themselves need 35 KB for
+// 256 and wait for them (436 ns a step; 24576 rows of 1536 x 1536 with a gelu: 64 against 49 us).  The accumulators fill half of tensor memory and the scales a fifth, so there is one set: the
+// epilogue takes them into registers at once, and the products of the next tile begin while it works on those.
+constexpr int kPairStages = 4;
+constexpr int kPairStage = 2 * kTile * 128 + 3 * kScaleBytes + 1024;  // (a stage starts on a 1024-byte boundary)
+constexpr int kPairBytes = 2 * kTile * 128 + 3 * kScaleBytes;
+constexpr int kPairShared = kPairStages * kPairStage + 4 * kPanelBytes + 1024;
+constexpr uint32_t kPairScales = 256;  // column of the scales
+
+template <int kOut, int kActivation>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_pair_kernel(const __grid_constant__ Mx4Args args) {
+    constexpr bool kBf16 = kOut == 0;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t bars[2 * kPairStages + 2];
+    __shared__ uint32_t tmem_at;
+    __shared__ volatile int given_up;
+    const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, bar0 = smem_addr(bars);
+    auto full = [&](int s) { return bar0 + 8 * s; };
+    auto empty = [&](int s) { return bar0 + 8 * (kPairStages + s); };
+    const uint32_t acc_full = bar0 + 16 * kPairStages, acc_empty = acc_full + 8;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = (int)pair_rank(), pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    if (threadIdx.x == 0) {
+        given_up = 0;
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 2 * kMxEpilogueWarps);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMxEpilogueWarps + 1) pair_tmem_alloc(smem_addr(&tmem_at), kMxTmem);
+    tc_fence_before();
+    __syncthreads();
+    pair_sync();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    const int tiles = args.tiles_m * args.tiles_n, steps = args.steps;
+
+    if (warp == kMxEpilogueWarps) {
+        if (lane == 0) {
+            tma_prefetch_map(&args.a);
+            tma_prefetch_map(&args.w);
+            tma_prefetch_map(&args.sa);
+            tma_prefetch_map(&args.sw);
+            uint32_t issued = 0;
+            bool ok = true;
+            for (int64_t tile = pair; ok && tile < tiles; tile += pairs) {
+                const int m = (int)(tile / args.tiles_n) * 2 + rank, n = (int)(tile % args.tiles_n) * 2;  // in 128 rows
+                for (int k = 0; k < steps; ++k, ++issued) {
+                    const int s = (int)(issued % kPairStages);
+                    if (issued >= kPairStages && !pair_wait(empty(s), (issued / kPairStages - 1) & 1, &given_up)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t a = ring + s * kPairStage, sa = a + 2 * kTile * 128, bar = in_leader(full(s));
+                    if (rank == 0) mbar_expect(full(s), 2 * kPairBytes);
+                    pair_load_2d(a, &args.a, k * 128, m * kTile, bar);
+                    pair_load_2d(a + kTile * 128, &args.w, k * 128, (n + rank) * kTile, bar);
+                    // (groups of 128 rows behind the last read as zeros)
+                    pair_load_2d(sa, &args.sa, 0, (m * steps + k) * 8, bar);
+                    for (int i = 0; i < 2; ++i) pair_load_2d(sa + (1 + i) * kScaleBytes, &args.sw, 0, ((n + i) * steps + k) * 8, bar);
+                }
+            }
+            if (!ok) let_settle();
+        }
+        __syncwarp();
+    } else if (warp == kMxEpilogueWarps + 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t used = 0;
+            int turn = 0;
+            bool ok = true;
+            for (int64_t tile = pair; ok && tile < tiles; tile += pairs, ++turn) {
+                if (turn >= 1 && !pair_wait(acc_empty, (uint32_t)(turn - 1) & 1, &given_up)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                for (int k = 0; k < steps; ++k, ++used) {
+                    const int s = (int)(used % kPairStages);
+                    if (!pair_wait(full(s), (used / kPairStages) & 1, &given_up)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = ring + s * kPairStage, w = a + kTile * 128, sa = w + kTile * 128, sw = sa + kScaleBytes;
+                    const uint32_t ta = tmem + kPairScales + (used % kScaleSets) * 24, tw = ta + 8;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {  // a piece of 128 columns of K: four columns for A, eight for the two groups of W
+                        pair_copy_scales(ta + 4 * i, scale_desc(sa + 512 * i));
+                        pair_copy_scales(tw + 8 * i, scale_desc(sw + 512 * i));
+                        pair_copy_scales(tw + 8 * i + 4, scale_desc(sw + kScaleBytes + 512 * i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        pair_mma_mx4(tmem, operand_desc(a + 32 * i, 1024, 16), operand_desc(w + 32 * i, 1024, 16), pair_mx4_idesc(256, i & 1), ta + 4 * (i >> 1),
+                                     tw + 8 * (i >> 1), k > 0 || i > 0);
+                    pair_commit(empty(s));
+                }
+                if (ok) pair_commit(acc_full);
+            }
+            if (!ok) let_settle();
+        }
+        __syncwarp();
+    } else {
+        // A warp has 32 rows and 64 columns: a panel's quarter of its own.
+        const int quadrant = warp % 4, part = warp / 4, r = quadrant * 32 + lane;
+        uint8_t* const panel = raw + (ring - smem_addr(raw)) + kPairStages * kPairStage + part * kPanelBytes;
+        int turn = 0;
+        for (int64_t tile = pair; tile < tiles; tile += pairs, ++turn) {
+            const int64_t row0 = tile / args.tiles_n * 256 + rank * 128 + quadrant * 32;
+            const int col = (int)(tile % args.tiles_n) * 256 + 64 * part;
+            const bool ok = pair_wait(acc_full, (uint32_t)turn & 1, &given_up);
+            tc_fence_after();
+            uint32_t g[2][32];
+            const uint32_t from = tmem + ((uint32_t)(quadrant * 32) << 16) + 64 * part;
+            tmem_load_32(from, g[0]);
+            tmem_load_32(from + 32, g[1]);
+            tmem_load_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                pair_arrive(in_leader(acc_empty));
+                store_wait_read<0>();
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t bias[8];
+                float v[16];
+                load_words(reinterpret_cast<const uint16_t*>(args.bias) + col + 16 * j, args.bias ? args.columns - col - 16 * j : 0, args.vector_bias, bias);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    Two slope;
+                    const uint32_t* two = g[j / 2] + j % 2 * 16 + 2 * i;
+                    const float2 y = activate<kActivation, false>(Two(__uint_as_float(two[0]), __uint_as_float(two[1])) + two_of<kBf16>(bias[i]), slope).apart();
+                    v[2 * i] = ok ? y.x : __int_as_float(0x7FC00000);
+                    v[2 * i + 1] = ok ? y.y : __int_as_float(0x7FC00000);
+                }
+                put_panel<kBf16>(panel, r, 16 * j, v);
+            }
+            if (args.align_out == 16) {
+                async_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    if (row0 < args.rows && col < args.columns) tma_store_2d(&args.to, col, (int)row0, smem_addr(panel) + quadrant * 4096);
+                    store_commit();
+                }
+            } else {
+                __syncwarp();
+                copy_panel(panel, quadrant * 32, 0, 1, args.out, args.out_stride, row0, args.rows, col, args.columns, args.align_out >= 4, lane);
+                __syncwarp();
+            }
+        }
+        if (lane == 0) store_wait();
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    pair_sync();
+    if (warp == kMxEpilogueWarps + 1) {
+        tc_fence_after();
+        pair_tmem_free(tmem, kMxTmem);
+    }
+}
+
 // Few rows of x as they are: every block quantises them for itself (a chunk of kChunk columns at a time, in shared memory as the
 // values they stand for), a warp takes a column of the product.  One launch, and no 128 rows of which most are empty: at 1 row,
 // 1536 x 1536, the two launches of the general way took 4 + 9 us.
@@ -461,9 +629,21 @@ static int launch_few(const void* x, int64_t x_stride, int rows, int width, cons
     return check_cuda(cudaGetLastError(), "mx4_few_kernel");
 }
 
-static SharedLimit g_limit[2][3];
+static SharedLimit g_limit[2][3], g_pair_limit[2][3];
+
+// Blocks by themselves while each gets at most one tile: a pair walks as long as a block and ends with twice the epilogue (1024 rows of
+// 1536 x 2720 with a gelu: 13.4 against 16.7 us); pairs beyond (2048 rows: 16.7 against 19.0; 24576: 71 against 101).
+static bool paired(int64_t rows, int64_t columns) { return blocks_of(rows, kTile) * blocks_of(columns, kTile) > sm_count(); }
 
 template <int kOut, int kActivation> static int launch_linear(const Mx4Args& args, cudaStream_t stream) {
+    if (args.pairs) {
+        auto* kernel = mx4_pair_kernel<kOut, kActivation>;
+        int rc = allow_shared(g_pair_limit[kOut][kActivation], (const void*)kernel, kPairShared);
+        if (rc) return rc;
+        const int tiles = args.tiles_m * args.tiles_n, most = sm_count() / 2;
+        kernel<<<2 * (tiles < most ? tiles : most), kMxThreads, kPairShared, stream>>>(args);
+        return check_cuda(cudaGetLastError(), "mx4_pair_kernel");
+    }
     auto* kernel = mx4_linear_kernel<kOut, kActivation>;
     int rc = allow_shared(g_limit[kOut][kActivation], (const void*)kernel, kMxShared);
     if (rc) return rc;
@@ -561,7 +741,9 @@ extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_
     int rc = check_matrix("p2b_mx4_linear", rows, width);
     if (!rc) rc = check_matrix("p2b_mx4_linear", columns, width);
     if (rc) return rc;
-    if (columns < 1 || blocks_of(rows, kTile) * blocks_of(columns, kTile) > 0x7FFF0000ll)
+    // (tiles and rows of 128 scale bytes are counted in 32 bits)
+    if (columns < 1 || blocks_of(rows, kTile) * blocks_of(columns, kTile) > 0x7FFF0000ll || (blocks_of(rows, kTile) + 1) * blocks_of(width, 256) > 0x0FFF0000ll ||
+        (blocks_of(columns, kTile) + 1) * blocks_of(width, 256) > 0x0FFF0000ll)
         return set_error(P2B_ERR_ARG, "p2b_mx4_linear: %lld x %d outputs are out of range", (long long)rows, columns);
     if (dtype < 0 || dtype > 1) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: unknown type %d (0 bf16, 1 fp16)", dtype);
     if (activation < 0 || activation > 2) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: unknown activation %d (0 gelu, 1 silu, 2 none)", activation);
@@ -581,7 +763,15 @@ extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_
     if (rc) return rc;
     args.a_scales = (const uint8_t*)a_scales, args.w_scales = (const uint8_t*)w_scales, args.bias = bias, args.out = out;
     args.out_stride = out_stride, args.rows = rows, args.columns = columns;
-    args.steps = (int)blocks_of(width, 256), args.tiles_m = (int)blocks_of(rows, kTile), args.tiles_n = (int)blocks_of(columns, kTile);
+    args.steps = (int)blocks_of(width, 256);
+    args.pairs = paired(rows, columns);
+    if (args.pairs) {
+        rc = encode_pieces(&args.sa, a_scales, blocks_of(rows, 128) * args.steps);
+        if (!rc) rc = encode_pieces(&args.sw, w_scales, blocks_of(columns, 128) * args.steps);
+        if (rc) return rc;
+    }
+    const int edge = args.pairs ? 256 : kTile;
+    args.tiles_m = (int)blocks_of(rows, edge), args.tiles_n = (int)blocks_of(columns, edge);
     args.vector_bias = aligned16(bias, 0);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == 0)

@@ -33,4 +33,15 @@ int encode_rows(CUtensorMap* map, const void* base, int element, int64_t columns
     return P2B_OK;
 }
 
+int encode_pieces(CUtensorMap* map, const void* base, int64_t pieces) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return set_error(P2B_ERR_STATE, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = {128, (cuuint64_t)pieces * 8}, strides[1] = {128};
+    const cuuint32_t box[2] = {128, 8}, steps[2] = {1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return set_error(P2B_ERR_ARG, "tensor map of %lld pieces refused (%d)", (long long)pieces, (int)rc);
+    return P2B_OK;
+}
+
 }  // namespace p2b

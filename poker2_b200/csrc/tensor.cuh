@@ -216,6 +216,8 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
 // Tensor map of a row-major matrix: boxes of `box_rows` rows x 128 bytes, 128-byte swizzle.  `element` is the size of an
 // element (2: 16-bit, 1: bytes); base and stride are multiples of 16 bytes (checked by the callers with a message of their own).
 int encode_rows(CUtensorMap* map, const void* base, int element, int64_t columns, int64_t rows, int64_t stride_bytes, int box_rows);
+// The same of packed bytes in pieces of 1024, without a swizzle: box y = 8 * piece.
+int encode_pieces(CUtensorMap* map, const void* base, int64_t pieces);
 
 namespace tc {
 
@@ -236,6 +238,21 @@ __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint
 // 512 bytes of shared memory (32 rows of 16 bytes, no swizzle) to 4 columns, the same for each of the four quadrants.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | (8ull << 32) | (1ull << 46);
+}
+// the pair's: 256 rows x n columns, the scales of its own 128 rows and of all n columns in either block's tensor memory
+__host__ __device__ constexpr uint32_t pair_mx4_idesc(int n, int scale_half) {
+    return ((uint32_t)(2 * scale_half) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (2u << 27) |
+           ((uint32_t)(2 * scale_half) << 29);
+}
+__device__ __forceinline__ void pair_mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void pair_copy_scales(uint32_t dst, uint64_t src) {  // in both blocks, each from its own shared memory
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void tmem_copy_scales(uint32_t dst, uint64_t src) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(dst), "l"(src) : "memory");
