@@ -94,7 +94,7 @@ _VALUE_FUNCS = {"p2b_cfr_scratch_floats": ([_i32, _i32], _i64), "p2b_cfr_default
                 "p2b_cfr_solve_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_solve_block_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_step_scratch_floats": ([_i32, _i32, _i64], _i64),
-                "p2b_gated_few_rows": ([], _i32), "p2b_gated_backward_scratch_bytes": ([_i64, _i32], _i64),
+                "p2b_gated_few_rows": ([], _i32), "p2b_gated_backward_scratch_bytes": ([_i64, _i32, _i32], _i64),
                 "p2b_mx4_few_rows": ([], _i32), "p2b_mx4_value_bytes": ([_i64, _i32], _i64), "p2b_mx4_scale_bytes": ([_i64, _i32], _i64),
                 "p2b_policy_loss_scratch_bytes": ([_i64, _i32], _i64),
                 "p2b_cfr_noalloc_scratch_floats": ([], _i64), "p2b_cfr_path_policy": ([_i32], _i32)}

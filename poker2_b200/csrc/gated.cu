@@ -20,7 +20,9 @@ struct GatedArgs {
     CUtensorMap to, to_wg, to_wu;  // the outputs out, dwg, dwu, where their rows start on 16-byte boundaries
     const void *bias_gate, *bias_up, *grad_h;
     void *out, *dwg, *dwu;   // h, dgate | dup or dx; the gradients of the weights
-    float* sums;             // kGradHidden: column sums of dgate | dup over 32 rows each (NULL: not wanted)
+    float* sums;             // column sums of dgate | dup over 32 rows each, left by kGradHidden for kGradients (NULL: not wanted)
+    void *dbg, *dbu;         // kGradients: the gradients of the biases, from the sums
+    int parts;               // 16-bit numbers that dgate and dup are kept in: 1, or 2 whose sum they are
     int64_t grad_stride, out_stride;
     int64_t rows;            // rows of x
     int width, hidden;       // columns of x, rows of either weight
@@ -109,11 +111,42 @@ __device__ __forceinline__ void split(const float (&v)[32], float (&lower)[16], 
 #pragma unroll
     for (int i = 0; i < 16; ++i) lower[i] = v[i], upper[i] = v[16 + i];
 }
+// v minus its value in 16 bits
+template <bool kBf16> __device__ __forceinline__ void take_rounded(float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float rest = v[i] - widen<kBf16>(narrow<kBf16>(v[i]));
+        v[i] = isfinite(rest) ? rest : 0.0f;  // (the first part says it already)
+    }
+}
 // Column sums of dgate and dup (16 columns each) over the warp's 32 rows.
 __device__ __forceinline__ void sum_hidden(const GatedArgs& args, float (&v)[32], int64_t row, int col, int lane) {
     if (!args.sums || row - lane >= args.rows) return;
     const float sum = lane_sums(v, lane);
     args.sums[(row / 32) * 2 * args.hidden_padded + (lane < 16 ? 0 : args.hidden_padded - 16) + col + lane] = sum;
+}
+
+// Gradients of the biases: the column sums of 32 rows each, added up.  512 threads (16 warps, barrier 5) take 32 columns at a time, a
+// warp every sixteenth of the sums.  kGradients does it while its first tile is on its way.
+template <bool kBf16> __device__ __forceinline__ void add_bias_gradients(const GatedArgs& args, float* area, int block, int blocks) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t sums = (args.rows + 31) / 32;
+    for (int c0 = block * 32; c0 < 2 * args.hidden_padded; c0 += blocks * 32) {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int64_t p = warp; p < sums; p += 16) sum += args.sums[p * 2 * args.hidden_padded + c0 + lane];
+        area[threadIdx.x] = sum;
+        group_sync(5, 512);
+        if (warp == 0) {
+#pragma unroll
+            for (int w = 1; w < 16; ++w) sum += area[w * 32 + lane];
+            const bool second = c0 >= args.hidden_padded;
+            const int f = c0 + lane - (second ? args.hidden_padded : 0);
+            uint16_t* out = reinterpret_cast<uint16_t*>(second ? args.dbu : args.dbg);
+            if (f < args.hidden && out) out[f] = narrow<kBf16>(sum);
+        }
+        group_sync(5, 512);
+    }
 }
 
 // Which tiles a pair takes, the same for its producers, its matrix instructions and its epilogues.  kGradients: first the tiles
@@ -217,6 +250,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
             while (ok && walk.take(args, tile, weights)) {
                 const int across = weights ? args.tiles_w_n : args.tiles_n, steps = weights ? args.steps_w : args.steps;
                 const int m0 = tile / across * 256 + rank * 128, n = tile % across;
+                // kGradients: the reduction goes over dgate (with Wg), dup (with Wu), then the rests of both; or twice over the rows of x
+                const int run = kMode != kGradients ? 0 : (weights ? steps / args.parts : steps / (2 * args.parts)) * kStep;
+                int side = 0, at = 0;
                 for (int k = 0; k < steps; ++k, ++issued) {
                     const int s = (int)(issued % kPairStages);
                     if (issued >= kPairStages && !pair_wait(empty(s), (issued / kPairStages - 1) & 1, &given_up)) {
@@ -230,16 +266,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                         pair_load_2d(b, rank == 0 ? &args.b0 : &args.b1, k * kStep, n * 128, bar);
                     } else if (weights) {
                         for (int c = 0; c < 2; ++c) {
-                            pair_load_2d(a + c * 8192, &args.at, m0 + 64 * c, k * kStep, bar);
-                            pair_load_2d(b + c * 8192, &args.bt, n * 256 + rank * 128 + 64 * c, k * kStep, bar);
+                            pair_load_2d(a + c * 8192, &args.at, m0 + 64 * c + 2 * side * args.hidden_padded, at, bar);
+                            pair_load_2d(b + c * 8192, &args.bt, n * 256 + rank * 128 + 64 * c, at, bar);
                         }
                     } else {
-                        const bool second = 2 * k >= steps;
-                        const int f0 = (second ? k - steps / 2 : k) * kStep;
-                        pair_load_2d(a, &args.a, f0 + (second ? args.hidden_padded : 0), m0, bar);
+                        pair_load_2d(a, &args.a, at + side * args.hidden_padded, m0, bar);
                         for (int c = 0; c < 2; ++c)
-                            pair_load_2d(b + c * 8192, second ? &args.b1 : &args.b0, n * 256 + rank * 128 + 64 * c, f0, bar);
+                            pair_load_2d(b + c * 8192, side & 1 ? &args.b1 : &args.b0, n * 256 + rank * 128 + 64 * c, at, bar);
                     }
+                    at += kStep;
+                    if (kMode == kGradients && at == run) at = 0, ++side;
                 }
             }
             if (!ok) let_settle();
@@ -285,6 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
         const int quadrant = warp % 4, part = warp / 4, r = quadrant * 32 + lane;
         const bool storer = part == 0 && lane == 0;
         const uint32_t lanes = (uint32_t)(quadrant * 32) << 16;
+        if (kMode == kGradients && args.sums) add_bias_gradients<kBf16>(args, reinterpret_cast<float*>(panels), blockIdx.x, gridDim.x);
         for (int turn = 0; walk.take(args, tile, weights); ++turn) {
             const int across = weights ? args.tiles_w_n : args.tiles_n, n = tile % across, acc = turn & 1;
             const int64_t row = (int64_t)(tile / across) * 256 + rank * 128 + r, row0 = row - lane;
@@ -357,6 +394,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                         for (int p = 0; p < (kMode == kGradients ? 2 : 1); ++p)
                             copy_panel(panels + (kMode == kForward ? j : p) * kPanelBytes, quadrant * 32, part, 4, out, stride, first, rows, col + 64 * p, columns,
                                        alignment >= 4, lane);
+                }
+                if (kMode == kGradHidden && args.parts == 2) {  // what the rounding left, behind dgate | dup
+                    float lower[16], upper[16];
+                    split(v, lower, upper);
+                    take_rounded<kBf16>(lower);
+                    take_rounded<kBf16>(upper);
+                    if (storer) store_wait_read<0>();
+                    group_sync(1 + quadrant, 128);
+                    put_panel<kBf16>(panels, r, 16 * part, lower);
+                    put_panel<kBf16>(panels + kPanelBytes, r, 16 * part, upper);
+                    async_fence();
+                    group_sync(1 + quadrant, 128);
+                    if (storer) {
+                        const uint32_t src = smem_addr(panels) + quadrant * 4096;
+                        if (first < rows) {
+                            tma_store_2d(map, 2 * args.hidden_padded + col, (int)first, src);
+                            tma_store_2d(map, 3 * args.hidden_padded + col, (int)first, src + kPanelBytes);
+                        }
+                        store_commit();
+                    }
                 }
                 if (kMode == kGradHidden) sum_hidden(args, v, row, n * 128 + 64 * j + 16 * part, lane);
             }
@@ -470,6 +527,12 @@ __global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constan
                 } else {
                     store_row<kBf16>(args.out, row * args.out_stride + col, lower, 16, 16);
                     store_row<kBf16>(args.out, row * args.out_stride + args.hidden_padded + col, upper, 16, 16);
+                    if (args.parts == 2) {
+                        take_rounded<kBf16>(lower);
+                        take_rounded<kBf16>(upper);
+                        store_row<kBf16>(args.out, row * args.out_stride + 2 * args.hidden_padded + col, lower, 16, 16);
+                        store_row<kBf16>(args.out, row * args.out_stride + 3 * args.hidden_padded + col, upper, 16, 16);
+                    }
                 }
             }
             if (kMode == kGradHidden) sum_hidden(args, v, row, col, lane);
@@ -540,23 +603,10 @@ __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64
         }
 }
 
-// Gradients of the biases: the column sums of 32 rows each, added up.  A block takes 32 columns, a warp every eighth part.
-template <bool kBf16>
-__global__ void __launch_bounds__(256) bias_gradient_kernel(const float* sums, int64_t parts, int hidden, int hidden_padded, uint16_t* gate, uint16_t* up) {
-    __shared__ float part[8][32];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int64_t p = warp; p < parts; p += 8) sum += sums[p * 2 * hidden_padded + c];
-    part[warp][lane] = sum;
-    __syncthreads();
-    if (warp > 0) return;
-#pragma unroll
-    for (int w = 1; w < 8; ++w) sum += part[w][lane];
-    const bool second = c >= hidden_padded;
-    const int f = second ? c - hidden_padded : c;
-    uint16_t* out = second ? up : gate;
-    if (f < hidden && out) out[f] = narrow<kBf16>(sum);
+// (by itself where no other gradient is wanted)
+template <bool kBf16> __global__ void __launch_bounds__(512) bias_gradient_kernel(const __grid_constant__ GatedArgs args) {
+    __shared__ float area[512];
+    add_bias_gradients<kBf16>(args, area, blockIdx.x, gridDim.x);
 }
 
 static SharedLimit g_pair_limit[3][2][2], g_slim_limit[2][2][2];
@@ -660,10 +710,15 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
     return rc ? rc : launch_hidden<kForward>(args, slim, bf16, activation, st);
 }
 
-extern "C" int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t hidden) {
-    if (rows < 0 || rows > kMostRows || hidden < 1 || hidden > kMostColumns) return -1;
+// dgate and dup are rounded to 16 bits on their way into the products, which makes the gradients' error 1.4 times that of their
+// last rounding alone.  Where the products take no longer than their launch, two 16-bit numbers carry each (0.4 us for 64 rows of
+// 2048 x 2048), and the last rounding is all.
+static int parts_of(int64_t rows, int64_t width, int64_t hidden) { return rows * hidden <= (1ll << 28) / width ? 2 : 1; }
+
+extern "C" int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t width, int32_t hidden) {
+    if (rows < 0 || rows > kMostRows || width < 1 || width > kMostColumns || hidden < 1 || hidden > kMostColumns) return -1;
     const int64_t columns = 2 * blocks_of(hidden, 128) * 128;
-    return 2 * rows * columns + 4 * columns * blocks_of(rows, 32);  // dgate | dup, their column sums
+    return 2 * rows * columns * parts_of(rows, width, hidden) + 4 * columns * blocks_of(rows, 32);  // dgate | dup, their column sums
 }
 
 extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride,
@@ -684,9 +739,9 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     if (dx && rows > 1 && dx_stride < width) return set_error(P2B_ERR_ARG, "p2b_gated_backward: rows of dx overlap");
     if (!aligned16(x, rows > 1 ? x_stride : 0) || !aligned16(wg, hidden > 1 ? wg_stride : 0) || !aligned16(wu, hidden > 1 ? wu_stride : 0))
         return set_error(P2B_ERR_ARG, "p2b_gated_backward: rows of x and of the weights must start on 16-byte boundaries");
-    if (!scratch || ((uintptr_t)scratch % 16) != 0 || scratch_bytes < p2b_gated_backward_scratch_bytes(rows, hidden))
+    if (!scratch || ((uintptr_t)scratch % 16) != 0 || scratch_bytes < p2b_gated_backward_scratch_bytes(rows, width, hidden))
         return set_error(P2B_ERR_ARG, "p2b_gated_backward: scratch of %lld bytes on a 16-byte boundary is needed",
-                         (long long)p2b_gated_backward_scratch_bytes(rows, hidden));
+                         (long long)p2b_gated_backward_scratch_bytes(rows, width, hidden));
     const bool bf16 = dtype == 0;
     const int64_t whole = blocks_of(width, 8) * 8;
     if (rows == 1) x_stride = whole;
@@ -694,46 +749,50 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     GatedArgs args{};
     args.rows = rows, args.width = width, args.hidden = hidden;
     args.hidden_padded = (int)blocks_of(hidden, 128) * 128;
-    const int64_t columns = 2 * (int64_t)args.hidden_padded;
+    args.parts = parts_of(rows, width, hidden);
+    const int64_t columns = 2 * (int64_t)args.hidden_padded, wide = columns * args.parts;
+    if (dbg || dbu) args.sums = (float*)((char*)scratch + 2 * rows * wide);
     GatedArgs next = args;
     args.bias_gate = bg, args.bias_up = bu, args.grad_h = grad_h, args.grad_stride = grad_stride;
     args.vector_in = aligned16(grad_h, rows > 1 ? grad_stride : 0), args.vector_bias = aligned16(bg, 0) && aligned16(bu, 0);
-    args.out = scratch, args.out_stride = columns;
-    args.sums = dbg || dbu ? (float*)((char*)scratch + 2 * rows * columns) : nullptr;
+    args.out = scratch, args.out_stride = wide;
     const bool slim = slim_tiles(rows, args.hidden_padded);
     rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
     // every column of the work space is written, those behind the last hidden unit as zeros
     args.tiles_n = args.hidden_padded / (slim ? 32 : 128);
     args.tiles = (int)blocks_of(rows, slim ? kRows : 256) * args.tiles_n;
     args.align_out = 16;
-    if (!rc && !slim) rc = encode_rows(&args.to, scratch, 2, columns, rows, 2 * columns, 32);
+    if (!rc && !slim) rc = encode_rows(&args.to, scratch, 2, wide, rows, 2 * wide, 32);
     if (!rc) rc = launch_hidden<kGradHidden>(args, slim, bf16, activation, st);
     if (rc) return rc;
     if (dx || dwg || dwu) {
         next.out = dx, next.out_stride = dx_stride, next.align_out = row_alignment(dx, rows > 1 ? dx_stride : 0);
         next.dwg = dwg, next.dwu = dwu, next.align_w = row_alignment((const void*)((uintptr_t)dwg | (uintptr_t)dwu), hidden > 1 ? width : 0);
-        rc = encode_rows(&next.a, scratch, 2, columns, rows, 2 * columns, kRows);
+        next.dbg = dbg, next.dbu = dbu;
+        rc = encode_rows(&next.a, scratch, 2, wide, rows, 2 * wide, kRows);
         if (!rc) rc = encode_rows(&next.b0, wg, 2, width, hidden, 2 * wg_stride, kStep);
         if (!rc) rc = encode_rows(&next.b1, wu, 2, width, hidden, 2 * wu_stride, kStep);
-        if (!rc) rc = encode_rows(&next.at, scratch, 2, columns, rows, 2 * columns, kStep);
+        if (!rc) rc = encode_rows(&next.at, scratch, 2, wide, rows, 2 * wide, kStep);
         if (!rc) rc = encode_rows(&next.bt, x, 2, width, rows, 2 * x_stride, kStep);
         if (!rc && dx && next.align_out == 16) rc = encode_rows(&next.to, dx, 2, width, rows, 2 * (rows > 1 ? dx_stride : whole), 32);
         for (int i = 0; i < 2; ++i)
             if (!rc && (i ? dwu : dwg) && next.align_w == 16)
                 rc = encode_rows(i ? &next.to_wu : &next.to_wg, i ? dwu : dwg, 2, width, hidden, 2 * (hidden > 1 ? (int64_t)width : whole), 32);
         if (rc) return rc;
-        next.steps = 2 * (int)blocks_of(hidden, kStep);
-        next.steps_w = (int)blocks_of(rows, kStep);
+        next.steps = 2 * args.parts * (int)blocks_of(hidden, kStep);
+        next.steps_w = args.parts * (int)blocks_of(rows, kStep);
         next.tiles_n = next.tiles_w_n = (int)blocks_of(width, 256);
         next.tiles = dx ? (int)blocks_of(rows, 256) * next.tiles_n : 0;
         next.tiles_w = dwg || dwu ? (int)(columns / 256) * next.tiles_w_n : 0;
         next.ahead = (next.steps_w + next.steps / 2) / next.steps;
         rc = bf16 ? launch_pairs<kGradients, true, 0>(next, st) : launch_pairs<kGradients, false, 0>(next, st);
-        if (rc) return rc;
-    }
-    if (args.sums) {
-        auto* kernel = bf16 ? bias_gradient_kernel<true> : bias_gradient_kernel<false>;
-        kernel<<<(unsigned)(columns / 32), 256, 0, st>>>(args.sums, blocks_of(rows, 32), hidden, args.hidden_padded, (uint16_t*)dbg, (uint16_t*)dbu);
+    } else if (args.sums) {
+        next.dbg = dbg, next.dbu = dbu;
+        const unsigned blocks = (unsigned)(columns / 32);
+        if (bf16)
+            bias_gradient_kernel<true><<<blocks, 512, 0, st>>>(next);
+        else
+            bias_gradient_kernel<false><<<blocks, 512, 0, st>>>(next);
         rc = check_cuda(cudaGetLastError(), "bias_gradient_kernel");
     }
     return rc;

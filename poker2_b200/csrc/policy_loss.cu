@@ -401,6 +401,7 @@ static bool loss_sizes(int64_t states, int32_t hands, int32_t actions) {
 }
 
 extern "C" int64_t p2b_policy_loss_scratch_bytes(int64_t states, int32_t hands) {
+    if (loss_sizes(states, hands, 1) && states * hands <= kAlone * kHands) return 0;
     return loss_sizes(states, hands, 1) ? 8 * (1 + kMassBlocks + kLossBlocks) + blocks_of(states, 2) * 8 : -1;
 }
 
@@ -412,9 +413,10 @@ extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, cons
         return set_error(P2B_ERR_ARG, "%s: %lld states of %d hands and %d actions are out of range (1 to %d actions)", name, (long long)states, hands, actions, kMostActions);
     if (dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "%s: unknown type %d (0 bf16, 1 fp16, 2 fp32)", name, dtype);
     if (!(clip >= 0.0 && clip < 1.0) || !(kl >= 0.0f && kl <= 3.4028234e38f)) return set_error(P2B_ERR_ARG, "%s: clip lies in [0, 1), kl is not negative", name);
-    if (!loss || !scratch || scratch_bytes < p2b_policy_loss_scratch_bytes(states, hands) || (uintptr_t)scratch % 8)
+    const int64_t bytes = p2b_policy_loss_scratch_bytes(states, hands);
+    if (!loss || (bytes > 0 && !scratch) || scratch_bytes < bytes || (uintptr_t)scratch % 8)
         return set_error(P2B_ERR_ARG, "%s: loss and scratch of %lld bytes on an 8-byte boundary are needed", name,
-                         (long long)p2b_policy_loss_scratch_bytes(states, hands));
+                         (long long)bytes);
     if ((old_policy == nullptr) != (advantages == nullptr)) return set_error(P2B_ERR_ARG, "%s: the old policy and the advantages come together", name);
     if (states > 0 && (!logits || !target || !legal)) return set_error(P2B_ERR_ARG, "%s: null array", name);
     const int size = dtype == 2 ? 4 : 2;

@@ -71,7 +71,7 @@ def _backward(grad_h, x, gate_weight, up_weight, gate_bias, up_bias, act, needs)
     xr, gw, uw, gh = _lib.wide_rows(xr), _lib.wide_rows(gate_weight), _lib.wide_rows(up_weight), _lib.plain_rows(gh)
     gb = None if gate_bias is None else gate_bias.contiguous()
     ub = None if up_bias is None else up_bias.contiguous()
-    size = _lib.lib().p2b_gated_backward_scratch_bytes(rows, hidden)
+    size = _lib.lib().p2b_gated_backward_scratch_bytes(rows, width, hidden)
     scratch = new((max(size, 16) // 2,))
     _lib.call_on(x.get_device(), "p2b_gated_backward", gh.data_ptr(), gh.stride(0), xr.data_ptr(), xr.stride(0), gw.data_ptr(), gw.stride(0),
                  uw.data_ptr(), uw.stride(0), p(gb), p(ub), rows, width, hidden, _TYPES[x.dtype], act, p(dx), width, p(dwg), p(dwu), p(dbg),

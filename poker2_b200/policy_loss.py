@@ -96,9 +96,9 @@ def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, with_
     grad = logits.new_empty((states, hands, actions)) if with_grad else None
     p = _lib.ptr
     size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
-    scratch = target.new_empty((size // 4,))
+    scratch = target.new_empty((size // 4,)) if size else None
     _lib.call_on(logits.get_device(), "p2b_policy_loss", logits.data_ptr(), p(old_policy), p(advantages), target.data_ptr(), legal.data_ptr(),
-                 p(weights), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(), p(grad), scratch.data_ptr(), size)
+                 p(weights), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(), p(grad), p(scratch), size)
     return loss, grad
 
 

@@ -55,7 +55,8 @@ def test_gated_addresses_off_their_boundaries_are_refused(handle):
     assert handle.p2b_gated_backward(*_gated_backward(p, scratch=p + 4)) == -1
     assert handle.p2b_gated_forward(*_gated_forward(None, rows=0, wg=p, wu=p)) == 0  # no rows: nothing to do
     assert handle.p2b_gated_few_rows() == gated.FEW_ROWS
-    assert handle.p2b_gated_backward_scratch_bytes(-1, 8) == -1 and handle.p2b_gated_backward_scratch_bytes(8, 0) == -1
+    for sizes in ((-1, 8, 8), (8, 0, 8), (8, 8, 0)):
+        assert handle.p2b_gated_backward_scratch_bytes(*sizes) == -1
 
 
 def test_gated_linear_wants_the_gpu():
@@ -175,8 +176,8 @@ def _loss(p, **change):
 
 
 @pytest.mark.parametrize("change", [dict(states=-1), dict(states=1 << 40), dict(hands=0), dict(actions=0), dict(actions=17), dict(dtype=3), dict(clip=1.0), dict(clip=-0.1),
-                                    dict(clip=float("nan")), dict(kl=-1.0), dict(kl=float("inf")), dict(kl=float("nan")), dict(loss=None), dict(scratch=None),
-                                    dict(size=8), dict(scratch=(4,)), dict(old=None), dict(adv=None), dict(logits=None), dict(target=None), dict(legal=None),
+                                    dict(clip=float("nan")), dict(kl=-1.0), dict(kl=float("inf")), dict(kl=float("nan")), dict(loss=None), dict(states=3000, scratch=None),
+                                    dict(states=3000, size=8), dict(states=3000, scratch=(4,)), dict(old=None), dict(adv=None), dict(logits=None), dict(target=None), dict(legal=None),
                                     dict(logits=(1,)), dict(old=(2,)), dict(target=(1,)), dict(weights=(2,)), dict(grad=(1,)), dict(loss=(2,)),
                                     dict(dtype=2, logits=(2,))])
 def test_policy_loss_refuses(handle, change):
