@@ -245,7 +245,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
             tma_prefetch_map(&args.a);
             tma_prefetch_map(&args.b0);
             tma_prefetch_map(&args.b1);
-            uint32_t issued = 0;
+            // (the thread that issues the copies sets the pace of the products: stages and coordinates are counted, not divided)
+            const uint32_t leader_full = in_leader(full(0));
+            int s = 0;
+            uint32_t phase = 1;  // (the stages begin empty)
             bool ok = true;
             while (ok && walk.take(args, tile, weights)) {
                 const int across = weights ? args.tiles_w_n : args.tiles_n, steps = weights ? args.steps_w : args.steps;
@@ -253,17 +256,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                 // kGradients: the reduction goes over dgate (with Wg), dup (with Wu), then the rests of both; or twice over the rows of x
                 const int run = kMode != kGradients ? 0 : (weights ? steps / args.parts : steps / (2 * args.parts)) * kStep;
                 int side = 0, at = 0;
-                for (int k = 0; k < steps; ++k, ++issued) {
-                    const int s = (int)(issued % kPairStages);
-                    if (issued >= kPairStages && !pair_wait(empty(s), (issued / kPairStages - 1) & 1, &given_up)) {
+                for (int k = 0; k < steps; ++k) {
+                    if (!pair_wait(empty(s), phase, &given_up)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t a = ring + s * kPairStage, b = a + kRows * 128, bar = in_leader(full(s));
+                    const uint32_t a = ring + s * kPairStage, b = a + kRows * 128, bar = leader_full + 8 * s;
                     if (rank == 0) mbar_expect(full(s), 2 * kPairStage);
                     if (kMode != kGradients) {
-                        pair_load_2d(a, &args.a, k * kStep, m0, bar);
-                        pair_load_2d(b, rank == 0 ? &args.b0 : &args.b1, k * kStep, n * 128, bar);
+                        pair_load_2d(a, &args.a, at, m0, bar);
+                        pair_load_2d(b, rank == 0 ? &args.b0 : &args.b1, at, n * 128, bar);
                     } else if (weights) {
                         for (int c = 0; c < 2; ++c) {
                             pair_load_2d(a + c * 8192, &args.at, m0 + 64 * c + 2 * side * args.hidden_padded, at, bar);
@@ -276,6 +278,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                     }
                     at += kStep;
                     if (kMode == kGradients && at == run) at = 0, ++side;
+                    if (++s == kPairStages) s = 0, phase ^= 1;
                 }
             }
             if (!ok) let_settle();
@@ -283,8 +286,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
         __syncwarp();
     } else if (warp == kEpilogueWarps + 1) {
         if (lane == 0 && rank == 0) {
-            uint32_t used = 0;
-            int turn = 0;
+            int s = 0, turn = 0;
+            uint32_t phase = 0;
             bool ok = true;
             for (; ok && walk.take(args, tile, weights); ++turn) {
                 const int acc = turn & 1, steps = weights ? args.steps_w : args.steps;
@@ -294,22 +297,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                 }
                 tc_fence_after();
                 const uint32_t idesc = f16_idesc(kBf16, weights, kMode == kGradients, 256, 256);
-                for (int k = 0; k < steps; ++k, ++used) {
-                    const int s = (int)(used % kPairStages);
-                    if (!pair_wait(full(s), (used / kPairStages) & 1, &given_up)) {
+                // rows along the reduction: 32 bytes on within the swizzled row, else 16 rows of 128 bytes
+                const uint64_t a0 = weights ? operand_desc(ring, 1024, 8192) : operand_desc(ring, 1024, 16);
+                const uint64_t b0 = kMode == kGradients ? operand_desc(ring + kRows * 128, 1024, 8192) : operand_desc(ring + kRows * 128, 1024, 16);
+                const uint32_t a_on = weights ? 2048 >> 4 : 32 >> 4, b_on = kMode == kGradients ? 2048 >> 4 : 32 >> 4;
+                uint32_t add = 0;
+                for (int k = 0; k < steps; ++k) {
+                    if (!pair_wait(full(s), phase, &given_up)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = ring + s * kPairStage, b = a + kRows * 128;
+                    const uint64_t da = a0 + s * (kPairStage >> 4), db = b0 + s * (kPairStage >> 4);
 #pragma unroll
                     for (int i = 0; i < kStep / 16; ++i) {
-                        // rows along the reduction: 32 bytes on within the swizzled row, else 16 rows of 128 bytes
-                        const uint64_t da = weights ? operand_desc(a + 2048 * i, 1024, 8192) : operand_desc(a + 32 * i, 1024, 16);
-                        const uint64_t db = kMode == kGradients ? operand_desc(b + 2048 * i, 1024, 8192) : operand_desc(b + 32 * i, 1024, 16);
-                        pair_mma_f16(tmem + acc * 256, da, db, idesc, k > 0 || i > 0);
+                        pair_mma_f16(tmem + acc * 256, da + i * a_on, db + i * b_on, idesc, add);
+                        add = 1;
                     }
                     pair_commit(empty(s));
+                    if (++s == kPairStages) s = 0, phase ^= 1;
                 }
                 if (ok) pair_commit(acc_full(acc));
             }

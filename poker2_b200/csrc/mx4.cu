@@ -210,7 +210,7 @@ template <int kOut, int kActivation>  // kOut 0 bf16, 1 fp16
 __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_constant__ Mx4Args args) {
     constexpr bool kBf16 = kOut == 0;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t bars[2 * kMxStages + 5];
+    __shared__ uint64_t bars[2 * kMxStages + 4];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int given_up;
     const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u, bar0 = smem_addr(bars);
@@ -218,7 +218,6 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
     auto empty = [&](int s) { return bar0 + 8 * (kMxStages + s); };
     auto acc_full = [&](int s) { return bar0 + 8 * (2 * kMxStages + s); };
     auto acc_empty = [&](int s) { return bar0 + 8 * (2 * kMxStages + 2 + s); };
-    const uint32_t last = bar0 + 8 * (2 * kMxStages + 4);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         given_up = 0;
@@ -230,7 +229,6 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
             mbar_init(acc_full(s), 1);
             mbar_init(acc_empty(s), kMxEpilogueWarps / 2);
         }
-        mbar_init(last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMxEpilogueWarps + 1) tmem_alloc(smem_addr(&tmem_at), kMxTmem);
@@ -244,13 +242,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
         if (lane == 0) {
             tma_prefetch_map(&args.a);
             tma_prefetch_map(&args.w);
-            int64_t issued = 0;
+            int s = 0;
+            uint32_t phase = 1;  // (the stages begin empty)
             bool ok = true;
             for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
                 const int m = (int)(tile / args.tiles_n), n = (int)(tile % args.tiles_n);
-                for (int k = 0; k < steps; ++k, ++issued) {
-                    const int s = (int)(issued % kMxStages);
-                    if (issued >= kMxStages && !mbar_wait(empty(s), (uint32_t)(issued / kMxStages - 1) & 1, &given_up)) {
+                for (int k = 0; k < steps; ++k) {
+                    if (!mbar_wait(empty(s), phase, &given_up)) {
                         ok = false;
                         break;
                     }
@@ -260,19 +258,16 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
                     tma_load_2d(a + kTile * 128, &args.w, k * 128, n * kTile, full(s));
                     bulk_load(a + 2 * kTile * 128, args.a_scales + ((int64_t)m * steps + k) * kScaleBytes, kScaleBytes, full(s));
                     bulk_load(a + 2 * kTile * 128 + kScaleBytes, args.w_scales + ((int64_t)n * steps + k) * kScaleBytes, kScaleBytes, full(s));
+                    if (++s == kMxStages) s = 0, phase ^= 1;
                 }
             }
-            if (!ok)  // the copies in flight land before the block's memory goes
-                for (int64_t i = issued > kMxStages ? issued - kMxStages : 0; i < issued; ++i) {
-                    volatile int still = 0;
-                    mbar_wait(full((int)(i % kMxStages)), (uint32_t)(i / kMxStages) & 1, &still);
-                }
+            if (!ok) let_settle();  // the copies in flight land before the block's memory goes
         }
         __syncwarp();
     } else if (warp == kMxEpilogueWarps + 1) {
         if (lane == 0) {
-            int64_t used = 0;
-            int turn = 0;
+            uint32_t used = 0, phase = 0;
+            int s = 0, turn = 0;
             bool ok = true;
             for (int64_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++turn) {
                 const int acc = turn & 1;
@@ -282,8 +277,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
                 }
                 tc_fence_after();
                 for (int k = 0; k < steps; ++k, ++used) {
-                    const int s = (int)(used % kMxStages);
-                    if (!mbar_wait(full(s), (uint32_t)(used / kMxStages) & 1, &given_up)) {
+                    if (!mbar_wait(full(s), phase, &given_up)) {
                         ok = false;
                         break;
                     }
@@ -300,14 +294,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
                         mma_mx4(tmem + acc * kTile, operand_desc(a + 32 * i, 1024, 16), operand_desc(w + 32 * i, 1024, 16), mx4_idesc(kTile, kTile, i & 1),
                                 ta + 4 * (i >> 1), tw + 4 * (i >> 1), k > 0 || i > 0);
                     tc_commit(empty(s));
+                    if (++s == kMxStages) s = 0, phase ^= 1;
                 }
                 if (ok) tc_commit(acc_full(acc));
             }
-            if (!ok) {  // the matrix instructions in flight end before their tensor memory is freed
-                volatile int still = 0;
-                tc_commit(last);
-                mbar_wait(last, 0, &still);
-            }
+            if (!ok) let_settle();  // the matrix instructions in flight end before their tensor memory is freed
         }
         __syncwarp();
     } else {
@@ -414,23 +405,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
             tma_prefetch_map(&args.w);
             tma_prefetch_map(&args.sa);
             tma_prefetch_map(&args.sw);
-            uint32_t issued = 0;
+            const uint32_t leader_full = in_leader(full(0));
+            int s = 0;
+            uint32_t phase = 1;  // (the stages begin empty)
             bool ok = true;
             for (int64_t tile = pair; ok && tile < tiles; tile += pairs) {
                 const int m = (int)(tile / args.tiles_n) * 2 + rank, n = (int)(tile % args.tiles_n) * 2;  // in 128 rows
-                for (int k = 0; k < steps; ++k, ++issued) {
-                    const int s = (int)(issued % kPairStages);
-                    if (issued >= kPairStages && !pair_wait(empty(s), (issued / kPairStages - 1) & 1, &given_up)) {
+                for (int k = 0; k < steps; ++k) {
+                    if (!pair_wait(empty(s), phase, &given_up)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t a = ring + s * kPairStage, sa = a + 2 * kTile * 128, bar = in_leader(full(s));
+                    const uint32_t a = ring + s * kPairStage, sa = a + 2 * kTile * 128, bar = leader_full + 8 * s;
                     if (rank == 0) mbar_expect(full(s), 2 * kPairBytes);
                     pair_load_2d(a, &args.a, k * 128, m * kTile, bar);
                     pair_load_2d(a + kTile * 128, &args.w, k * 128, (n + rank) * kTile, bar);
                     // (groups of 128 rows behind the last read as zeros)
                     pair_load_2d(sa, &args.sa, 0, (m * steps + k) * 8, bar);
                     for (int i = 0; i < 2; ++i) pair_load_2d(sa + (1 + i) * kScaleBytes, &args.sw, 0, ((n + i) * steps + k) * 8, bar);
+                    if (++s == kPairStages) s = 0, phase ^= 1;
                 }
             }
             if (!ok) let_settle();
@@ -438,8 +431,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
         __syncwarp();
     } else if (warp == kMxEpilogueWarps + 1) {
         if (lane == 0 && rank == 0) {
-            uint32_t used = 0;
-            int turn = 0;
+            uint32_t used = 0, phase = 0;
+            int s = 0, turn = 0;
             bool ok = true;
             for (int64_t tile = pair; ok && tile < tiles; tile += pairs, ++turn) {
                 if (turn >= 1 && !pair_wait(acc_empty, (uint32_t)(turn - 1) & 1, &given_up)) {
@@ -448,8 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
                 }
                 tc_fence_after();
                 for (int k = 0; k < steps; ++k, ++used) {
-                    const int s = (int)(used % kPairStages);
-                    if (!pair_wait(full(s), (used / kPairStages) & 1, &given_up)) {
+                    if (!pair_wait(full(s), phase, &given_up)) {
                         ok = false;
                         break;
                     }
@@ -467,6 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
                         pair_mma_mx4(tmem, operand_desc(a + 32 * i, 1024, 16), operand_desc(w + 32 * i, 1024, 16), pair_mx4_idesc(256, i & 1), ta + 4 * (i >> 1),
                                      tw + 8 * (i >> 1), k > 0 || i > 0);
                     pair_commit(empty(s));
+                    if (++s == kPairStages) s = 0, phase ^= 1;
                 }
                 if (ok) pair_commit(acc_full);
             }
