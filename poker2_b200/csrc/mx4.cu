@@ -83,15 +83,44 @@ __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as
 __device__ __forceinline__ float scale_of(uint32_t byte) {
     return byte == 255u ? __int_as_float(0x7FC00000) : byte ? __uint_as_float(byte << 23) : 5.8774717541114375e-39f;
 }
-__device__ __forceinline__ uint32_t four_bit_pair(float lo, float hi) {
-    uint32_t v;
-    asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\tcvt.u32.u8 %0, q;\n\t}" : "=r"(v) : "f"(lo), "f"(hi));
-    return v;
+// Eight values of magnitude 6 at most, two a byte, and back.
+__device__ __forceinline__ uint32_t four_bit_codes(const float2 (&v)[4]) {
+    uint32_t word;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(word)
+        : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
+    return word;
 }
-__device__ __forceinline__ float2 four_bit_values(uint32_t byte) {
-    uint32_t v;
-    asm("{\n\t.reg .b8 q;\n\tcvt.u8.u32 q, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, q;\n\t}" : "=r"(v) : "r"(byte));
-    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+__device__ __forceinline__ void four_bit_values(uint32_t word, float scale, float2 (&v)[4]) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(word));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        v[i] = (Two(f.x, f.y) * Two(scale)).apart();
+    }
+}
+
+// A block's code: what eight of its values become, and its scale byte.  (Four lanes have a block.)
+template <typename T> __device__ __forceinline__ uint32_t quantise_eight(const Eight<T>& x, uint32_t& byte) {
+    uint32_t top = x.top();
+    top = max(top, __shfl_xor_sync(~0u, top, 1));
+    top = max(top, __shfl_xor_sync(~0u, top, 2));
+    byte = scale_byte(Eight<T>::magnitude(top));
+    const Two inverse(byte == 255u ? 0.0f : inverse_scale(byte));
+    float2 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 two = x.pair(i);
+        v[i] = (Two(two.x, two.y) * inverse).apart();
+    }
+    return four_bit_codes(v);
 }
 
 // Four lanes take a block, a warp kSpans times 256 neighbouring columns of a row: 16-byte loads (16-bit types), kSpans of them on
@@ -107,37 +136,33 @@ __global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t s
     for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < all; job += (int64_t)gridDim.x * 8) {
         const int64_t row = all < (1ll << 31) ? (uint32_t)job / (uint32_t)row_jobs : job / row_jobs;
         const int first = (int)(job - row * row_jobs) * kSpans;
-        const T* p = x + row * stride + first * 256 + lane * 8;
+        const int col0 = first * 256 + lane * 8, inside = width - col0;
+        const T* const p = x + row * stride + col0;
+        const bool there = row < rows;
         Eight<T> v[kSpans];
+        if (there && vector && (first + kSpans) * 256 <= width) {
 #pragma unroll
-        for (int i = 0; i < kSpans; ++i) {
-            const int col = (first + i) * 256 + lane * 8;
-            if (row < rows && vector && col + 8 <= width)
-                v[i].load(p + i * 256);
-            else
-                v[i].load_some(p + i * 256, row < rows ? width - col : 0);
+            for (int i = 0; i < kSpans; ++i) v[i].load(p + i * 256);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSpans; ++i)
+                if (there && vector && inside >= i * 256 + 8)
+                    v[i].load(p + i * 256);
+                else
+                    v[i].load_some(p + i * 256, there ? inside - i * 256 : 0);
         }
-        uint8_t* const row_scales = scales + (row / 128 * spans * 2 + lane / 16) * 512 + row % 32 * 16 + row % 128 / 32 * 4;
+        uint32_t* const out = reinterpret_cast<uint32_t*>(values + row * row_bytes + col0 / 2);
+        uint32_t* const row_scales = reinterpret_cast<uint32_t*>(scales + ((row / 128 * spans + first) * 2 + lane / 16) * 512 + row % 32 * 16 + row % 128 / 32 * 4);
+        const int left = there ? blocks * 32 - col0 : 0, left_spans = spans - first;
 #pragma unroll
         for (int i = 0; i < kSpans; ++i) {
-            if (first + i >= spans) break;
-            uint32_t top = v[i].top();
-            top = max(top, __shfl_xor_sync(~0u, top, 1));
-            top = max(top, __shfl_xor_sync(~0u, top, 2));
-            const uint32_t byte = scale_byte(Eight<T>::magnitude(top));
-            const float inverse = byte == 255u ? 0.0f : inverse_scale(byte);
-            uint32_t word = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 two = v[i].pair(j);
-                word |= four_bit_pair(two.x * inverse, two.y * inverse) << (8 * j);
-            }
-            const int col = (first + i) * 256 + lane * 8;
-            if (row < rows && col < blocks * 32) *reinterpret_cast<uint32_t*>(values + row * row_bytes + col / 2) = word;
+            uint32_t byte;
+            const uint32_t word = quantise_eight<T>(v[i], byte);
+            if (left > i * 256) out[i * 32] = word;
             uint32_t four = byte << (8 * (lane / 4 % 4));
             four |= __shfl_xor_sync(~0u, four, 4);
             four |= __shfl_xor_sync(~0u, four, 8);
-            if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(row_scales + (int64_t)(first + i) * 1024) = four;
+            if (lane % 16 == 0 && left_spans > i) row_scales[i * 256] = four;
         }
     }
 }
@@ -162,13 +187,8 @@ __global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* valu
 #pragma unroll
         for (int i = 0; i < kSpans; ++i) {
             const int col = (first + i) * 256 + lane * 8;
-            const float scale = scale_of(byte[i]);
             float2 v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = four_bit_values(word[i] >> (8 * j) & 255u);
-                v[j].x *= scale, v[j].y *= scale;
-            }
+            four_bit_values(word[i], scale_of(byte[i]), v);
             T* p = out + row * stride + col;
             if (vector && col + 8 <= width) {
                 Eight<T>::store(p, v);
@@ -563,27 +583,20 @@ __global__ void __launch_bounds__(256) mx4_few_kernel(const T* x, int64_t x_stri
                 v.load(x + r * x_stride + col);
             else
                 v.load_some(x + r * x_stride + col, width - col);
-            uint32_t top = v.top();
-            top = max(top, __shfl_xor_sync(~0u, top, 1));
-            top = max(top, __shfl_xor_sync(~0u, top, 2));
-            const uint32_t b = scale_byte(Eight<T>::magnitude(top));
-            const float inverse = b == 255u ? 0.0f : inverse_scale(b), scale = scale_of(b);
+            uint32_t b;
+            // (by way of a shuffle: codes handed straight from their packing to their unpacking came out as zeros, nvcc 12.9)
+            const uint32_t word_x = __shfl_sync(~0u, quantise_eight<T>(v, b), lane);
+            float2 q[4];
+            four_bit_values(word_x, scale_of(b), q);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 two = v.pair(j), q = four_bit_values(four_bit_pair(two.x * inverse, two.y * inverse));
-                *reinterpret_cast<float2*>(&values[r][i * 256 + lane * 8 + 2 * j]) = make_float2(q.x * scale, q.y * scale);
-            }
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(&values[r][i * 256 + lane * 8 + 2 * j]) = q[j];
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kChunk / 256; ++i) {
             if (first + i >= spans) break;
             float2 f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[j] = four_bit_values(word[i] >> (8 * j) & 255u);
-                f[j].x *= scale_of(byte[i]), f[j].y *= scale_of(byte[i]);
-            }
+            four_bit_values(word[i], scale_of(byte[i]), f);
 #pragma unroll
             for (int r = 0; r < kMost; ++r)
                 if (r < rows) {
