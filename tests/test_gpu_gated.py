@@ -10,6 +10,8 @@ pytestmark = pytest.mark.gpu
 SIZES = [  # rows, width, hidden: single tokens, the step to the tensor cores, tiles and blocks just full, one over, odd numbers
     (1, 64, 32), (1, 1536, 1024), (1, 77, 5), (2, 2720, 40), (8, 65, 33), (9, 64, 1), (9, 1, 8), (13, 72, 64), (77, 100, 72),
     (128, 64, 128), (129, 63, 129), (257, 1536, 200), (300, 8, 1024), (700, 2720, 96), (1000, 333, 257),
+    (40, 64, 2500), (600, 72, 2100),  # biases beyond what is staged
+    (2000, 1536, 1024), (5200, 600, 300),  # several tiles a pair, both kinds of gradients' tiles
 ]
 
 
@@ -175,3 +177,61 @@ def test_capture_through_autograd_is_refused(cuda_device):
     graph.replay()
     assert torch.equal(h, alive.detach())
     assert torch.isfinite(torch.autograd.grad(alive, wg, dh)[0]).all()
+
+
+def test_outputs_beyond_32_bits(cuda_device):
+    """1.6 million rows of 1400 hidden units: 2.2e9 outputs; the first and last rows against their own call."""
+    rows, width, hidden = 1_600_000, 64, 1400
+    _, wg, wu, bg, bu, _ = _layer(1, width, hidden, torch.bfloat16, cuda_device)
+    x = torch.randn(rows, width, device=cuda_device, dtype=torch.bfloat16)
+    h = gated.gated_linear(x, wg, wu, bg, bu)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        refs.assert_within(h[part], *refs.gated(x[part], wg, wu, bg, bu, "gelu", x.dtype))
+    del h
+    dh = torch.randn(rows, hidden, device=cuda_device, dtype=torch.bfloat16)
+    dx = gated.gated_linear_backward(dh, x, wg, wu, bg, bu, needs=(True, False, False, False, False))[0]
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        refs.assert_within(dx[part], *refs.gated_backward(dh[part], x[part], wg, wu, bg, bu, "gelu", x.dtype)["dx"])
+
+
+def test_another_current_device_and_two_threads(cuda_device, monkeypatch):
+    """The way a call takes when its tensors' device is not the current one (the same device here), and calls from two threads."""
+    import threading
+
+    from poker2_b200 import _lib
+
+    x, wg, wu, bg, bu, dh = _layer(300, 256, 160, torch.bfloat16, cuda_device)
+    want = gated.gated_linear(x, wg, wu, bg, bu), gated.gated_linear_backward(dh, x, wg, wu, bg, bu)
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = gated.gated_linear(x, wg, wu, bg, bu), gated.gated_linear_backward(dh, x, wg, wu, bg, bu)
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    monkeypatch.setattr(_lib, "_get_device", lambda: -1)
+    got[2] = gated.gated_linear(x, wg, wu, bg, bu), gated.gated_linear_backward(dh, x, wg, wu, bg, bu)
+    for h, grads in got.values():
+        assert torch.equal(h, want[0]) and all(torch.equal(a, b) for a, b in zip(grads, want[1]))
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    x, wg, wu, bg, bu, dh = _layer(16, 64, 32, torch.bfloat16, cuda_device)
+    x.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(gated.gated_linear(x, wg, wu, bg, bu), x, dh, create_graph=True)
+
+
+def test_the_leaf_of_a_broadcast_input_gets_its_sum(cuda_device):
+    x, wg, wu, bg, bu, dh = _layer(200, 72, 40, torch.bfloat16, cuda_device)
+    row = x[0].clone().requires_grad_(True)
+    got, = torch.autograd.grad(gated.gated_linear(row.expand(200, 72), wg, wu, bg, bu), row, dh)
+    each = gated.gated_linear_backward(dh, x[:1].expand(200, 72), wg, wu, bg, bu)[0]
+    assert torch.equal(got, each.sum(0))

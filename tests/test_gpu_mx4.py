@@ -148,3 +148,46 @@ def test_streams_and_capture(cuda_device):
     graphs[1].replay()
     for a, b in outs:
         assert torch.equal(a, mx4.linear(x, q, activation="silu")) and torch.equal(b, mx4.quantise(x).dequantise(x.dtype))
+
+
+def test_offsets_beyond_32_bits_and_unaligned_biases(cuda_device):
+    """1.6 million rows of 1400 values, and as many outputs; the first and last rows against their own call."""
+    rows, width = 1_600_000, 1400
+    x = torch.randn(rows, width, device=cuda_device, dtype=torch.bfloat16)
+    q = mx4.quantise(x)
+    back = q.dequantise(torch.bfloat16)
+    ends = (slice(0, 200), slice(rows - 200, rows))
+    for part in ends:
+        assert torch.equal(back[part].double(), refs.mx4_values(x[part]))
+    del back
+    w = mx4.quantise(torch.randn(1400, width, device=cuda_device) / 37)
+    bias = torch.randn(1401, device=cuda_device).bfloat16()[1:]
+    y = mx4.linear(q, w, bias, activation="silu")
+    for part in ends:
+        refs.assert_within(y[part], *refs.mx4_linear(refs.mx4_values(x[part]), w.dequantise().double(), bias, "silu", torch.bfloat16))
+
+
+def test_threads_and_another_current_device(cuda_device, monkeypatch):
+    import threading
+
+    from poker2_b200 import _lib
+
+    x = torch.randn(2000, 512, device=cuda_device).bfloat16()
+    q = mx4.quantise(torch.randn(1500, 512, device=cuda_device))
+    want, got = mx4.linear(x, q), {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = mx4.linear(x, q)
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    monkeypatch.setattr(_lib, "_get_device", lambda: -1)
+    got[2] = mx4.linear(x, q)
+    assert all(torch.equal(y, want) for y in got.values()) and torch.equal(mx4.linear(x[:2], q), mx4.linear(x[:2].clone(), q))

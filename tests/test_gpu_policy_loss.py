@@ -203,3 +203,29 @@ def test_hand_weights(cuda_device):
             want[i, (c1 == card) | (c2 == card)] = 0.0
     # the mass is summed in 64 bits and rounded, and rounded again by the product
     refs.assert_within(got, want, want * 2.0 ** -22)
+
+
+def test_arrays_beyond_32_bits(cuda_device):
+    """105,000 states of 1326 hands and 16 actions, 2.2e9 entries: every state the same, so loss and gradients are those of one."""
+    states, A = 105_000, 16
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    one = torch.randn(1, 1326, A, device=cuda_device, generator=g)
+    policy = torch.softmax(torch.randn(1, 1326, A, device=cuda_device, generator=g), -1)
+    legal = torch.ones(1, A, dtype=torch.bool, device=cuda_device)
+    logits, many = one.bfloat16().repeat(states, 1, 1), policy.repeat(states, 1, 1)
+    loss, grad = pl.clipped_policy_loss_and_grad(logits, many, many, many, legal.expand(states, A))
+    want = refs.policy_loss(one.bfloat16(), policy, policy, policy, legal, None, 0.2, 1.0, torch.float32)
+    refs.assert_within(loss, want[0], want[1])
+    for part in (0, states // 2, states - 1):
+        value = want[2] / states
+        refs.assert_within(grad[part: part + 1], value, want[3] / states + refs.rounded(value.abs() * 1.001, torch.bfloat16))
+
+
+def test_second_derivatives_are_refused_and_factors_scale(cuda_device):
+    logits, *rest = _batch(5, 100, 4, torch.bfloat16, cuda_device)
+    logits.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(pl.clipped_policy_loss(logits, *rest), logits, create_graph=True)
+    plain, = torch.autograd.grad(pl.clipped_policy_loss(logits, *rest), logits)
+    scaled, = torch.autograd.grad(0.3 * pl.clipped_policy_loss(logits, *rest), logits)
+    assert torch.equal(scaled, (plain.float() * torch.tensor(0.3, device=cuda_device)).bfloat16())
