@@ -472,7 +472,7 @@ int p2b_indexed_add_rows(float* out, const int64_t* index, const float* src, int
  *   h = act(x gate_weight^T + gate_bias) * (x up_weight^T + up_bias)        [rows,hidden], one rounding
  * Rows of x and of the weights start on 16-byte boundaries, unless there are at most p2b_gated_few_rows() rows
  * (forward only).  A wait that runs out inside a kernel leaves NaN in the outputs that hung on it.
- * p2b_gated_backward: gradients of sum(grad_h * h); where rows * width * hidden is above 2^28, dgate = grad_h * up * act' and
+ * p2b_gated_backward: gradients of sum(grad_h * h); where rows * width * hidden is above 2^24, dgate = grad_h * up * act' and
  * dup = grad_h * act are rounded to the type once on their way into the products of dx, dwg and dwu.  dx [rows,width] (dx_stride), dwg and dwu [hidden,width], dbg and dbu [hidden]
  * packed; any of the five may be NULL.  scratch: p2b_gated_backward_scratch_bytes(rows, width, hidden), 16-byte aligned.
  * The same inputs give the same bits. */
@@ -523,7 +523,7 @@ int p2b_mx4_linear_few(const void* x, int64_t x_stride, int32_t x_dtype, int64_t
  *  negative (NULL: 1).  All packed.  1 to 16 actions, 0 <= clip < 1, kl >= 0.
  * Nothing is read into the result from illegal actions, hands of weight 0 and hands whose legal logits are all -inf; their
  * gradients are 0.  loss: one fp32, summed in 64 bits in a fixed order.  scratch: p2b_policy_loss_scratch_bytes(states, hands),
- * 8-byte aligned (0 bytes for up to 2048 hands: NULL will do).  p2b_policy_loss_scale: out = grad * *factor (device), n values. */
+ * 8-byte aligned (0 bytes for up to 1536 hands: NULL will do).  p2b_policy_loss_scale: out = grad * *factor (device), n values. */
 int64_t p2b_policy_loss_scratch_bytes(int64_t states, int32_t hands);
 int p2b_policy_loss(const void* logits, const float* old_policy, const float* advantages, const float* target,
                     const uint8_t* legal, const float* weights, int64_t states, int32_t hands, int32_t actions, int32_t dtype,

@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constan
 }
 
 // Few rows: a warp takes one gate and one up row of the weights, which pass through the chip once, against all rows of x.
-// Bound by the way from L2 and the launch: at 1 row, width 1536, hidden 1024 the weights are 6.3 MB.
+// Bound by the way from L2 and by the launch: 1 row, width 1536, hidden 1024 (6.3 MB of weights) take 3.1 us, 2 TB/s.
 template <int kMost, bool kBf16, int kActivation>
 __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64_t x_stride, const uint16_t* wg, int64_t wg_stride,
                                                         const uint16_t* wu, int64_t wu_stride, const uint16_t* bg, const uint16_t* bu,
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64
     for (int r = 0; r < kMost; ++r) g[r] = u[r] = 0.0f;
     const uint16_t *pg = wg + f * wg_stride, *pu = wu + f * wu_stride;
     if (vector) {
-#pragma unroll(kMost == 1 ? 6 : kMost == 4 ? 3 : 2)
+#pragma unroll(kMost == 1 ? 6 : 3)
         for (int k = lane * 8; k + 8 <= width; k += 256) {
             const uint4 a = __ldg(reinterpret_cast<const uint4*>(pg + k)), b = __ldg(reinterpret_cast<const uint4*>(pu + k));
             const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
@@ -640,7 +640,8 @@ template <int kMode> static int launch_hidden(const GatedArgs& args, bool slim, 
                                : (bf16 ? launch_pairs<kMode, true, kSilu>(args, st) : launch_pairs<kMode, false, kSilu>(args, st));
 }
 
-constexpr int kFewRows = 8;
+// From five rows on the slim tiles are as fast (1536 x 1024: 3.1 us at 1 row, 7.4 at 4, 10.8 at 6, 13.3 at 8; slim 10.7 at any).
+constexpr int kFewRows = 4;
 constexpr int64_t kMostRows = 1ll << 30;
 constexpr int kMostColumns = 1 << 20;
 
@@ -659,7 +660,8 @@ static int check_layer(const char* name, const void* x, int64_t x_stride, const 
     return P2B_OK;
 }
 
-// Slim tiles where they fit the chip at once.
+// Slim tiles where they fit the chip at once: 512 rows of 1536 x 1024 take 11.8 us in slim tiles, 14.3 in pairs; 600 rows, a wave and
+// some, 20.8 and 14.4.
 static bool slim_tiles(int64_t rows, int32_t hidden) { return blocks_of(rows, kRows) * blocks_of(hidden, 32) <= sm_count(); }
 
 // Tiles and maps of x and the weights for the products that end in hidden columns.
@@ -677,7 +679,7 @@ template <bool kBf16, int kActivation>
 static int launch_few(const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride, const void* bg,
                       const void* bu, int rows, int width, int hidden, void* h, int64_t h_stride, cudaStream_t stream) {
     const int vector = aligned16(x, rows > 1 ? x_stride : 0) && aligned16(wg, wg_stride) && aligned16(wu, wu_stride);
-    auto* kernel = rows == 1 ? gated_few_kernel<1, kBf16, kActivation> : rows <= 4 ? gated_few_kernel<4, kBf16, kActivation> : gated_few_kernel<kFewRows, kBf16, kActivation>;
+    auto* kernel = rows == 1 ? gated_few_kernel<1, kBf16, kActivation> : rows == 2 ? gated_few_kernel<2, kBf16, kActivation> : gated_few_kernel<kFewRows, kBf16, kActivation>;
     kernel<<<(unsigned)blocks_of(hidden, 4), 128, 0, stream>>>((const uint16_t*)x, x_stride, (const uint16_t*)wg, wg_stride, (const uint16_t*)wu, wu_stride,
                                                               (const uint16_t*)bg, (const uint16_t*)bu, rows, width, hidden, (uint16_t*)h, h_stride, vector);
     return check_cuda(cudaGetLastError(), "gated_few_kernel");
@@ -717,9 +719,11 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
 }
 
 // dgate and dup are rounded to 16 bits on their way into the products, which makes the gradients' error 1.4 times that of their
-// last rounding alone.  Where the products take no longer than their launch, two 16-bit numbers carry each (0.4 us for 64 rows of
-// 2048 x 2048), and the last rounding is all.
-static int parts_of(int64_t rows, int64_t width, int64_t hidden) { return rows * hidden <= (1ll << 28) / width ? 2 : 1; }
+// last rounding alone.  Two 16-bit numbers for each would take it away and make the products twice as long (1000 rows of 1536 x 1024: 35
+// -> 48 us for the whole pass).  So only small layers have them (16 rows of 72 x 64: 11.1 -> 11.9 us), where few values
+// let the error of a single gradient stray further from that mean.
+constexpr int64_t kSmallProducts = 1ll << 24;
+static int parts_of(int64_t rows, int64_t width, int64_t hidden) { return rows * hidden <= kSmallProducts / width ? 2 : 1; }
 
 extern "C" int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t width, int32_t hidden) {
     if (rows < 0 || rows > kMostRows || width < 1 || width > kMostColumns || hidden < 1 || hidden > kMostColumns) return -1;

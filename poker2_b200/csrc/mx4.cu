@@ -549,9 +549,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
 }
 
 // Few rows of x as they are: every block quantises them for itself (a chunk of kChunk columns at a time, in shared memory as the
-// values they stand for), a warp takes a column of the product.  One launch, and no 128 rows of which most are empty: at 1 row,
-// 1536 x 1536, the two launches of the general way took 4 + 9 us.
-constexpr int kFewRows = 8;
+// values they stand for), a warp takes a column of the product.  One launch, and no 128 rows of which most are empty: 1 row of 1536 x
+// 1536 takes 3.6 us, in the two launches of the general way 9.6; 4 rows 7.1 and 9.6; at 8 rows it would be 12.3 and 9.4.
+constexpr int kFewRows = 4;
 constexpr int kChunk = 1024;
 
 template <typename T, int kMost, bool kBf16, int kActivation>
@@ -629,7 +629,7 @@ template <typename T, bool kBf16, int kActivation>
 static int launch_few(const void* x, int64_t x_stride, int rows, int width, const void* w_values, const void* w_scales, const void* bias, int columns, void* out,
                       int64_t out_stride, cudaStream_t stream) {
     const int vector = (uintptr_t)x % 16 == 0 && (rows == 1 || x_stride % (16 / (int)sizeof(T)) == 0);
-    auto* kernel = rows == 1 ? mx4_few_kernel<T, 1, kBf16, kActivation> : rows <= 4 ? mx4_few_kernel<T, 4, kBf16, kActivation> : mx4_few_kernel<T, kFewRows, kBf16, kActivation>;
+    auto* kernel = rows == 1 ? mx4_few_kernel<T, 1, kBf16, kActivation> : rows == 2 ? mx4_few_kernel<T, 2, kBf16, kActivation> : mx4_few_kernel<T, kFewRows, kBf16, kActivation>;
     kernel<<<(unsigned)blocks_of(columns, 8), 256, 0, stream>>>((const T*)x, x_stride, rows, width, (const uint8_t*)w_values, (const uint8_t*)w_scales,
                                                                (const uint16_t*)bias, columns, (uint16_t*)out, out_stride, vector);
     return check_cuda(cudaGetLastError(), "mx4_few_kernel");

@@ -13,7 +13,7 @@ from . import _lib
 
 ACTIVATIONS = {"gelu": 0, "silu": 1}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
-FEW_ROWS = 8  # up to so many rows the forward pass reads operands of any alignment (p2b_gated_few_rows)
+FEW_ROWS = 4  # up to so many rows the forward pass reads operands of any alignment (p2b_gated_few_rows)
 
 
 def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, gate_bias: torch.Tensor | None = None,

@@ -15,7 +15,7 @@ from . import _lib
 
 ACTIVATIONS = {"gelu": 0, "silu": 1, "none": 2}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-FEW_ROWS = 8  # up to so many rows are quantised by the product itself (p2b_mx4_few_rows)
+FEW_ROWS = 4  # up to so many rows are quantised by the product itself (p2b_mx4_few_rows)
 
 
 @dataclass

@@ -8,7 +8,7 @@ import network_refs as refs
 pytestmark = pytest.mark.gpu
 
 SIZES = [  # rows, width, hidden: single tokens, the step to the tensor cores, tiles and blocks just full, one over, odd numbers
-    (1, 64, 32), (1, 1536, 1024), (1, 77, 5), (2, 2720, 40), (8, 65, 33), (9, 64, 1), (9, 1, 8), (13, 72, 64), (77, 100, 72),
+    (1, 64, 32), (1, 1536, 1024), (1, 77, 5), (2, 2720, 40), (4, 65, 33), (5, 64, 1), (8, 65, 33), (9, 64, 1), (9, 1, 8), (13, 72, 64), (77, 100, 72),
     (128, 64, 128), (129, 63, 129), (257, 1536, 200), (300, 8, 1024), (700, 2720, 96), (1000, 333, 257),
     (40, 64, 2500), (600, 72, 2100),  # biases beyond what is staged
     (2000, 1536, 1024), (5200, 600, 300),  # several tiles a pair, both kinds of gradients' tiles

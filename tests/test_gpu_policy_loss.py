@@ -7,7 +7,7 @@ from poker2_b200 import policy_loss as pl
 
 pytestmark = pytest.mark.gpu
 SIZES = [(1, 1326, 5), (1, 1, 1), (3, 1326, 8), (7, 100, 2), (40, 7, 3), (2, 256, 4), (5, 1326, 7), (300, 1, 6), (17, 300, 16), (9, 511, 11),
-         (8, 256, 4), (2049, 1, 3), (1201, 1326, 2), (700, 1326, 5)]  # one block's work just full, one over; blocks that take many tiles
+         (6, 256, 4), (1537, 1, 3), (1201, 1326, 2), (700, 1326, 5)]  # one block's work just full, one over; blocks that take many tiles
 
 
 def _batch(states, hands, actions, dtype, device, seed=0):

@@ -128,7 +128,7 @@ def test_mx4_linear_refuses(handle, change):
     assert _refused(handle, "p2b_mx4_linear", **change)
 
 
-@pytest.mark.parametrize("change", [dict(rows=-1), dict(rows=9), dict(width=0), dict(columns=0), dict(columns=1 << 30), dict(dtype=2), dict(xdtype=3), dict(xdtype=-1), dict(act=3),
+@pytest.mark.parametrize("change", [dict(rows=-1), dict(rows=5), dict(width=0), dict(columns=0), dict(columns=1 << 30), dict(dtype=2), dict(xdtype=3), dict(xdtype=-1), dict(act=3),
                                     dict(x=None), dict(w=None), dict(sw=None), dict(out=None), dict(xs=-1), dict(stride=7), dict(w=(8,)), dict(sw=(4,)), dict(x=(1,)),
                                     dict(xdtype=2, x=(2,)), dict(out=(1,)), dict(bias=(1,))])
 def test_mx4_linear_few_refuses(handle, change):
