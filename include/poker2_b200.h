@@ -470,8 +470,9 @@ int p2b_indexed_add_rows(float* out, const int64_t* index, const float* src, int
  * all of one type: dtype 0 bf16, 1 fp16; rows x_stride, ... elements apart, elements of a row next to each other.
  * activation 0: gelu (with erf), 1: silu.  Sums in fp32.
  *   h = act(x gate_weight^T + gate_bias) * (x up_weight^T + up_bias)        [rows,hidden], one rounding
- * Rows of x and of the weights start on 16-byte boundaries, unless there are at most p2b_gated_few_rows() rows
- * (forward only).  A wait that runs out inside a kernel leaves NaN in the outputs that hung on it.
+ * Rows of x and of the weights that start on 16-byte boundaries are read in place (forward with at most p2b_gated_few_rows()
+ * rows: any); others by way of copies in scratch, of p2b_gated_align_bytes(rows, width, hidden) bytes, 16-byte aligned
+ * (p2b_gated_backward: behind its own).  scratch of the forward pass may be NULL where none is copied.  A wait that runs out inside a kernel leaves NaN in the outputs that hung on it.
  * p2b_gated_backward: gradients of sum(grad_h * h); where rows * width * hidden is above 2^24, dgate = grad_h * up * act' and
  * dup = grad_h * act are rounded to the type once on their way into the products of dx, dwg and dwu.  dx [rows,width] (dx_stride), dwg and dwu [hidden,width], dbg and dbu [hidden]
  * packed; any of the five may be NULL.  scratch: p2b_gated_backward_scratch_bytes(rows, width, hidden), 16-byte aligned.
@@ -480,7 +481,8 @@ int p2b_gated_few_rows(void);
 int p2b_gated_forward(const void* x, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
                       const void* up_weight, int64_t up_stride, const void* gate_bias, const void* up_bias,
                       int64_t rows, int32_t width, int32_t hidden, int32_t dtype, int32_t activation, void* h,
-                      int64_t h_stride, void* stream);
+                      int64_t h_stride, void* scratch, int64_t scratch_bytes, void* stream);
+int64_t p2b_gated_align_bytes(int64_t rows, int32_t width, int32_t hidden);
 int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t width, int32_t hidden);
 int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, int64_t x_stride,
                        const void* gate_weight, int64_t gate_stride, const void* up_weight, int64_t up_stride,

@@ -77,7 +77,7 @@ _SIGNATURES = {
     "p2b_mean_over_hand_perms": [_vp, _vp, _i32, _i64, _vp, _vp],
     "p2b_tree_count": [_vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp],
     "p2b_tree_records": [_vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
-    "p2b_gated_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
+    "p2b_gated_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
     "p2b_gated_backward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp,
                            _vp, _vp, _vp, _vp, _i64, _vp],
     "p2b_mx4_quantise": [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp],
@@ -94,7 +94,7 @@ _VALUE_FUNCS = {"p2b_cfr_scratch_floats": ([_i32, _i32], _i64), "p2b_cfr_default
                 "p2b_cfr_solve_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_solve_block_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_step_scratch_floats": ([_i32, _i32, _i64], _i64),
-                "p2b_gated_few_rows": ([], _i32), "p2b_gated_backward_scratch_bytes": ([_i64, _i32, _i32], _i64),
+                "p2b_gated_few_rows": ([], _i32), "p2b_gated_align_bytes": ([_i64, _i32, _i32], _i64), "p2b_gated_backward_scratch_bytes": ([_i64, _i32, _i32], _i64),
                 "p2b_mx4_few_rows": ([], _i32), "p2b_mx4_value_bytes": ([_i64, _i32], _i64), "p2b_mx4_scale_bytes": ([_i64, _i32], _i64),
                 "p2b_policy_loss_scratch_bytes": ([_i64, _i32], _i64),
                 "p2b_cfr_noalloc_scratch_floats": ([], _i64), "p2b_cfr_path_policy": ([_i32], _i32)}
@@ -199,12 +199,3 @@ def plain_rows(t: torch.Tensor) -> torch.Tensor:
     apart, step = t.stride()
     return t if (step == 1 or columns == 1) and (apart >= columns or rows <= 1) else t.contiguous()
 
-
-def wide_rows(t: torch.Tensor) -> torch.Tensor:
-    """The same with every row of 16-bit elements on a 16-byte boundary, as the tensor-memory kernels load them: copied where it
-    is not."""
-    rows, columns = t.shape
-    apart, step = t.stride()
-    if (step == 1 or columns == 1) and (apart >= columns and apart % 8 == 0 or rows <= 1) and t.data_ptr() % 16 == 0:
-        return t
-    return t.new_empty((rows, (columns + 7) // 8 * 8))[:, :columns].copy_(t)

@@ -660,6 +660,55 @@ static int check_layer(const char* name, const void* x, int64_t x_stride, const 
     return P2B_OK;
 }
 
+// Operands whose rows do not start on 16-byte boundaries, as the copies into shared memory want them, are copied to rows that do: all that
+// need it in one launch, 16 bytes a thread.
+struct AlignJob {
+    const uint16_t* from;
+    int64_t stride, rows;
+    uint16_t* to;
+};
+struct AlignArgs {
+    AlignJob job[3];
+    int width, whole;  // columns, and rounded up to a multiple of 8
+};
+__global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ AlignArgs args) {
+    const AlignJob job = args.job[blockIdx.y];
+    const int groups = args.whole / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < job.rows * groups; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / groups;
+        const int col = (int)(i - row * groups) * 8;
+        const uint16_t* p = job.from + row * job.stride + col;
+        uint32_t q[4];
+        load_words(p, args.width - col, false, q);
+        *reinterpret_cast<uint4*>(job.to + row * args.whole + col) = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+}
+static int64_t align_bytes(int64_t rows, int64_t width, int64_t hidden) { return 2 * (rows + 2 * hidden) * (blocks_of(width, 8) * 8); }
+// x, gate and up weights with rows and strides; those that need it become copies in `area`.
+static int align_operands(const char* name, const void** at, int64_t* stride, const int64_t* rows, int width, void* area, int64_t bytes, cudaStream_t st) {
+    AlignArgs args{};
+    args.width = width, args.whole = (int)blocks_of(width, 8) * 8;
+    uint16_t* to = (uint16_t*)area;
+    int jobs = 0;
+    int64_t most = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (aligned16(at[i], rows[i] > 1 ? stride[i] : 0)) {
+            if (rows[i] <= 1) stride[i] = args.whole;
+            continue;
+        }
+        args.job[jobs++] = {(const uint16_t*)at[i], stride[i], rows[i], to};
+        at[i] = to, stride[i] = args.whole;
+        to += rows[i] * args.whole;
+        most = rows[i] > most ? rows[i] : most;
+    }
+    if (!jobs) return P2B_OK;
+    if (!area || (uintptr_t)area % 16 || (char*)to - (char*)area > bytes)
+        return set_error(P2B_ERR_ARG, "%s: rows of x or of a weight start on no 16-byte boundaries, and there is no scratch for copies that do", name);
+    const int64_t blocks = blocks_of(most * (args.whole / 8), 256), fit = 8 * sm_count();
+    align_rows_kernel<<<dim3((unsigned)(blocks < fit ? blocks : fit), jobs), 256, 0, st>>>(args);
+    return check_cuda(cudaGetLastError(), "align_rows_kernel");
+}
+
 // Slim tiles where they fit the chip at once: 512 rows of 1536 x 1024 take 11.8 us in slim tiles, 14.3 in pairs; 600 rows, a wave and
 // some, 20.8 and 14.4.
 static bool slim_tiles(int64_t rows, int32_t hidden) { return blocks_of(rows, kRows) * blocks_of(hidden, 32) <= sm_count(); }
@@ -691,9 +740,13 @@ using namespace p2b;
 
 extern "C" int p2b_gated_few_rows(void) { return kFewRows; }
 
+extern "C" int64_t p2b_gated_align_bytes(int64_t rows, int32_t width, int32_t hidden) {
+    return rows < 0 || rows > kMostRows || width < 1 || width > kMostColumns || hidden < 1 || hidden > kMostColumns ? -1 : align_bytes(rows, width, hidden);
+}
+
 extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride,
                                  const void* bg, const void* bu, int64_t rows, int32_t width, int32_t hidden, int32_t dtype,
-                                 int32_t activation, void* h, int64_t h_stride, void* stream) {
+                                 int32_t activation, void* h, int64_t h_stride, void* scratch, int64_t scratch_bytes, void* stream) {
     int rc = check_layer("p2b_gated_forward", x, x_stride, wg, wg_stride, wu, wu_stride, rows, width, hidden, dtype, activation);
     if (rc) return rc;
     if (rows == 0) return P2B_OK;
@@ -704,16 +757,18 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
         auto* few = activation == kGelu ? (bf16 ? launch_few<true, kGelu> : launch_few<false, kGelu>) : (bf16 ? launch_few<true, kSilu> : launch_few<false, kSilu>);
         return few(x, x_stride, wg, wg_stride, wu, wu_stride, bg, bu, (int)rows, width, hidden, h, h_stride, st);
     }
-    if (!aligned16(x, x_stride) || !aligned16(wg, hidden > 1 ? wg_stride : 0) || !aligned16(wu, hidden > 1 ? wu_stride : 0))
-        return set_error(P2B_ERR_ARG, "p2b_gated_forward: rows of x and of the weights must start on 16-byte boundaries");
+    const void* at[3] = {x, wg, wu};
+    int64_t stride[3] = {x_stride, wg_stride, wu_stride};
+    const int64_t count[3] = {rows, hidden, hidden};
+    rc = align_operands("p2b_gated_forward", at, stride, count, width, scratch, scratch_bytes, st);
+    if (rc) return rc;
     GatedArgs args{};
     args.rows = rows, args.width = width, args.hidden = hidden;
     args.hidden_padded = (int)blocks_of(hidden, 128) * 128;
     args.bias_gate = bg, args.bias_up = bu, args.out = h, args.out_stride = h_stride, args.align_out = row_alignment(h, rows > 1 ? h_stride : 0);
     args.vector_bias = aligned16(bg, 0) && aligned16(bu, 0);
-    if (hidden == 1) wg_stride = wu_stride = blocks_of(width, 8) * 8;
     const bool slim = slim_tiles(rows, hidden);
-    rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
+    rc = hidden_maps(args, slim, at[0], stride[0], at[1], stride[1], at[2], stride[2]);
     if (!rc && !slim && args.align_out == 16) rc = encode_rows(&args.to, h, 2, hidden, rows, 2 * (rows > 1 ? h_stride : blocks_of(hidden, 8) * 8), 32);
     return rc ? rc : launch_hidden<kForward>(args, slim, bf16, activation, st);
 }
@@ -747,15 +802,18 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     }
     if (!grad_h || (rows > 1 && grad_stride < hidden)) return set_error(P2B_ERR_ARG, "p2b_gated_backward: null gradient or rows that overlap");
     if (dx && rows > 1 && dx_stride < width) return set_error(P2B_ERR_ARG, "p2b_gated_backward: rows of dx overlap");
-    if (!aligned16(x, rows > 1 ? x_stride : 0) || !aligned16(wg, hidden > 1 ? wg_stride : 0) || !aligned16(wu, hidden > 1 ? wu_stride : 0))
-        return set_error(P2B_ERR_ARG, "p2b_gated_backward: rows of x and of the weights must start on 16-byte boundaries");
     if (!scratch || ((uintptr_t)scratch % 16) != 0 || scratch_bytes < p2b_gated_backward_scratch_bytes(rows, width, hidden))
         return set_error(P2B_ERR_ARG, "p2b_gated_backward: scratch of %lld bytes on a 16-byte boundary is needed",
                          (long long)p2b_gated_backward_scratch_bytes(rows, width, hidden));
     const bool bf16 = dtype == 0;
-    const int64_t whole = blocks_of(width, 8) * 8;
-    if (rows == 1) x_stride = whole;
-    if (hidden == 1) wg_stride = wu_stride = whole;
+    const int64_t whole = blocks_of(width, 8) * 8, own = p2b_gated_backward_scratch_bytes(rows, width, hidden);
+    const void* at[3] = {x, wg, wu};
+    int64_t stride[3] = {x_stride, wg_stride, wu_stride};
+    const int64_t count[3] = {rows, hidden, hidden};
+    rc = align_operands("p2b_gated_backward", at, stride, count, width, (char*)scratch + own, scratch_bytes - own, st);
+    if (rc) return rc;
+    x = at[0], wg = at[1], wu = at[2];
+    x_stride = stride[0], wg_stride = stride[1], wu_stride = stride[2];
     GatedArgs args{};
     args.rows = rows, args.width = width, args.hidden = hidden;
     args.hidden_padded = (int)blocks_of(hidden, 128) * 128;

@@ -48,13 +48,14 @@ def _forward(x, gate_weight, up_weight, gate_bias, up_bias, act):
     xr = x if len(shape) == 2 else x.reshape(-1, width)
     rows = xr.shape[0]
     h = x.new_empty((rows, hidden))
-    whole = _lib.wide_rows if rows > FEW_ROWS else _lib.plain_rows
-    xr, gw, uw = whole(xr), whole(gate_weight), whole(up_weight)
+    xr, gw, uw = _lib.plain_rows(xr), _lib.plain_rows(gate_weight), _lib.plain_rows(up_weight)
+    size = 0 if rows <= FEW_ROWS else _align_bytes(xr, gw, uw)
+    scratch = x.new_empty((size // 2,)) if size else None
     gb = None if gate_bias is None else gate_bias.contiguous()
     ub = None if up_bias is None else up_bias.contiguous()
     _lib.call_on(x.get_device(), "p2b_gated_forward", xr.data_ptr(), xr.stride(0), gw.data_ptr(), gw.stride(0), uw.data_ptr(), uw.stride(0),
                  None if gb is None else gb.data_ptr(), None if ub is None else ub.data_ptr(), rows, width, hidden, _TYPES[x.dtype], act,
-                 h.data_ptr(), hidden)
+                 h.data_ptr(), hidden, None if scratch is None else scratch.data_ptr(), size)
     return h if len(shape) == 2 else h.view(*shape[:-1], hidden)
 
 
@@ -68,15 +69,24 @@ def _backward(grad_h, x, gate_weight, up_weight, gate_bias, up_bias, act, needs)
     dwu = new((hidden, width)) if needs[2] else None
     dbg = new((hidden,)) if needs[3] and gate_bias is not None else None
     dbu = new((hidden,)) if needs[4] and up_bias is not None else None
-    xr, gw, uw, gh = _lib.wide_rows(xr), _lib.wide_rows(gate_weight), _lib.wide_rows(up_weight), _lib.plain_rows(gh)
+    xr, gw, uw, gh = _lib.plain_rows(xr), _lib.plain_rows(gate_weight), _lib.plain_rows(up_weight), _lib.plain_rows(gh)
     gb = None if gate_bias is None else gate_bias.contiguous()
     ub = None if up_bias is None else up_bias.contiguous()
-    size = _lib.lib().p2b_gated_backward_scratch_bytes(rows, width, hidden)
+    size = _lib.lib().p2b_gated_backward_scratch_bytes(rows, width, hidden) + _align_bytes(xr, gw, uw)
     scratch = new((max(size, 16) // 2,))
     _lib.call_on(x.get_device(), "p2b_gated_backward", gh.data_ptr(), gh.stride(0), xr.data_ptr(), xr.stride(0), gw.data_ptr(), gw.stride(0),
                  uw.data_ptr(), uw.stride(0), p(gb), p(ub), rows, width, hidden, _TYPES[x.dtype], act, p(dx), width, p(dwg), p(dwu), p(dbg),
                  p(dbu), scratch.data_ptr(), size)
     return dx if dx is None or len(shape) == 2 else dx.view(shape), dwg, dwu, dbg, dbu
+
+
+def _align_bytes(*matrices) -> int:
+    """Bytes for copies whose rows start on 16-byte boundaries; 0 where all do already."""
+    for t in matrices:
+        if t.data_ptr() % 16 or t.stride(0) % 8 and t.shape[0] > 1:
+            x, weight, _ = matrices
+            return _lib.lib().p2b_gated_align_bytes(x.shape[0], x.shape[1], weight.shape[0])
+    return 0
 
 
 class _Gated(torch.autograd.Function):

@@ -19,15 +19,17 @@ def _area():
 
 
 def _gated_forward(p, **change):
-    a = dict(x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=None, bu=None, rows=16, width=64, hidden=8, dtype=0, act=0, h=p, hs=8)
+    a = dict(x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=None, bu=None, rows=16, width=64, hidden=8, dtype=0, act=0, h=p, hs=8, scratch=None, size=0)
     a.update(change)
     return [*a.values(), None]
 
 
 def _gated_backward(p, **change):
     a = dict(dh=p, ds=8, x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=None, bu=None, rows=16, width=64, hidden=8, dtype=0, act=0, dx=p, dxs=64,
-             dwg=None, dwu=None, dbg=None, dbu=None, scratch=p, size=1 << 30)
+             dwg=None, dwu=None, dbg=None, dbu=None, scratch=p, size=None)
     a.update(change)
+    if a["size"] is None:  # what the layer itself needs, nothing for copies
+        a["size"] = max(0, _lib.lib().p2b_gated_backward_scratch_bytes(max(0, min(a["rows"], 1 << 29)), 64, 8))
     return [*a.values(), None]
 
 
@@ -52,7 +54,10 @@ def test_gated_addresses_off_their_boundaries_are_refused(handle):
     for name in ("x", "wg", "wu"):
         assert handle.p2b_gated_forward(*_gated_forward(p, **{name: p + 2})) == -1 and b"16-byte" in handle.p2b_last_error()
         assert handle.p2b_gated_backward(*_gated_backward(p, **{name: p + 8})) == -1 and b"16-byte" in handle.p2b_last_error()
+        assert handle.p2b_gated_forward(*_gated_forward(p, **{name: p + 2}, scratch=p, size=100)) == -1 and b"16-byte" in handle.p2b_last_error()
+        assert handle.p2b_gated_forward(*_gated_forward(p, **{name: p + 2}, scratch=p + 8, size=1 << 20)) == -1 and b"16-byte" in handle.p2b_last_error()
     assert handle.p2b_gated_backward(*_gated_backward(p, scratch=p + 4)) == -1
+    assert handle.p2b_gated_align_bytes(16, 65, 8) == 2 * 32 * 72 and handle.p2b_gated_align_bytes(-1, 65, 8) == -1
     assert handle.p2b_gated_forward(*_gated_forward(None, rows=0, wg=p, wu=p)) == 0  # no rows: nothing to do
     assert handle.p2b_gated_few_rows() == gated.FEW_ROWS
     for sizes in ((-1, 8, 8), (8, 0, 8), (8, 8, 0)):
