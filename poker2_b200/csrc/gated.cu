@@ -2,8 +2,10 @@
 //
 // One tile of 128 rows holds 128 gate and 128 up columns next to each other in tensor memory (one matrix instruction of
 // 256 columns, its operand half from Wg, half from Wu), so the activation and the product happen on the accumulators and
-// neither projection goes through memory.  The backward pass takes the same products again instead of keeping them: its first
-// kernel ends in dgate = dh * up * act'(gate), dup = dh * act(gate) (16-bit, side by side in work space), from which
+// neither projection goes through memory.  Bound by the matrix instructions and what feeds them: 24576 rows of 1536 -> 1024 (155
+// GFLOP, 2 x 1024 x 1536 weights in L2) take 110 to 125 us, 1.24 to 1.41 PFLOP/s, at 13 TB/s out of L2.  The backward pass takes the
+// same products again instead of keeping gate and up in fp32, which would trade 4 rows x hidden x width operations for 22 bytes of
+// traffic a hidden value and 8 held over the whole step (even in time at width 1280).  Its first kernel ends in dgate = dh * up * act'(gate), dup = dh * act(gate) (16-bit, side by side in work space), from which
 // dx = dgate Wg + dup Wu, dWg = dgate^T x, dWu = dup^T x and the column sums follow.
 #include "layer.cuh"
 #include "tensor.cuh"

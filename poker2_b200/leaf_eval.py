@@ -7,8 +7,9 @@ pre-chance state is the expectation over the next public card of the network's v
 the post-card beliefs (`ChanceNodeHelper.single_card_chance_values`,
 p2/search/chance_node_helper.py:359-479).  `ChanceLeafEvaluator` computes that expectation
 explicitly: the expansion over the next card and the per-leaf averaging are this library's
-kernels (`chance.expand_next_card`, `chance.indexed_add_rows`); the network's GEMMs are
-torch / cuBLAS.
+kernels (`chance.expand_next_card`, `chance.indexed_add_rows`); the GEMMs of `ValueMLP` are
+torch / cuBLAS, `GatedValueMLP` and `Mx4ValueMLP` are made of this library's gated and 4-bit
+layers.
 """
 from __future__ import annotations
 
