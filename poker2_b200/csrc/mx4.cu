@@ -107,13 +107,7 @@ __device__ __forceinline__ void four_bit_values(uint32_t word, float scale, floa
     }
 }
 
-// A block's code: what eight of its values become, and its scale byte.  (Four lanes have a block.)
-template <typename T> __device__ __forceinline__ uint32_t quantise_eight(const Eight<T>& x, uint32_t& byte) {
-    uint32_t top = x.top();
-    top = max(top, __shfl_xor_sync(~0u, top, 1));
-    top = max(top, __shfl_xor_sync(~0u, top, 2));
-    byte = scale_byte(Eight<T>::magnitude(top));
-    const Two inverse(byte == 255u ? 0.0f : inverse_scale(byte));
+template <typename T> __device__ __forceinline__ uint32_t codes_of(const Eight<T>& x, Two inverse) {
     float2 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -122,48 +116,63 @@ template <typename T> __device__ __forceinline__ uint32_t quantise_eight(const E
     }
     return four_bit_codes(v);
 }
+// What eight values of a block become that four lanes have, and its scale byte.
+template <typename T> __device__ __forceinline__ uint32_t quantise_eight(const Eight<T>& x, uint32_t& byte) {
+    uint32_t top = x.top();
+    top = max(top, __shfl_xor_sync(~0u, top, 1));
+    top = max(top, __shfl_xor_sync(~0u, top, 2));
+    byte = scale_byte(Eight<T>::magnitude(top));
+    return codes_of(x, Two(byte == 255u ? 0.0f : inverse_scale(byte)));
+}
 
-// Four lanes take a block, a warp kSpans times 256 neighbouring columns of a row: 16-byte loads (16-bit types), kSpans of them on
-// their way at once, 128 bytes of values and two scale words out.  Bound by its instructions: 24576 x 2720 bf16 take 38 us (169 MB, 4.5
-// TB/s, 0.77 of the issue slots).
-constexpr int kSpans = 4;
+// Two lanes take a block, a warp kWide times 512 neighbouring columns of a row: four 16-byte loads (16-bit types) on their way at once,
+// 256 bytes of values and four scale words out a time.  Bound by memory and its instructions alike: 24576 x 2720 bf16 take QUANT us (169 MB);
+// with four lanes a block, which spend as much on every scale for half as many values, 37.
+constexpr int kWide = 2;
+constexpr int kSpans = 4;  // times 256 columns of a row for a warp that reads back
 
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t stride, int64_t rows, int width, uint8_t* values, uint8_t* scales,
                                                            int vector) {
     const int lane = threadIdx.x % 32;
-    const int blocks = (width + 31) / 32, spans = (width + 255) / 256, row_jobs = (spans + kSpans - 1) / kSpans;
+    const int blocks = (width + 31) / 32, pieces = (width + 255) / 256 * 2, row_jobs = (width + 512 * kWide - 1) / (512 * kWide);
     const int64_t row_bytes = (int64_t)blocks * 16, all = (rows + 127) / 128 * 128 * row_jobs;
     for (int64_t job = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; job < all; job += (int64_t)gridDim.x * 8) {
         const int64_t row = all < (1ll << 31) ? (uint32_t)job / (uint32_t)row_jobs : job / row_jobs;
-        const int first = (int)(job - row * row_jobs) * kSpans;
-        const int col0 = first * 256 + lane * 8, inside = width - col0;
+        const int first = (int)(job - row * row_jobs) * 512 * kWide, col0 = first + lane * 16, inside = width - col0;
         const T* const p = x + row * stride + col0;
         const bool there = row < rows;
-        Eight<T> v[kSpans];
-        if (there && vector && (first + kSpans) * 256 <= width) {
+        Eight<T> v[2 * kWide];
+        if (there && vector && first + 512 * kWide <= width) {
 #pragma unroll
-            for (int i = 0; i < kSpans; ++i) v[i].load(p + i * 256);
+            for (int i = 0; i < 2 * kWide; ++i) v[i].load(p + i / 2 * 512 + i % 2 * 8);
         } else {
 #pragma unroll
-            for (int i = 0; i < kSpans; ++i)
-                if (there && vector && inside >= i * 256 + 8)
-                    v[i].load(p + i * 256);
+            for (int i = 0; i < 2 * kWide; ++i) {
+                const int at = i / 2 * 512 + i % 2 * 8;
+                if (there && vector && inside >= at + 8)
+                    v[i].load(p + at);
                 else
-                    v[i].load_some(p + i * 256, there ? inside - i * 256 : 0);
+                    v[i].load_some(p + at, there ? inside - at : 0);
+            }
         }
-        uint32_t* const out = reinterpret_cast<uint32_t*>(values + row * row_bytes + col0 / 2);
-        uint32_t* const row_scales = reinterpret_cast<uint32_t*>(scales + ((row / 128 * spans + first) * 2 + lane / 16) * 512 + row % 32 * 16 + row % 128 / 32 * 4);
-        const int left = there ? blocks * 32 - col0 : 0, left_spans = spans - first;
+        uint2* const out = reinterpret_cast<uint2*>(values + row * row_bytes + col0 / 2);
+        const int piece = first / 128 + lane / 8;
+        uint32_t* const row_scales = reinterpret_cast<uint32_t*>(scales + (row / 128 * pieces + piece) * 512 + row % 32 * 16 + row % 128 / 32 * 4);
+        const int left = there ? blocks * 32 - col0 : 0;
 #pragma unroll
-        for (int i = 0; i < kSpans; ++i) {
-            uint32_t byte;
-            const uint32_t word = quantise_eight<T>(v[i], byte);
-            if (left > i * 256) out[i * 32] = word;
-            uint32_t four = byte << (8 * (lane / 4 % 4));
+        for (int i = 0; i < kWide; ++i) {
+            if (first + 512 * i >= width) break;
+            uint32_t top = max(v[2 * i].top(), v[2 * i + 1].top());
+            top = max(top, __shfl_xor_sync(~0u, top, 1));
+            const uint32_t byte = scale_byte(Eight<T>::magnitude(top));
+            const Two inverse(byte == 255u ? 0.0f : inverse_scale(byte));
+            const uint2 codes = make_uint2(codes_of(v[2 * i], inverse), codes_of(v[2 * i + 1], inverse));
+            if (left > i * 512) out[i * 32] = codes;
+            uint32_t four = byte << (8 * (lane / 2 % 4));
+            four |= __shfl_xor_sync(~0u, four, 2);
             four |= __shfl_xor_sync(~0u, four, 4);
-            four |= __shfl_xor_sync(~0u, four, 8);
-            if (lane % 16 == 0 && left_spans > i) row_scales[i * 256] = four;
+            if (lane % 8 == 0 && piece + 4 * i < pieces) row_scales[i * 512] = four;
         }
     }
 }
@@ -187,6 +196,7 @@ __global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* valu
         }
 #pragma unroll
         for (int i = 0; i < kSpans; ++i) {
+            if (first + i >= spans) break;
             const int col = (first + i) * 256 + lane * 8;
             float2 v[4];
             four_bit_values(word[i], scale_of(byte[i]), v);
@@ -690,7 +700,7 @@ extern "C" int p2b_mx4_quantise(const void* x, int64_t x_stride, int64_t rows, i
     if (((uintptr_t)values % 16) || ((uintptr_t)scales % 16) || (uintptr_t)x % (dtype == 2 ? 4 : 2))
         return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: values and scales must lie on 16-byte boundaries, x on its element's");
     const int vector = (uintptr_t)x % 16 == 0 && x_stride % (dtype == 2 ? 4 : 8) == 0;
-    const unsigned grid = warp_grid(blocks_of(rows, 128) * 128 * blocks_of(width, 256 * kSpans));
+    const unsigned grid = warp_grid(blocks_of(rows, 128) * 128 * blocks_of(width, 512 * kWide));
     cudaStream_t st = (cudaStream_t)stream;
     uint8_t *v = (uint8_t*)values, *s = (uint8_t*)scales;
     if (dtype == 0) mx4_quantise_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, x_stride, rows, width, v, s, vector);
