@@ -474,7 +474,7 @@ int p2b_indexed_add_rows(float* out, const int64_t* index, const float* src, int
  * rows: any); others by way of copies in scratch, of p2b_gated_align_bytes(rows, width, hidden) bytes, 16-byte aligned
  * (p2b_gated_backward: behind its own).  scratch of the forward pass may be NULL where none is copied.  A wait that runs out inside a kernel leaves NaN in the outputs that hung on it.
  * p2b_gated_backward: gradients of sum(grad_h * h); where rows * width * hidden is above 2^24, dgate = grad_h * up * act' and
- * dup = grad_h * act are rounded to the type once on their way into the products of dx, dwg and dwu.  dx [rows,width] (dx_stride), dwg and dwu [hidden,width], dbg and dbu [hidden]
+ * dup = grad_h * act are rounded to the type once on their way into the products of dx, dwg and dwu (fp16: they end at 65504).  dx [rows,width] (dx_stride), dwg and dwu [hidden,width], dbg and dbu [hidden]
  * packed; any of the five may be NULL.  scratch: p2b_gated_backward_scratch_bytes(rows, width, hidden), 16-byte aligned.
  * The same inputs give the same bits. */
 int p2b_gated_few_rows(void);

@@ -34,7 +34,8 @@ def gated_linear_backward(grad_h: torch.Tensor, x: torch.Tensor, gate_weight: to
                           gate_bias: torch.Tensor | None = None, up_bias: torch.Tensor | None = None, *, activation: str = "gelu",
                           needs: tuple = (True, True, True, True, True)):
     """Gradients of sum(grad_h * gated_linear(x, ...)) for (x, gate_weight, up_weight, gate_bias, up_bias); None where `needs` says
-    so or the bias is None.  The same inputs give the same bits."""
+    so or the bias is None.  The same inputs give the same bits.  Like the layer's own intermediate values in fp16, those of the
+    gradients (grad_h times gate or up) end at 65504 and lose bits below 6e-5: scale an fp16 loss as for any other layer."""
     act = _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
     if grad_h.shape != (*x.shape[:-1], gate_weight.shape[0]) or grad_h.dtype != x.dtype or grad_h.get_device() != x.get_device():
         raise ValueError("the gradient of the hidden layer must have its shape, type and device")

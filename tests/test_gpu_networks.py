@@ -173,3 +173,13 @@ def test_gated_network_trains_through_autograd(cuda_device):
     net.net(x).float().square().mean().backward()
     for name, p in net.named_parameters():
         assert p.grad is not None and torch.isfinite(p.grad.double()).all() and bool(p.grad.any()), name
+
+
+def test_policy_loss_of_batches_without_rows_or_targets(cuda_device):
+    none = torch.zeros(0, 1326, 5, device=cuda_device)
+    view = ua.FeatureView(torch.zeros(0, 4, device=cuda_device), *(torch.zeros(0, dtype=torch.long, device=cuda_device) for _ in range(2)),
+                          torch.zeros(0, 5, dtype=torch.long, device=cuda_device), torch.zeros(0, 2652, device=cuda_device))
+    legal = torch.zeros(0, 5, dtype=torch.bool, device=cuda_device)
+    assert ua.RebelBatchLike(view, legal, policy_targets=none).policy_loss(none.clone().requires_grad_(True)).item() == 0.0
+    with pytest.raises(ValueError, match="targets"):
+        ua.RebelBatchLike(view, legal).policy_loss(none)

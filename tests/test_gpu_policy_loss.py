@@ -221,11 +221,13 @@ def test_arrays_beyond_32_bits(cuda_device):
         refs.assert_within(grad[part: part + 1], value, want[3] / states + refs.rounded(value.abs() * 1.001, torch.bfloat16))
 
 
-def test_second_derivatives_are_refused_and_factors_scale(cuda_device):
-    logits, *rest = _batch(5, 100, 4, torch.bfloat16, cuda_device)
+@pytest.mark.parametrize("size", [(5, 100, 4), (3, 77, 5), (400, 1326, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_second_derivatives_are_refused_and_factors_scale(cuda_device, size, dtype):
+    logits, *rest = _batch(*size, dtype, cuda_device)
     logits.requires_grad_(True)
     with pytest.raises(RuntimeError, match="second"):
         torch.autograd.grad(pl.clipped_policy_loss(logits, *rest), logits, create_graph=True)
     plain, = torch.autograd.grad(pl.clipped_policy_loss(logits, *rest), logits)
     scaled, = torch.autograd.grad(0.3 * pl.clipped_policy_loss(logits, *rest), logits)
-    assert torch.equal(scaled, (plain.float() * torch.tensor(0.3, device=cuda_device)).bfloat16())
+    assert torch.equal(scaled, (plain.float() * torch.tensor(0.3, device=cuda_device)).to(dtype))
