@@ -510,7 +510,12 @@ int p2b_mx4_dequantise(const void* values, const void* scales, int64_t rows, int
 int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales,
                    int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out,
                    int64_t out_stride, void* stream);
-/* The same of at most p2b_mx4_few_rows() rows of x (x_dtype 0 bf16, 1 fp16, 2 fp32), quantised on the way, in one launch. */
+/* The same with the result quantised in place of written out: what p2b_mx4_quantise would make of it (dtype: the bias's, to which the
+ * result is rounded before). */
+int p2b_mx4_linear_mx4(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales,
+                       int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out_values,
+                       void* out_scales, void* stream);
+/* The same (written out) of at most p2b_mx4_few_rows() rows of x (x_dtype 0 bf16, 1 fp16, 2 fp32), quantised on the way, in one launch. */
 int p2b_mx4_few_rows(void);
 int p2b_mx4_linear_few(const void* x, int64_t x_stride, int32_t x_dtype, int64_t rows, const void* w_values, const void* w_scales,
                        int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out,

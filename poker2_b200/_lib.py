@@ -83,6 +83,7 @@ _SIGNATURES = {
     "p2b_mx4_quantise": [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp],
     "p2b_mx4_dequantise": [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp],
     "p2b_mx4_linear": [_vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp],
+    "p2b_mx4_linear_mx4": [_vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp],
     "p2b_mx4_linear_few": [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp],
     "p2b_policy_loss": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, ctypes.c_double, _f32, _vp, _vp, _vp, _i64, _vp],
     "p2b_policy_loss_scale": [_vp, _vp, _i64, _i32, _vp, _vp],

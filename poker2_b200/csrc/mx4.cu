@@ -223,6 +223,7 @@ struct Mx4Args {
     const uint8_t *a_scales, *w_scales;
     const void* bias;
     void* out;
+    uint8_t *out_values, *out_scales;  // the result quantised, instead of out
     int64_t out_stride, rows;
     int columns, steps, tiles_m, tiles_n;
     int vector_bias, align_out, pairs;
@@ -239,7 +240,57 @@ constexpr int kScaleSets = 4;      // sets of scale columns in tensor memory, us
 constexpr uint32_t kMxTmem = 512;  // two accumulators, scales behind them
 constexpr uint32_t kScaleColumn = 2 * kTile;
 
-template <int kOut, int kActivation>  // kOut 0 bf16, 1 fp16
+// 32 accumulators of a row from column `col` on to act(. + bias), rounded to 16 bits: two to a word of y.
+template <bool kBf16, int kActivation>
+__device__ __forceinline__ void finish_block(const Mx4Args& args, const uint32_t (&g)[32], int col, bool ok, uint32_t (&y)[16]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        uint32_t bias[8];
+        load_words(reinterpret_cast<const uint16_t*>(args.bias) + col + 16 * j, args.bias ? args.columns - col - 16 * j : 0, args.vector_bias, bias);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            Two slope;
+            const uint32_t* two = g + 16 * j + 2 * i;
+            const float2 v = activate<kActivation, false>(Two(__uint_as_float(two[0]), __uint_as_float(two[1])) + two_of<kBf16>(bias[i]), slope).apart();
+            y[8 * j + i] = ok ? pack<kBf16>(v.x, v.y) : 0x7FFF7FFFu;  // (a NaN in either type)
+        }
+    }
+}
+// A row's 64 neighbouring results from column `col` on, quantised as mx4_quantise_kernel would: 32 bytes of values, two scales.  Rows behind
+// the last have scales of zero, columns behind the last are zeros by themselves (no weight, no bias).
+template <bool kBf16> __device__ __forceinline__ void store_quantised(const Mx4Args& args, int64_t row, int col, const uint32_t (&y)[2][16]) {
+    using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+    if (col >= (args.columns + 255) / 256 * 256 || row >= (args.rows + 127) / 128 * 128) return;
+    const int64_t row_bytes = (int64_t)((args.columns + 31) / 32) * 16, pieces = scale_pieces(args.columns);
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        Eight<T> v[4];
+        uint32_t top = 0, codes[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i].w[k] = y[j][4 * i + k];
+            top = max(top, v[i].top());
+        }
+        const uint32_t byte = row < args.rows ? scale_byte(Eight<T>::magnitude(top)) : 0;
+        const Two inverse(byte == 255u ? 0.0f : inverse_scale(byte));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes[i] = codes_of(v[i], inverse);
+        bytes |= byte << (8 * j);
+        if (row < args.rows && col + 32 * j < args.columns)
+            *reinterpret_cast<uint4*>(args.out_values + row * row_bytes + (col + 32 * j) / 2) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    }
+    uint8_t* at = args.out_scales + (row / 128 * pieces + col / 128) * 512 + row % 32 * 16 + row % 128 / 32 * 4 + col / 32 % 4;
+    *reinterpret_cast<uint16_t*>(at) = (uint16_t)bytes;
+}
+template <bool kBf16> __device__ __forceinline__ void put_block(uint8_t* panel, int r, int col, const uint32_t (&y)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(panel + r * 128 + ((col / 8 + i) ^ (r & 7)) * 16) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+}
+
+template <int kOut, int kActivation, bool kQuantised>  // kOut 0 bf16, 1 fp16
 __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_constant__ Mx4Args args) {
     constexpr bool kBf16 = kOut == 0;
     extern __shared__ uint8_t raw[];
@@ -345,28 +396,30 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
             const int col = (int)(tile % args.tiles_n) * kTile + 64 * half;
             const bool ok = mbar_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
             tc_fence_after();
-            if (lane == 0) store_wait_read<0>();
+            if (!kQuantised && lane == 0) store_wait_read<0>();
             __syncwarp();
+            uint32_t y[2][16];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                uint32_t g[32], bias[16];
-                float v[32];
+                uint32_t g[32];
                 tmem_load_32(tmem + ((uint32_t)(quadrant * 32) << 16) + acc * kTile + 64 * half + 32 * j, g);
-                load_words(reinterpret_cast<const uint16_t*>(args.bias) + col + 32 * j, args.bias ? args.columns - col - 32 * j : 0, args.vector_bias, bias);
                 tmem_load_wait();
                 if (j == 1) {  // the accumulator is read
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty(acc));
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    Two slope;
-                    const float2 y = activate<kActivation, false>(Two(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])) + two_of<kBf16>(bias[i]), slope).apart();
-                    v[2 * i] = ok ? y.x : __int_as_float(0x7FC00000);
-                    v[2 * i + 1] = ok ? y.y : __int_as_float(0x7FC00000);
+                finish_block<kBf16, kActivation>(args, g, col + 32 * j, ok, y[j]);
+                if (!kQuantised) put_block<kBf16>(panel, r, 32 * j, y[j]);
+            }
+            if (kQuantised) {
+                store_quantised<kBf16>(args, row0 + lane, col, y);
+                // (the odd piece behind a last tile of 128 columns has none of its own)
+                if (col + 128 >= args.columns) {
+                    const uint32_t none[2][16] = {};
+                    if (col / 128 % 2 == 0) store_quantised<kBf16>(args, row0 + lane, col + 128, none);
                 }
-                put_panel<kBf16>(panel, r, 32 * j, v);
+                continue;
             }
             if (args.align_out == 16) {
                 async_fence();
@@ -401,7 +454,7 @@ constexpr int kPairBytes = 2 * kTile * 128 + 3 * kScaleBytes;
 constexpr int kPairShared = kPairStages * kPairStage + 4 * kPanelBytes + 1024;
 constexpr uint32_t kPairScales = 256;  // column of the scales
 
-template <int kOut, int kActivation>
+template <int kOut, int kActivation, bool kQuantised>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_pair_kernel(const __grid_constant__ Mx4Args args) {
     constexpr bool kBf16 = kOut == 0;
     extern __shared__ uint8_t raw[];
@@ -518,23 +571,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
             __syncwarp();
             if (lane == 0) {
                 pair_arrive(in_leader(acc_empty));
-                store_wait_read<0>();
+                if (!kQuantised) store_wait_read<0>();
             }
             __syncwarp();
+            uint32_t y[2][16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t bias[8];
-                float v[16];
-                load_words(reinterpret_cast<const uint16_t*>(args.bias) + col + 16 * j, args.bias ? args.columns - col - 16 * j : 0, args.vector_bias, bias);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    Two slope;
-                    const uint32_t* two = g[j / 2] + j % 2 * 16 + 2 * i;
-                    const float2 y = activate<kActivation, false>(Two(__uint_as_float(two[0]), __uint_as_float(two[1])) + two_of<kBf16>(bias[i]), slope).apart();
-                    v[2 * i] = ok ? y.x : __int_as_float(0x7FC00000);
-                    v[2 * i + 1] = ok ? y.y : __int_as_float(0x7FC00000);
-                }
-                put_panel<kBf16>(panel, r, 16 * j, v);
+            for (int j = 0; j < 2; ++j) {
+                finish_block<kBf16, kActivation>(args, g[j], col + 32 * j, ok, y[j]);
+                if (!kQuantised) put_block<kBf16>(panel, r, 32 * j, y[j]);
+            }
+            if (kQuantised) {
+                store_quantised<kBf16>(args, row0 + lane, col, y);
+                continue;
             }
             if (args.align_out == 16) {
                 async_fence();
@@ -648,23 +696,23 @@ static int launch_few(const void* x, int64_t x_stride, int rows, int width, cons
     return check_cuda(cudaGetLastError(), "mx4_few_kernel");
 }
 
-static SharedLimit g_limit[2][3], g_pair_limit[2][3];
+static SharedLimit g_limit[2][3][2], g_pair_limit[2][3][2];
 
 // Blocks by themselves while each gets at most one tile: a pair walks as long as a block and ends with twice the epilogue (1024 rows of
 // 1536 x 2720 with a gelu: 13.4 against 16.7 us); pairs beyond (2048 rows: 16.7 against 19.0; 24576: 71 against 101).
 static bool paired(int64_t rows, int64_t columns) { return blocks_of(rows, kTile) * blocks_of(columns, kTile) > sm_count(); }
 
-template <int kOut, int kActivation> static int launch_linear(const Mx4Args& args, cudaStream_t stream) {
+template <int kOut, int kActivation, bool kQuantised> static int launch_linear(const Mx4Args& args, cudaStream_t stream) {
     if (args.pairs) {
-        auto* kernel = mx4_pair_kernel<kOut, kActivation>;
-        int rc = allow_shared(g_pair_limit[kOut][kActivation], (const void*)kernel, kPairShared);
+        auto* kernel = mx4_pair_kernel<kOut, kActivation, kQuantised>;
+        int rc = allow_shared(g_pair_limit[kOut][kActivation][kQuantised], (const void*)kernel, kPairShared);
         if (rc) return rc;
         const int tiles = args.tiles_m * args.tiles_n, most = sm_count() / 2;
         kernel<<<2 * (tiles < most ? tiles : most), kMxThreads, kPairShared, stream>>>(args);
         return check_cuda(cudaGetLastError(), "mx4_pair_kernel");
     }
-    auto* kernel = mx4_linear_kernel<kOut, kActivation>;
-    int rc = allow_shared(g_limit[kOut][kActivation], (const void*)kernel, kMxShared);
+    auto* kernel = mx4_linear_kernel<kOut, kActivation, kQuantised>;
+    int rc = allow_shared(g_limit[kOut][kActivation][kQuantised], (const void*)kernel, kMxShared);
     if (rc) return rc;
     const int tiles = args.tiles_m * args.tiles_n;
     kernel<<<tiles < sm_count() ? tiles : sm_count(), kMxThreads, kMxShared, stream>>>(args);
@@ -755,30 +803,33 @@ extern "C" int p2b_mx4_linear_few(const void* x, int64_t x_stride, int32_t x_dty
     return x_dtype == 0 ? few(__nv_bfloat16()) : x_dtype == 1 ? few(__half()) : few(0.0f);
 }
 
-extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
-                              int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* stream) {
-    int rc = check_matrix("p2b_mx4_linear", rows, width);
-    if (!rc) rc = check_matrix("p2b_mx4_linear", columns, width);
+static int linear_of_quantised(const char* name, const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
+                              int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* out_values, void* out_scales,
+                              void* stream) {
+    const bool quantised = out_values || out_scales;
+    int rc = check_matrix(name, rows, width);
+    if (!rc) rc = check_matrix(name, columns, width);
     if (rc) return rc;
     // (tiles and rows of 128 scale bytes are counted in 32 bits)
     if (columns < 1 || blocks_of(rows, kTile) * blocks_of(columns, kTile) > 0x7FFF0000ll || (blocks_of(rows, kTile) + 1) * blocks_of(width, 256) > 0x0FFF0000ll ||
         (blocks_of(columns, kTile) + 1) * blocks_of(width, 256) > 0x0FFF0000ll)
-        return set_error(P2B_ERR_ARG, "p2b_mx4_linear: %lld x %d outputs are out of range", (long long)rows, columns);
-    if (dtype < 0 || dtype > 1) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: unknown type %d (0 bf16, 1 fp16)", dtype);
-    if (activation < 0 || activation > 2) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: unknown activation %d (0 gelu, 1 silu, 2 none)", activation);
+        return set_error(P2B_ERR_ARG, "%s: %lld x %d outputs are out of range", name, (long long)rows, columns);
+    if (dtype < 0 || dtype > 1) return set_error(P2B_ERR_ARG, "%s: unknown type %d (0 bf16, 1 fp16)", name, dtype);
+    if (activation < 0 || activation > 2) return set_error(P2B_ERR_ARG, "%s: unknown activation %d (0 gelu, 1 silu, 2 none)", name, activation);
     if (rows == 0) return P2B_OK;
-    if (!a_values || !a_scales || !w_values || !w_scales || !out || (rows > 1 && out_stride < columns))
-        return set_error(P2B_ERR_ARG, "p2b_mx4_linear: null array or rows that overlap");
-    for (const void* p : {a_values, a_scales, w_values, w_scales})
-        if ((uintptr_t)p % 16) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: values and scales must lie on 16-byte boundaries");
-    if ((uintptr_t)out % 2 || (uintptr_t)bias % 2) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: out and bias must lie on 2-byte boundaries");
+    if (!a_values || !a_scales || !w_values || !w_scales || (quantised ? !out_values || !out_scales : !out || (rows > 1 && out_stride < columns)))
+        return set_error(P2B_ERR_ARG, "%s: null array or rows that overlap", name);
+    for (const void* p : {a_values, a_scales, w_values, w_scales, (const void*)out_values, (const void*)out_scales})
+        if ((uintptr_t)p % 16) return set_error(P2B_ERR_ARG, "%s: values and scales must lie on 16-byte boundaries", name);
+    if ((uintptr_t)out % 2 || (uintptr_t)bias % 2) return set_error(P2B_ERR_ARG, "%s: out and bias must lie on 2-byte boundaries", name);
     Mx4Args args{};
     const int64_t row_bytes = blocks_of(width, 32) * 16;
     rc = encode_rows(&args.a, a_values, 1, row_bytes, rows, row_bytes, kTile);
     if (!rc) rc = encode_rows(&args.w, w_values, 1, row_bytes, columns, row_bytes, kTile);
     if (rc) return rc;
+    args.out_values = (uint8_t*)out_values, args.out_scales = (uint8_t*)out_scales;
     args.align_out = row_alignment(out, rows > 1 ? out_stride : 0);
-    if (args.align_out == 16) rc = encode_rows(&args.to, out, 2, columns, rows, 2 * (rows > 1 ? out_stride : blocks_of(columns, 8) * 8), 32);
+    if (!quantised && args.align_out == 16) rc = encode_rows(&args.to, out, 2, columns, rows, 2 * (rows > 1 ? out_stride : blocks_of(columns, 8) * 8), 32);
     if (rc) return rc;
     args.a_scales = (const uint8_t*)a_scales, args.w_scales = (const uint8_t*)w_scales, args.bias = bias, args.out = out;
     args.out_stride = out_stride, args.rows = rows, args.columns = columns;
@@ -792,8 +843,25 @@ extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_
     const int edge = args.pairs ? 256 : kTile;
     args.tiles_m = (int)blocks_of(rows, edge), args.tiles_n = (int)blocks_of(columns, edge);
     args.vector_bias = aligned16(bias, 0);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == 0)
-        return activation == 0 ? launch_linear<0, 0>(args, st) : activation == 1 ? launch_linear<0, 1>(args, st) : launch_linear<0, 2>(args, st);
-    return activation == 0 ? launch_linear<1, 0>(args, st) : activation == 1 ? launch_linear<1, 1>(args, st) : launch_linear<1, 2>(args, st);
+    auto launch = [&](auto type) {
+        constexpr int kOut = decltype(type)::value;
+        auto* f = quantised ? (activation == 0 ? launch_linear<kOut, 0, true> : activation == 1 ? launch_linear<kOut, 1, true> : launch_linear<kOut, 2, true>)
+                            : (activation == 0 ? launch_linear<kOut, 0, false> : activation == 1 ? launch_linear<kOut, 1, false> : launch_linear<kOut, 2, false>);
+        return f(args, (cudaStream_t)stream);
+    };
+    return dtype == 0 ? launch(std::integral_constant<int, 0>()) : launch(std::integral_constant<int, 1>());
+}
+
+extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
+                              int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* stream) {
+    if (rows > 0 && !out) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: null array");
+    return linear_of_quantised("p2b_mx4_linear", a_values, a_scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, out, out_stride, nullptr, nullptr,
+                               stream);
+}
+
+extern "C" int p2b_mx4_linear_mx4(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
+                                  int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out_values, void* out_scales, void* stream) {
+    if (rows > 0 && (!out_values || !out_scales)) return set_error(P2B_ERR_ARG, "p2b_mx4_linear_mx4: null array");
+    return linear_of_quantised("p2b_mx4_linear_mx4", a_values, a_scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, nullptr, 0, out_values,
+                               out_scales, stream);
 }

@@ -115,16 +115,18 @@ class GatedValueMLP(ValueMLP):
 
 
 class Mx4Linear(torch.nn.Module):
-    """act(q(x) q(W)^T + b) with W quantised once, when the layer is made."""
+    """act(q(x) q(W)^T + b) with W quantised once, when the layer is made.  `hands_on`: the result stays in 4 bits, as the next such
+    layer would make of it (but for few rows, which that one takes as they are)."""
 
-    def __init__(self, linear: torch.nn.Linear, activation: str = "none"):
+    def __init__(self, linear: torch.nn.Linear, activation: str = "none", hands_on: bool = False):
         super().__init__()
         self.weight = mx4.quantise(linear.weight.detach())
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
-        self.activation = activation
+        self.activation, self.hands_on, self.dtype = activation, hands_on, linear.weight.dtype
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return mx4.linear(x, self.weight, self.bias, activation=self.activation)
+    def forward(self, x: torch.Tensor | mx4.Mx4) -> torch.Tensor | mx4.Mx4:
+        rows = x.rows if isinstance(x, mx4.Mx4) else x.shape[:-1].numel()
+        return mx4.linear(x, self.weight, self.bias, activation=self.activation, dtype=self.dtype, quantised=self.hands_on and rows > mx4.FEW_ROWS)
 
 
 class Mx4ValueMLP(ValueMLP):
@@ -141,7 +143,8 @@ class Mx4ValueMLP(ValueMLP):
         if any(type(m) is torch.nn.GELU and (i == 0 or type(layers[i - 1]) is not torch.nn.Linear) for i, m in enumerate(layers)):
             raise ValueError("a GELU follows a linear layer")
         after = lambda i: "gelu" if i + 1 < len(layers) and type(layers[i + 1]) is torch.nn.GELU else "none"  # noqa: E731
-        self.net = torch.nn.Sequential(*(Mx4Linear(m, after(i)) for i, m in enumerate(layers) if type(m) is torch.nn.Linear))
+        last = max(i for i, m in enumerate(layers) if type(m) is torch.nn.Linear)
+        self.net = torch.nn.Sequential(*(Mx4Linear(m, after(i), i < last) for i, m in enumerate(layers) if type(m) is torch.nn.Linear))
         self.dtype = source.dtype
 
 

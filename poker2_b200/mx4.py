@@ -1,5 +1,5 @@
 """Microscaled 4-bit values: 32 neighbouring values of a row share a power-of-two scale.  `quantise` writes them, `dequantise`
-reads them back, `linear` multiplies two such matrices on the block-scaled matrix instructions.
+reads them back, `linear` multiplies two such matrices on the block-scaled matrix instructions and can leave its result in the same form.
 
 The scale of a block is the smallest power of two that brings its largest magnitude to 6 or below, so nothing is cut off; a
 value is then the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with its sign, ties to the even code.  A block that holds an infinity
@@ -72,10 +72,11 @@ def quantise(x: torch.Tensor) -> Mx4:
 
 
 def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None, *, activation: str = "none",
-           dtype: torch.dtype | None = None) -> torch.Tensor:
+           dtype: torch.dtype | None = None, quantised: bool = False) -> torch.Tensor | Mx4:
     """act(q(x) weight^T + bias) [..., columns]: x [..., width] as a tensor (quantised here) or quantised already, weight a quantised
     [columns, width] matrix, bias [columns] in the type of the result, which is x's (bf16 where x is fp32 or quantised)
-    unless `dtype` says bf16 or fp16.  `activation`: "none", "gelu" (with erf) or "silu".  Sums are fp32, one rounding at the end."""
+    unless `dtype` says bf16 or fp16.  `activation`: "none", "gelu" (with erf) or "silu".  Sums are fp32, one rounding at the end.
+    `quantised`: the result as `quantise` would make of it, without its way through memory, for the next such layer."""
     if not isinstance(weight, Mx4) or len(weight.shape) != 2:
         raise ValueError("the weight is a quantised matrix [columns, width]")
     act = ACTIVATIONS.get(activation)
@@ -98,7 +99,7 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
         if bias.dim() != 1 or bias.shape[0] != columns or bias.dtype != dtype or bias.get_device() != device:
             raise ValueError("the bias has one entry for each output, in the type of the result and on its device")
         bias = bias.contiguous()
-    if tensor and x.numel() <= FEW_ROWS * width and x.dtype in _TYPES:
+    if tensor and x.numel() <= FEW_ROWS * width and x.dtype in _TYPES and not quantised:
         flat = x if x.dim() == 2 else x.reshape(-1, width)
         if width > 1 and flat.stride(1) != 1:
             flat = flat.contiguous()
@@ -108,6 +109,13 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
                      weight.scales.data_ptr(), columns, width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, out.data_ptr(), columns)
         return out if x.dim() == 2 else out.view(*x.shape[:-1], columns)
     a = quantise(x) if tensor else x
+    if quantised:
+        rows, v = a.values.shape[0], a.values
+        values = v.new_empty((rows, (columns + 31) // 32 * 16))
+        scales = v.new_empty(((rows + 127) // 128 * ((columns + 255) // 256) * 1024,))
+        _lib.call_on(device, "p2b_mx4_linear_mx4", v.data_ptr(), a.scales.data_ptr(), rows, weight.values.data_ptr(), weight.scales.data_ptr(), columns,
+                     width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, values.data_ptr(), scales.data_ptr())
+        return Mx4(values, scales, (*a.shape[:-1], columns))
     out = a.values.new_empty((*a.shape[:-1], columns), dtype=dtype)
     _lib.call_on(device, "p2b_mx4_linear", a.values.data_ptr(), a.scales.data_ptr(), a.values.shape[0], weight.values.data_ptr(),
                  weight.scales.data_ptr(), columns, width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, out.data_ptr(), columns)

@@ -100,6 +100,35 @@ def test_linear(cuda_device, rows, width, columns, dtype, activation):
         refs.assert_within(mx4.linear(x, q), *refs.mx4_linear(refs.mx4_values(x), refs.mx4_values(w), None, activation, dtype))
 
 
+@pytest.mark.parametrize("activation", ["none", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("rows,width,columns", [(1, 64, 1), (5, 1536, 1536), (33, 256, 100), (128, 300, 129), (129, 64, 40), (300, 520, 256), (385, 1000, 257),
+                                                (600, 513, 2652), (1700, 300, 1500), (2500, 512, 1031), (5000, 64, 700), (2400, 96, 1537)])
+def test_linear_that_stays_quantised(cuda_device, rows, width, columns, dtype, activation):
+    """To the bit what quantising the result gives, scales behind the last row and column included."""
+    g = torch.Generator(device=cuda_device).manual_seed(rows + width + columns)
+    x = mx4.quantise(torch.randn(rows, width, device=cuda_device, generator=g))
+    w = mx4.quantise(torch.randn(columns, width, device=cuda_device, generator=g) / width ** 0.5)
+    bias = torch.randn(columns, device=cuda_device, generator=g).to(dtype)
+    for b in (bias, None):
+        want = mx4.quantise(mx4.linear(x, w, b, activation=activation, dtype=dtype))
+        # what was in memory before does not matter
+        torch.full((rows * (columns + 300) * 2,), 255, dtype=torch.uint8, device=cuda_device)
+        got = mx4.linear(x, w, b, activation=activation, dtype=dtype, quantised=True)
+        assert got.shape == (rows, columns) and torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
+        refs.assert_within(mx4.linear(got, mx4.quantise(torch.ones(3, columns, device=cuda_device))),
+                           *refs.mx4_linear(got.dequantise().double(), torch.ones(3, columns, device=cuda_device).double(), None, "none", torch.bfloat16))
+
+
+def test_linear_that_stays_quantised_shapes_and_bad_rows(cuda_device):
+    x, w = torch.randn(140, 96, device=cuda_device), mx4.quantise(torch.randn(50, 96, device=cuda_device))
+    assert mx4.linear(x.view(14, 10, 96), w, quantised=True).shape == (14, 10, 50)
+    assert mx4.linear(x[0], w, quantised=True).shape == (50,) and mx4.linear(x[:0], w, quantised=True).dequantise().shape == (0, 50)
+    x[5, 40] = float("nan")
+    bad = mx4.linear(x, w, quantised=True).dequantise()
+    assert torch.isnan(bad[5]).all() and torch.isfinite(bad[:5]).all() and torch.isfinite(bad[6:]).all()
+
+
 def test_linear_types_shapes_and_bad_rows(cuda_device):
     x = torch.randn(140, 96, device=cuda_device)
     q = mx4.quantise(torch.randn(50, 96, device=cuda_device))

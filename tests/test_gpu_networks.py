@@ -80,9 +80,10 @@ def test_quantised_network_is_its_layers(cuda_device):
     x = torch.randn(40, net.IN_PADDED, device=cuda_device).bfloat16()
     got, y = net.net(x), x
     layers = [m for m in source.net if isinstance(m, torch.nn.Linear)]
+    assert all(isinstance(net.net[0](x[:r]), torch.Tensor) == (r <= mx4.FEW_ROWS) for r in (1, 4, 5, 40))
     for i, m in enumerate(layers):
         last = i + 1 == len(layers)
-        a = net.net[i](y)
+        a = mx4.linear(y, net.net[i].weight, net.net[i].bias, activation="none" if last else "gelu")
         refs.assert_within(a, *refs.mx4_linear(refs.mx4_values(y), refs.mx4_values(m.weight.detach()), m.bias.detach(), "none" if last else "gelu", y.dtype))
         y = a
     assert torch.equal(got, y)

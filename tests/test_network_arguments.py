@@ -105,6 +105,7 @@ def _refused(handle, name, **change):
     calls = {
         "p2b_mx4_quantise": dict(x=p, stride=64, rows=4, width=64, dtype=0, values=p, scales=p, stream=None),
         "p2b_mx4_dequantise": dict(values=p, scales=p, rows=4, width=64, dtype=0, out=p, stride=64, stream=None),
+        "p2b_mx4_linear_mx4": dict(a=p, sa=p, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, values=p, scales=p, stream=None),
         "p2b_mx4_linear_few": dict(x=p, xs=64, xdtype=0, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
         "p2b_mx4_linear": dict(a=p, sa=p, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
     }
@@ -138,6 +139,12 @@ def test_mx4_linear_refuses(handle, change):
                                     dict(xdtype=2, x=(2,)), dict(out=(1,)), dict(bias=(1,))])
 def test_mx4_linear_few_refuses(handle, change):
     assert _refused(handle, "p2b_mx4_linear_few", **change)
+
+
+@pytest.mark.parametrize("change", MATRIX + [dict(dtype=2), dict(act=3), dict(columns=0), dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(values=None),
+                                             dict(scales=None), dict(values=(8,)), dict(scales=(4,)), dict(a=(8,)), dict(bias=(1,)), dict(rows=1 << 30, columns=1 << 20)])
+def test_mx4_linear_mx4_refuses(handle, change):
+    assert _refused(handle, "p2b_mx4_linear_mx4", **change)
 
 
 def test_mx4_sizes(handle):
