@@ -401,7 +401,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                     if (out)
                         for (int p = 0; p < (kMode == kGradients ? 2 : 1); ++p)
                             copy_panel(panels + (kMode == kForward ? j : p) * kPanelBytes, quadrant * 32, part, 4, out, stride, first, rows, col + 64 * p, columns,
-                                       alignment >= 4, lane);
+                                       alignment, lane);
                 }
                 if (kMode == kGradHidden && args.parts == 2) {  // what the rounding left, behind dgate | dup
                     float lower[16], upper[16];

@@ -171,15 +171,26 @@ template <bool kBf16, int kCount> __device__ __forceinline__ void put_panel(uint
                        pack<kBf16>(v[8 * i + 6], v[8 * i + 7]));
     }
 }
-// 32 rows of a panel, from r0 on, by `warps` warps to a matrix whose rows start on no 16-byte boundaries: a row an instruction.
+// 32 rows of a panel, from r0 on, by `warps` warps to a matrix whose rows start on no 16-byte boundaries: two rows an instruction where
+// they start on 8-byte ones, else one.
 __device__ __forceinline__ void copy_panel(const uint8_t* panel, int r0, int warp, int warps, void* out, int64_t stride, int64_t row, int64_t rows, int col,
-                                           int columns, bool pairs, int lane) {
+                                           int columns, int alignment, int lane) {
+    if (alignment >= 8 && col + 64 <= columns) {
+        const int c = lane % 16;
+        uint16_t* p = reinterpret_cast<uint16_t*>(out) + (row + lane / 16 + 2 * warp) * stride + col + 4 * c;
+#pragma unroll 4
+        for (int i = 2 * warp + lane / 16; i < 32; i += 2 * warps, p += 2 * warps * stride) {
+            const int r = r0 + i;
+            if (row + i < rows) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(panel + r * 128 + ((c / 2) ^ (r & 7)) * 16 + c % 2 * 8);
+        }
+        return;
+    }
     for (int i = warp; i < 32 && row + i < rows; i += warps) {
         const int r = r0 + i;
         const uint32_t two = *reinterpret_cast<const uint32_t*>(panel + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4);
         uint16_t* p = reinterpret_cast<uint16_t*>(out) + (row + i) * stride + col + 2 * lane;
         const int left = columns - col - 2 * lane;
-        if (pairs && left >= 2) {
+        if (alignment >= 4 && left >= 2) {
             *reinterpret_cast<uint32_t*>(p) = two;
         } else {
             if (left >= 1) p[0] = (uint16_t)two;

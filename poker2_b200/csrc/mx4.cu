@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
                 }
             } else {
                 __syncwarp();
-                copy_panel(panel, quadrant * 32, 0, 1, args.out, args.out_stride, row0, args.rows, col, args.columns, args.align_out >= 4, lane);
+                copy_panel(panel, quadrant * 32, 0, 1, args.out, args.out_stride, row0, args.rows, col, args.columns, args.align_out, lane);
             }
         }
         if (lane == 0) store_wait();
@@ -593,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1) mx4_p
                 }
             } else {
                 __syncwarp();
-                copy_panel(panel, quadrant * 32, 0, 1, args.out, args.out_stride, row0, args.rows, col, args.columns, args.align_out >= 4, lane);
+                copy_panel(panel, quadrant * 32, 0, 1, args.out, args.out_stride, row0, args.rows, col, args.columns, args.align_out, lane);
                 __syncwarp();
             }
         }

@@ -76,7 +76,7 @@ def test_strides_and_shapes(cuda_device):
 @pytest.mark.parametrize("activation", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("dtype", TYPES[:2])
 @pytest.mark.parametrize("rows,width,columns", [(1, 1536, 1536), (1, 32, 1), (2, 31, 7), (4, 1023, 9), (3, 2720, 130), (4, 1025, 16), (5, 1025, 16), (33, 256, 128), (128, 300, 129), (129, 64, 40),
-                                                (200, 2720, 333), (385, 1000, 257), (600, 513, 2652),
+                                                (200, 2720, 333), (385, 1000, 257), (600, 513, 2652), (3001, 128, 2652), (2800, 64, 1330),
                                                 (1700, 300, 1500), (2500, 512, 1031), (5000, 64, 700)])
 def test_linear(cuda_device, rows, width, columns, dtype, activation):
     g = torch.Generator(device=cuda_device).manual_seed(rows + width + columns)
