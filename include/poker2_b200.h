@@ -515,11 +515,17 @@ int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, con
 int p2b_mx4_linear_mx4(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales,
                        int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out_values,
                        void* out_scales, void* stream);
-/* The same (written out) of at most p2b_mx4_few_rows() rows of x (x_dtype 0 bf16, 1 fp16, 2 fp32), quantised on the way, in one launch. */
+/* The same (written out) of rows of x that are not quantised yet (x_dtype 0 bf16, 1 fp16, 2 fp32; any alignment), in one call: scratch of
+ * p2b_mx4_linear_rows_scratch_bytes(rows, width), 16-byte aligned, takes the quantised rows.  p2b_mx4_linear_few: at most
+ * p2b_mx4_few_rows() rows, without scratch and in one launch, as p2b_mx4_linear_rows does it. */
 int p2b_mx4_few_rows(void);
 int p2b_mx4_linear_few(const void* x, int64_t x_stride, int32_t x_dtype, int64_t rows, const void* w_values, const void* w_scales,
                        int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out,
                        int64_t out_stride, void* stream);
+int64_t p2b_mx4_linear_rows_scratch_bytes(int64_t rows, int32_t width);
+int p2b_mx4_linear_rows(const void* x, int64_t x_stride, int32_t x_dtype, int64_t rows, const void* w_values, const void* w_scales,
+                        int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out,
+                        int64_t out_stride, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* Clipped policy loss with a KL term over the hands of a batch of states, and its gradient.  Per state and hand, over the legal
  * actions a, p = softmax(logits) and q = old_policy:

@@ -84,6 +84,7 @@ _SIGNATURES = {
     "p2b_mx4_dequantise": [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp],
     "p2b_mx4_linear": [_vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp],
     "p2b_mx4_linear_mx4": [_vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp],
+    "p2b_mx4_linear_rows": [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
     "p2b_mx4_linear_few": [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp],
     "p2b_policy_loss": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, ctypes.c_double, _f32, _vp, _vp, _vp, _i64, _vp],
     "p2b_policy_loss_scale": [_vp, _vp, _i64, _i32, _vp, _vp],
@@ -96,7 +97,7 @@ _VALUE_FUNCS = {"p2b_cfr_scratch_floats": ([_i32, _i32], _i64), "p2b_cfr_default
                 "p2b_cfr_solve_block_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_step_scratch_floats": ([_i32, _i32, _i64], _i64),
                 "p2b_gated_few_rows": ([], _i32), "p2b_gated_align_bytes": ([_i64, _i32, _i32], _i64), "p2b_gated_backward_scratch_bytes": ([_i64, _i32, _i32], _i64),
-                "p2b_mx4_few_rows": ([], _i32), "p2b_mx4_value_bytes": ([_i64, _i32], _i64), "p2b_mx4_scale_bytes": ([_i64, _i32], _i64),
+                "p2b_mx4_few_rows": ([], _i32), "p2b_mx4_linear_rows_scratch_bytes": ([_i64, _i32], _i64), "p2b_mx4_value_bytes": ([_i64, _i32], _i64), "p2b_mx4_scale_bytes": ([_i64, _i32], _i64),
                 "p2b_policy_loss_scratch_bytes": ([_i64, _i32], _i64),
                 "p2b_cfr_noalloc_scratch_floats": ([], _i64), "p2b_cfr_path_policy": ([_i32], _i32)}
 

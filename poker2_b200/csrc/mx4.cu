@@ -741,14 +741,20 @@ extern "C" int64_t p2b_mx4_scale_bytes(int64_t rows, int32_t width) {
     return rows < 0 || width < 1 ? -1 : blocks_of(rows, 128) * scale_pieces(width) * 512;
 }
 
-extern "C" int p2b_mx4_quantise(const void* x, int64_t x_stride, int64_t rows, int32_t width, int32_t dtype, void* values, void* scales, void* stream) {
-    int rc = check_matrix("p2b_mx4_quantise", rows, width);
+static int check_source(const char* name, const void* x, int64_t x_stride, int64_t rows, int32_t width, int32_t dtype) {
+    int rc = check_matrix(name, rows, width);
     if (rc) return rc;
-    if (dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: unknown type %d (0 bf16, 1 fp16, 2 fp32)", dtype);
-    if (rows == 0) return P2B_OK;
-    if (!x || !values || !scales || x_stride < 0) return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: null array or negative stride");
-    if (((uintptr_t)values % 16) || ((uintptr_t)scales % 16) || (uintptr_t)x % (dtype == 2 ? 4 : 2))
-        return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: values and scales must lie on 16-byte boundaries, x on its element's");
+    if (dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "%s: unknown type %d (0 bf16, 1 fp16, 2 fp32)", name, dtype);
+    if (rows > 0 && (!x || x_stride < 0 || (uintptr_t)x % (dtype == 2 ? 4 : 2)))
+        return set_error(P2B_ERR_ARG, "%s: x must lie on its elements' boundaries, its rows no negative number apart", name);
+    return P2B_OK;
+}
+
+extern "C" int p2b_mx4_quantise(const void* x, int64_t x_stride, int64_t rows, int32_t width, int32_t dtype, void* values, void* scales, void* stream) {
+    int rc = check_source("p2b_mx4_quantise", x, x_stride, rows, width, dtype);
+    if (rc || rows == 0) return rc;
+    if (!values || !scales || ((uintptr_t)values % 16) || ((uintptr_t)scales % 16))
+        return set_error(P2B_ERR_ARG, "p2b_mx4_quantise: values and scales must lie on 16-byte boundaries");
     const int vector = (uintptr_t)x % 16 == 0 && x_stride % (dtype == 2 ? 4 : 8) == 0;
     const unsigned grid = warp_grid(blocks_of(rows, 128) * 128 * blocks_of(width, 512 * kWide));
     cudaStream_t st = (cudaStream_t)stream;
@@ -803,9 +809,9 @@ extern "C" int p2b_mx4_linear_few(const void* x, int64_t x_stride, int32_t x_dty
     return x_dtype == 0 ? few(__nv_bfloat16()) : x_dtype == 1 ? few(__half()) : few(0.0f);
 }
 
-static int linear_of_quantised(const char* name, const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
-                              int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* out_values, void* out_scales,
-                              void* stream) {
+static int prepare_linear(const char* name, Mx4Args& args, const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales,
+                          int32_t columns, int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* out_values,
+                          void* out_scales) {
     const bool quantised = out_values || out_scales;
     int rc = check_matrix(name, rows, width);
     if (!rc) rc = check_matrix(name, columns, width);
@@ -822,7 +828,6 @@ static int linear_of_quantised(const char* name, const void* a_values, const voi
     for (const void* p : {a_values, a_scales, w_values, w_scales, (const void*)out_values, (const void*)out_scales})
         if ((uintptr_t)p % 16) return set_error(P2B_ERR_ARG, "%s: values and scales must lie on 16-byte boundaries", name);
     if ((uintptr_t)out % 2 || (uintptr_t)bias % 2) return set_error(P2B_ERR_ARG, "%s: out and bias must lie on 2-byte boundaries", name);
-    Mx4Args args{};
     const int64_t row_bytes = blocks_of(width, 32) * 16;
     rc = encode_rows(&args.a, a_values, 1, row_bytes, rows, row_bytes, kTile);
     if (!rc) rc = encode_rows(&args.w, w_values, 1, row_bytes, columns, row_bytes, kTile);
@@ -843,11 +848,15 @@ static int linear_of_quantised(const char* name, const void* a_values, const voi
     const int edge = args.pairs ? 256 : kTile;
     args.tiles_m = (int)blocks_of(rows, edge), args.tiles_n = (int)blocks_of(columns, edge);
     args.vector_bias = aligned16(bias, 0);
+    return P2B_OK;
+}
+
+static int run_linear(const Mx4Args& args, int32_t dtype, int32_t activation, cudaStream_t stream) {
     auto launch = [&](auto type) {
         constexpr int kOut = decltype(type)::value;
-        auto* f = quantised ? (activation == 0 ? launch_linear<kOut, 0, true> : activation == 1 ? launch_linear<kOut, 1, true> : launch_linear<kOut, 2, true>)
-                            : (activation == 0 ? launch_linear<kOut, 0, false> : activation == 1 ? launch_linear<kOut, 1, false> : launch_linear<kOut, 2, false>);
-        return f(args, (cudaStream_t)stream);
+        auto* f = args.out_values ? (activation == 0 ? launch_linear<kOut, 0, true> : activation == 1 ? launch_linear<kOut, 1, true> : launch_linear<kOut, 2, true>)
+                                  : (activation == 0 ? launch_linear<kOut, 0, false> : activation == 1 ? launch_linear<kOut, 1, false> : launch_linear<kOut, 2, false>);
+        return f(args, stream);
     };
     return dtype == 0 ? launch(std::integral_constant<int, 0>()) : launch(std::integral_constant<int, 1>());
 }
@@ -855,13 +864,40 @@ static int linear_of_quantised(const char* name, const void* a_values, const voi
 extern "C" int p2b_mx4_linear(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
                               int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* stream) {
     if (rows > 0 && !out) return set_error(P2B_ERR_ARG, "p2b_mx4_linear: null array");
-    return linear_of_quantised("p2b_mx4_linear", a_values, a_scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, out, out_stride, nullptr, nullptr,
-                               stream);
+    Mx4Args args{};
+    const int rc = prepare_linear("p2b_mx4_linear", args, a_values, a_scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, out, out_stride, nullptr,
+                                  nullptr);
+    return rc || rows == 0 ? rc : run_linear(args, dtype, activation, (cudaStream_t)stream);
 }
 
 extern "C" int p2b_mx4_linear_mx4(const void* a_values, const void* a_scales, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
                                   int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out_values, void* out_scales, void* stream) {
     if (rows > 0 && (!out_values || !out_scales)) return set_error(P2B_ERR_ARG, "p2b_mx4_linear_mx4: null array");
-    return linear_of_quantised("p2b_mx4_linear_mx4", a_values, a_scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, nullptr, 0, out_values,
-                               out_scales, stream);
+    Mx4Args args{};
+    const int rc = prepare_linear("p2b_mx4_linear_mx4", args, a_values, a_scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, nullptr, 0, out_values,
+                                  out_scales);
+    return rc || rows == 0 ? rc : run_linear(args, dtype, activation, (cudaStream_t)stream);
+}
+
+extern "C" int64_t p2b_mx4_linear_rows_scratch_bytes(int64_t rows, int32_t width) {
+    if (rows < 0 || width < 1) return -1;
+    return rows <= kFewRows ? 0 : p2b_mx4_scale_bytes(rows, width) + p2b_mx4_value_bytes(rows, width);
+}
+
+extern "C" int p2b_mx4_linear_rows(const void* x, int64_t x_stride, int32_t x_dtype, int64_t rows, const void* w_values, const void* w_scales, int32_t columns,
+                                   int32_t width, const void* bias, int32_t dtype, int32_t activation, void* out, int64_t out_stride, void* scratch,
+                                   int64_t scratch_bytes, void* stream) {
+    if (rows <= kFewRows)
+        return p2b_mx4_linear_few(x, x_stride, x_dtype, rows, w_values, w_scales, columns, width, bias, dtype, activation, out, out_stride, stream);
+    int rc = check_source("p2b_mx4_linear_rows", x, x_stride, rows, width, x_dtype);
+    if (rc) return rc;
+    if (!scratch || (uintptr_t)scratch % 16 || scratch_bytes < p2b_mx4_linear_rows_scratch_bytes(rows, width))
+        return set_error(P2B_ERR_ARG, "p2b_mx4_linear_rows: scratch of %lld bytes on a 16-byte boundary is needed",
+                         (long long)p2b_mx4_linear_rows_scratch_bytes(rows, width));
+    uint8_t *scales = (uint8_t*)scratch, *values = scales + p2b_mx4_scale_bytes(rows, width);
+    // (the product's arguments are looked at before anything is launched)
+    Mx4Args args{};
+    rc = prepare_linear("p2b_mx4_linear_rows", args, values, scales, rows, w_values, w_scales, columns, width, bias, dtype, activation, out, out_stride, nullptr, nullptr);
+    if (!rc) rc = p2b_mx4_quantise(x, x_stride, rows, width, x_dtype, values, scales, stream);
+    return rc ? rc : run_linear(args, dtype, activation, (cudaStream_t)stream);
 }

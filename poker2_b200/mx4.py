@@ -99,14 +99,18 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
         if bias.dim() != 1 or bias.shape[0] != columns or bias.dtype != dtype or bias.get_device() != device:
             raise ValueError("the bias has one entry for each output, in the type of the result and on its device")
         bias = bias.contiguous()
-    if tensor and x.numel() <= FEW_ROWS * width and x.dtype in _TYPES and not quantised:
+    if tensor and not quantised and x.dtype in _TYPES:
         flat = x if x.dim() == 2 else x.reshape(-1, width)
         if width > 1 and flat.stride(1) != 1:
             flat = flat.contiguous()
         rows = flat.shape[0]
-        out = x.new_empty((rows, columns), dtype=dtype)
-        _lib.call_on(device, "p2b_mx4_linear_few", flat.data_ptr(), flat.stride(0), _TYPES[x.dtype], rows, weight.values.data_ptr(),
-                     weight.scales.data_ptr(), columns, width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, out.data_ptr(), columns)
+        out, scratch, size = x.new_empty((rows, columns), dtype=dtype), None, 0
+        if rows > FEW_ROWS:
+            size = (rows + 127) // 128 * ((width + 255) // 256) * 1024 + rows * ((width + 31) // 32 * 16)
+            scratch = x.new_empty((size,), dtype=torch.uint8)
+        _lib.call_on(device, "p2b_mx4_linear_rows", flat.data_ptr(), flat.stride(0), _TYPES[x.dtype], rows, weight.values.data_ptr(),
+                     weight.scales.data_ptr(), columns, width, None if bias is None else bias.data_ptr(), _TYPES[dtype], act, out.data_ptr(), columns,
+                     None if scratch is None else scratch.data_ptr(), size)
         return out if x.dim() == 2 else out.view(*x.shape[:-1], columns)
     a = quantise(x) if tensor else x
     if quantised:

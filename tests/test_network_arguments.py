@@ -106,6 +106,8 @@ def _refused(handle, name, **change):
         "p2b_mx4_quantise": dict(x=p, stride=64, rows=4, width=64, dtype=0, values=p, scales=p, stream=None),
         "p2b_mx4_dequantise": dict(values=p, scales=p, rows=4, width=64, dtype=0, out=p, stride=64, stream=None),
         "p2b_mx4_linear_mx4": dict(a=p, sa=p, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, values=p, scales=p, stream=None),
+        "p2b_mx4_linear_rows": dict(x=p, xs=64, xdtype=0, rows=40, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, scratch=p, size=4096,
+                                    stream=None),
         "p2b_mx4_linear_few": dict(x=p, xs=64, xdtype=0, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
         "p2b_mx4_linear": dict(a=p, sa=p, rows=4, w=p, sw=p, columns=8, width=64, bias=p, dtype=0, act=0, out=p, stride=8, stream=None),
     }
@@ -147,10 +149,19 @@ def test_mx4_linear_mx4_refuses(handle, change):
     assert _refused(handle, "p2b_mx4_linear_mx4", **change)
 
 
+@pytest.mark.parametrize("change", MATRIX[1:] + [dict(dtype=2), dict(act=3), dict(columns=0), dict(w=None), dict(sw=None), dict(out=None), dict(stride=7), dict(w=(8,)),
+                                                 dict(sw=(4,)), dict(out=(1,)), dict(bias=(1,)), dict(scratch=None), dict(scratch=(8,)), dict(size=1663),
+                                                 dict(x=None), dict(xs=-1), dict(xdtype=3), dict(x=(1,))])
+def test_mx4_linear_rows_refuses(handle, change):
+    assert _refused(handle, "p2b_mx4_linear_rows", **change)
+
+
 def test_mx4_sizes(handle):
     from poker2_b200 import mx4
 
     assert handle.p2b_mx4_few_rows() == mx4.FEW_ROWS
+    assert handle.p2b_mx4_linear_rows_scratch_bytes(4, 64) == 0 and handle.p2b_mx4_linear_rows_scratch_bytes(40, 65) == 1024 + 40 * 48
+    assert handle.p2b_mx4_linear_rows_scratch_bytes(-1, 64) == -1
     assert handle.p2b_mx4_value_bytes(3, 33) == 96 and handle.p2b_mx4_scale_bytes(129, 257) == 2 * 4 * 512
     assert handle.p2b_mx4_value_bytes(-1, 33) == -1 and handle.p2b_mx4_scale_bytes(1, 0) == -1
     assert handle.p2b_mx4_quantise(None, 0, 0, 64, 0, None, None, None) == 0
