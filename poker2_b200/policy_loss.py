@@ -85,20 +85,21 @@ class _Loss(torch.autograd.Function):
 
 
 def _packed(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
+    return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
 def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, with_grad):
     states, hands, actions = logits.shape
-    with torch.no_grad():
-        logits, old_policy, advantages, target, legal, weights = map(_packed, (logits, old_policy, advantages, target, legal, weights))
+    logits, target, legal = _packed(logits), _packed(target), _packed(legal)
+    old_policy, advantages, weights = _packed(old_policy), _packed(advantages), _packed(weights)
     loss = target.new_empty(())
     grad = logits.new_empty((states, hands, actions)) if with_grad else None
-    p = _lib.ptr
     size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
     scratch = target.new_empty((size // 4,)) if size else None
-    _lib.call_on(logits.get_device(), "p2b_policy_loss", logits.data_ptr(), p(old_policy), p(advantages), target.data_ptr(), legal.data_ptr(),
-                 p(weights), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(), p(grad), p(scratch), size)
+    _lib.call_on(logits.get_device(), "p2b_policy_loss", logits.data_ptr(), None if old_policy is None else old_policy.data_ptr(),
+                 None if advantages is None else advantages.data_ptr(), target.data_ptr(), legal.data_ptr(),
+                 None if weights is None else weights.data_ptr(), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(),
+                 None if grad is None else grad.data_ptr(), None if scratch is None else scratch.data_ptr(), size)
     return loss, grad
 
 
