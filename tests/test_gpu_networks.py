@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import network_refs as refs
-from poker2_b200 import chance, evaluator, leaf_eval, mx4, policy_loss, tree as ptree, upstream_adapter as ua
+from poker2_b200 import chance, evaluator, gated, leaf_eval, mx4, policy_loss, tree as ptree, upstream_adapter as ua
 from poker2_b200.replay import ReplayRing
 
 pytestmark = pytest.mark.gpu
@@ -184,3 +184,39 @@ def test_policy_loss_of_batches_without_rows_or_targets(cuda_device):
     assert ua.RebelBatchLike(view, legal, policy_targets=none).policy_loss(none.clone().requires_grad_(True)).item() == 0.0
     with pytest.raises(ValueError, match="targets"):
         ua.RebelBatchLike(view, legal).policy_loss(none)
+
+
+def test_threads_that_have_made_no_call_yet(cuda_device):
+    """A thread's first call finds memory in the allocator's cache, so that no call of the runtime has gone before the operator's."""
+    import threading
+
+    x, dh = (torch.randn(300, 256, device=cuda_device).bfloat16() for _ in range(2))
+    wg, wu = (torch.randn(256, 256, device=cuda_device).div(16).bfloat16() for _ in range(2))
+    rows, weight = mx4.quantise(x), mx4.quantise(wg)
+    weights, state = torch.rand(3, 1326, device=cuda_device), [torch.randn(3, 1326, 4, device=cuda_device) for _ in range(4)]
+    calls = {
+        "gated_linear": lambda: gated.gated_linear(x, wg, wu), "few rows": lambda: gated.gated_linear(x[:2], wg, wu),
+        "gated_linear_backward": lambda: torch.cat(gated.gated_linear_backward(dh, x, wg, wu)[:3]),
+        "linear": lambda: mx4.linear(rows, weight), "linear of rows": lambda: mx4.linear(x, weight), "few": lambda: mx4.linear(x[:2], weight),
+        "quantised": lambda: mx4.linear(rows, weight, quantised=True).values, "quantise": lambda: mx4.quantise(x).values,
+        "dequantise": lambda: rows.dequantise(),
+        "loss": lambda: policy_loss.clipped_policy_loss_and_grad(*[state[0], state[1].softmax(-1), state[2], state[3].softmax(-1)],
+                                                                torch.ones(3, 4, dtype=torch.bool, device=cuda_device), weights)[1],
+    }
+    for name, call in calls.items():
+        want, got = call().clone(), {}
+        call()
+
+        def work():
+            try:
+                got["value"] = call()
+            except RuntimeError as error:
+                got["value"] = str(error)
+
+        torch.cuda.synchronize()
+        thread = threading.Thread(target=work)
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert not isinstance(got["value"], str), (name, got["value"])
+        assert torch.equal(got["value"], want), name
