@@ -476,19 +476,22 @@ int p2b_indexed_add_rows(float* out, const int64_t* index, const float* src, int
  * p2b_gated_backward: gradients of sum(grad_h * h); where rows * width * hidden is above 2^24, dgate = grad_h * up * act' and
  * dup = grad_h * act are rounded to the type once on their way into the products of dx, dwg and dwu (fp16: they end at 65504).  dx [rows,width] (dx_stride), dwg and dwu [hidden,width], dbg and dbu [hidden]
  * packed; any of the five may be NULL.  scratch: p2b_gated_backward_scratch_bytes(rows, width, hidden), 16-byte aligned.
- * The same inputs give the same bits. */
+ * kept (NULL: none): an area of p2b_gated_kept_bytes(rows, width, hidden) bytes, 16-byte aligned, in which the forward pass leaves gate
+ * and up for the backward pass of the same inputs, which then need not take the projections again; NULL where that is 0.
+ * The same inputs give the same bits, with and without it. */
 int p2b_gated_few_rows(void);
 int p2b_gated_forward(const void* x, int64_t x_stride, const void* gate_weight, int64_t gate_stride,
                       const void* up_weight, int64_t up_stride, const void* gate_bias, const void* up_bias,
                       int64_t rows, int32_t width, int32_t hidden, int32_t dtype, int32_t activation, void* h,
-                      int64_t h_stride, void* scratch, int64_t scratch_bytes, void* stream);
+                      int64_t h_stride, void* kept, void* scratch, int64_t scratch_bytes, void* stream);
+int64_t p2b_gated_kept_bytes(int64_t rows, int32_t width, int32_t hidden);
 int64_t p2b_gated_align_bytes(int64_t rows, int32_t width, int32_t hidden);
 int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t width, int32_t hidden);
 int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, int64_t x_stride,
                        const void* gate_weight, int64_t gate_stride, const void* up_weight, int64_t up_stride,
                        const void* gate_bias, const void* up_bias, int64_t rows, int32_t width, int32_t hidden,
                        int32_t dtype, int32_t activation, void* dx, int64_t dx_stride, void* dwg, void* dwu,
-                       void* dbg, void* dbu, void* scratch, int64_t scratch_bytes, void* stream);
+                       void* dbg, void* dbu, const void* kept, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* Microscaled 4-bit values: a row in blocks of 32, each with a power-of-two scale, the smallest that brings the block's largest
  * magnitude to 6 or below; values are the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, ties to the even code.  A

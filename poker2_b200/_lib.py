@@ -77,9 +77,9 @@ _SIGNATURES = {
     "p2b_mean_over_hand_perms": [_vp, _vp, _i32, _i64, _vp, _vp],
     "p2b_tree_count": [_vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp],
     "p2b_tree_records": [_vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
-    "p2b_gated_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
+    "p2b_gated_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _i64, _vp],
     "p2b_gated_backward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp,
-                           _vp, _vp, _vp, _vp, _i64, _vp],
+                           _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "p2b_mx4_quantise": [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp],
     "p2b_mx4_dequantise": [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp],
     "p2b_mx4_linear": [_vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp],
@@ -96,7 +96,7 @@ _VALUE_FUNCS = {"p2b_cfr_scratch_floats": ([_i32, _i32], _i64), "p2b_cfr_default
                 "p2b_cfr_solve_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_solve_block_scratch_floats": ([_i32, _i32, _i32, _i32, _i64], _i64),
                 "p2b_cfr_step_scratch_floats": ([_i32, _i32, _i64], _i64),
-                "p2b_gated_few_rows": ([], _i32), "p2b_gated_align_bytes": ([_i64, _i32, _i32], _i64), "p2b_gated_backward_scratch_bytes": ([_i64, _i32, _i32], _i64),
+                "p2b_gated_few_rows": ([], _i32), "p2b_gated_kept_bytes": ([_i64, _i32, _i32], _i64), "p2b_gated_align_bytes": ([_i64, _i32, _i32], _i64), "p2b_gated_backward_scratch_bytes": ([_i64, _i32, _i32], _i64),
                 "p2b_mx4_few_rows": ([], _i32), "p2b_mx4_linear_rows_scratch_bytes": ([_i64, _i32], _i64), "p2b_mx4_value_bytes": ([_i64, _i32], _i64), "p2b_mx4_scale_bytes": ([_i64, _i32], _i64),
                 "p2b_policy_loss_scratch_bytes": ([_i64, _i32], _i64),
                 "p2b_cfr_noalloc_scratch_floats": ([], _i64), "p2b_cfr_path_policy": ([_i32], _i32)}

@@ -4,9 +4,9 @@
 // 256 columns, its operand half from Wg, half from Wu), so the activation and the product happen on the accumulators and
 // neither projection goes through memory.  Bound by the matrix instructions and what feeds them: 24576 rows of 1536 -> 1024 (155
 // GFLOP, 2 x 1024 x 1536 weights in L2) take 110 to 125 us, 1.24 to 1.41 PFLOP/s, at 13 TB/s out of L2.  The backward pass takes the
-// same products again instead of keeping gate and up in fp32, which would trade 4 rows x hidden x width operations for 22 bytes of
-// traffic a hidden value and 8 held over the whole step (even in time at width 1280).  Its first kernel ends in dgate = dh * up * act'(gate), dup = dh * act(gate) (16-bit, side by side in work space), from which
-// dx = dgate Wg + dup Wu, dWg = dgate^T x, dWu = dup^T x and the column sums follow.
+// same products again or, in large layers, finds gate and up in fp32 as the forward pass of the step kept them (`keeps` below).  From
+// them come dgate = dh * up * act'(gate) and dup = dh * act(gate) (16-bit, side by side in work space), and from these
+// dx = dgate Wg + dup Wu, dWg = dgate^T x, dWu = dup^T x and the column sums.
 #include "layer.cuh"
 #include "tensor.cuh"
 
@@ -14,12 +14,13 @@ namespace p2b {
 
 using namespace tc;
 
-enum GatedMode { kForward = 0, kGradHidden = 1, kGradients = 2 };
+enum GatedMode { kForward = 0, kGradHidden = 1, kGradients = 2, kForwardKept = 3 };
 
 struct GatedArgs {
     CUtensorMap a, b0, b1;   // kForward, kGradHidden: x, Wg, Wu; kGradients: dgate | dup by rows, Wg, Wu
     CUtensorMap at, bt;      // kGradients: dgate | dup and x with the reduction along their rows
     CUtensorMap to, to_wg, to_wu;  // the outputs out, dwg, dwu, where their rows start on 16-byte boundaries
+    CUtensorMap kept;              // kForwardKept: gate and up in fp32, upper halves and then lower halves side by side
     const void *bias_gate, *bias_up, *grad_h;
     void *out, *dwg, *dwu;   // h, dgate | dup or dx; the gradients of the weights
     float* sums;             // column sums of dgate | dup over 32 rows each, left by kGradHidden for kGradients (NULL: not wanted)
@@ -75,11 +76,25 @@ __device__ __forceinline__ Biases stage_biases(const GatedArgs& args, uint16_t* 
     return {area, area + args.hidden_padded, args.hidden_padded, args.hidden_padded, true};
 }
 
+// Two fp32 numbers as their upper and their lower halves, and back.
+__device__ __forceinline__ void keep(float2 v, uint32_t& upper, uint32_t& lower) {
+    upper = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+    lower = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x5410);
+}
+__device__ __forceinline__ Two kept_pair(uint32_t upper, uint32_t lower) {
+    return Two(__uint_as_float(__byte_perm(lower, upper, 0x5410)), __uint_as_float(__byte_perm(lower, upper, 0x7632)));
+}
+__device__ __forceinline__ void put_words(uint8_t* panel, int r, int col, const uint32_t (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint4*>(panel + r * 128 + ((col / 8 + i) ^ (r & 7)) * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
 // 16 hidden columns of a warp's 32 rows, from the accumulators of gate and up to h (v[0..15]) or to dgate and dup (v[0..15], v[16..31]).
-// (grad: 16 columns of grad_h, loaded before the accumulators were waited for.)
+// (grad: 16 columns of grad_h, loaded before the accumulators were waited for; kept: kForwardKept, the halves of gate and up.)
 template <int kMode, bool kBf16, int kActivation>
 __device__ __forceinline__ void finish_hidden(const GatedArgs& args, const Biases& bias, const uint32_t (&grad)[8], uint32_t gate_at, uint32_t up_at,
-                                              int64_t row, int col, bool ok, float (&v)[32]) {
+                                              int64_t row, int col, bool ok, float (&v)[32], uint32_t (&kept)[4][8]) {
     uint32_t g[16], u[16], bg[8], bu[8];
     tmem_load_16(gate_at, g);
     tmem_load_16(up_at, u);
@@ -93,10 +108,15 @@ __device__ __forceinline__ void finish_hidden(const GatedArgs& args, const Biase
         const Two gate = Two(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])) + two_of<kBf16>(bg[i]);
         const Two up = Two(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])) + two_of<kBf16>(bu[i]);
         const Two a = activate<kActivation, kMode == kGradHidden>(gate, slope);
-        if (kMode == kForward) {
+        if (kMode == kForward || kMode == kForwardKept) {
             const float2 h = (a * up).apart();
             v[2 * i] = ok ? h.x : __int_as_float(0x7FC00000);
             v[2 * i + 1] = ok ? h.y : __int_as_float(0x7FC00000);
+            if (kMode == kForwardKept) {
+                const float2 gates = gate.apart(), ups = up.apart();
+                keep(ok ? gates : make_float2(__int_as_float(0x7FC00000), __int_as_float(0x7FC00000)), kept[0][i], kept[2][i]);
+                keep(ups, kept[1][i], kept[3][i]);
+            }
         } else {
             const Two dh = two_of<kBf16>(grad[i]);
             const float2 dgate = (dh * up * slope).apart(), dup = (dh * a).apart();
@@ -362,6 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                 group_sync(1 + quadrant, 128);
                 const int col = kMode == kGradients ? n * 256 + 128 * j : n * 128 + 64 * j;
                 float v[32];
+                uint32_t kept[4][8];
                 if (kMode == kGradients) {
                     uint32_t g[32];
                     tmem_load_32(from + 128 * j + 32 * part, g);
@@ -372,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                 } else {
                     float lower[16], upper[16];
                     const int c = 64 * j + 16 * part;
-                    finish_hidden<kMode, kBf16, kActivation>(args, bias, grad[j], from + c, from + 128 + c, row, n * 128 + c, ok, v);
+                    finish_hidden<kMode, kBf16, kActivation>(args, bias, grad[j], from + c, from + 128 + c, row, n * 128 + c, ok, v, kept);
                     split(v, lower, upper);
                     put_panel<kBf16>(panels + (kMode == kForward ? j : 0) * kPanelBytes, r, 16 * part, lower);
                     if (kMode == kGradHidden) put_panel<kBf16>(panels + kPanelBytes, r, 16 * part, upper);
@@ -388,7 +409,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                     if (storer) {
                         if (first < rows && out) {
                             const uint32_t src = smem_addr(panels) + quadrant * 4096;
-                            const int columns = kMode == kForward ? args.hidden : kMode == kGradHidden ? args.hidden_padded : args.width;
+                            const int columns = kMode == kForward || kMode == kForwardKept ? args.hidden : kMode == kGradHidden ? args.hidden_padded : args.width;
                             if (col < columns) tma_store_2d(map, col, (int)first, src + (kMode == kForward ? j : 0) * kPanelBytes);
                             if (kMode == kGradHidden) tma_store_2d(map, args.hidden_padded + col, (int)first, src + kPanelBytes);
                             if (kMode == kGradients && col + 64 < columns) tma_store_2d(map, col + 64, (int)first, src + kPanelBytes);
@@ -397,12 +418,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_p
                     }
                 } else {
                     group_sync(1 + quadrant, 128);
-                    const int columns = kMode == kForward ? args.hidden : args.width;
+                    const int columns = kMode == kForward || kMode == kForwardKept ? args.hidden : args.width;
                     if (out)
                         for (int p = 0; p < (kMode == kGradients ? 2 : 1); ++p)
                             copy_panel(panels + (kMode == kForward ? j : p) * kPanelBytes, quadrant * 32, part, 4, out, stride, first, rows, col + 64 * p, columns,
                                        alignment, lane);
                 }
+                if (kMode == kForwardKept)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {  // the upper halves of gate and up, then the lower ones
+                        if (storer) store_wait_read<0>();
+                        group_sync(1 + quadrant, 128);
+                        put_words(panels, r, 16 * part, kept[2 * p]);
+                        put_words(panels + kPanelBytes, r, 16 * part, kept[2 * p + 1]);
+                        async_fence();
+                        group_sync(1 + quadrant, 128);
+                        if (storer) {
+                            const uint32_t src = smem_addr(panels) + quadrant * 4096;
+                            if (first < rows) {
+                                tma_store_2d(&args.kept, 2 * p * args.hidden_padded + col, (int)first, src);
+                                tma_store_2d(&args.kept, (2 * p + 1) * args.hidden_padded + col, (int)first, src + kPanelBytes);
+                            }
+                            store_commit();
+                        }
+                    }
                 if (kMode == kGradHidden && args.parts == 2) {  // what the rounding left, behind dgate | dup
                     float lower[16], upper[16];
                     split(v, lower, upper);
@@ -527,7 +566,8 @@ __global__ void __launch_bounds__(192, 1) gated_slim_kernel(const __grid_constan
         for (int j = 0; j < 2; ++j) {
             float v[32], lower[16], upper[16];
             const int col = n0 + 16 * j;
-            finish_hidden<kMode, kBf16, kActivation>(args, bias, grad[j], from + 16 * j, from + 32 + 16 * j, row, col, ok, v);
+            uint32_t none[4][8];
+            finish_hidden<kMode, kBf16, kActivation>(args, bias, grad[j], from + 16 * j, from + 32 + 16 * j, row, col, ok, v, none);
             split(v, lower, upper);
             if (row < args.rows) {
                 if (kMode == kForward) {
@@ -611,13 +651,69 @@ __global__ void __launch_bounds__(128) gated_few_kernel(const uint16_t* x, int64
         }
 }
 
+// dgate and dup (and their sums over 32 rows) from gate and up as the forward pass kept them, with the bits that kGradHidden would give:
+// the same numbers, the sums in the order of lane_sums.  A block takes 32 rows x 128 hidden columns, a thread 8 columns of rows ty
+// and ty + 16.  Bound by memory, 14 bytes a hidden value: 8192 x 1024 take 22 us, 5.3 TB/s.
+template <bool kBf16, int kActivation>
+__global__ void __launch_bounds__(256) gated_kept_kernel(const __grid_constant__ GatedArgs args, const uint16_t* kept) {
+    __shared__ float sums[8][16][17];  // half of the sixteen rows at a time, 8 columns of dgate and dup for each of 16 threads
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, col = blockIdx.x * 128 + 8 * tx;
+    const int64_t row0 = (int64_t)blockIdx.y * 32, wide = 4 * (int64_t)args.hidden_padded;
+    float total[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int64_t row = row0 + ty + 16 * k;
+        const bool inside = row < args.rows;
+        uint32_t dh[4], half[4][4];
+        load_words(reinterpret_cast<const uint16_t*>(args.grad_h) + row * args.grad_stride + col, inside ? args.hidden - col : 0, args.vector_in, dh);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) load_words(kept + row * wide + p * args.hidden_padded + col, inside ? 8 : 0, true, half[p]);
+        float d[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            Two slope;
+            const Two gate = kept_pair(half[0][i], half[2][i]), up = kept_pair(half[1][i], half[3][i]), grad = two_of<kBf16>(dh[i]);
+            const Two a = activate<kActivation, true>(gate, slope);
+            const float2 dgate = (grad * up * slope).apart(), dup = (grad * a).apart();
+            const bool first = inside && col + 2 * i < args.hidden, second = inside && col + 2 * i + 1 < args.hidden;
+            d[2 * i] = first ? dgate.x : 0.0f, d[2 * i + 1] = second ? dgate.y : 0.0f;
+            d[8 + 2 * i] = first ? dup.x : 0.0f, d[9 + 2 * i] = second ? dup.y : 0.0f;
+        }
+        if (inside) {
+            uint16_t* out = reinterpret_cast<uint16_t*>(args.out) + row * args.out_stride + col;
+            *reinterpret_cast<uint4*>(out) = make_uint4(pack<kBf16>(d[0], d[1]), pack<kBf16>(d[2], d[3]), pack<kBf16>(d[4], d[5]), pack<kBf16>(d[6], d[7]));
+            *reinterpret_cast<uint4*>(out + args.hidden_padded) =
+                make_uint4(pack<kBf16>(d[8], d[9]), pack<kBf16>(d[10], d[11]), pack<kBf16>(d[12], d[13]), pack<kBf16>(d[14], d[15]));
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total[i] = k == 0 ? d[i] : total[i] + d[i];
+    }
+    if (!args.sums) return;
+#pragma unroll
+    for (int o = 8; o > 0; o /= 2) {
+        if (ty >= o && ty < 2 * o)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[ty - o][tx][i] = total[i];
+        __syncthreads();
+        if (ty < o)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) total[i] += sums[ty][tx][i];
+        __syncthreads();
+    }
+    if (ty == 0) {
+        float* to = args.sums + (int64_t)blockIdx.y * 2 * args.hidden_padded + col;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = total[i], to[args.hidden_padded + i] = total[8 + i];
+    }
+}
+
 // (by itself where no other gradient is wanted)
 template <bool kBf16> __global__ void __launch_bounds__(512) bias_gradient_kernel(const __grid_constant__ GatedArgs args) {
     __shared__ float area[512];
     add_bias_gradients<kBf16>(args, area, blockIdx.x, gridDim.x);
 }
 
-static SharedLimit g_pair_limit[3][2][2], g_slim_limit[2][2][2];
+static SharedLimit g_pair_limit[4][2][2], g_slim_limit[2][2][2];
 
 template <int kMode, bool kBf16, int kActivation> static int launch_pairs(const GatedArgs& args, cudaStream_t stream) {
     auto* kernel = gated_pair_kernel<kMode, kBf16, kActivation>;
@@ -736,11 +832,27 @@ static int launch_few(const void* x, int64_t x_stride, const void* wg, int64_t w
     return check_cuda(cudaGetLastError(), "gated_few_kernel");
 }
 
+// Whether the forward pass of a training step keeps gate and up for the backward pass, or that takes the projections again.  Kept
+// they are 8 bytes a hidden value to write and to read, taken again 4 * width operations.  Both passes of 8192 rows to 1024, taken
+// again and kept: width 512 115 and 110 us, 1024 133 and 121, 1536 180 and 156, 2720 306 and 248.  Below a width of 1024 that is not
+// worth the memory, and below 2^33 products autograd takes longer on the host than the kernels (1000 rows of 1536 to 1024: 57 and 47 us
+// of kernels, 125 and 132 for the call).  The kernels that keep them are the pairs'.
+constexpr int kKeptWidth = 1024;
+constexpr int64_t kKeptProducts = 1ll << 33;
+static bool keeps(int64_t rows, int64_t width, int64_t hidden) {
+    return width >= kKeptWidth && rows * hidden >= blocks_of(kKeptProducts, width) && rows > kFewRows && !slim_tiles(rows, (int32_t)hidden);
+}
+
 }  // namespace p2b
 
 using namespace p2b;
 
 extern "C" int p2b_gated_few_rows(void) { return kFewRows; }
+
+extern "C" int64_t p2b_gated_kept_bytes(int64_t rows, int32_t width, int32_t hidden) {
+    if (rows < 0 || rows > kMostRows || width < 1 || width > kMostColumns || hidden < 1 || hidden > kMostColumns) return -1;
+    return keeps(rows, width, hidden) ? 8 * rows * blocks_of(hidden, 128) * 128 : 0;
+}
 
 extern "C" int64_t p2b_gated_align_bytes(int64_t rows, int32_t width, int32_t hidden) {
     return rows < 0 || rows > kMostRows || width < 1 || width > kMostColumns || hidden < 1 || hidden > kMostColumns ? -1 : align_bytes(rows, width, hidden);
@@ -748,11 +860,13 @@ extern "C" int64_t p2b_gated_align_bytes(int64_t rows, int32_t width, int32_t hi
 
 extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride,
                                  const void* bg, const void* bu, int64_t rows, int32_t width, int32_t hidden, int32_t dtype,
-                                 int32_t activation, void* h, int64_t h_stride, void* scratch, int64_t scratch_bytes, void* stream) {
+                                 int32_t activation, void* h, int64_t h_stride, void* kept, void* scratch, int64_t scratch_bytes, void* stream) {
     int rc = check_layer("p2b_gated_forward", x, x_stride, wg, wg_stride, wu, wu_stride, rows, width, hidden, dtype, activation);
     if (rc) return rc;
     if (rows == 0) return P2B_OK;
     if (!h || (rows > 1 && h_stride < hidden)) return set_error(P2B_ERR_ARG, "p2b_gated_forward: null output or rows that overlap");
+    if (kept && ((uintptr_t)kept % 16 || !p2b_gated_kept_bytes(rows, width, hidden)))
+        return set_error(P2B_ERR_ARG, "p2b_gated_forward: kept lies on a 16-byte boundary and is NULL where p2b_gated_kept_bytes is 0");
     const bool bf16 = dtype == 0;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows <= kFewRows) {
@@ -772,6 +886,13 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
     const bool slim = slim_tiles(rows, hidden);
     rc = hidden_maps(args, slim, at[0], stride[0], at[1], stride[1], at[2], stride[2]);
     if (!rc && !slim && args.align_out == 16) rc = encode_rows(&args.to, h, 2, hidden, rows, 2 * (rows > 1 ? h_stride : blocks_of(hidden, 8) * 8), 32);
+    if (!rc && kept) {
+        const int64_t wide = 4 * (int64_t)args.hidden_padded;
+        rc = encode_rows(&args.kept, kept, 2, wide, rows, 2 * wide, 32);
+        if (rc) return rc;
+        return activation == kGelu ? (bf16 ? launch_pairs<kForwardKept, true, kGelu>(args, st) : launch_pairs<kForwardKept, false, kGelu>(args, st))
+                                   : (bf16 ? launch_pairs<kForwardKept, true, kSilu>(args, st) : launch_pairs<kForwardKept, false, kSilu>(args, st));
+    }
     return rc ? rc : launch_hidden<kForward>(args, slim, bf16, activation, st);
 }
 
@@ -791,7 +912,7 @@ extern "C" int64_t p2b_gated_backward_scratch_bytes(int64_t rows, int32_t width,
 extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride,
                                   const void* wu, int64_t wu_stride, const void* bg, const void* bu, int64_t rows, int32_t width,
                                   int32_t hidden, int32_t dtype, int32_t activation, void* dx, int64_t dx_stride, void* dwg, void* dwu,
-                                  void* dbg, void* dbu, void* scratch, int64_t scratch_bytes, void* stream) {
+                                  void* dbg, void* dbu, const void* kept, void* scratch, int64_t scratch_bytes, void* stream) {
     int rc = check_layer("p2b_gated_backward", x, x_stride, wg, wg_stride, wu, wu_stride, rows, width, hidden, dtype, activation);
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
@@ -807,6 +928,8 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     if (!scratch || ((uintptr_t)scratch % 16) != 0 || scratch_bytes < p2b_gated_backward_scratch_bytes(rows, width, hidden))
         return set_error(P2B_ERR_ARG, "p2b_gated_backward: scratch of %lld bytes on a 16-byte boundary is needed",
                          (long long)p2b_gated_backward_scratch_bytes(rows, width, hidden));
+    if (kept && ((uintptr_t)kept % 16 || !p2b_gated_kept_bytes(rows, width, hidden)))
+        return set_error(P2B_ERR_ARG, "p2b_gated_backward: kept lies on a 16-byte boundary and is NULL where p2b_gated_kept_bytes is 0");
     const bool bf16 = dtype == 0;
     const int64_t whole = blocks_of(width, 8) * 8, own = p2b_gated_backward_scratch_bytes(rows, width, hidden);
     const void* at[3] = {x, wg, wu};
@@ -826,15 +949,30 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
     args.bias_gate = bg, args.bias_up = bu, args.grad_h = grad_h, args.grad_stride = grad_stride;
     args.vector_in = aligned16(grad_h, rows > 1 ? grad_stride : 0), args.vector_bias = aligned16(bg, 0) && aligned16(bu, 0);
     args.out = scratch, args.out_stride = wide;
-    const bool slim = slim_tiles(rows, args.hidden_padded);
-    rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
-    // every column of the work space is written, those behind the last hidden unit as zeros
-    args.tiles_n = args.hidden_padded / (slim ? 32 : 128);
-    args.tiles = (int)blocks_of(rows, slim ? kRows : 256) * args.tiles_n;
-    args.align_out = 16;
-    if (!rc && !slim) rc = encode_rows(&args.to, scratch, 2, wide, rows, 2 * wide, 32);
-    if (!rc) rc = launch_hidden<kGradHidden>(args, slim, bf16, activation, st);
-    if (rc) return rc;
+    if (kept) {
+        auto* kernel = activation == kGelu ? (bf16 ? gated_kept_kernel<true, kGelu> : gated_kept_kernel<false, kGelu>)
+                                           : (bf16 ? gated_kept_kernel<true, kSilu> : gated_kept_kernel<false, kSilu>);
+        for (int64_t done = 0; done < rows; done += 32ll * 65535) {  // (blocks of 32 rows, 65,535 to a launch)
+            GatedArgs part = args;
+            part.rows = rows - done < 32ll * 65535 ? rows - done : 32ll * 65535;
+            part.grad_h = (const uint16_t*)grad_h + done * grad_stride;
+            part.out = (uint16_t*)scratch + done * wide;
+            if (args.sums) part.sums = args.sums + done / 32 * columns;
+            const dim3 grid((unsigned)(args.hidden_padded / 128), (unsigned)blocks_of(part.rows, 32));
+            kernel<<<grid, 256, 0, st>>>(part, (const uint16_t*)kept + done * 4 * args.hidden_padded);
+            if ((rc = check_cuda(cudaGetLastError(), "gated_kept_kernel"))) return rc;
+        }
+    } else {
+        const bool slim = slim_tiles(rows, args.hidden_padded);
+        rc = hidden_maps(args, slim, x, x_stride, wg, wg_stride, wu, wu_stride);
+        // every column of the work space is written, those behind the last hidden unit as zeros
+        args.tiles_n = args.hidden_padded / (slim ? 32 : 128);
+        args.tiles = (int)blocks_of(rows, slim ? kRows : 256) * args.tiles_n;
+        args.align_out = 16;
+        if (!rc && !slim) rc = encode_rows(&args.to, scratch, 2, wide, rows, 2 * wide, 32);
+        if (!rc) rc = launch_hidden<kGradHidden>(args, slim, bf16, activation, st);
+        if (rc) return rc;
+    }
     if (dx || dwg || dwu) {
         next.out = dx, next.out_stride = dx_stride, next.align_out = row_alignment(dx, rows > 1 ? dx_stride : 0);
         next.dwg = dwg, next.dwu = dwu, next.align_w = row_alignment((const void*)((uintptr_t)dwg | (uintptr_t)dwu), hidden > 1 ? width : 0);

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from poker2_b200 import gated
+from poker2_b200 import _lib, gated
 import network_refs as refs
 
 pytestmark = pytest.mark.gpu
@@ -235,3 +235,43 @@ def test_the_leaf_of_a_broadcast_input_gets_its_sum(cuda_device):
     got, = torch.autograd.grad(gated.gated_linear(row.expand(200, 72), wg, wu, bg, bu), row, dh)
     each = gated.gated_linear_backward(dh, x[:1].expand(200, 72), wg, wu, bg, bu)[0]
     assert torch.equal(got, each.sum(0))
+
+
+@pytest.mark.parametrize("dtype,activation", [(torch.bfloat16, "gelu"), (torch.float16, "silu")])
+@pytest.mark.parametrize("size,keeps", [
+    ((8192, 1024, 1024), True), ((8195, 1100, 1000), True), ((20001, 1027, 701), True), ((40, 65536, 4800), True),
+    ((8191, 1024, 1024), False), ((9000, 1016, 1024), False), ((512, 16392, 1024), False),
+])
+def test_what_the_forward_pass_keeps(cuda_device, size, keeps, dtype, activation):
+    """Gate and up as the forward pass left them give the bits that the projections taken again give."""
+    x, wg, wu, bg, bu, dh = _layer(*size, dtype, cuda_device)
+    assert (_lib.lib().p2b_gated_kept_bytes(*size) > 0) == keeps
+    if size[0] == 8195:
+        leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, bg, bu)]
+        got = torch.autograd.grad(gated.gated_linear(*leaves, activation=activation), leaves, dh)
+        for g, (name, (value, bound)) in zip(got, refs.gated_backward(dh, x, wg, wu, bg, bu, activation, dtype).items()):
+            refs.assert_within(g, value, bound, name)
+    x[2, 1], x[3, 0], dh[1, 0] = float("inf"), float("nan"), float("nan")
+    for bias in (True, False):
+        plain = (x, wg, wu, bg, bu) if bias else (x, wg, wu)
+        leaves = [t.clone().requires_grad_(True) for t in plain]
+        h = gated.gated_linear(*leaves, activation=activation)
+        assert torch.equal(h.detach().view(torch.int16), gated.gated_linear(*plain, activation=activation).view(torch.int16))
+        apart = gated.gated_linear_backward(dh, *plain, activation=activation)
+        for _ in range(2):
+            for a, b in zip(torch.autograd.grad(h, leaves, dh, retain_graph=True), apart):
+                assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+        for i, leaf in enumerate(leaves):  # one gradient by itself
+            (a,) = torch.autograd.grad(h, [leaf], dh, retain_graph=True)
+            assert torch.equal(a.view(torch.int16), apart[i].view(torch.int16))
+
+
+def test_kept_rows_beyond_one_launch(cuda_device):
+    rows, width, hidden = 65535 * 32 + 45, 1024, 5
+    x, wg, wu, bg, bu, dh = _layer(rows, width, hidden, torch.bfloat16, cuda_device)
+    assert _lib.lib().p2b_gated_kept_bytes(rows, width, hidden) > 1 << 31
+    leaves = [t.clone().requires_grad_(True) for t in (wg, wu, bg, bu)]
+    got = torch.autograd.grad(gated.gated_linear(x, *leaves), leaves, dh)
+    apart = gated.gated_linear_backward(dh, x, wg, wu, bg, bu, needs=(False, True, True, True, True))
+    for a, b in zip(got, apart[1:]):
+        assert torch.equal(a, b)

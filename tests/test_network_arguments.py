@@ -19,14 +19,14 @@ def _area():
 
 
 def _gated_forward(p, **change):
-    a = dict(x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=None, bu=None, rows=16, width=64, hidden=8, dtype=0, act=0, h=p, hs=8, scratch=None, size=0)
+    a = dict(x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=None, bu=None, rows=16, width=64, hidden=8, dtype=0, act=0, h=p, hs=8, kept=None, scratch=None, size=0)
     a.update(change)
     return [*a.values(), None]
 
 
 def _gated_backward(p, **change):
     a = dict(dh=p, ds=8, x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=None, bu=None, rows=16, width=64, hidden=8, dtype=0, act=0, dx=p, dxs=64,
-             dwg=None, dwu=None, dbg=None, dbu=None, scratch=p, size=None)
+             dwg=None, dwu=None, dbg=None, dbu=None, kept=None, scratch=p, size=None)
     a.update(change)
     if a["size"] is None:  # what the layer itself needs, nothing for copies
         a["size"] = max(0, _lib.lib().p2b_gated_backward_scratch_bytes(max(0, min(a["rows"], 1 << 29)), 64, 8))
@@ -37,13 +37,13 @@ LAYER = [dict(rows=-1), dict(rows=1 << 40), dict(width=0), dict(width=1 << 24), 
          dict(act=2), dict(x=None), dict(wg=None), dict(wu=None), dict(xs=63), dict(gs=8), dict(us=0), dict(rows=1 << 29, hidden=1 << 19)]
 
 
-@pytest.mark.parametrize("change", LAYER + [dict(h=None), dict(hs=7), dict(xs=65), dict(gs=68), dict(us=66)])
+@pytest.mark.parametrize("change", LAYER + [dict(h=None), dict(hs=7), dict(kept=64), dict(xs=65), dict(gs=68), dict(us=66)])
 def test_gated_forward_refuses(handle, change):
     area, p = _area()
     assert handle.p2b_gated_forward(*_gated_forward(p, **change)) == -1 and b"p2b_gated_forward" in handle.p2b_last_error()
 
 
-@pytest.mark.parametrize("change", LAYER + [dict(dh=None), dict(ds=7), dict(dxs=63), dict(scratch=None), dict(size=100), dict(xs=68), dict(us=65)])
+@pytest.mark.parametrize("change", LAYER + [dict(dh=None), dict(ds=7), dict(dxs=63), dict(scratch=None), dict(size=100), dict(kept=64), dict(xs=68), dict(us=65)])
 def test_gated_backward_refuses(handle, change):
     area, p = _area()
     assert handle.p2b_gated_backward(*_gated_backward(p, **change)) == -1 and b"p2b_gated_backward" in handle.p2b_last_error()
@@ -61,7 +61,11 @@ def test_gated_addresses_off_their_boundaries_are_refused(handle):
     assert handle.p2b_gated_forward(*_gated_forward(None, rows=0, wg=p, wu=p)) == 0  # no rows: nothing to do
     assert handle.p2b_gated_few_rows() == gated.FEW_ROWS
     for sizes in ((-1, 8, 8), (8, 0, 8), (8, 8, 0)):
-        assert handle.p2b_gated_backward_scratch_bytes(*sizes) == -1
+        assert handle.p2b_gated_backward_scratch_bytes(*sizes) == -1 and handle.p2b_gated_kept_bytes(*sizes) == -1
+    assert gated.KEPT_PRODUCTS == 8192 * 1024 * 1024 and handle.p2b_gated_kept_bytes(8192, 1024, 1024) == 8 * 8192 * 1024
+    assert handle.p2b_gated_kept_bytes(8192, 1024, 1025) == 8 * 8192 * 1152
+    for sizes in ((8191, 1024, 1024), (8192, 1024, 1023), (9000, 1016, 1024), (4, 1 << 19, 4800), (512, 1 << 16, 1024)):
+        assert handle.p2b_gated_kept_bytes(*sizes) == 0
 
 
 def test_gated_linear_wants_the_gpu():
