@@ -191,6 +191,8 @@ def call_on(device: int, name: str, *args) -> None:
     if device == _get_device():
         call(name, *args, _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
     else:
+        if device < 0:  # (what torch.cuda.device would take for the current one, and a kernel the host's addresses for its own)
+            raise ValueError(f"{name} requires CUDA tensors.")
         with torch.cuda.device(device):
             call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 

@@ -44,6 +44,8 @@ class Mx4:
         kind, values = _TYPES.get(dtype), self.values
         if kind is None:
             raise ValueError("values are read back in bf16, fp16 or fp32")
+        if values.get_device() < 0:
+            _lib.require_cuda(values, "dequantise")
         out, width = values.new_empty(self.shape, dtype=dtype), self.shape[-1]
         _lib.call_on(values.get_device(), "p2b_mx4_dequantise", values.data_ptr(), self.scales.data_ptr(), values.shape[0], width, kind,
                      out.data_ptr(), width)
@@ -91,6 +93,8 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
         raise ValueError("the result is bf16 or fp16")
     columns, width = weight.shape
     device = weight.values.get_device()
+    if device < 0:
+        _lib.require_cuda(weight.values, "mx4.linear")
     if len(x.shape) < 1 or x.shape[-1] != width or (x if tensor else x.values).get_device() != device:
         raise ValueError("x must have the weight's width and device")
     if columns == 0:
