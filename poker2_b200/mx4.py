@@ -7,6 +7,7 @@ or a NaN reads back as NaN.  For serving: there are no gradients.  `leaf_eval.Mx
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -46,10 +47,20 @@ class Mx4:
             raise ValueError("values are read back in bf16, fp16 or fp32")
         if values.get_device() < 0:
             _lib.require_cuda(values, "dequantise")
+        _check_layout(self)
         out, width = values.new_empty(self.shape, dtype=dtype), self.shape[-1]
         _lib.call_on(values.get_device(), "p2b_mx4_dequantise", values.data_ptr(), self.scales.data_ptr(), values.shape[0], width, kind,
                      out.data_ptr(), width)
         return out
+
+
+def _check_layout(m: Mx4) -> None:
+    """The arrays hold what `shape` says (a kernel reads as far as that goes)."""
+    values, scales, shape = m.values, m.scales, m.shape
+    width, rows = shape[-1], shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    if (values.nbytes != rows * ((width + 31) // 32 * 16) or scales.nbytes != (rows + 127) // 128 * ((width + 255) // 256) * 1024
+            or values.shape[0] != rows or not values.is_contiguous() or not scales.is_contiguous() or scales.get_device() != values.get_device()):
+        raise ValueError("the values and scales of a quantised matrix are packed, lie on one device and are as many as its shape says")
 
 
 def quantise(x: torch.Tensor) -> Mx4:
@@ -99,6 +110,9 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
         raise ValueError("x must have the weight's width and device")
     if columns == 0:
         raise ValueError("the weight has no row")
+    _check_layout(weight)
+    if not tensor:
+        _check_layout(x)
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != columns or bias.dtype != dtype or bias.get_device() != device:
             raise ValueError("the bias has one entry for each output, in the type of the result and on its device")

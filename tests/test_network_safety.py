@@ -39,3 +39,42 @@ def test_calls_without_a_device_are_refused(launches):
     with pytest.raises(ValueError, match="CUDA"):
         _lib.call_on(-1, "p2b_mx4_quantise")
     assert not launches
+
+
+class _Elsewhere(torch.Tensor):
+    """A CPU tensor that says it lies on a GPU."""
+
+    def get_device(self):
+        return 0
+
+
+def _there(m):
+    return mx4.Mx4(m.values.as_subclass(_Elsewhere), m.scales.as_subclass(_Elsewhere), m.shape)
+
+
+def test_matrices_smaller_than_they_say_are_refused(launches):
+    good = _there(_quantised(40, 300))
+    mx4.linear(good, good)
+    mx4.linear(good, good, quantised=True)
+    good.dequantise()
+    row = _there(_quantised(1, 300))
+    row.shape = (300,)
+    assert row.dequantise().shape == (300,)
+    assert launches == ["p2b_mx4_linear", "p2b_mx4_linear_mx4", "p2b_mx4_dequantise", "p2b_mx4_dequantise"]
+    launches.clear()
+    v, s = good.values, good.scales
+    for values, scales, shape in ((v[:39], s, (40, 300)), (v, s[:-1], (40, 300)), (v, s, (41, 300)), (v, s, (2, 21, 300)), (v, s, (40, 321)), (v, s, (40, 513)),
+                                  (torch.zeros(40, 320, dtype=torch.uint8).as_subclass(_Elsewhere)[:, ::2], s, (40, 300)),
+                                  (v, torch.zeros(4096, dtype=torch.uint8).as_subclass(_Elsewhere)[::2], (40, 300)), (v, torch.zeros(2048, dtype=torch.uint8), (40, 300)),
+                                  (v.view(80, 80), s, (40, 300))):
+        bad, width = mx4.Mx4(values, scales, shape), shape[-1]
+        with pytest.raises(ValueError, match="shape says"):
+            bad.dequantise()
+        other = _there(_quantised(40, width))
+        for call in (lambda: mx4.linear(bad, other), lambda: mx4.linear(bad, other, quantised=True)):
+            with pytest.raises(ValueError, match="shape says"):
+                call()
+        if len(shape) == 2:
+            with pytest.raises(ValueError, match="shape says"):
+                mx4.linear(other, bad)
+    assert not launches
