@@ -48,7 +48,8 @@ def clipped_policy_loss_and_grad(logits: torch.Tensor, old_policy: torch.Tensor 
 
 def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tensor) -> torch.Tensor:
     """[n, 1326] fp32: the chance that the player to act holds a hand, times the chance that the other player's range leaves it
-    open; 0 for hands with a card on the board.  beliefs [n, 2*1326], to_act [n], board [n, L] with -1 for cards not dealt."""
+    open; 0 for hands with a card on the board.  beliefs [n, 2*1326], to_act [n], board [n, L] with -1 for cards not dealt.  A state
+    whose player is neither 0 nor 1, or with a card above 51, has NaN for all its weights."""
     from .fused_cfr import unblocked_mass_triton
 
     _lib.require_cuda(beliefs, "hand_weights")
@@ -57,12 +58,15 @@ def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tenso
         raise ValueError("beliefs [n, 2652], to_act [n] and board [n, L] are wanted")
     device = beliefs.device
     ranges = beliefs.to(torch.float32).view(n, 2, NUM_HANDS)
-    actor, rows = to_act.to(device=device, dtype=torch.int64), torch.arange(n, device=device)
+    player, rows = to_act.to(device=device, dtype=torch.int64), torch.arange(n, device=device)
+    actor = player.clamp(0, 1)  # (an index outside would end the process's use of the device)
     held = ranges[rows, actor] * unblocked_mass_triton(ranges[rows, 1 - actor].contiguous()).clamp(min=0.0)
     c1, c2 = torch.triu_indices(52, 52, 1, device=device)
     board = board.to(device=device, dtype=torch.int64)
-    dealt = torch.zeros(n, 53, dtype=torch.bool, device=device).scatter_(1, torch.where(board >= 0, board, 52), True)
-    return torch.where(dealt[:, c1] | dealt[:, c2], 0.0, held)
+    dealt = torch.zeros(n, 53, dtype=torch.bool, device=device).scatter_(1, torch.where(board >= 0, board.clamp(max=52), 52), True)
+    undefined = ((player != actor) | (board > 51).any(dim=1))[:, None]
+    dealt |= undefined
+    return torch.where(dealt[:, c1] | dealt[:, c2], torch.where(undefined, float("nan"), 0.0), held)
 
 
 class _Loss(torch.autograd.Function):

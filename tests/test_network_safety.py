@@ -78,3 +78,30 @@ def test_matrices_smaller_than_they_say_are_refused(launches):
             with pytest.raises(ValueError, match="shape says"):
                 mx4.linear(other, bad)
     assert not launches
+
+
+def test_hand_weights_of_players_and_cards_that_do_not_exist(monkeypatch):
+    """An index outside its range is an error on the CPU and the end of the context on a GPU: such states' weights are NaN instead."""
+    from poker2_b200 import fused_cfr, policy_loss
+
+    c1, c2 = torch.triu_indices(52, 52, 1)
+    apart = ((c1[:, None] != c1) & (c1[:, None] != c2) & (c2[:, None] != c1) & (c2[:, None] != c2)).float()
+    monkeypatch.setattr(_lib, "require_cuda", lambda t, what: None)
+    monkeypatch.setattr(fused_cfr, "unblocked_mass_triton", lambda ranges: ranges @ apart)
+    beliefs = torch.rand(8, 2 * 1326)
+    to_act = torch.tensor([0, 1, 2, -1, 0, 1, 0, 7])
+    board = torch.tensor([[3, 9, 20, -1, -1]] * 8)
+    board[4, 1], board[5, 4], board[6, 3] = 52, 1 << 40, -7
+    got = policy_loss.hand_weights(beliefs, to_act, board)
+    wrong = torch.tensor([False, False, True, True, True, True, False, True])
+    assert got.dtype == torch.float32 and torch.isnan(got[wrong]).all()
+    assert torch.equal(got[~wrong], policy_loss.hand_weights(beliefs[~wrong], to_act[~wrong], board[~wrong]))
+    ranges = beliefs.view(8, 2, 1326)
+    for row in (0, 1, 6):
+        blocked = torch.zeros(1326, dtype=torch.bool)
+        for card in board[row].tolist():
+            blocked |= (c1 == card) | (c2 == card)
+        want = torch.where(blocked, 0.0, ranges[row, to_act[row]].double() * (ranges[row, 1 - to_act[row]].double() @ apart.double()))
+        # 1326 terms in fp32 and a product: 2^-24 each
+        assert ((got[row] - want).abs() <= want * 1400 * 2.0 ** -24).all()
+    assert policy_loss.hand_weights(beliefs[:0], to_act[:0], board[:0]).shape == (0, 1326)
