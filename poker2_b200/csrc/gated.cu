@@ -744,7 +744,7 @@ constexpr int64_t kMostRows = 1ll << 30;
 constexpr int kMostColumns = 1 << 20;
 
 static int check_layer(const char* name, const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride,
-                       int64_t rows, int32_t width, int32_t hidden, int32_t dtype, int32_t activation) {
+                       const void* bg, const void* bu, int64_t rows, int32_t width, int32_t hidden, int32_t dtype, int32_t activation) {
     if (rows < 0 || rows > kMostRows || width < 1 || width > kMostColumns || hidden < 1 || hidden > kMostColumns)
         return set_error(P2B_ERR_ARG, "%s: %lld rows, width %d, hidden %d are out of range", name, (long long)rows, width, hidden);
     // (tiles are counted in 32 bits)
@@ -753,6 +753,8 @@ static int check_layer(const char* name, const void* x, int64_t x_stride, const 
     if (dtype < 0 || dtype > 1) return set_error(P2B_ERR_ARG, "%s: unknown type %d (0 bf16, 1 fp16)", name, dtype);
     if (activation < 0 || activation > 1) return set_error(P2B_ERR_ARG, "%s: unknown activation %d (0 gelu, 1 silu)", name, activation);
     if ((rows > 0 && !x) || !wg || !wu) return set_error(P2B_ERR_ARG, "%s: null operand", name);
+    if ((uintptr_t)x % 2 || (uintptr_t)wg % 2 || (uintptr_t)wu % 2 || (uintptr_t)bg % 2 || (uintptr_t)bu % 2)
+        return set_error(P2B_ERR_ARG, "%s: an operand lies on no 2-byte boundary", name);
     if ((rows > 1 && x_stride < width) || (hidden > 1 && (wg_stride < width || wu_stride < width)))
         return set_error(P2B_ERR_ARG, "%s: rows overlap", name);
     return P2B_OK;
@@ -861,10 +863,11 @@ extern "C" int64_t p2b_gated_align_bytes(int64_t rows, int32_t width, int32_t hi
 extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg, int64_t wg_stride, const void* wu, int64_t wu_stride,
                                  const void* bg, const void* bu, int64_t rows, int32_t width, int32_t hidden, int32_t dtype,
                                  int32_t activation, void* h, int64_t h_stride, void* kept, void* scratch, int64_t scratch_bytes, void* stream) {
-    int rc = check_layer("p2b_gated_forward", x, x_stride, wg, wg_stride, wu, wu_stride, rows, width, hidden, dtype, activation);
+    int rc = check_layer("p2b_gated_forward", x, x_stride, wg, wg_stride, wu, wu_stride, bg, bu, rows, width, hidden, dtype, activation);
     if (rc) return rc;
     if (rows == 0) return P2B_OK;
     if (!h || (rows > 1 && h_stride < hidden)) return set_error(P2B_ERR_ARG, "p2b_gated_forward: null output or rows that overlap");
+    if ((uintptr_t)h % 2) return set_error(P2B_ERR_ARG, "p2b_gated_forward: the output lies on no 2-byte boundary");
     if (kept && ((uintptr_t)kept % 16 || !p2b_gated_kept_bytes(rows, width, hidden)))
         return set_error(P2B_ERR_ARG, "p2b_gated_forward: kept lies on a 16-byte boundary and is NULL where p2b_gated_kept_bytes is 0");
     const bool bf16 = dtype == 0;
@@ -913,8 +916,10 @@ extern "C" int p2b_gated_backward(const void* grad_h, int64_t grad_stride, const
                                   const void* wu, int64_t wu_stride, const void* bg, const void* bu, int64_t rows, int32_t width,
                                   int32_t hidden, int32_t dtype, int32_t activation, void* dx, int64_t dx_stride, void* dwg, void* dwu,
                                   void* dbg, void* dbu, const void* kept, void* scratch, int64_t scratch_bytes, void* stream) {
-    int rc = check_layer("p2b_gated_backward", x, x_stride, wg, wg_stride, wu, wu_stride, rows, width, hidden, dtype, activation);
+    int rc = check_layer("p2b_gated_backward", x, x_stride, wg, wg_stride, wu, wu_stride, bg, bu, rows, width, hidden, dtype, activation);
     if (rc) return rc;
+    for (const void* p : {grad_h, (const void*)dx, (const void*)dwg, (const void*)dwu, (const void*)dbg, (const void*)dbu})
+        if ((uintptr_t)p % 2) return set_error(P2B_ERR_ARG, "p2b_gated_backward: a gradient lies on no 2-byte boundary");
     cudaStream_t st = (cudaStream_t)stream;
     if (rows == 0) {  // no row: gradients of the weights are zero
         for (void* w : {dwg, dwu})

@@ -461,6 +461,8 @@ extern "C" int p2b_policy_loss_scale(const void* grad, const float* factor, int6
     if (n < 0 || dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "p2b_policy_loss_scale: %lld values of type %d", (long long)n, dtype);
     if (n == 0) return P2B_OK;
     if (!grad || !factor || !out) return set_error(P2B_ERR_ARG, "p2b_policy_loss_scale: null array");
+    if ((uintptr_t)factor % 4 || ((uintptr_t)grad | (uintptr_t)out) % (dtype == 2 ? 4 : 2))
+        return set_error(P2B_ERR_ARG, "p2b_policy_loss_scale: an array lies off its elements' boundaries");
     const int64_t each = dtype == 2 ? 4 : 8, whole = ((uintptr_t)grad | (uintptr_t)out) % 16 ? 0 : n / each * each;
     const int64_t blocks = blocks_of(n, 256 * each), most = 8 * sm_count();
     const unsigned grid = (unsigned)(blocks < most ? blocks : most);

@@ -105,3 +105,29 @@ def test_hand_weights_of_players_and_cards_that_do_not_exist(monkeypatch):
         # 1326 terms in fp32 and a product: 2^-24 each
         assert ((got[row] - want).abs() <= want * 1400 * 2.0 ** -24).all()
     assert policy_loss.hand_weights(beliefs[:0], to_act[:0], board[:0]).shape == (0, 1326)
+
+
+@pytest.fixture(scope="module")
+def handle():
+    from poker2_b200 import build
+
+    build.build()
+    return _lib.lib()
+
+
+def test_addresses_between_elements_are_refused(handle):
+    """An odd address would be a misaligned access of the kernel."""
+    import ctypes
+
+    area = (ctypes.c_char * 8192)()
+    p = (ctypes.addressof(area) + 63) // 64 * 64
+    for rows in (2, 16):
+        good = dict(x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=p, bu=p, rows=rows, width=64, hidden=8, dtype=0, act=0, h=p, hs=8, kept=None, scratch=p, size=1 << 20, stream=None)
+        for name in ("x", "wg", "wu", "bg", "bu", "h"):
+            assert handle.p2b_gated_forward(*{**good, name: p + 1}.values()) == -1 and b"2-byte" in handle.p2b_last_error(), name
+        good = dict(dh=p, ds=8, x=p, xs=64, wg=p, gs=64, wu=p, us=64, bg=p, bu=p, rows=rows, width=64, hidden=8, dtype=0, act=0, dx=p, dxs=64, dwg=p, dwu=p, dbg=p,
+                    dbu=p, kept=None, scratch=p, size=1 << 20, stream=None)
+        for name in ("dh", "x", "wg", "wu", "bg", "bu", "dx", "dwg", "dwu", "dbg", "dbu"):
+            assert handle.p2b_gated_backward(*{**good, name: p + 1}.values()) == -1 and b"2-byte" in handle.p2b_last_error(), name
+    for args in ((p + 1, p, 4, 0, p), (p, p + 2, 4, 0, p), (p, p, 4, 1, p + 1), (p + 2, p, 4, 2, p), (p, p, 4, 2, p + 2)):
+        assert handle.p2b_policy_loss_scale(*args, None) == -1 and b"boundaries" in handle.p2b_last_error()
