@@ -257,7 +257,8 @@ __device__ __forceinline__ void finish_block(const Mx4Args& args, const uint32_t
     }
 }
 // A row's 64 neighbouring results from column `col` on, quantised as mx4_quantise_kernel would: 32 bytes of values, two scales.  Rows behind
-// the last have scales of zero, columns behind the last are zeros by themselves (no weight, no bias).
+// the last have scales of zero; columns behind the last count as zeros (no weight, no bias: they are, but where the row holds a block that
+// is not finite).
 template <bool kBf16> __device__ __forceinline__ void store_quantised(const Mx4Args& args, int64_t row, int col, const uint32_t (&y)[2][16]) {
     using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
     if (col >= (args.columns + 255) / 256 * 256 || row >= (args.rows + 127) / 128 * 128) return;
@@ -271,8 +272,14 @@ template <bool kBf16> __device__ __forceinline__ void store_quantised(const Mx4A
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[i].w[k] = y[j][4 * i + k];
-            top = max(top, v[i].top());
         }
+        const int left = args.columns - col - 32 * j;
+        if (left < 32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i / 4].w[i % 4] &= (2 * i < left ? 0xFFFFu : 0u) | (2 * i + 1 < left ? 0xFFFF0000u : 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, v[i].top());
         const uint32_t byte = row < args.rows ? scale_byte(Eight<T>::magnitude(top)) : 0;
         const Two inverse(byte == 255u ? 0.0f : inverse_scale(byte));
 #pragma unroll
@@ -393,7 +400,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
         int turn = acc;
         for (int64_t tile = blockIdx.x + (int64_t)acc * gridDim.x; tile < tiles; tile += 2 * (int64_t)gridDim.x, turn += 2) {
             const int64_t row0 = tile / args.tiles_n * kTile + quadrant * 32;
-            const int col = (int)(tile % args.tiles_n) * kTile + 64 * half;
+            const int n = (int)(tile % args.tiles_n), col = n * kTile + 64 * half;
             const bool ok = mbar_wait(acc_full(acc), (uint32_t)(turn / 2) & 1, &given_up);
             tc_fence_after();
             if (!kQuantised && lane == 0) store_wait_read<0>();
@@ -414,10 +421,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx4_linear_kernel(const __grid_
             }
             if (kQuantised) {
                 store_quantised<kBf16>(args, row0 + lane, col, y);
-                // (the odd piece behind a last tile of 128 columns has none of its own)
-                if (col + 128 >= args.columns) {
+                // (the odd piece behind a last tile of 128 columns has no tile of its own)
+                if (n + 1 == args.tiles_n && n % 2 == 0) {
                     const uint32_t none[2][16] = {};
-                    if (col / 128 % 2 == 0) store_quantised<kBf16>(args, row0 + lane, col + 128, none);
+                    store_quantised<kBf16>(args, row0 + lane, col + 128, none);
                 }
                 continue;
             }
