@@ -87,6 +87,8 @@ _SIGNATURES = {
     "p2b_mx4_linear_rows": [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp, _i64, _vp],
     "p2b_mx4_linear_few": [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp],
     "p2b_policy_loss": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, ctypes.c_double, _f32, _vp, _vp, _vp, _i64, _vp],
+    "p2b_policy_loss_scaled": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, ctypes.c_double, _f32, _vp, _vp, _i32, _f32, _vp, _vp, _i64, _vp],
+    "p2b_policy_loss_scale_fp32": [_vp, _vp, _i64, _vp, _vp],
     "p2b_policy_loss_scale": [_vp, _vp, _i64, _i32, _vp, _vp],
     "p2b_selftest_division": [ctypes.c_uint64, ctypes.c_uint32, _vp, _vp, _vp],
     "p2b_selftest_division_sweep": [_vp, _vp, _vp],

@@ -44,6 +44,9 @@ struct LossArgs {
     uint64_t magic;   // ceil(2^64 / hands)
     float* loss;
     void* grad;
+    int wide;                // grad is fp32 whatever the logits are
+    float factor;            // of the gradient, times *factor_at (NULL: 1), before its only rounding
+    const float* factor_at;
 };
 
 __device__ __forceinline__ double block_sum(double v, double* area) {
@@ -165,7 +168,8 @@ __device__ __noinline__ uint32_t settle_hand(const T* z, const float* old, const
 }
 
 // Blocks stay: each takes every gridDim.x-th tile of 256 hands, with the tiles after the present one on their way into the other
-// two of three stages (two stages in all: 225 us instead of 146 for the states above).  The gradient overwrites the logits of its stage and leaves from there.
+// two of three stages (two stages in all: 225 us instead of 146 for the states above).  The gradient overwrites the logits (in fp32: the
+// targets) of its stage and leaves from there.
 template <int kActions, typename T>
 __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_constant__ LossArgs args) {
     extern __shared__ __align__(16) uint8_t area[];
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
         }
     }
     mass = block_sum(mass, sums);
-    const float inverse = mass > 0.0 ? (float)(1.0 / mass) : 0.0f;
+    const float inverse = mass > 0.0 ? (float)(1.0 / mass) : 0.0f, share = inverse * (args.factor_at ? args.factor * *args.factor_at : args.factor);
     const float low_end = (float)(1.0 - args.clip), high_end = (float)(1.0 + args.clip);
 
     double loss_sum = 0.0;
@@ -286,7 +290,7 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                     divergence = t[a] > 0.0f ? more : divergence;
                 }
                 divergence = 0.69314718055994531f * fmaf(targets, log_two(total), divergence);
-                const float rcp = reciprocal(total), scale = weight * inverse, pulled = scale * args.kl;
+                const float rcp = reciprocal(total), scale = weight * share, pulled = scale * args.kl;
                 float surrogate = 0.0f, pull = 0.0f;
                 if (args.old_policy) {
                     uint32_t doubtful = 0;
@@ -330,15 +334,19 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                 if (!ok)
 #pragma unroll
                     for (int a = 0; a < kActions; ++a) p[a] = __int_as_float(0x7FC00000);
-                write_hand<kActions, T>(z_own, p);
+                if (args.wide)  // (in the place of the targets, which are read)
+                    write_hand<kActions, float>(target_s + tid * kActions, p);
+                else
+                    write_hand<kActions, T>(z_own, p);
             }
         }
         if (bulk) async_fence();
         __syncthreads();
         if (bulk && tid == 0) {
             if (args.grad)
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<T*>(args.grad) + first * kActions),
-                             "r"(smem_addr(z_s)), "r"((uint32_t)kLogits)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                                 reinterpret_cast<uint8_t*>(args.grad) + first * kActions * (args.wide ? 4 : (int)sizeof(T))),
+                             "r"(args.wide ? smem_addr(target_s) : smem_addr(z_s)), "r"((uint32_t)(args.wide ? kWords : kLogits))
                              : "memory");
             store_commit();
             store_wait_read<1>();  // the gradient of the tile before has left its stage, which takes the tile after the next
@@ -346,7 +354,12 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
             if (whole(next)) fetch(next, (turn + kLossStages - 1) % kLossStages);
         }
         if (!bulk && args.grad)
-            for (int i = tid; i < count * kActions; i += kHands) reinterpret_cast<T*>(args.grad)[first * kActions + i] = z_s[i];
+            for (int i = tid; i < count * kActions; i += kHands) {
+                if (args.wide)
+                    reinterpret_cast<float*>(args.grad)[first * kActions + i] = target_s[i];
+                else
+                    reinterpret_cast<T*>(args.grad)[first * kActions + i] = z_s[i];
+            }
         if (!args.bulk) __syncthreads();
     }
     loss_sum = block_sum(loss_sum, sums);
@@ -386,6 +399,22 @@ template <typename T> __global__ void __launch_bounds__(256) scale_kernel(const 
     for (int64_t i = whole + begin; i < n; i += step) out[i] = from_float<T>(as_float(in[i]) * f);
 }
 
+// The same of a gradient in fp32, for fp16 logits: an entry is of the size of 1 / (states * hands), 2e-7 for 4096 states, and fp16 ends at
+// 6e-8, so it takes the factor before it is rounded.  Up to a factor of 2, where that can bring nothing back, it is rounded before as well,
+// as the gradient by itself is: the same bits times the factor, two half steps of fp16 more at most.
+__global__ void __launch_bounds__(256) scale_wide_kernel(const float* in, const float* factor, __half* out, int64_t n, int64_t whole) {
+    const float f = *factor;
+    const bool before = fabsf(f) <= 2.0f;
+    auto scaled = [&](float g) { return __float2half((before ? __half2float(__float2half(g)) : g) * f); };
+    const int64_t step = (int64_t)gridDim.x * 256, begin = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t i = begin; i < whole / 8; i += step) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(in) + 2 * i), b = __ldg(reinterpret_cast<const float4*>(in) + 2 * i + 1);
+        __align__(16) const __half v[8] = {scaled(a.x), scaled(a.y), scaled(a.z), scaled(a.w), scaled(b.x), scaled(b.y), scaled(b.z), scaled(b.w)};
+        reinterpret_cast<uint4*>(out)[i] = *reinterpret_cast<const uint4*>(v);
+    }
+    for (int64_t i = whole + begin; i < n; i += step) out[i] = scaled(in[i]);
+}
+
 static SharedLimit g_limit[kMostActions + 1][3];
 
 template <int kActions, typename T> static int launch_loss(const LossArgs& args, int type, cudaStream_t stream) {
@@ -417,9 +446,10 @@ extern "C" int64_t p2b_policy_loss_scratch_bytes(int64_t states, int32_t hands) 
     return loss_sizes(states, hands, 1) ? 8 * (1 + kMassBlocks + kLossBlocks) + blocks_of(states, 2) * 8 : -1;
 }
 
-extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, const float* advantages, const float* target, const uint8_t* legal,
-                               const float* weights, int64_t states, int32_t hands, int32_t actions, int32_t dtype, double clip, float kl,
-                               float* loss, void* grad, void* scratch, int64_t scratch_bytes, void* stream) {
+extern "C" int p2b_policy_loss_scaled(const void* logits, const float* old_policy, const float* advantages, const float* target, const uint8_t* legal,
+                                      const float* weights, int64_t states, int32_t hands, int32_t actions, int32_t dtype, double clip, float kl,
+                                      float* loss, void* grad, int32_t grad_dtype, float factor, const float* factor_at, void* scratch,
+                                      int64_t scratch_bytes, void* stream) {
     const char* name = "p2b_policy_loss";
     if (!loss_sizes(states, hands, actions))
         return set_error(P2B_ERR_ARG, "%s: %lld states of %d hands and %d actions are out of range (1 to %d actions)", name, (long long)states, hands, actions, kMostActions);
@@ -431,14 +461,16 @@ extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, cons
                          (long long)bytes);
     if ((old_policy == nullptr) != (advantages == nullptr)) return set_error(P2B_ERR_ARG, "%s: the old policy and the advantages come together", name);
     if (states > 0 && (!logits || !target || !legal)) return set_error(P2B_ERR_ARG, "%s: null array", name);
-    const int size = dtype == 2 ? 4 : 2;
-    const uintptr_t four = (uintptr_t)old_policy | (uintptr_t)advantages | (uintptr_t)target | (uintptr_t)weights | (uintptr_t)loss;
-    if (four % 4 || ((uintptr_t)logits | (uintptr_t)grad) % size) return set_error(P2B_ERR_ARG, "%s: an array lies off its elements' boundaries", name);
+    if (grad_dtype != dtype && grad_dtype != 2) return set_error(P2B_ERR_ARG, "%s: the gradient has the logits' type or is fp32", name);
+    if (!(factor >= -3.4028234e38f && factor <= 3.4028234e38f)) return set_error(P2B_ERR_ARG, "%s: the gradient's factor is not finite", name);
+    const uintptr_t four = (uintptr_t)old_policy | (uintptr_t)advantages | (uintptr_t)target | (uintptr_t)weights | (uintptr_t)loss | (uintptr_t)factor_at;
+    if (four % 4 || (uintptr_t)logits % (dtype == 2 ? 4 : 2) || (uintptr_t)grad % (grad_dtype == 2 ? 4 : 2)) return set_error(P2B_ERR_ARG, "%s: an array lies off its elements' boundaries", name);
     cudaStream_t st = (cudaStream_t)stream;
     if (states == 0) return check_cuda(cudaMemsetAsync(loss, 0, 4, st), name);
     LossArgs args{};
     args.logits = logits, args.old_policy = old_policy, args.advantages = advantages, args.target = target, args.weights = weights, args.legal = legal;
     args.states = states, args.total = states * hands, args.hands = hands, args.clip = clip, args.kl = kl, args.loss = loss, args.grad = grad;
+    args.wide = grad_dtype != dtype, args.factor = factor, args.factor_at = factor_at;
     args.bulk = (((uintptr_t)old_policy | (uintptr_t)advantages | (uintptr_t)target | (uintptr_t)weights | (uintptr_t)logits | (uintptr_t)grad) % 16) == 0;
     args.done = (unsigned long long*)scratch;
     args.mass = (double*)scratch + 1;
@@ -457,6 +489,13 @@ extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, cons
     return launch_actions<float>(args, actions, 2, st);
 }
 
+extern "C" int p2b_policy_loss(const void* logits, const float* old_policy, const float* advantages, const float* target, const uint8_t* legal,
+                               const float* weights, int64_t states, int32_t hands, int32_t actions, int32_t dtype, double clip, float kl,
+                               float* loss, void* grad, void* scratch, int64_t scratch_bytes, void* stream) {
+    return p2b_policy_loss_scaled(logits, old_policy, advantages, target, legal, weights, states, hands, actions, dtype, clip, kl, loss, grad, dtype, 1.0f, nullptr,
+                                  scratch, scratch_bytes, stream);
+}
+
 extern "C" int p2b_policy_loss_scale(const void* grad, const float* factor, int64_t n, int32_t dtype, void* out, void* stream) {
     if (n < 0 || dtype < 0 || dtype > 2) return set_error(P2B_ERR_ARG, "p2b_policy_loss_scale: %lld values of type %d", (long long)n, dtype);
     if (n == 0) return P2B_OK;
@@ -471,4 +510,15 @@ extern "C" int p2b_policy_loss_scale(const void* grad, const float* factor, int6
     if (dtype == 1) scale_kernel<<<grid, 256, 0, st>>>((const __half*)grad, factor, (__half*)out, n, whole);
     if (dtype == 2) scale_kernel<<<grid, 256, 0, st>>>((const float*)grad, factor, (float*)out, n, whole);
     return check_cuda(cudaGetLastError(), "scale_kernel");
+}
+
+extern "C" int p2b_policy_loss_scale_fp32(const float* grad, const float* factor, int64_t n, void* out, void* stream) {
+    const char* name = "p2b_policy_loss_scale_fp32";
+    if (n < 0) return set_error(P2B_ERR_ARG, "%s: %lld values", name, (long long)n);
+    if (n == 0) return P2B_OK;
+    if (!grad || !factor || !out) return set_error(P2B_ERR_ARG, "%s: null array", name);
+    if (((uintptr_t)factor | (uintptr_t)grad) % 4 || (uintptr_t)out % 2) return set_error(P2B_ERR_ARG, "%s: an array lies off its elements' boundaries", name);
+    const int64_t whole = ((uintptr_t)grad | (uintptr_t)out) % 16 ? 0 : n / 8 * 8, blocks = blocks_of(n, 256 * 8), most = 8 * sm_count();
+    scale_wide_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, (cudaStream_t)stream>>>(grad, factor, (__half*)out, n, whole);
+    return check_cuda(cudaGetLastError(), "scale_wide_kernel");
 }

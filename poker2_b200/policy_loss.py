@@ -27,23 +27,34 @@ def clipped_policy_loss(logits: torch.Tensor, old_policy: torch.Tensor | None, a
     that differentiates to the logits.
 
     Illegal actions, hands of weight 0, states without a legal action and hands whose legal logits are all -inf add nothing
-    and get a zero gradient, whatever their entries hold.  With gradients wanted the gradient is computed in the same pass (rounded
-    to the logits' type; a factor that the backward pass brings is rounded in once more) and the call is refused while a CUDA graph is
-    being captured: use `clipped_policy_loss_and_grad` there."""
+    and get a zero gradient, whatever their entries hold.  With gradients wanted the gradient is computed in the same pass and
+    the call is refused while a CUDA graph is being captured: use `clipped_policy_loss_and_grad` there.  bf16 and fp32 logits: it is
+    rounded to their type, and once more with the factor that the backward pass brings.  fp16 logits: it stays in fp32 until that
+    factor is known, so that a gradient scaler's reaches entries of the size 1 / (states * hands), which fp16 has no room for
+    (factors up to 2, which raise nothing into its range, multiply the rounded gradient)."""
     _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
     if not (torch.is_grad_enabled() and logits.requires_grad):
-        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, False)[0]
+        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, None)[0]
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("clipped_policy_loss cannot be captured into a CUDA graph through autograd; call clipped_policy_loss_and_grad, which can.")
     return _Loss.apply(logits, old_policy, advantages, target, legal, weights, clip, kl)
 
 
 def clipped_policy_loss_and_grad(logits: torch.Tensor, old_policy: torch.Tensor | None, advantages: torch.Tensor | None, target: torch.Tensor,
-                                 legal: torch.Tensor, weights: torch.Tensor | None = None, *, clip: float = 0.2, kl: float = 1.0):
+                                 legal: torch.Tensor, weights: torch.Tensor | None = None, *, clip: float = 0.2, kl: float = 1.0,
+                                 scale: float | torch.Tensor = 1.0):
     """(loss, its gradient to the logits in their type) of `clipped_policy_loss`, in one pass and without autograd: hand the gradient
-    to `logits.backward(grad)`, or scale it first."""
+    to `logits.backward(grad)`.  `scale`, a number or an fp32 tensor of one element on the logits' device, multiplies the gradient (the
+    loss stays as it is) before it is rounded: what a gradient scaler brings, without which entries of the size 1 / (states * hands)
+    are lost in fp16."""
     _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
-    return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, True)
+    if isinstance(scale, torch.Tensor):
+        if scale.numel() != 1 or scale.dtype != torch.float32 or scale.get_device() != logits.get_device():
+            raise ValueError("the scale is a number, or an fp32 tensor of one element on the logits' device")
+        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, logits.dtype, 1.0, scale.data_ptr())
+    if not abs(scale) <= 3.4028234e38:
+        raise ValueError("the scale is finite")
+    return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, logits.dtype, scale)
 
 
 def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tensor) -> torch.Tensor:
@@ -72,8 +83,9 @@ def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tenso
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, old_policy, advantages, target, legal, weights, clip, kl):
-        loss, grad = _run(logits, old_policy, advantages, target, legal, weights, clip, kl, True)
+        loss, grad = _run(logits, old_policy, advantages, target, legal, weights, clip, kl, torch.float32 if logits.dtype == torch.float16 else logits.dtype)
         ctx.save_for_backward(grad)
+        ctx.dtype = logits.dtype
         return loss
 
     @staticmethod
@@ -83,8 +95,11 @@ class _Loss(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("clipped_policy_loss has no second derivatives (create_graph=True)")
         grad, = ctx.saved_tensors
-        out = torch.empty_like(grad)
-        _lib.call_on(grad.get_device(), "p2b_policy_loss_scale", grad.data_ptr(), factor.data_ptr(), grad.numel(), _TYPES[grad.dtype], out.data_ptr())
+        out = torch.empty_like(grad, dtype=ctx.dtype)
+        if ctx.dtype != grad.dtype:
+            _lib.call_on(grad.get_device(), "p2b_policy_loss_scale_fp32", grad.data_ptr(), factor.data_ptr(), grad.numel(), out.data_ptr())
+        else:
+            _lib.call_on(grad.get_device(), "p2b_policy_loss_scale", grad.data_ptr(), factor.data_ptr(), grad.numel(), _TYPES[grad.dtype], out.data_ptr())
         return out, None, None, None, None, None, None, None
 
 
@@ -92,18 +107,19 @@ def _packed(t):
     return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
-def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, with_grad):
+def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, grad_dtype, scale=1.0, scale_at=None):
+    """(loss, the gradient times scale and *scale_at in grad_dtype, or None)."""
     states, hands, actions = logits.shape
     logits, target, legal = _packed(logits), _packed(target), _packed(legal)
     old_policy, advantages, weights = _packed(old_policy), _packed(advantages), _packed(weights)
     loss = target.new_empty(())
-    grad = logits.new_empty((states, hands, actions)) if with_grad else None
+    grad = None if grad_dtype is None else logits.new_empty((states, hands, actions), dtype=grad_dtype)
     size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
     scratch = target.new_empty((size // 4,)) if size else None
-    _lib.call_on(logits.get_device(), "p2b_policy_loss", logits.data_ptr(), None if old_policy is None else old_policy.data_ptr(),
+    _lib.call_on(logits.get_device(), "p2b_policy_loss_scaled", logits.data_ptr(), None if old_policy is None else old_policy.data_ptr(),
                  None if advantages is None else advantages.data_ptr(), target.data_ptr(), legal.data_ptr(),
                  None if weights is None else weights.data_ptr(), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(),
-                 None if grad is None else grad.data_ptr(), None if scratch is None else scratch.data_ptr(), size)
+                 None if grad is None else grad.data_ptr(), _TYPES[grad_dtype or logits.dtype], scale, scale_at, None if scratch is None else scratch.data_ptr(), size)
     return loss, grad
 
 

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from poker2_b200 import mx4
+import network_refs as refs
+from poker2_b200 import mx4, policy_loss as pl
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,73 @@ def test_rows_that_are_not_finite_stay_quantised(cuda_device, rows, width, colum
         assert torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
     again = mx4.linear(got, mx4.quantise(torch.ones(3, columns, device=cuda_device)))
     assert torch.isnan(again[[0, 7, 31, rows - 1]]).all() and torch.isfinite(again[1:7]).all()
+
+
+def _loss_batch(states, hands, actions, dtype, device, seed=0):
+    g = torch.Generator(device=device).manual_seed(seed + states + hands + actions)
+    new = lambda *s: torch.randn(*s, device=device, generator=g)  # noqa: E731
+    logits = new(states, hands, actions).to(dtype)
+    legal = torch.rand(states, actions, device=device, generator=g) < 0.8
+    legal[:, min(1, actions - 1)] = True
+    old = torch.softmax(logits.float() + 0.3 * new(states, hands, actions), -1)
+    target = (new(states, hands, actions) + 0.3).clamp(min=0.0)
+    target = target / target.sum(-1, keepdim=True).clamp(min=1e-6)
+    return logits, old, 0.1 * new(states, hands, actions), target, legal, torch.rand(states, hands, device=device, generator=g)
+
+
+@pytest.mark.parametrize("factor", [65536.0, 1000.0, 3.0])
+@pytest.mark.parametrize("states,hands,actions", [(4096, 1326, 5), (513, 1326, 8), (2, 255, 3), (77, 300, 4)])
+def test_a_loss_scale_reaches_gradients_that_fp16_has_no_room_for(cuda_device, states, hands, actions, factor):
+    """The factor of a gradient scaler times the 64-bit gradient, rounded once: entries of the size 1/(states*hands) survive in fp16."""
+    batch = _loss_batch(states, hands, actions, torch.float16, cuda_device)
+    _, _, grad, bound = refs.policy_loss(*batch, 0.2, 0.5, torch.float32)
+    leaf = batch[0].clone().requires_grad_(True)
+    got, = torch.autograd.grad(factor * pl.clipped_policy_loss(leaf, *batch[1:], clip=0.2, kl=0.5), leaf)
+    # the fp32 gradient (its bound holds a rounding to fp32), the product's own step, the rounding to fp16
+    value, err = factor * grad, factor * (bound + grad.abs() * 2.0 ** -24)
+    refs.assert_within(got, value, err + refs.rounded(value.abs() + err, torch.float16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("states,hands,actions", [(1, 1326, 5), (700, 1326, 5), (33, 256, 16), (3, 77, 3), (520, 511, 8), (2, 1, 1)])
+def test_a_scale_is_taken_in_before_the_gradient_is_rounded(cuda_device, states, hands, actions, dtype):
+    """The explicit form with a scale, on the host or on the device, in a captured graph too; without the policy term as well."""
+    batch = _loss_batch(states, hands, actions, dtype, cuda_device, seed=5)
+    plain = pl.clipped_policy_loss_and_grad(*batch)
+    assert all(torch.equal(a, b) for a, b in zip(plain, pl.clipped_policy_loss_and_grad(*batch, scale=1.0)))
+    for scale in (4096.0, 300.0, -0.7):
+        for args in (batch, (batch[0], None, None, *batch[3:])):
+            _, _, grad, bound = refs.policy_loss(*args, 0.2, 1.0, torch.float32)
+            loss, got = pl.clipped_policy_loss_and_grad(*args, scale=scale)
+            assert torch.equal(loss, pl.clipped_policy_loss(*args)) and got.dtype == dtype
+            value, err = scale * grad, abs(scale) * (bound + grad.abs() * 2.0 ** -23)  # (two products in fp32)
+            refs.assert_within(got, value, err + refs.rounded(value.abs() + err, dtype))
+        held = torch.tensor([[scale]], device=cuda_device)
+        assert torch.equal(pl.clipped_policy_loss_and_grad(*args, scale=held)[1], got)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _, later = pl.clipped_policy_loss_and_grad(*args, scale=held)
+        held.mul_(2.0)
+        graph.replay()
+        assert torch.equal(later, pl.clipped_policy_loss_and_grad(*args, scale=2.0 * scale)[1])
+        # arrays off 16-byte boundaries take the other way into shared memory
+        shifted = [t if t is None else torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t) for t in args]
+        assert torch.equal(pl.clipped_policy_loss_and_grad(*shifted, scale=scale)[1], got)
+
+
+def test_small_factors_multiply_the_rounded_fp16_gradient(cuda_device):
+    batch = _loss_batch(600, 1326, 4, torch.float16, cuda_device)
+    leaf = batch[0].clone().requires_grad_(True)
+    loss, (_, _, grad, bound) = pl.clipped_policy_loss(leaf, *batch[1:]), refs.policy_loss(*batch, 0.2, 1.0, torch.float32)
+    _, once = pl.clipped_policy_loss_and_grad(*batch)
+    for factor in (1.0, 2.0, -2.0, 0.3, 0.0, 2.25, float("inf"), float("nan")):
+        got, = torch.autograd.grad(loss, leaf, torch.tensor(factor, device=cuda_device), retain_graph=True)
+        if abs(factor) <= 2.0:
+            assert torch.equal(got, (once.float() * factor).half())
+            value, err = factor * grad, abs(factor) * (bound + grad.abs() * 2.0 ** -24 + refs.rounded(grad.abs() + bound, torch.float16))
+        elif factor == 2.25:
+            value, err = factor * grad, factor * (bound + grad.abs() * 2.0 ** -24)
+        else:
+            assert not torch.isfinite(got[grad != 0]).any()
+            continue
+        refs.assert_within(got, value, err + refs.rounded(value.abs() + err, torch.float16))

@@ -131,3 +131,25 @@ def test_addresses_between_elements_are_refused(handle):
             assert handle.p2b_gated_backward(*{**good, name: p + 1}.values()) == -1 and b"2-byte" in handle.p2b_last_error(), name
     for args in ((p + 1, p, 4, 0, p), (p, p + 2, 4, 0, p), (p, p, 4, 1, p + 1), (p + 2, p, 4, 2, p), (p, p, 4, 2, p + 2)):
         assert handle.p2b_policy_loss_scale(*args, None) == -1 and b"boundaries" in handle.p2b_last_error()
+
+
+def test_policy_loss_scales_that_are_refused(handle):
+    import ctypes
+
+    from poker2_b200 import policy_loss as pl
+
+    area = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(area) + 63) // 64 * 64
+    good = dict(logits=p, old=p, adv=p, target=p, legal=p, weights=p, states=2, hands=3, actions=4, dtype=1, clip=0.2, kl=1.0, loss=p, grad=p, gdtype=1, factor=1.0, at=p,
+                scratch=p, size=1 << 20, stream=None)
+    for change in (dict(gdtype=0), dict(gdtype=3), dict(gdtype=-1), dict(factor=float("inf")), dict(factor=float("nan")), dict(at=p + 2), dict(gdtype=2, grad=p + 2),
+                   dict(grad=p + 1), dict(dtype=2, gdtype=1), dict(logits=None), dict(states=-1), dict(scratch=None, states=3000)):
+        assert handle.p2b_policy_loss_scaled(*{**good, **change}.values()) == -1 and b"p2b_policy_loss" in handle.p2b_last_error(), change
+    for args in ((None, p, 4, p), (p, None, 4, p), (p, p, 4, None), (p, p, -1, p), (p + 2, p, 4, p), (p, p + 2, 4, p), (p, p, 4, p + 1)):
+        assert handle.p2b_policy_loss_scale_fp32(*args, None) == -1
+    assert handle.p2b_policy_loss_scale_fp32(None, None, 0, None, None) == 0
+    there = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype).as_subclass(_Elsewhere)  # noqa: E731
+    call = lambda scale: pl.clipped_policy_loss_and_grad(there(2, 3, 4), None, None, there(2, 3, 4), there(2, 4, dtype=torch.bool), scale=scale)  # noqa: E731
+    for scale in (float("inf"), float("nan"), 1e300, there(2), there(1, dtype=torch.float64), torch.ones(1)):
+        with pytest.raises(ValueError, match="scale"):
+            call(scale)
