@@ -13,6 +13,8 @@
 #include "layer.cuh"
 #include "tensor.cuh"
 
+#include <type_traits>
+
 namespace p2b {
 
 using namespace tc;
@@ -44,7 +46,7 @@ struct LossArgs {
     uint64_t magic;   // ceil(2^64 / hands)
     float* loss;
     void* grad;
-    int wide;                // grad is fp32 whatever the logits are
+    int wide;                // fp16 logits: grad is fp32
     float factor;            // of the gradient, times *factor_at (NULL: 1), before its only rounding
     const float* factor_at;
 };
@@ -143,11 +145,12 @@ template <int kActions, typename T> __device__ __forceinline__ void write_hand(T
     }
 }
 
-__device__ __forceinline__ float log_two(float x) {  // of a positive number (a subnormal one counts as the smallest normal)
+__device__ __forceinline__ float log_two(float x) {  // of a normal number; a NaN stays one
     float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 1.17549435e-38f)));
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float log_two_of_target(float x) { return log_two(fmaxf(x, 1.17549435e-38f)); }  // (a subnormal number counts as the smallest normal)
 
 // Which of the doubtful actions of a hand are free: probabilities so near an end of their interval that 32 bits may put them on the
 // wrong side are compared in 64.  (Masks go in and out: an address taken of the caller's arrays would put them into memory.)
@@ -170,8 +173,12 @@ __device__ __noinline__ uint32_t settle_hand(const T* z, const float* old, const
 // Blocks stay: each takes every gridDim.x-th tile of 256 hands, with the tiles after the present one on their way into the other
 // two of three stages (two stages in all: 225 us instead of 146 for the states above).  The gradient overwrites the logits (in fp32: the
 // targets) of its stage and leaves from there.
+// Blocks a multiprocessor that registers are to leave room for, as many as shared memory does.  (6 to 8 actions: two fit by themselves, in up
+// to 128 registers; held to that, 4096 states of 8 actions take 2 us longer.)
+constexpr int blocks_held(int actions) { return actions <= 4 ? 4 : actions == 5 ? 3 : actions == 9 || actions == 10 ? 2 : 1; }
+
 template <int kActions, typename T>
-__global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_constant__ LossArgs args) {
+__global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_kernel(const __grid_constant__ LossArgs args) {
     extern __shared__ __align__(16) uint8_t area[];
     __shared__ double sums[kHands / 32];
     __shared__ uint64_t bar_words[kLossStages];
@@ -179,6 +186,7 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
     __shared__ bool last_block;
     constexpr int kStage = kHands * (kActions * ((int)sizeof(T) + 12) + 4), kWords = kHands * kActions * 4, kLogits = kHands * kActions * (int)sizeof(T);
     const int tid = threadIdx.x;
+    const bool wide = std::is_same<T, __half>::value && args.wide;
     const int64_t tiles = (args.total + kHands - 1) / kHands;
     auto bar = [&](int s) { return smem_addr(bar_words + s); };
     auto whole = [&](int64_t tile) { return args.bulk && tile < tiles && (tile + 1) * kHands <= args.total; };
@@ -276,8 +284,8 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                 g[a] = legal ? g[a] : 0.0f;
                 top = fmaxf(top, p[a]);
             }
-            // no legal action, or none that the logits leave, or a hand that does not count: nothing, whatever else is there
-            if (weight != 0.0f && top != -INFINITY) {
+            // no legal action, or a hand that does not count: nothing, whatever else is there
+            if (weight != 0.0f && open != 0) {
                 float d[kActions], total = 0.0f, targets = 0.0f, divergence = 0.0f;
                 // (in powers of two; logarithms are lg2.approx, off by 2^-22, of which the loss averages a whole batch)
 #pragma unroll
@@ -286,12 +294,25 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                     p[a] = small_power_of_two(d[a]);
                     total += p[a];
                     targets += t[a];
-                    const float more = fmaf(t[a], log_two(t[a]) - d[a], divergence);
+                    const float more = fmaf(t[a], log_two_of_target(t[a]) - d[a], divergence);
                     divergence = t[a] > 0.0f ? more : divergence;
                 }
                 divergence = 0.69314718055994531f * fmaf(targets, log_two(total), divergence);
                 const float rcp = reciprocal(total), scale = weight * share, pulled = scale * args.kl;
                 float surrogate = 0.0f, pull = 0.0f;
+                // A sum that is NaN: no action that the logits leave is nothing, something undefined stays so at the legal actions.  (Of the
+                // logits again: a maximum passes over NaN, which is no -inf.)
+                auto undefined = [&] {
+                    uint32_t left = 0;
+#pragma unroll 1
+                    for (int a = 0; a < kActions; ++a) left = open >> a & 1 && as_float(z_own[a]) != -INFINITY ? open : left;
+#pragma unroll
+                    for (int a = 0; a < kActions; ++a) {
+                        p[a] = left & 1u << a ? p[a] : 0.0f;
+                        t[a] = left ? t[a] : 0.0f;
+                    }
+                    if (left == 0) divergence = surrogate = targets = 0.0f;
+                };
                 if (args.old_policy) {
                     uint32_t doubtful = 0;
 #pragma unroll
@@ -299,14 +320,17 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                         p[a] *= rcp;
                         q[a] *= g[a] > 0.0f ? high_end : low_end;
                         // p is off by 1.5e-6 of itself and 1e-7 for every halving below the top, and by its last bits where those are few
-                        doubtful |= fabsf(p[a] - q[a]) <= fmaf(q[a], fmaf(fminf(-d[a], 200.0f), 1e-7f, 2e-6f), 1e-43f) ? 1u << a : 0u;
+                        // (undefined counts as doubtful)
+                        doubtful |= fabsf(p[a] - q[a]) > fmaf(q[a], fmaf(fminf(-d[a], 200.0f), 1e-7f, 2e-6f), 1e-43f) ? 0u : 1u << a;
                         const float moving = p[a] * g[a], fixed = q[a] * g[a];
                         const bool free = moving <= fixed;
                         surrogate += free ? moving : fixed;
                         d[a] = free ? g[a] : 0.0f;
                         pull += free ? moving : 0.0f;
                     }
-                    if (doubtful) {
+                    if (doubtful && total != total) {
+                        undefined();
+                    } else if (doubtful) {
                         const uint32_t free = settle_hand<kActions, T>(z_own, old_s + tid * kActions, adv_s + tid * kActions, open, doubtful, args.clip);
                         surrogate = pull = 0.0f;
 #pragma unroll
@@ -322,7 +346,10 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                     for (int a = 0; a < kActions; ++a) p[a] = fmaf(p[a], fmaf(-scale, d[a], base), -pulled * t[a]);
                 } else {
 #pragma unroll
-                    for (int a = 0; a < kActions; ++a) p[a] = pulled * fmaf(p[a] * rcp, targets, -t[a]);
+                    for (int a = 0; a < kActions; ++a) p[a] *= rcp;
+                    if (total != total) undefined();
+#pragma unroll
+                    for (int a = 0; a < kActions; ++a) p[a] = pulled * fmaf(p[a], targets, -t[a]);
                 }
                 loss_sum += (double)weight * (double)(args.kl * divergence - surrogate);
             } else {
@@ -334,7 +361,7 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
                 if (!ok)
 #pragma unroll
                     for (int a = 0; a < kActions; ++a) p[a] = __int_as_float(0x7FC00000);
-                if (args.wide)  // (in the place of the targets, which are read)
+                if (wide)  // (in the place of the targets, which are read)
                     write_hand<kActions, float>(target_s + tid * kActions, p);
                 else
                     write_hand<kActions, T>(z_own, p);
@@ -345,8 +372,8 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
         if (bulk && tid == 0) {
             if (args.grad)
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
-                                 reinterpret_cast<uint8_t*>(args.grad) + first * kActions * (args.wide ? 4 : (int)sizeof(T))),
-                             "r"(args.wide ? smem_addr(target_s) : smem_addr(z_s)), "r"((uint32_t)(args.wide ? kWords : kLogits))
+                                 reinterpret_cast<uint8_t*>(args.grad) + first * kActions * (wide ? 4 : (int)sizeof(T))),
+                             "r"(wide ? smem_addr(target_s) : smem_addr(z_s)), "r"((uint32_t)(wide ? kWords : kLogits))
                              : "memory");
             store_commit();
             store_wait_read<1>();  // the gradient of the tile before has left its stage, which takes the tile after the next
@@ -355,7 +382,7 @@ __global__ void __launch_bounds__(kHands) policy_loss_kernel(const __grid_consta
         }
         if (!bulk && args.grad)
             for (int i = tid; i < count * kActions; i += kHands) {
-                if (args.wide)
+                if (wide)
                     reinterpret_cast<float*>(args.grad)[first * kActions + i] = target_s[i];
                 else
                     reinterpret_cast<T*>(args.grad)[first * kActions + i] = z_s[i];
@@ -461,7 +488,7 @@ extern "C" int p2b_policy_loss_scaled(const void* logits, const float* old_polic
                          (long long)bytes);
     if ((old_policy == nullptr) != (advantages == nullptr)) return set_error(P2B_ERR_ARG, "%s: the old policy and the advantages come together", name);
     if (states > 0 && (!logits || !target || !legal)) return set_error(P2B_ERR_ARG, "%s: null array", name);
-    if (grad_dtype != dtype && grad_dtype != 2) return set_error(P2B_ERR_ARG, "%s: the gradient has the logits' type or is fp32", name);
+    if (grad_dtype != dtype && (grad_dtype != 2 || dtype != 1)) return set_error(P2B_ERR_ARG, "%s: the gradient has the logits' type, or is fp32 where they are fp16", name);
     if (!(factor >= -3.4028234e38f && factor <= 3.4028234e38f)) return set_error(P2B_ERR_ARG, "%s: the gradient's factor is not finite", name);
     const uintptr_t four = (uintptr_t)old_policy | (uintptr_t)advantages | (uintptr_t)target | (uintptr_t)weights | (uintptr_t)loss | (uintptr_t)factor_at;
     if (four % 4 || (uintptr_t)logits % (dtype == 2 ? 4 : 2) || (uintptr_t)grad % (grad_dtype == 2 ? 4 : 2)) return set_error(P2B_ERR_ARG, "%s: an array lies off its elements' boundaries", name);

@@ -27,7 +27,8 @@ def clipped_policy_loss(logits: torch.Tensor, old_policy: torch.Tensor | None, a
     that differentiates to the logits.
 
     Illegal actions, hands of weight 0, states without a legal action and hands whose legal logits are all -inf add nothing
-    and get a zero gradient, whatever their entries hold.  With gradients wanted the gradient is computed in the same pass and
+    and get a zero gradient, whatever their entries hold; a NaN or +inf among the legal logits of a hand that counts makes the loss and the
+    hand's gradient NaN.  With gradients wanted the gradient is computed in the same pass and
     the call is refused while a CUDA graph is being captured: use `clipped_policy_loss_and_grad` there.  bf16 and fp32 logits: it is
     rounded to their type, and once more with the factor that the backward pass brings.  fp16 logits: it stays in fp32 until that
     factor is known, so that a gradient scaler's reaches entries of the size 1 / (states * hands), which fp16 has no room for

@@ -100,3 +100,57 @@ def test_small_factors_multiply_the_rounded_fp16_gradient(cuda_device):
             assert not torch.isfinite(got[grad != 0]).any()
             continue
         refs.assert_within(got, value, err + refs.rounded(value.abs() + err, torch.float16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("states,hands,actions", [(3, 40, 5), (300, 256, 5), (40, 77, 8), (6, 256, 1)])
+def test_undefined_logits_are_not_taken_for_hands_without_actions(cuda_device, states, hands, actions, dtype):
+    """NaN (or +inf, whose softmax is undefined) at a legal action of a hand that counts: the loss and that hand's legal gradients are
+    NaN, all others what they were; at hands that do not count it is nothing."""
+    nan = float("nan")
+    logits, old, adv, target, legal, weights = _loss_batch(states, hands, actions, dtype, cuda_device)
+    legal[2] = False
+    legal[1, -1] = actions == 1  # (an illegal action beside the undefined ones)
+    weights[0, 7] = 0.0
+    weights[1:, :] += 0.01
+    where = torch.zeros(states, hands, dtype=torch.bool, device=cuda_device)
+    where[1, 5] = True
+    undefined = where[:, :, None] & legal[:, None, :]
+    for policies in ((old, adv), (None, None)):
+        for kl in (0.0, 0.7):
+            rest = (*policies, target, legal, weights)
+            loss, grad = pl.clipped_policy_loss_and_grad(logits, *rest, kl=kl)
+            for fill in ("all", "one", "one and -inf", "inf"):
+                bad = logits.clone()
+                if fill == "all":
+                    bad[1, 5] = nan
+                elif fill == "one":
+                    bad[1, 5, 0] = nan
+                    legal_target = target.clone()
+                    legal_target[1, 5, 0] = 0.0  # (nothing of the KL term hangs on the undefined logit itself)
+                    rest = (*policies, legal_target, legal, weights)
+                    if not legal[1, 0]:
+                        continue
+                elif fill == "one and -inf":
+                    bad[1, 5] = float("-inf")
+                    bad[1, 5, 0] = nan
+                    if not legal[1, 0]:
+                        continue
+                else:
+                    bad[1, 5, 0] = float("inf")
+                    if not legal[1, 0]:
+                        continue
+                got_loss, got = pl.clipped_policy_loss_and_grad(bad, *rest, kl=kl)
+                assert torch.isnan(got_loss) and torch.isnan(pl.clipped_policy_loss(bad, *rest, kl=kl)), fill
+                assert torch.isnan(got[undefined]).all(), fill
+                assert torch.equal(got[~undefined], grad[~undefined]), fill
+            quiet = logits.clone()
+            quiet[0, 7] = quiet[2] = nan
+            again = pl.clipped_policy_loss_and_grad(quiet, *policies, target, legal, weights, kl=kl)
+            assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
+    everywhere = pl.clipped_policy_loss_and_grad(torch.full_like(logits, nan), old, adv, target, legal, weights)
+    assert torch.isnan(everywhere[0]) and torch.isnan(everywhere[1][(weights != 0)[:, :, None] & legal[:, None, :]]).all()
+    assert not everywhere[1][~legal[:, None, :].expand_as(logits)].any()
+    leaf = torch.full_like(logits, nan).requires_grad_(True)
+    value = pl.clipped_policy_loss(leaf, old, adv, target, legal, weights)
+    assert torch.isnan(value) and torch.isnan(torch.autograd.grad(value, leaf)[0][1:2][legal[1:2, None, :].expand(1, hands, actions)]).all()
