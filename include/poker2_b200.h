@@ -538,7 +538,8 @@ int p2b_mx4_linear_rows(const void* x, int64_t x_stride, int32_t x_dtype, int64_
  *  KL term alone), target [states,hands,actions] fp32; legal [states,actions] bytes; weights [states,hands] fp32, none
  *  negative (NULL: 1).  All packed.  1 to 16 actions, 0 <= clip < 1, kl >= 0.
  * Nothing is read into the result from illegal actions, hands of weight 0 and hands whose legal logits are all -inf; their
- * gradients are 0; a NaN or +inf among the legal logits of another hand makes the loss and its gradient NaN.  loss: one fp32, summed in 64 bits in a fixed order.  scratch: p2b_policy_loss_scratch_bytes(states, hands),
+ * gradients are 0; a NaN or +inf among the legal logits of another hand makes the loss and its gradient NaN, a NaN among the
+ * weights all of them.  loss: one fp32, summed in 64 bits in a fixed order.  scratch: p2b_policy_loss_scratch_bytes(states, hands),
  * 8-byte aligned (0 bytes for up to 1536 hands: NULL will do).
  * p2b_policy_loss_scaled: the gradient times factor * *factor_at (device; NULL: 1) before its only rounding, to grad_dtype: dtype, or for fp16 2 (fp32).
  * Entries are of the size of 1 / (states * hands), which fp16 has no room for: it wants a factor, or fp32 until that is known.

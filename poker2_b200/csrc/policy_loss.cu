@@ -173,9 +173,9 @@ __device__ __noinline__ uint32_t settle_hand(const T* z, const float* old, const
 // Blocks stay: each takes every gridDim.x-th tile of 256 hands, with the tiles after the present one on their way into the other
 // two of three stages (two stages in all: 225 us instead of 146 for the states above).  The gradient overwrites the logits (in fp32: the
 // targets) of its stage and leaves from there.
-// Blocks a multiprocessor that registers are to leave room for, as many as shared memory does.  (6 to 8 actions: two fit by themselves, in up
-// to 128 registers; held to that, 4096 states of 8 actions take 2 us longer.)
-constexpr int blocks_held(int actions) { return actions <= 4 ? 4 : actions == 5 ? 3 : actions == 9 || actions == 10 ? 2 : 1; }
+// Blocks a multiprocessor that registers are to leave room for, as many as shared memory does (8 actions, one block instead of two: 217 us
+// instead of 150 for the states above).
+constexpr int blocks_held(int actions) { return actions <= 4 ? 4 : actions == 5 ? 3 : actions <= 10 ? 2 : 1; }
 
 template <int kActions, typename T>
 __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_kernel(const __grid_constant__ LossArgs args) {
@@ -221,7 +221,9 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
         }
     }
     mass = block_sum(mass, sums);
-    const float inverse = mass > 0.0 ? (float)(1.0 / mass) : 0.0f, share = inverse * (args.factor_at ? args.factor * *args.factor_at : args.factor);
+    const bool nothing = mass <= 0.0;  // (an undefined mass is not nothing)
+    const float inverse = nothing ? 0.0f : (float)(1.0 / mass), share = inverse * (args.factor_at ? args.factor * *args.factor_at : args.factor);
+    const float undefined_mass = mass < INFINITY ? 0.0f : __int_as_float(0x7FC00000);  // (goes the way of undefined logits)
     const float low_end = (float)(1.0 - args.clip), high_end = (float)(1.0 + args.clip);
 
     double loss_sum = 0.0;
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
             }
             // no legal action, or a hand that does not count: nothing, whatever else is there
             if (weight != 0.0f && open != 0) {
-                float d[kActions], total = 0.0f, targets = 0.0f, divergence = 0.0f;
+                float d[kActions], total = undefined_mass, targets = 0.0f, divergence = 0.0f;
                 // (in powers of two; logarithms are lg2.approx, off by 2^-22, of which the loss averages a whole batch)
 #pragma unroll
                 for (int a = 0; a < kActions; ++a) {
@@ -298,7 +300,8 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
                     divergence = t[a] > 0.0f ? more : divergence;
                 }
                 divergence = 0.69314718055994531f * fmaf(targets, log_two(total), divergence);
-                const float rcp = reciprocal(total), scale = weight * share, pulled = scale * args.kl;
+                const float rcp = reciprocal(total);
+                float scale = weight * share, pulled = scale * args.kl;
                 float surrogate = 0.0f, pull = 0.0f;
                 // A sum that is NaN: no action that the logits leave is nothing, something undefined stays so at the legal actions.  (Of the
                 // logits again: a maximum passes over NaN, which is no -inf.)
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
                         p[a] = left & 1u << a ? p[a] : 0.0f;
                         t[a] = left ? t[a] : 0.0f;
                     }
+                    scale = pulled = 1.0f;
                     if (left == 0) divergence = surrogate = targets = 0.0f;
                 };
                 if (args.old_policy) {
@@ -392,7 +396,7 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
     loss_sum = block_sum(loss_sum, sums);
     // the block that comes last adds the parts up, in their order
     if (gridDim.x == 1) {
-        if (tid == 0) *args.loss = mass > 0.0 ? (float)(loss_sum / mass) : 0.0f;
+        if (tid == 0) *args.loss = nothing ? 0.0f : (float)(loss_sum / mass);
     } else {
         if (tid == 0) {
             args.sums[blockIdx.x] = loss_sum;
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
             double sum = 0.0;
             for (int i = tid; i < (int)gridDim.x; i += kHands) sum += __ldcg(args.sums + i);
             sum = block_sum(sum, sums);
-            if (tid == 0) *args.loss = mass > 0.0 ? (float)(sum / mass) : 0.0f;
+            if (tid == 0) *args.loss = nothing ? 0.0f : (float)(sum / mass);
         }
     }
     if (tid == 0) store_wait();

@@ -28,11 +28,13 @@ def clipped_policy_loss(logits: torch.Tensor, old_policy: torch.Tensor | None, a
 
     Illegal actions, hands of weight 0, states without a legal action and hands whose legal logits are all -inf add nothing
     and get a zero gradient, whatever their entries hold; a NaN or +inf among the legal logits of a hand that counts makes the loss and the
-    hand's gradient NaN.  With gradients wanted the gradient is computed in the same pass and
-    the call is refused while a CUDA graph is being captured: use `clipped_policy_loss_and_grad` there.  bf16 and fp32 logits: it is
-    rounded to their type, and once more with the factor that the backward pass brings.  fp16 logits: it stays in fp32 until that
-    factor is known, so that a gradient scaler's reaches entries of the size 1 / (states * hands), which fp16 has no room for
-    (factors up to 2, which raise nothing into its range, multiply the rounded gradient)."""
+    hand's gradient NaN, a NaN among the weights (of states with a legal action) the loss and the gradients of all hands.
+
+    With gradients wanted the gradient is computed in the same pass and the call is refused while a CUDA graph is being captured: use
+    `clipped_policy_loss_and_grad` there.  bf16 and fp32 logits: it is rounded to their type, and once more with the factor that the
+    backward pass brings.  fp16 logits: it stays in fp32 until that factor is known, so that a gradient scaler's reaches entries of the
+    size 1 / (states * hands), which fp16 has no room for (factors up to 2, which raise nothing into its range, multiply the rounded
+    gradient)."""
     _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, None)[0]

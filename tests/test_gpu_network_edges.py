@@ -154,3 +154,42 @@ def test_undefined_logits_are_not_taken_for_hands_without_actions(cuda_device, s
     leaf = torch.full_like(logits, nan).requires_grad_(True)
     value = pl.clipped_policy_loss(leaf, old, adv, target, legal, weights)
     assert torch.isnan(value) and torch.isnan(torch.autograd.grad(value, leaf)[0][1:2][legal[1:2, None, :].expand(1, hands, actions)]).all()
+
+
+@pytest.mark.parametrize("states,hands,actions", [(3, 40, 5), (300, 256, 5), (40, 77, 8)])
+def test_undefined_weights_are_no_batch_without_weight(cuda_device, states, hands, actions):
+    nan = float("nan")
+    logits, old, adv, target, legal, weights = _loss_batch(states, hands, actions, torch.float32, cuda_device)
+    legal[2] = False
+    weights[:, 3] = 0.0
+    loss, grad = pl.clipped_policy_loss_and_grad(logits, old, adv, target, legal, weights)
+    bad = weights.clone()
+    bad[2] = nan  # a state that does not count
+    got = pl.clipped_policy_loss_and_grad(logits, old, adv, target, legal, bad)
+    assert torch.equal(got[0], loss) and torch.equal(got[1], grad)
+    bad[1, 7] = nan
+    counts = (bad != 0)[:, :, None] & legal[:, None, :]
+    for policies in ((old, adv), (None, None)):
+        for scale in (1.0, 1024.0):
+            got = pl.clipped_policy_loss_and_grad(logits, *policies, target, legal, bad, scale=scale)
+            assert torch.isnan(got[0]) and torch.isnan(got[1][counts]).all() and not got[1][~counts].any()
+    leaf = logits.clone().requires_grad_(True)
+    value = pl.clipped_policy_loss(leaf, old, adv, target, legal, bad)
+    assert torch.isnan(value) and torch.isnan(torch.autograd.grad(value, leaf)[0][counts]).all()
+    endless = weights.clone()
+    endless[1, 7] = float("inf")
+    got = pl.clipped_policy_loss_and_grad(logits, old, adv, target, legal, endless)
+    assert torch.isnan(got[0]) and torch.isnan(got[1][1, 7][legal[1]]).all() and not got[1][~legal[:, None, :].expand_as(logits)].any()
+
+
+def test_hand_weights_hand_an_undefined_player_on(cuda_device):
+    """From a player that does not exist to the loss of a minibatch."""
+    beliefs, to_act = torch.rand(4, 2 * 1326, device=cuda_device), torch.tensor([0, 1, 2, 1], device=cuda_device)
+    board = torch.full((4, 5), -1, device=cuda_device)
+    weights = pl.hand_weights(beliefs, to_act, board)
+    assert torch.isnan(weights[2]).all() and torch.isfinite(weights[[0, 1, 3]]).all()
+    logits, target = torch.randn(4, 1326, 3, device=cuda_device), torch.full((4, 1326, 3), 1 / 3, device=cuda_device)
+    legal = torch.ones(4, 3, dtype=torch.bool, device=cuda_device)
+    assert torch.isnan(pl.clipped_policy_loss(logits, None, None, target, legal, weights))
+    board[1, 0] = 52
+    assert torch.isnan(pl.hand_weights(beliefs, to_act, board)[[1, 2]]).all()
