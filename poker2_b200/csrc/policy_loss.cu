@@ -222,7 +222,9 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
     }
     mass = block_sum(mass, sums);
     const bool nothing = mass <= 0.0;  // (an undefined mass is not nothing)
-    const float inverse = nothing ? 0.0f : (float)(1.0 / mass), share = inverse * (args.factor_at ? args.factor * *args.factor_at : args.factor);
+    // (masses whose reciprocal fp32 has no room for: weights and mass are lifted alike, a power of two)
+    const float lift = mass < 0x1p-100 ? 0x1p100f : mass > 0x1p100 ? 0x1p-100f : 1.0f;
+    const float inverse = nothing ? 0.0f : (float)(1.0 / (mass * lift)), share = inverse * (args.factor_at ? args.factor * *args.factor_at : args.factor);
     const float undefined_mass = mass < INFINITY ? 0.0f : __int_as_float(0x7FC00000);  // (goes the way of undefined logits)
     const float low_end = (float)(1.0 - args.clip), high_end = (float)(1.0 + args.clip);
 
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(kHands, blocks_held(kActions)) policy_loss_ker
                 }
                 divergence = 0.69314718055994531f * fmaf(targets, log_two(total), divergence);
                 const float rcp = reciprocal(total);
-                float scale = weight * share, pulled = scale * args.kl;
+                float scale = weight * lift * share, pulled = scale * args.kl;
                 float surrogate = 0.0f, pull = 0.0f;
                 // A sum that is NaN: no action that the logits leave is nothing, something undefined stays so at the legal actions.  (Of the
                 // logits again: a maximum passes over NaN, which is no -inf.)

@@ -193,3 +193,16 @@ def test_hand_weights_hand_an_undefined_player_on(cuda_device):
     assert torch.isnan(pl.clipped_policy_loss(logits, None, None, target, legal, weights))
     board[1, 0] = 52
     assert torch.isnan(pl.hand_weights(beliefs, to_act, board)[[1, 2]]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("size", [1e-44, 1e-42, 1e-39, 1e-30, 1e30, 1e36, 3e38])
+def test_weights_at_both_ends_of_fp32(cuda_device, size, dtype):
+    """Their size falls out of loss and gradient, also where the reciprocal of their sum lies outside fp32."""
+    for states, hands, actions in ((2, 60, 4), (40, 77, 3)):
+        logits, old, adv, target, legal, weights = _loss_batch(states, hands, actions, dtype, cuda_device)
+        weights = weights.clamp(min=0.1) * size
+        loss, grad = pl.clipped_policy_loss_and_grad(logits, old, adv, target, legal, weights)
+        want = refs.policy_loss(logits, old, adv, target, legal, weights, 0.2, 1.0, dtype)
+        refs.assert_within(loss, want[0], want[1])
+        refs.assert_within(grad, want[2], want[3])
