@@ -116,22 +116,48 @@ class GatedValueMLP(ValueMLP):
 
 class Mx4Linear(torch.nn.Module):
     """act(q(x) q(W)^T + b) with W quantised once, when the layer is made.  `hands_on`: the result stays in 4 bits, as the next such
-    layer would make of it (but for few rows, which that one takes as they are)."""
+    layer would make of it (but for few rows, which that one takes as they are).  W is in the state dict in 4 bits; the layer moves
+    between devices and keeps its type."""
 
     def __init__(self, linear: torch.nn.Linear, activation: str = "none", hands_on: bool = False):
         super().__init__()
-        self.weight = mx4.quantise(linear.weight.detach())
+        weight = mx4.quantise(linear.weight.detach())
+        self.register_buffer("values", weight.values)
+        self.register_buffer("scales", weight.scales)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+        self.shape = weight.shape
         self.activation, self.hands_on, self.dtype = activation, hands_on, linear.weight.dtype
+
+    @property
+    def weight(self) -> mx4.Mx4:
+        return mx4.Mx4(self._buffers["values"], self._buffers["scales"], self.shape)
 
     def forward(self, x: torch.Tensor | mx4.Mx4) -> torch.Tensor | mx4.Mx4:
         rows = x.rows if isinstance(x, mx4.Mx4) else x.shape[:-1].numel()
         return mx4.linear(x, self.weight, self.bias, activation=self.activation, dtype=self.dtype, quantised=self.hands_on and rows > mx4.FEW_ROWS)
 
+    def _apply(self, fn, recurse=True):
+        if fn(torch.empty(0, dtype=self.dtype, device=self.values.device)).dtype != self.dtype:
+            raise ValueError("a 4-bit layer keeps its type: quantise a layer of the other one")
+        return super()._apply(fn, recurse)
+
+    def get_extra_state(self):  # (widths up to 31 apart have arrays of one size)
+        return {"shape": self.shape}
+
+    def set_extra_state(self, state):
+        pass
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        saved = state_dict.get(prefix + "_extra_state")
+        if saved is not None and tuple(saved["shape"]) != self.shape:
+            error_msgs.append(f"a 4-bit weight of {tuple(saved['shape'])} does not fit {prefix[:-1] or 'the layer'}, whose weight is {self.shape}")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
 
 class Mx4ValueMLP(ValueMLP):
     """A `ValueMLP` as it serves in 4 bits: every linear layer with its GELU becomes an `Mx4Linear`.  A copy of the weights as
-    they are now, on the GPU where they lie; for leaf values, not for training."""
+    they are now, on the GPU where they lie, saved and moved as other networks are; for leaf values, not for training."""
 
     def __init__(self, source: ValueMLP):
         torch.nn.Module.__init__(self)

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import network_refs as refs
-from poker2_b200 import mx4, policy_loss as pl
+from poker2_b200 import leaf_eval, mx4, policy_loss as pl
 
 pytestmark = pytest.mark.gpu
 
@@ -206,3 +206,29 @@ def test_weights_at_both_ends_of_fp32(cuda_device, size, dtype):
         want = refs.policy_loss(logits, old, adv, target, legal, weights, 0.2, 1.0, dtype)
         refs.assert_within(loss, want[0], want[1])
         refs.assert_within(grad, want[2], want[3])
+
+
+def test_a_4_bit_network_saved_loaded_copied_and_moved(cuda_device, tmp_path):
+    import copy
+
+    one, two = (leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(96, 2, seed=seed).to(cuda_device)) for seed in (1, 2))
+    x = torch.randn(40, one.IN_PADDED, device=cuda_device).bfloat16()
+    want, other = one.net(x), two.net(x)
+    assert not torch.equal(want, other)
+    torch.save(one.state_dict(), tmp_path / "net.pt")
+    two.load_state_dict(torch.load(tmp_path / "net.pt", weights_only=True))
+    assert torch.equal(two.net(x), want)
+    torch.save(one, tmp_path / "whole.pt")
+    assert torch.equal(torch.load(tmp_path / "whole.pt", weights_only=False).net(x), want)
+    assert torch.equal(copy.deepcopy(one).net(x), want)
+    home = two.cpu()
+    assert all(m.values.device.type == m.scales.device.type == m.bias.device.type == "cpu" for m in home.net)
+    for rows in (x[:2], x):
+        with pytest.raises(ValueError):
+            home.net(rows)
+        with pytest.raises(ValueError, match="CUDA"):
+            home.net(rows.cpu())
+    assert torch.equal(home.to(cuda_device).net(x), want) and torch.equal(home.net(x[:1]), one.net(x[:1]))
+    with pytest.raises(ValueError, match="type"):
+        one.half()
+    assert torch.equal(one.net(x), want)

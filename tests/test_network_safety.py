@@ -153,3 +153,76 @@ def test_policy_loss_scales_that_are_refused(handle):
     for scale in (float("inf"), float("nan"), 1e300, there(2), there(1, dtype=torch.float64), torch.ones(1)):
         with pytest.raises(ValueError, match="scale"):
             call(scale)
+
+
+def _quantise_here(x):
+    """A stand-in for the kernel: different arrays for different weights."""
+    rows, width = x.shape
+    m = _quantised(rows, width)
+    m.values.copy_(torch.arange(m.values.numel()).view_as(m.values).add_(int(1e6 * x.double().abs().sum())).remainder_(251))
+    m.scales.fill_(int(1e6 * x.double().abs().sum()) % 250)
+    return m
+
+
+@pytest.fixture
+def networks(monkeypatch):
+    from poker2_b200 import leaf_eval
+
+    monkeypatch.setattr(mx4, "quantise", _quantise_here)
+    return lambda seed, width=64, dtype=torch.bfloat16: leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(width, 2, seed=seed, dtype=dtype))
+
+
+def _same_weights(a, b):
+    return all(torch.equal(x.weight.values, y.weight.values) and torch.equal(x.weight.scales, y.weight.scales) and torch.equal(x.bias, y.bias)
+               for x, y in zip(a.net, b.net))
+
+
+def test_a_4_bit_network_is_saved_and_loaded_with_its_weights(networks, tmp_path):
+    import copy
+
+    one, two = networks(1), networks(2)
+    assert not _same_weights(one, two)
+    torch.save(one.state_dict(), tmp_path / "net.pt")
+    state = torch.load(tmp_path / "net.pt", weights_only=True)
+    assert {f"net.{i}.{k}" for i in range(3) for k in ("values", "scales", "bias")} <= set(state)
+    for assign in (False, True):
+        two = networks(2)
+        two.load_state_dict(state, strict=True, assign=assign)
+        assert _same_weights(one, two)
+    assert _same_weights(copy.deepcopy(one), one)
+    with pytest.raises(RuntimeError, match="Missing"):
+        two.load_state_dict({k: v for k, v in state.items() if "bias" in k})
+    with pytest.raises(RuntimeError, match="size mismatch|does not fit"):
+        networks(3, 128).load_state_dict(state)
+    # 60 and 64 columns have arrays of one size, and are not one matrix
+    other = networks(3, 60)
+    before = copy.deepcopy(other)
+    with pytest.raises(RuntimeError, match="does not fit"):
+        other.net[2].load_state_dict({k[6:]: v for k, v in state.items() if k.startswith("net.2.")})
+    assert _same_weights(before, other)
+    bias = one.net[0].bias
+    one.net[0].bias = None
+    assert "bias" not in one.net[0].state_dict() and bias is not None
+
+
+def test_a_4_bit_network_keeps_its_type_and_moves_as_a_whole(networks):
+    net = networks(1)
+    same = networks(1)
+    for change in (lambda: net.half(), lambda: net.float(), lambda: net.to(torch.float16), lambda: net.double(), lambda: net.type(torch.float32)):
+        with pytest.raises(ValueError, match="type"):
+            change()
+        assert _same_weights(net, same) and net.net[0].bias.dtype == torch.bfloat16
+    net.to(torch.bfloat16).to("cpu")
+    assert _same_weights(net, same)
+    away = net.to("meta")
+    for layer in away.net:
+        assert {layer.values.device.type, layer.scales.device.type, layer.bias.device.type} == {"meta"}
+    assert networks(1, dtype=torch.float16).half().net[0].dtype == torch.float16
+
+
+def test_a_4_bit_network_in_host_memory_refuses_its_calls(networks, launches):
+    net = networks(1)
+    for rows in (2, 40):
+        with pytest.raises(ValueError, match="CUDA"):
+            net.net(torch.zeros(rows, net.IN_PADDED, dtype=torch.bfloat16))
+    assert not launches
