@@ -199,6 +199,18 @@ def call_on(device: int, name: str, *args) -> None:
             call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
+_forward_ad = torch.autograd.forward_ad
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """RuntimeError where one of them carries a forward-mode tangent, which the kernels would drop: its owner would take the result for
+    a constant.  (Such a tensor does not require a gradient.  Outside of `dual_level` this is one comparison.)"""
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivatives")
+
+
 def plain_rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix whose rows are packed and do not overlap: `t` itself where it is one."""
     rows, columns = t.shape

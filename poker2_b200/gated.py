@@ -25,6 +25,7 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
     "gelu" (with erf) or "silu".  Any strides; rows that start on 16-byte boundaries (and weights likewise) are read in place.
     With gradients wanted the call is refused while a CUDA graph is being captured: use `gated_linear_backward` there."""
     act = _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
+    _lib.refuse_tangents("gated_linear", x, gate_weight, up_weight, gate_bias, up_bias)
     if torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad
                                     or gate_bias is not None and gate_bias.requires_grad or up_bias is not None and up_bias.requires_grad):
         _refuse_capture("gated_linear")
@@ -41,6 +42,7 @@ def gated_linear_backward(grad_h: torch.Tensor, x: torch.Tensor, gate_weight: to
     act = _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
     if grad_h.shape != (*x.shape[:-1], gate_weight.shape[0]) or grad_h.dtype != x.dtype or grad_h.get_device() != x.get_device():
         raise ValueError("the gradient of the hidden layer must have its shape, type and device")
+    _lib.refuse_tangents("gated_linear_backward", grad_h, x, gate_weight, up_weight, gate_bias, up_bias)
     with torch.no_grad():
         return _backward(grad_h, x, gate_weight, up_weight, gate_bias, up_bias, None, act, needs)
 
@@ -111,6 +113,7 @@ class _Gated(torch.autograd.Function):
         _refuse_capture("the backward pass of gated_linear")
         if torch.is_grad_enabled():
             raise RuntimeError("gated_linear has no second derivatives (create_graph=True)")
+        _lib.refuse_tangents("the backward pass of gated_linear", grad_h)
         return (*_backward(grad_h, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad), None)
 
 

@@ -66,6 +66,7 @@ def _check_layout(m: Mx4) -> None:
 def quantise(x: torch.Tensor) -> Mx4:
     """x [..., width], bf16, fp16 or fp32, any strides; the blocks lie along the last dimension, the last one may be short."""
     kind, shape, device = _TYPES.get(x.dtype), x.shape, x.get_device()
+    _lib.refuse_tangents("quantise", x)
     if device < 0:
         _lib.require_cuda(x, "quantise")
     if kind is None:
@@ -98,6 +99,7 @@ def linear(x: torch.Tensor | Mx4, weight: Mx4, bias: torch.Tensor | None = None,
     tensor = isinstance(x, torch.Tensor)
     if torch.is_grad_enabled() and (tensor and x.requires_grad or bias is not None and bias.requires_grad):
         raise RuntimeError("mx4.linear has no gradient: call it under torch.no_grad(), or train the layer that was quantised")
+    _lib.refuse_tangents("mx4.linear", x if tensor else None, bias)
     if dtype is None:
         dtype = torch.float16 if tensor and x.dtype == torch.float16 else torch.bfloat16
     elif dtype not in (torch.bfloat16, torch.float16):

@@ -97,6 +97,7 @@ class _Loss(torch.autograd.Function):
             raise RuntimeError("the backward pass of clipped_policy_loss cannot be captured into a CUDA graph; call clipped_policy_loss_and_grad, which can.")
         if torch.is_grad_enabled():
             raise RuntimeError("clipped_policy_loss has no second derivatives (create_graph=True)")
+        _lib.refuse_tangents("the backward pass of clipped_policy_loss", factor)
         grad, = ctx.saved_tensors
         out = torch.empty_like(grad, dtype=ctx.dtype)
         if ctx.dtype != grad.dtype:
@@ -143,5 +144,6 @@ def _check(logits, old_policy, advantages, target, legal, weights, clip, kl) -> 
         raise ValueError("weights [states, hands] fp32 on the logits' device are wanted")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (old_policy, advantages, target, weights)):
         raise RuntimeError("the loss differentiates to the logits alone: detach the policies, advantages and weights")
+    _lib.refuse_tangents("the policy loss", logits, old_policy, advantages, target, weights)
     if not 0.0 <= clip < 1.0 or not 0.0 <= kl < float("inf"):
         raise ValueError("clip lies in [0, 1), kl is not negative")

@@ -226,3 +226,36 @@ def test_a_4_bit_network_in_host_memory_refuses_its_calls(networks, launches):
         with pytest.raises(ValueError, match="CUDA"):
             net.net(torch.zeros(rows, net.IN_PADDED, dtype=torch.bfloat16))
     assert not launches
+
+
+def test_forward_mode_tangents_are_refused(launches):
+    """A dual tensor requires no gradient, so it would pass for a constant and its tangent be lost."""
+    from poker2_b200 import gated, policy_loss as pl
+
+    bf16 = lambda *s: torch.zeros(*s, dtype=torch.bfloat16).as_subclass(_Elsewhere)  # noqa: E731
+    f32 = lambda *s: torch.zeros(*s).as_subclass(_Elsewhere)  # noqa: E731
+    legal, w = torch.ones(2, 4, dtype=torch.bool).as_subclass(_Elsewhere), _there(_quantised(4, 32))
+    layer = [lambda: bf16(5, 32), lambda: bf16(8, 32), lambda: bf16(8, 32), lambda: bf16(8), lambda: bf16(8)]
+    loss = [lambda: f32(2, 3, 4), lambda: f32(2, 3, 4), lambda: f32(2, 3, 4), lambda: f32(2, 3, 4), lambda: f32(2, 3)]
+    calls = [
+        (gated.gated_linear, layer), (gated.gated_linear_backward, [lambda: bf16(5, 8), *layer]), (mx4.quantise, [lambda: f32(3, 32)]),
+        (lambda x, b: mx4.linear(x, w, b), [lambda: bf16(3, 32), lambda: bf16(4)]), (lambda b: mx4.linear(_there(_quantised(6, 32)), w, b), [lambda: bf16(4)]),
+        (lambda x: mx4.linear(x, w, quantised=True), [lambda: bf16(3, 32)]),
+        (lambda z, o, a, t, h: pl.clipped_policy_loss(z, o, a, t, legal, h), loss),
+        (lambda z, o, a, t, h: pl.clipped_policy_loss_and_grad(z, o, a, t, legal, h), loss),
+    ]
+    for call, make in calls:
+        with torch.autograd.forward_ad.dual_level():
+            for i in range(len(make)):
+                args = [m() for m in make]
+                args[i] = torch.autograd.forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*args)
+            assert not launches
+            call(*(m() for m in make))  # (without a tangent it goes through there too)
+            assert launches
+            launches.clear()
+        call(*(m() for m in make))
+        launches.clear()
