@@ -67,6 +67,9 @@ def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tenso
     from .fused_cfr import unblocked_mass_triton
 
     _lib.require_cuda(beliefs, "hand_weights")
+    if torch.is_grad_enabled() and beliefs.requires_grad:
+        raise RuntimeError("hand_weights has no gradient: detach the beliefs")  # (half of the product's would be lost in the kernel)
+    _lib.refuse_tangents("hand_weights", beliefs)
     n = beliefs.shape[0]
     if tuple(beliefs.shape) != (n, 2 * NUM_HANDS) or tuple(to_act.shape) != (n,) or board.dim() != 2 or board.shape[0] != n:
         raise ValueError("beliefs [n, 2652], to_act [n] and board [n, L] are wanted")

@@ -259,3 +259,20 @@ def test_forward_mode_tangents_are_refused(launches):
             launches.clear()
         call(*(m() for m in make))
         launches.clear()
+
+
+def test_hand_weights_have_no_gradient(monkeypatch):
+    """One factor of the product comes from a kernel: a gradient through the other alone would be half of it."""
+    from poker2_b200 import fused_cfr, policy_loss
+
+    monkeypatch.setattr(_lib, "require_cuda", lambda t, what: None)
+    monkeypatch.setattr(fused_cfr, "unblocked_mass_triton", lambda ranges: ranges.detach() * 0 + 1)
+    beliefs, to_act, board = torch.rand(2, 2 * 1326), torch.tensor([0, 1]), torch.full((2, 5), -1)
+    want = policy_loss.hand_weights(beliefs, to_act, board)
+    leaf = beliefs.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="detach"):
+        policy_loss.hand_weights(leaf, to_act, board)
+    with torch.no_grad():
+        assert torch.equal(policy_loss.hand_weights(leaf, to_act, board), want)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        policy_loss.hand_weights(torch.autograd.forward_ad.make_dual(beliefs, torch.ones_like(beliefs)), to_act, board)
