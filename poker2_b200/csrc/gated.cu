@@ -835,7 +835,7 @@ static int launch_few(const void* x, int64_t x_stride, const void* wg, int64_t w
 }
 
 // Whether the forward pass of a training step keeps gate and up for the backward pass, or that takes the projections again.  Kept
-// they are 8 bytes a hidden value to write and to read, taken again 4 * width operations.  Both passes of 8192 rows to 1024, taken
+// they are 8 bytes a hidden value (of hidden rounded up to 128) to write and to read, taken again 4 * width operations.  Both passes of 8192 rows to 1024, taken
 // again and kept: width 512 115 and 110 us, 1024 133 and 121, 1536 180 and 156, 2720 306 and 248.  Below a width of 1024 that is not
 // worth the memory, and below 2^33 products autograd takes longer on the host than the kernels (1000 rows of 1536 to 1024: 57 and 47 us
 // of kernels, 125 and 132 for the call).  The kernels that keep them are the pairs'.

@@ -3,7 +3,8 @@
 `gated_linear` is the layer, with gradients through autograd; `gated_linear_backward` gives the gradients by themselves, for
 callers that keep their own tape or capture a training step in a CUDA graph.  Both projections, the activation and the
 product are one kernel; the backward pass takes the projections anew or, in large layers where that takes longer, finds gate and up
-as autograd's forward pass kept them, 8 bytes a hidden value: the same bits either way.
+as autograd's forward pass kept them: the same bits either way.  What is kept takes 8 bytes a hidden value (of `hidden` rounded up to 128,
+so up to 16; narrower layers keep nothing), four times h, from forward to backward; `keep=False`, or no memory for it, takes them anew.
 `leaf_eval.GatedValueMLP` is a value network made of such layers.
 """
 from __future__ import annotations
@@ -19,17 +20,18 @@ FEW_ROWS = 4  # up to so many rows the forward pass reads operands of any alignm
 
 
 def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, gate_bias: torch.Tensor | None = None,
-                 up_bias: torch.Tensor | None = None, *, activation: str = "gelu") -> torch.Tensor:
+                 up_bias: torch.Tensor | None = None, *, activation: str = "gelu", keep: bool = True) -> torch.Tensor:
     """x [..., width], gate_weight and up_weight [hidden, width], biases [hidden] or None, all bf16 or all fp16 on one GPU
     -> act(x Wg^T + bg) * (x Wu^T + bu) [..., hidden].  Sums are fp32 and the result is rounded once.  `activation` is
     "gelu" (with erf) or "silu".  Any strides; rows that start on 16-byte boundaries (and weights likewise) are read in place.
+    `keep`: large training steps may hold gate and up for the backward pass, 8 to 16 bytes a hidden value.
     With gradients wanted the call is refused while a CUDA graph is being captured: use `gated_linear_backward` there."""
     act = _check(x, gate_weight, up_weight, gate_bias, up_bias, activation)
     _lib.refuse_tangents("gated_linear", x, gate_weight, up_weight, gate_bias, up_bias)
     if torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad
                                     or gate_bias is not None and gate_bias.requires_grad or up_bias is not None and up_bias.requires_grad):
         _refuse_capture("gated_linear")
-        return _Gated.apply(x, gate_weight, up_weight, gate_bias, up_bias, act)
+        return _Gated.apply(x, gate_weight, up_weight, gate_bias, up_bias, act, keep)
     return _forward(x, gate_weight, up_weight, gate_bias, up_bias, act)
 
 
@@ -98,12 +100,24 @@ def _align_bytes(*matrices) -> int:
     return 0
 
 
+def _kept_area(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor | None:
+    """Where the forward pass keeps gate and up; None where it does not, where most of it would be what `hidden` is rounded up by, and
+    where there is no room."""
+    hidden, width = weight.shape
+    rows = x.numel() // width
+    size = _lib.lib().p2b_gated_kept_bytes(rows, width, hidden)
+    if not 0 < size <= 16 * rows * hidden:
+        return None
+    try:
+        return x.new_empty((size // 2,))
+    except torch.cuda.OutOfMemoryError:
+        return None
+
+
 class _Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, act):
-        hidden, width = gate_weight.shape
-        size = _lib.lib().p2b_gated_kept_bytes(x.numel() // width, width, hidden) if x.numel() * hidden >= KEPT_PRODUCTS else 0
-        kept = x.new_empty((size // 2,)) if size > 0 else None
+    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, act, keep):
+        kept = _kept_area(x, gate_weight) if keep and x.numel() * gate_weight.shape[0] >= KEPT_PRODUCTS else None
         ctx.save_for_backward(x, gate_weight, up_weight, gate_bias, up_bias, kept)
         ctx.act = act
         return _forward(x, gate_weight, up_weight, gate_bias, up_bias, act, kept)
@@ -114,7 +128,7 @@ class _Gated(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("gated_linear has no second derivatives (create_graph=True)")
         _lib.refuse_tangents("the backward pass of gated_linear", grad_h)
-        return (*_backward(grad_h, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad), None)
+        return (*_backward(grad_h, *ctx.saved_tensors, ctx.act, ctx.needs_input_grad), None, None)
 
 
 def _refuse_capture(what: str) -> None:

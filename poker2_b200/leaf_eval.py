@@ -83,9 +83,10 @@ class ValueMLP(torch.nn.Module):
 
 
 class GatedBlock(torch.nn.Module):
-    """x + Wd (act(Wg n(x) + bg) * (Wu n(x) + bu)) + bd with n a layer norm: the gated hidden layer as a residual block."""
+    """x + Wd (act(Wg n(x) + bg) * (Wu n(x) + bu)) + bd with n a layer norm: the gated hidden layer as a residual block.  `keep`: as in
+    `gated.gated_linear`."""
 
-    def __init__(self, width: int, hidden: int, *, activation: str = "gelu", generator: torch.Generator | None = None):
+    def __init__(self, width: int, hidden: int, *, activation: str = "gelu", keep: bool = True, generator: torch.Generator | None = None):
         super().__init__()
         self.norm = torch.nn.LayerNorm(width)
         new = lambda rows, columns: torch.nn.Parameter(torch.randn(rows, columns, generator=generator) / columns ** 0.5)  # noqa: E731
@@ -95,10 +96,10 @@ class GatedBlock(torch.nn.Module):
         with torch.no_grad():
             self.down.weight.copy_(new(width, hidden))
             self.down.bias.zero_()
-        self.activation = activation
+        self.activation, self.keep = activation, keep
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        h = gated.gated_linear(self.norm(x), self.gate_weight, self.up_weight, self.gate_bias, self.up_bias, activation=self.activation)
+        h = gated.gated_linear(self.norm(x), self.gate_weight, self.up_weight, self.gate_bias, self.up_bias, activation=self.activation, keep=self.keep)
         return x + self.down(h)
 
 
@@ -106,11 +107,11 @@ class GatedValueMLP(ValueMLP):
     """`ValueMLP` with `depth - 1` gated residual blocks of `hidden` units for its inner layers; same input and output rows, so
     the leaf evaluators take it on the same paths.  Runs on the GPU, bf16 or fp16."""
 
-    def __init__(self, width: int = 1536, depth: int = 4, *, hidden: int | None = None, activation: str = "gelu", dtype=torch.bfloat16, seed: int = 0):
+    def __init__(self, width: int = 1536, depth: int = 4, *, hidden: int | None = None, activation: str = "gelu", keep: bool = True, dtype=torch.bfloat16, seed: int = 0):
         super().__init__(width, 1, dtype=dtype, seed=seed)
         g = torch.Generator().manual_seed(seed + 1)
         first, act, last = self.net
-        blocks = [GatedBlock(width, hidden or 2 * width // 3, activation=activation, generator=g) for _ in range(depth - 1)]
+        blocks = [GatedBlock(width, hidden or 2 * width // 3, activation=activation, keep=keep, generator=g) for _ in range(depth - 1)]
         self.net = torch.nn.Sequential(first, act, *blocks, last).to(dtype)
 
 

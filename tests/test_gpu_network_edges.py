@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import network_refs as refs
-from poker2_b200 import leaf_eval, mx4, policy_loss as pl
+from poker2_b200 import _lib, gated, leaf_eval, mx4, policy_loss as pl
 
 pytestmark = pytest.mark.gpu
 
@@ -232,3 +232,60 @@ def test_a_4_bit_network_saved_loaded_copied_and_moved(cuda_device, tmp_path):
     with pytest.raises(ValueError, match="type"):
         one.half()
     assert torch.equal(one.net(x), want)
+
+
+def _gated_layer(rows, width, hidden, device):
+    g = torch.Generator(device=device).manual_seed(rows + width + hidden)
+    new = lambda *s: torch.randn(*s, device=device, generator=g)  # noqa: E731
+    return [t.bfloat16() for t in (new(rows, width), new(hidden, width) / width ** 0.5, new(hidden, width) / width ** 0.5, new(hidden), new(hidden), new(rows, hidden))]
+
+
+def _training_step(inputs, dh, **options):
+    """Gradients of a step, and the bytes that were held between its passes."""
+    leaves = [t.clone().requires_grad_(True) for t in inputs]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    h = gated.gated_linear(*leaves, **options)
+    held = torch.cuda.memory_allocated() - before
+    return torch.autograd.grad(h, leaves, dh), held
+
+
+@pytest.mark.parametrize("rows,width,hidden,keeps", [(131080, 1024, 64, True), (131080, 1024, 63, False), (840000, 2048, 5, False), (8200, 1536, 1024, True), (50000, 1024, 193, True)])
+def test_what_a_training_step_holds_is_bounded(cuda_device, rows, width, hidden, keeps, monkeypatch):
+    """At most 16 bytes a hidden value beside h; nothing with keep=False or without the memory; the same gradients in every way."""
+    *inputs, dh = _gated_layer(rows, width, hidden, cuda_device)
+    output, whole = 2 * rows * hidden, 8 * rows * ((hidden + 127) // 128 * 128)
+    got, held = _training_step(inputs, dh)
+    slack = 1 << 21  # (the allocator's rounding)
+    assert held <= output + 16 * rows * hidden + slack and (held >= output + whole) == keeps
+    apart = gated.gated_linear_backward(dh, *inputs)
+    none, held = _training_step(inputs, dh, keep=False)
+    assert held <= output + slack
+
+    def full(*args, **kwargs):
+        raise torch.cuda.OutOfMemoryError("no room")
+
+    real = torch.Tensor.new_empty
+    monkeypatch.setattr(torch.Tensor, "new_empty", lambda t, size, **k: full() if len(size) == 1 and size[0] == whole // 2 else real(t, size, **k))
+    short, held = _training_step(inputs, dh)
+    assert held <= output + slack
+    for a, b, c, d in zip(got, apart, none, short):
+        assert torch.equal(a, b) and torch.equal(c, b) and torch.equal(d, b)
+
+
+def test_kept_values_of_more_rows_than_one_launch_takes(cuda_device):
+    rows, width, hidden = 65535 * 32 + 45, 1024, 5
+    *inputs, dh = _gated_layer(rows, width, hidden, cuda_device)
+    size = _lib.lib().p2b_gated_kept_bytes(rows, width, hidden)
+    kept = torch.empty(size // 2, dtype=torch.bfloat16, device=cuda_device)
+    gated._forward(*inputs, 0, kept)
+    needs = (False, True, True, True, True)
+    for a, b in zip(gated._backward(dh, *inputs, kept, 0, needs)[1:], gated.gated_linear_backward(dh, *inputs, needs=needs)[1:]):
+        assert torch.equal(a, b)
+
+
+def test_networks_take_the_switch(cuda_device):
+    kept, anew = (leaf_eval.GatedValueMLP(1024, 2, hidden=1024, keep=keep, seed=3).to(cuda_device) for keep in (True, False))
+    x = torch.randn(8200, 1024, device=cuda_device).bfloat16()
+    grads = [torch.autograd.grad(net.net[2](x).float().sum(), net.net[2].gate_weight)[0] for net in (kept, anew)]
+    assert kept.net[2].keep and not anew.net[2].keep and torch.equal(*grads)
