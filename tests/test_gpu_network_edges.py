@@ -289,3 +289,37 @@ def test_networks_take_the_switch(cuda_device):
     x = torch.randn(8200, 1024, device=cuda_device).bfloat16()
     grads = [torch.autograd.grad(net.net[2](x).float().sum(), net.net[2].gate_weight)[0] for net in (kept, anew)]
     assert kept.net[2].keep and not anew.net[2].keep and torch.equal(*grads)
+
+
+def _leaves(device, leaves=70, seed=1):
+    g = torch.Generator(device=device).manual_seed(seed)
+    boards = torch.rand(leaves, 48, device=device, generator=g).argsort(dim=1)[:, :5] + 4  # none of cards 0 to 3
+    boards[:, 4] = -1
+    beliefs = torch.zeros(leaves, 2, 1344, device=device)
+    beliefs[..., :1326] = torch.rand(leaves, 2, 1326, device=device, generator=g)
+    beliefs /= beliefs.sum(-1, keepdim=True)
+    return boards, beliefs, torch.rand(leaves, 3, device=device, generator=g)
+
+
+def test_a_first_layer_in_16_bits_sees_what_a_shared_scale_hides(cuda_device):
+    """A one-hot card of 1 in a block leaves nothing of range entries below 1/16 beside it; in 16 bits it does."""
+    source = leaf_eval.ValueMLP(96, 2, seed=5).to(cuda_device)
+    with torch.no_grad():
+        source.net[0].weight[:, 2624:2652] *= 30.0
+    whole, mixed = leaf_eval.Mx4ValueMLP(source), leaf_eval.Mx4ValueMLP(source, quantise_first=False)
+    boards, beliefs, context = _leaves(cuda_device)
+    other = beliefs.clone()
+    other[:, 1, 1298:1326] *= 20.0  # columns 2624 to 2651
+    assert other[:, 1, 1298:1326].max() < 1 / 16
+    for card, hidden in ((3, True), (4, False)):
+        boards[:, 0] = card
+        same = [torch.equal(net(beliefs[..., :1326], boards, context), net(other[..., :1326], boards, context)) for net in (whole, mixed)]
+        assert same == [hidden, False]
+    x = torch.randn(50, 2720, device=cuda_device).bfloat16()
+    with torch.no_grad():
+        y = torch.nn.functional.gelu(source.net[0](x))
+        for layer, last in zip(list(mixed.net)[2:], (False, True)):
+            y = mx4.linear(y, layer.weight, layer.bias, activation="none" if last else "gelu")
+    assert torch.equal(mixed.net(x), y) and torch.equal(mixed.layers(x), y)
+    direct = leaf_eval.DirectLeafEvaluator(mixed, boards, context, cuda_device)
+    assert direct._direct() and torch.equal(direct(beliefs), mixed(beliefs[..., :1326], boards, context))

@@ -276,3 +276,21 @@ def test_hand_weights_have_no_gradient(monkeypatch):
         assert torch.equal(policy_loss.hand_weights(leaf, to_act, board), want)
     with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         policy_loss.hand_weights(torch.autograd.forward_ad.make_dual(beliefs, torch.ones_like(beliefs)), to_act, board)
+
+
+def test_a_4_bit_network_whose_first_layer_stays(networks):
+    from poker2_b200 import leaf_eval
+
+    source = leaf_eval.ValueMLP(64, 2, seed=4)
+    net = leaf_eval.Mx4ValueMLP(source, quantise_first=False)
+    assert [type(m) for m in net.net] == [torch.nn.Linear, torch.nn.GELU, leaf_eval.Mx4Linear, leaf_eval.Mx4Linear]
+    assert [m.hands_on for m in list(net.net)[2:]] == [True, False] and [m.activation for m in list(net.net)[2:]] == ["gelu", "none"]
+    assert torch.equal(net.net[0].weight, source.net[0].weight) and net.net[0].weight is not source.net[0].weight and not net.net[0].weight.requires_grad
+    other = leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(64, 2, seed=5), quantise_first=False)
+    other.load_state_dict(net.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(net.buffers(), other.buffers())) and torch.equal(net.net[0].weight, other.net[0].weight)
+    with pytest.raises(ValueError, match="type"):
+        net.half()
+    assert net.net[0].weight.dtype == torch.bfloat16
+    with pytest.raises(ValueError, match="nothing"):
+        leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(64, 0), quantise_first=False)
