@@ -137,7 +137,10 @@ class Mx4Linear(torch.nn.Module):
 
     @property
     def weight(self) -> mx4.Mx4:
-        return mx4.Mx4(self._buffers["values"], self._buffers["scales"], self.shape)
+        own, m = self._buffers, self.__dict__.get("_weight")
+        if m is None or m.values is not own["values"] or m.scales is not own["scales"]:
+            m = self.__dict__["_weight"] = mx4.Mx4(own["values"], own["scales"], self.shape)
+        return m
 
     def forward(self, x: torch.Tensor | mx4.Mx4) -> torch.Tensor | mx4.Mx4:
         rows = x.rows if isinstance(x, mx4.Mx4) else x.shape[:-1].numel()
@@ -145,6 +148,7 @@ class Mx4Linear(torch.nn.Module):
 
     def _apply(self, fn, recurse=True):
         _refuse_type_change(fn, self.dtype, self.values.device)
+        self.__dict__.pop("_weight", None)  # (it holds the arrays that are left behind)
         return super()._apply(fn, recurse)
 
     def get_extra_state(self):  # (widths up to 31 apart have arrays of one size)

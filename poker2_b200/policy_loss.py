@@ -37,7 +37,7 @@ def clipped_policy_loss(logits: torch.Tensor, old_policy: torch.Tensor | None, a
     gradient)."""
     _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
     if not (torch.is_grad_enabled() and logits.requires_grad):
-        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, None)[0]
+        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, False)[0]
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("clipped_policy_loss cannot be captured into a CUDA graph through autograd; call clipped_policy_loss_and_grad, which can.")
     return _Loss.apply(logits, old_policy, advantages, target, legal, weights, clip, kl)
@@ -51,13 +51,14 @@ def clipped_policy_loss_and_grad(logits: torch.Tensor, old_policy: torch.Tensor 
     loss stays as it is) before it is rounded: what a gradient scaler brings, without which entries of the size 1 / (states * hands)
     are lost in fp16."""
     _check(logits, old_policy, advantages, target, legal, weights, clip, kl)
-    if isinstance(scale, torch.Tensor):
+    at = None
+    if type(scale) is not float and isinstance(scale, torch.Tensor):
         if scale.numel() != 1 or scale.dtype != torch.float32 or scale.get_device() != logits.get_device():
             raise ValueError("the scale is a number, or an fp32 tensor of one element on the logits' device")
-        return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, logits.dtype, 1.0, scale.data_ptr())
-    if not abs(scale) <= 3.4028234e38:
+        scale, at = 1.0, scale.data_ptr()
+    elif not abs(scale) <= 3.4028234e38:
         raise ValueError("the scale is finite")
-    return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, logits.dtype, scale)
+    return _run(logits, old_policy, advantages, target, legal, weights, clip, kl, True, scale, at)
 
 
 def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tensor) -> torch.Tensor:
@@ -89,9 +90,9 @@ def hand_weights(beliefs: torch.Tensor, to_act: torch.Tensor, board: torch.Tenso
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, old_policy, advantages, target, legal, weights, clip, kl):
-        loss, grad = _run(logits, old_policy, advantages, target, legal, weights, clip, kl, torch.float32 if logits.dtype == torch.float16 else logits.dtype)
+        ctx.wide = logits.dtype is torch.float16
+        loss, grad = _run(logits, old_policy, advantages, target, legal, weights, clip, kl, True, wide=ctx.wide)
         ctx.save_for_backward(grad)
-        ctx.dtype = logits.dtype
         return loss
 
     @staticmethod
@@ -102,10 +103,11 @@ class _Loss(torch.autograd.Function):
             raise RuntimeError("clipped_policy_loss has no second derivatives (create_graph=True)")
         _lib.refuse_tangents("the backward pass of clipped_policy_loss", factor)
         grad, = ctx.saved_tensors
-        out = torch.empty_like(grad, dtype=ctx.dtype)
-        if ctx.dtype != grad.dtype:
+        if ctx.wide:
+            out = torch.empty_like(grad, dtype=torch.float16)
             _lib.call_on(grad.get_device(), "p2b_policy_loss_scale_fp32", grad.data_ptr(), factor.data_ptr(), grad.numel(), out.data_ptr())
         else:
+            out = torch.empty_like(grad)
             _lib.call_on(grad.get_device(), "p2b_policy_loss_scale", grad.data_ptr(), factor.data_ptr(), grad.numel(), _TYPES[grad.dtype], out.data_ptr())
         return out, None, None, None, None, None, None, None
 
@@ -114,19 +116,21 @@ def _packed(t):
     return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
-def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, grad_dtype, scale=1.0, scale_at=None):
-    """(loss, the gradient times scale and *scale_at in grad_dtype, or None)."""
+def _run(logits, old_policy, advantages, target, legal, weights, clip, kl, with_grad, scale=1.0, scale_at=None, wide=False):
+    """(loss, the gradient times scale and *scale_at, of the logits' type or fp32 where `wide`; None where it is not wanted)."""
     states, hands, actions = logits.shape
     logits, target, legal = _packed(logits), _packed(target), _packed(legal)
     old_policy, advantages, weights = _packed(old_policy), _packed(advantages), _packed(weights)
     loss = target.new_empty(())
-    grad = None if grad_dtype is None else logits.new_empty((states, hands, actions), dtype=grad_dtype)
+    grad = None if not with_grad else target.new_empty((states, hands, actions)) if wide else logits.new_empty((states, hands, actions))
     size = _lib.lib().p2b_policy_loss_scratch_bytes(states, hands)
     scratch = target.new_empty((size // 4,)) if size else None
-    _lib.call_on(logits.get_device(), "p2b_policy_loss_scaled", logits.data_ptr(), None if old_policy is None else old_policy.data_ptr(),
+    kind = _TYPES[logits.dtype]
+    scaled = (2 if wide else kind, scale, scale_at) if wide or scale != 1.0 or scale_at else ()
+    _lib.call_on(logits.get_device(), "p2b_policy_loss_scaled" if scaled else "p2b_policy_loss", logits.data_ptr(), None if old_policy is None else old_policy.data_ptr(),
                  None if advantages is None else advantages.data_ptr(), target.data_ptr(), legal.data_ptr(),
-                 None if weights is None else weights.data_ptr(), states, hands, actions, _TYPES[logits.dtype], clip, kl, loss.data_ptr(),
-                 None if grad is None else grad.data_ptr(), _TYPES[grad_dtype or logits.dtype], scale, scale_at, None if scratch is None else scratch.data_ptr(), size)
+                 None if weights is None else weights.data_ptr(), states, hands, actions, kind, clip, kl, loss.data_ptr(),
+                 None if grad is None else grad.data_ptr(), *scaled, None if scratch is None else scratch.data_ptr(), size)
     return loss, grad
 
 
