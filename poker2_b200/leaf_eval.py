@@ -178,9 +178,13 @@ class Mx4ValueMLP(ValueMLP):
 
     def __init__(self, source: ValueMLP, *, quantise_first: bool = True):
         torch.nn.Module.__init__(self)
-        if type(source) is not ValueMLP or source.dtype not in (torch.bfloat16, torch.float16):
+        if type(source) is not ValueMLP:
             raise ValueError("a bf16 or fp16 ValueMLP is quantised")
         layers = list(source.net)
+        # (of the layers themselves: a source that was turned into another type still says the one it was made in)
+        types = {t.dtype for t in source.net.parameters()}
+        if len(types) != 1 or not types <= {torch.bfloat16, torch.float16}:
+            raise ValueError("a bf16 or fp16 ValueMLP is quantised, all its layers of one type")
         if any(type(m) not in (torch.nn.Linear, torch.nn.GELU) or type(m) is torch.nn.GELU and m.approximate != "none" for m in layers):
             raise ValueError("linear layers and GELUs are quantised, nothing else")
         if any(type(m) is torch.nn.GELU and (i == 0 or type(layers[i - 1]) is not torch.nn.Linear) for i, m in enumerate(layers)):
@@ -192,7 +196,7 @@ class Mx4ValueMLP(ValueMLP):
         quantised = [Mx4Linear(m, after(i), i < last) for i, m in enumerate(layers) if type(m) is torch.nn.Linear and (quantise_first or i > 0)]
         kept = [] if quantise_first else [copy.deepcopy(layers[0]).requires_grad_(False)] + [torch.nn.GELU()] * (after(0) == "gelu")
         self.net = torch.nn.Sequential(*kept, *quantised)
-        self.dtype = source.dtype
+        self.dtype = types.pop()
 
     def _apply(self, fn, recurse=True):
         _refuse_type_change(fn, self.dtype, next(self.buffers()).device)  # (before any layer is changed)
@@ -326,7 +330,7 @@ class DirectLeafEvaluator:
 
     def _direct(self) -> bool:
         """The model's layers may be called on rows kept here instead of the model itself."""
-        return self._rows is not None and type(self.model) in _ROW_NETWORKS and _bare(self.model)
+        return self._rows is not None and type(self.model) in _ROW_NETWORKS and self.model.dtype == torch.bfloat16 and _bare(self.model)
 
     def __call__(self, leaf_beliefs: torch.Tensor) -> torch.Tensor:
         if not self._direct():

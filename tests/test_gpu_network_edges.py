@@ -323,3 +323,18 @@ def test_a_first_layer_in_16_bits_sees_what_a_shared_scale_hides(cuda_device):
     assert torch.equal(mixed.net(x), y) and torch.equal(mixed.layers(x), y)
     direct = leaf_eval.DirectLeafEvaluator(mixed, boards, context, cuda_device)
     assert direct._direct() and torch.equal(direct(beliefs), mixed(beliefs[..., :1326], boards, context))
+
+
+@pytest.mark.parametrize("kind", [leaf_eval.DirectLeafEvaluator, leaf_eval.ChanceLeafEvaluator])
+def test_evaluators_read_a_4_bit_network_in_its_type(cuda_device, kind):
+    source = leaf_eval.ValueMLP(96, 2, seed=6).to(cuda_device)
+    half = leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(96, 2, seed=6).to(cuda_device).half())
+    boards, beliefs, context = _leaves(cuda_device, leaves=9)
+    got, want = (kind(net, boards, context, cuda_device)(beliefs) for net in (half, leaf_eval.Mx4ValueMLP(source)))
+    # (of one network in two types: roundings to 8 bits and the 4-bit steps that these change)
+    assert torch.isfinite(got).all() and (got[..., :1326] - want[..., :1326]).norm() < 0.5 * want.norm()
+    if kind is leaf_eval.DirectLeafEvaluator:  # another network put in place of the one it was made for
+        short = kind(leaf_eval.Mx4ValueMLP(source), boards, context, cuda_device)
+        assert short._direct()
+        short.model = half
+        assert not short._direct() and torch.equal(short(beliefs), got)

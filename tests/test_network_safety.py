@@ -294,3 +294,19 @@ def test_a_4_bit_network_whose_first_layer_stays(networks):
     assert net.net[0].weight.dtype == torch.bfloat16
     with pytest.raises(ValueError, match="nothing"):
         leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(64, 0), quantise_first=False)
+
+
+def test_a_4_bit_network_has_the_type_of_its_layers(networks):
+    """A source made in bf16 and turned into fp16 gives fp16 outputs, which the evaluators' short paths would read as bf16."""
+    from poker2_b200 import leaf_eval
+
+    source = leaf_eval.ValueMLP(64, 1)
+    assert leaf_eval.Mx4ValueMLP(source).dtype == torch.bfloat16
+    net = leaf_eval.Mx4ValueMLP(source.half())
+    assert net.dtype == torch.float16 and all(layer.dtype == torch.float16 for layer in net.net)
+    assert not leaf_eval.ChanceLeafEvaluator(net, torch.full((2, 5), -1), torch.zeros(2, 3), torch.device("cpu")).fused
+    source.net[0].bfloat16()
+    with pytest.raises(ValueError, match="one type"):
+        leaf_eval.Mx4ValueMLP(source)
+    with pytest.raises(ValueError, match="one type"):
+        leaf_eval.Mx4ValueMLP(leaf_eval.ValueMLP(64, 1).float())
