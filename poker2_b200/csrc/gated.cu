@@ -3,7 +3,8 @@
 // One tile of 128 rows holds 128 gate and 128 up columns next to each other in tensor memory (one matrix instruction of
 // 256 columns, its operand half from Wg, half from Wu), so the activation and the product happen on the accumulators and
 // neither projection goes through memory.  Bound by the matrix instructions and what feeds them: 24576 rows of 1536 -> 1024 (155
-// GFLOP, 2 x 1024 x 1536 weights in L2) take 110 to 125 us, 1.24 to 1.41 PFLOP/s, at 13 TB/s out of L2.  The backward pass takes the
+// GFLOP, 2 x 1024 x 1536 weights in L2) take 110 to 125 us, 1.24 to 1.41 PFLOP/s; 1.21 GB of operand tiles come
+// out of L2 meanwhile, 9.7 to 11 TB/s.  The backward pass takes the
 // same products again or, in large layers, finds gate and up in fp32 as the forward pass of the step kept them (`keeps` below).  From
 // them come dgate = dh * up * act'(gate) and dup = dh * act(gate) (16-bit, side by side in work space), and from these
 // dx = dgate Wg + dup Wu, dWg = dgate^T x, dWu = dup^T x and the column sums.
@@ -901,8 +902,8 @@ extern "C" int p2b_gated_forward(const void* x, int64_t x_stride, const void* wg
 
 // dgate and dup are rounded to 16 bits on their way into the products, which makes the gradients' error 1.4 times that of their
 // last rounding alone.  Two 16-bit numbers for each would take it away and make the products twice as long (1000 rows of 1536 x 1024: 35
-// -> 48 us for the whole pass).  So only small layers have them (16 rows of 72 x 64: 11.1 -> 11.9 us), where few values
-// let the error of a single gradient stray further from that mean.
+// -> 48 us for the whole pass).  Small layers have them all the same, for 1 us (16 rows of 72 x 64: 11.1 -> 11.9
+// us): a layer's gradients are therefore more exact on few rows than on many.
 constexpr int64_t kSmallProducts = 1ll << 24;
 static int parts_of(int64_t rows, int64_t width, int64_t hidden) { return rows * hidden <= kSmallProducts / width ? 2 : 1; }
 

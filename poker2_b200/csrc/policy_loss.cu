@@ -7,7 +7,7 @@
 // r = p/q, summed over the actions instead of sampled; written without the division, so q = 0 is no special case.)
 //
 // Bound by memory: an action's logit, three fp32 policies and the gradient; 4096 states of 1326 hands and 8 actions, bf16 logits (708
-// MB) take 136 us, 5.2 TB/s.  A block takes 256 hands, whose arrays come as one
+// MB) take 140 us, 5.1 TB/s.  A block takes 256 hands, whose arrays come as one
 // bulk copy each (hands of 5 actions are 20 bytes: read by thread they would be five sectors an instruction).  Which side
 // of the min is taken is decided in 64 bits where 32 might get it wrong: the gradient jumps there.
 #include "layer.cuh"
@@ -171,7 +171,7 @@ __device__ __noinline__ uint32_t settle_hand(const T* z, const float* old, const
 }
 
 // Blocks stay: each takes every gridDim.x-th tile of 256 hands, with the tiles after the present one on their way into the other
-// two of three stages (two stages in all: 225 us instead of 146 for the states above).  The gradient overwrites the logits (in fp32: the
+// two of three stages (two stages in all: half as long again for the states above).  The gradient overwrites the logits (in fp32: the
 // targets) of its stage and leaves from there.
 // Blocks a multiprocessor that registers are to leave room for, as many as shared memory does (8 actions, one block instead of two: 217 us
 // instead of 150 for the states above).
